@@ -258,6 +258,95 @@ int maivs_concurrent_kernel_times(maivs_concurrent* cx, int reset, const char** 
 int maivs_concurrent_array(maivs_concurrent* cx, long long segment, const char* name, const void** data,
                            size_t* count, size_t* elem_bytes);
 
+/* The attention cache (no counterpart in the reference): the read-out that follows a search. A cache
+ * holds key and value rows of n_seqs sequences in 4 bits, and answers queries with the
+ * softmax-weighted sum of the values: over every row of a sequence, or over the rows that a search
+ * named. Rows leave by the attention weight they gathered, as an index's rows leave by id.
+ *
+ * A row of one head is stored per group of 64 dimensions as step =
+ * bf16(f32(f32(max - min) * f32(1 / 15))), low = bf16(min) and 4-bit codes; a code c stands for f32(low + step * c) and is the nearest level
+ * to its element (ties to the even code). Groups that hold a NaN or an infinity, or whose range
+ * overflows f32, read back as NaN. dim is padded to 64, 128, 256 or 384; a padded row of one head
+ * takes 36 bytes per 64 dimensions for its key and as many for its value.
+ *
+ * All pointers are device memory of the cache's device, all tensors row-major; work is enqueued on
+ * `stream` (a cudaStream_t; NULL is the default stream) and the call returns without waiting. No
+ * call allocates: storage is the handle's, everything else the caller's, so a step can be captured
+ * into a graph. Work of one cache that overlaps on the GPU must not write what the other uses: a
+ * workspace serves one call at a time, rows are written by append and evict only.
+ *
+ * Tokens of a call are packed: sequence s has the tokens d_offsets[s] .. d_offsets[s + 1] - 1
+ * (int32, n_seqs + 1 of them, ascending within 0..n_tokens); d_lengths[s] (int32) is the number of
+ * rows it held before this step. Tokens before the first or behind the last sequence are padding:
+ * nothing is read or written for them. Row tables (weights f32, ids u64) are [n_seqs][capacity].
+ * dtype is that of keys, values, queries and outputs. A stride counts elements from token to token
+ * (0: packed); a token's heads are adjacent. */
+typedef struct maivs_cache maivs_cache;
+
+typedef enum { MAIVS_F32 = 0, MAIVS_F16 = 1, MAIVS_BF16 = 2 } maivs_dtype;
+
+/* n_seqs 1..65535, capacity (rows per sequence) 1..2^27, n_heads 1..1024, dim 1..384. device < 0
+ * makes a handle without storage, for sizes and argument checks (its calls return
+ * MAIVS_NO_DEVICE). On failure *out still holds a handle carrying the message. */
+int maivs_cache_new(size_t n_seqs, size_t capacity, size_t n_heads, size_t dim, int device, maivs_cache** out);
+void maivs_cache_free(maivs_cache* cx);
+const char* maivs_cache_last_error(maivs_cache* cx);
+/* "n_seqs", "capacity", "n_heads", "dim", "device", "device_bytes", "row_bytes" (key and value of one
+ * row of one head) */
+int maivs_cache_stat(maivs_cache* cx, const char* name, double* value);
+/* Token i of sequence s becomes row d_lengths[s] + i - d_offsets[s] (keys and values
+ * [n_tokens][n_heads][dim]). Rows past the capacity are left out and set flag 1. The new rows'
+ * entries of d_weights are set to 0 and those of d_ids to d_token_ids[i] (each NULL: not kept). */
+int maivs_cache_append(maivs_cache* cx, const void* d_keys, const void* d_values, int dtype, size_t n_tokens,
+                       size_t key_stride, size_t value_stride, const int32_t* d_offsets, const int32_t* d_lengths,
+                       float* d_weights, uint64_t* d_ids, const uint64_t* d_token_ids, void* stream);
+/* The values of the same rows, [n_tokens][n_heads][dim] rounded to dtype. */
+int maivs_cache_read(maivs_cache* cx, void* d_keys, void* d_values, int dtype, size_t n_tokens,
+                     const int32_t* d_offsets, const int32_t* d_lengths, void* stream);
+/* out[token][head] = sum over visible rows r of softmax(scale * q . key_r) value_r; query heads
+ * h * g .. h * g + g - 1 read head h, g = n_query_heads / n_heads. With causal set, token i of its
+ * sequence sees rows below d_lengths[s] + i + 1 (this step's appended rows up to its own); else rows
+ * below d_lengths[s]. A token that sees no row gives 0. d_lse (f32 [n_tokens][n_query_heads], may be
+ * NULL) receives log(sum(exp(scale * q . key))), -inf where no row is seen. With d_weights_in /
+ * d_weights_out (both or neither; they may be the same), out[row] = decay * in[row] + the softmax
+ * weights of all the call's tokens and heads, for the rows that the step's last token may see (every
+ * row below d_lengths[s] for a sequence without tokens); other entries are left as they are.
+ * max_rows (0: capacity) bounds the rows of a sequence: a longer one is read up to it and sets flag
+ * 2. max_tokens (0: n_tokens) is the expected number of tokens of a sequence; it only sizes the
+ * launch. Offsets that do not ascend within 0..n_tokens set flag 4; those sequences are skipped. */
+int maivs_cache_attend(maivs_cache* cx, const void* d_queries, int dtype, size_t n_tokens, size_t query_stride,
+                       size_t n_query_heads, const int32_t* d_offsets, const int32_t* d_lengths, int causal,
+                       float scale, size_t max_rows, size_t max_tokens, void* d_out, float* d_lse,
+                       const float* d_weights_in, float* d_weights_out, float decay, void* d_workspace,
+                       size_t workspace_bytes, void* stream);
+/* Bytes of workspace that such a call needs (16-byte aligned; contents need not be kept or set). */
+int maivs_cache_attend_workspace(maivs_cache* cx, size_t n_tokens, size_t n_query_heads, size_t max_rows,
+                                 size_t max_tokens, int weights, size_t* bytes);
+/* attend over the rows d_rows[token][0 .. k), as maivs_search_batch_device writes ids: an entry that
+ * is not a row the token sees (UINT64_MAX padding among them) is left out, one that occurs twice
+ * counts twice. d_weights ([n_tokens][k], may be NULL) receives each entry's softmax weight summed
+ * over the query heads (0 for entries left out). */
+int maivs_cache_attend_found(maivs_cache* cx, const void* d_queries, int dtype, size_t n_tokens, size_t query_stride,
+                             size_t n_query_heads, const int32_t* d_offsets, const int32_t* d_lengths,
+                             const uint64_t* d_rows, size_t k, int causal, float scale, void* d_out, float* d_lse,
+                             float* d_weights, void* d_workspace, size_t workspace_bytes, void* stream);
+int maivs_cache_attend_found_workspace(maivs_cache* cx, size_t n_tokens, size_t n_query_heads, size_t k, int weights,
+                                       size_t* bytes);
+/* Keeps the min(keep, length) heaviest rows of every sequence by d_weights_in, ties to the lower row.
+ * Rows whose id is d_protect_from[s] or above, and rows of NaN weight, rank as +inf. Kept rows below
+ * the new length stay in place; the others, in ascending order, move into the freed rows, in
+ * ascending order, with their weights and ids. d_weights_out, d_ids_out: entries below the new
+ * length (the inputs' own memory or other memory that does not overlap it). d_evicted ([n_seqs][capacity],
+ * may be NULL): the first length - new length entries receive the ids that left, by ascending row.
+ * Ids, protection and d_evicted are optional; the latter two need ids. */
+int maivs_cache_evict(maivs_cache* cx, const int32_t* d_lengths, size_t keep, const float* d_weights_in,
+                      float* d_weights_out, int32_t* d_new_lengths, const uint64_t* d_ids_in, uint64_t* d_ids_out,
+                      const uint64_t* d_protect_from, uint64_t* d_evicted, void* d_workspace, size_t workspace_bytes,
+                      void* stream);
+int maivs_cache_evict_workspace(maivs_cache* cx, size_t* bytes);
+/* Flags that earlier work set (see above), cleared by the call; synchronises `stream`. */
+int maivs_cache_flags(maivs_cache* cx, void* stream, uint32_t* flags);
+
 /* profile(on) / profile_read(reset=True) (src/prof.rs:76-98): device time per query phase. The
  * reader fills up to `cap` (name, milliseconds) pairs; names are static strings. */
 int maivs_profile(int on);

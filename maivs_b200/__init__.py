@@ -14,7 +14,7 @@ import numpy as np
 
 from . import _lib
 
-__all__ = ["FlatCellIndex", "ConcurrentIndex", "profile", "profile_read", "MaivsError", "nccl_unique_id",
+__all__ = ["FlatCellIndex", "ConcurrentIndex", "AttentionCache", "profile", "profile_read", "MaivsError", "nccl_unique_id",
            "shard_over_torch"]
 
 
@@ -593,6 +593,158 @@ class ConcurrentIndex:
             return np.zeros(0, dtype=dt)
         raw = np.ctypeslib.as_array(C.cast(p, C.POINTER(C.c_uint8)), shape=(n.value * eb.value,))
         return raw.view(dt).copy()
+
+
+_CACHE_DTYPES = {"f32": 0, "f16": 1, "bf16": 2}
+
+
+def _cache_dtype(dtype: str) -> int:
+    if dtype not in _CACHE_DTYPES:
+        raise ValueError(f"dtype must be one of {', '.join(_CACHE_DTYPES)}")
+    return _CACHE_DTYPES[dtype]
+
+
+def _size(x, name: str) -> int:
+    x = int(x)
+    if x < 0:
+        raise ValueError(f"{name} must not be negative")
+    return x
+
+
+class AttentionCache:
+    """Key and value rows of `n_seqs` sequences in 4 bits, and the softmax attention that reads them:
+    the read-out that follows a search, or a decoder's cache (no counterpart in the reference).
+
+    As `FlatCellIndex.search_batch_device`, the calls take device pointers (e.g. torch tensors'
+    data_ptr()) and enqueue on `stream` (0: the default stream) without waiting. Tokens of a call
+    are packed: sequence s has tokens offsets[s] .. offsets[s + 1] - 1 (int32 [n_seqs + 1]) and held
+    lengths[s] rows (int32) before the step. Row tables (weights f32, ids u64) are
+    [n_seqs, capacity]. The caller keeps lengths, tables and workspaces; the cache keeps the rows.
+    See include/maivs_b200.h for the formulas and every argument.
+
+    device=None makes a cache without storage, for sizes and argument checks."""
+
+    def __init__(self, n_seqs: int, capacity: int, n_heads: int, dim: int, device: int | None = 0):
+        L = _lib.lib()
+        h = C.c_void_p()
+        self._h = None
+        rc = L.maivs_cache_new(_size(n_seqs, "n_seqs"), _size(capacity, "capacity"), _size(n_heads, "n_heads"),
+                               _size(dim, "dim"), -1 if device is None else _size(device, "device"), C.byref(h))
+        self._h = h
+        self._dim = int(dim)
+        if rc != _lib.OK:
+            try:
+                self._check(rc)
+            finally:
+                L.maivs_cache_free(h)
+                self._h = None
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        if h:
+            _lib.lib().maivs_cache_free(h)
+            self._h = None
+
+    def _check(self, rc: int) -> None:
+        if rc == _lib.OK:
+            return
+        L = _lib.lib()
+        msg = L.maivs_cache_last_error(self._h).decode() if self._h else "allocation failed"
+        if rc in (_lib.BAD_SHAPE, _lib.BAD_ARG, _lib.BAD_STATE):
+            raise ValueError(msg)
+        raise MaivsError(f"{L.maivs_status_string(rc).decode()}: {msg}")
+
+    def append(self, d_keys: int, d_values: int, n_tokens: int, d_offsets: int, d_lengths: int, dtype: str = "bf16",
+               key_stride: int = 0, value_stride: int = 0, d_weights: int = 0, d_ids: int = 0, d_token_ids: int = 0,
+               stream: int = 0) -> None:
+        """Store tokens [n_tokens, n_heads, dim] as rows lengths[s], lengths[s] + 1, ... of their
+        sequences; the new rows' weights become 0 and their ids the tokens'."""
+        self._check(_lib.lib().maivs_cache_append(
+            self._h, d_keys, d_values, _cache_dtype(dtype), _size(n_tokens, "n_tokens"), _size(key_stride, "key_stride"),
+            _size(value_stride, "value_stride"), d_offsets, d_lengths, d_weights, d_ids, d_token_ids, stream))
+
+    def read(self, d_keys: int, d_values: int, n_tokens: int, d_offsets: int, d_lengths: int, dtype: str = "bf16",
+             stream: int = 0) -> None:
+        """The values of those rows, [n_tokens, n_heads, dim]."""
+        self._check(_lib.lib().maivs_cache_read(self._h, d_keys, d_values, _cache_dtype(dtype),
+                                                _size(n_tokens, "n_tokens"), d_offsets, d_lengths, stream))
+
+    def attend(self, d_queries: int, n_tokens: int, n_query_heads: int, d_offsets: int, d_lengths: int, d_out: int,
+               dtype: str = "bf16", query_stride: int = 0, causal: bool = True, scale: Optional[float] = None,
+               max_rows: int = 0, max_tokens: int = 0, d_lse: int = 0, d_weights_in: int = 0, d_weights_out: int = 0,
+               decay: float = 1.0, d_workspace: int = 0, workspace_bytes: int = 0, stream: int = 0) -> None:
+        """Attention of the tokens' queries over their sequences' rows; causal: up to the token's own
+        row of this step. scale: 1 / sqrt(dim) by default. Accumulates the rows' attention weights
+        when the weight tables are given."""
+        self._check(_lib.lib().maivs_cache_attend(
+            self._h, d_queries, _cache_dtype(dtype), _size(n_tokens, "n_tokens"), _size(query_stride, "query_stride"),
+            _size(n_query_heads, "n_query_heads"), d_offsets, d_lengths, int(bool(causal)), self._scale(scale),
+            _size(max_rows, "max_rows"), _size(max_tokens, "max_tokens"), d_out, d_lse, d_weights_in, d_weights_out,
+            float(decay), d_workspace, _size(workspace_bytes, "workspace_bytes"), stream))
+
+    def attend_workspace(self, n_tokens: int, n_query_heads: int, max_rows: int = 0, max_tokens: int = 0,
+                         weights: bool = False) -> int:
+        """Bytes of workspace that such an attend call needs."""
+        n = C.c_size_t(0)
+        self._check(_lib.lib().maivs_cache_attend_workspace(
+            self._h, _size(n_tokens, "n_tokens"), _size(n_query_heads, "n_query_heads"), _size(max_rows, "max_rows"),
+            _size(max_tokens, "max_tokens"), int(bool(weights)), C.byref(n)))
+        return n.value
+
+    def attend_found(self, d_queries: int, n_tokens: int, n_query_heads: int, d_offsets: int, d_lengths: int,
+                     d_rows: int, k: int, d_out: int, dtype: str = "bf16", query_stride: int = 0, causal: bool = False,
+                     scale: Optional[float] = None, d_lse: int = 0, d_weights: int = 0, d_workspace: int = 0,
+                     workspace_bytes: int = 0, stream: int = 0) -> None:
+        """Attention over the rows [n_tokens, k] that a search named, as search_batch_device writes
+        its ids (padded with 2^64 - 1)."""
+        self._check(_lib.lib().maivs_cache_attend_found(
+            self._h, d_queries, _cache_dtype(dtype), _size(n_tokens, "n_tokens"), _size(query_stride, "query_stride"),
+            _size(n_query_heads, "n_query_heads"), d_offsets, d_lengths, d_rows, _size(k, "k"), int(bool(causal)),
+            self._scale(scale), d_out, d_lse, d_weights, d_workspace, _size(workspace_bytes, "workspace_bytes"),
+            stream))
+
+    def attend_found_workspace(self, n_tokens: int, n_query_heads: int, k: int, weights: bool = True) -> int:
+        """Bytes of workspace that such an attend_found call needs."""
+        n = C.c_size_t(0)
+        self._check(_lib.lib().maivs_cache_attend_found_workspace(
+            self._h, _size(n_tokens, "n_tokens"), _size(n_query_heads, "n_query_heads"), _size(k, "k"),
+            int(bool(weights)), C.byref(n)))
+        return n.value
+
+    def evict(self, d_lengths: int, keep: int, d_weights_in: int, d_weights_out: int, d_new_lengths: int,
+              d_ids_in: int = 0, d_ids_out: int = 0, d_protect_from: int = 0, d_evicted: int = 0,
+              d_workspace: int = 0, workspace_bytes: int = 0, stream: int = 0) -> None:
+        """Keep every sequence's `keep` heaviest rows (and rows with ids from protect_from[s] on before
+        all others) and close the gaps; the ids that left go to `evicted`."""
+        self._check(_lib.lib().maivs_cache_evict(
+            self._h, d_lengths, _size(keep, "keep"), d_weights_in, d_weights_out, d_new_lengths, d_ids_in, d_ids_out,
+            d_protect_from, d_evicted, d_workspace, _size(workspace_bytes, "workspace_bytes"), stream))
+
+    def evict_workspace(self) -> int:
+        """Bytes of workspace that evict needs."""
+        n = C.c_size_t(0)
+        self._check(_lib.lib().maivs_cache_evict_workspace(self._h, C.byref(n)))
+        return n.value
+
+    def flags(self, stream: int = 0) -> int:
+        """Flags set since the last call (1: append past the capacity, 2: a sequence longer than
+        max_rows, 4: offsets out of order); synchronises `stream`."""
+        f = C.c_uint32(0)
+        self._check(_lib.lib().maivs_cache_flags(self._h, stream, C.byref(f)))
+        return int(f.value)
+
+    _STATS = ("n_seqs", "capacity", "n_heads", "dim", "device", "device_bytes", "row_bytes")
+
+    def stats(self) -> dict:
+        out = {}
+        v = C.c_double(0.0)
+        for name in self._STATS:
+            self._check(_lib.lib().maivs_cache_stat(self._h, name.encode(), C.byref(v)))
+            out[name] = float(v.value)
+        return out
+
+    def _scale(self, scale: Optional[float]) -> float:
+        return self._dim ** -0.5 if scale is None else float(scale)
 
 
 def nccl_unique_id() -> bytes:

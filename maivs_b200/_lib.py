@@ -106,6 +106,28 @@ _SIGS = {
                                                 C.POINTER(C.c_uint64), C.c_size_t, C.POINTER(C.c_size_t)]),
     "maivs_concurrent_array": (C.c_int, [C.c_void_p, C.c_longlong, C.c_char_p, C.POINTER(C.c_void_p),
                                          C.POINTER(C.c_size_t), C.POINTER(C.c_size_t)]),
+    "maivs_cache_new": (C.c_int, [C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t, C.c_int, C.POINTER(C.c_void_p)]),
+    "maivs_cache_free": (None, [C.c_void_p]),
+    "maivs_cache_last_error": (C.c_char_p, [C.c_void_p]),
+    "maivs_cache_stat": (C.c_int, [C.c_void_p, C.c_char_p, C.POINTER(C.c_double)]),
+    "maivs_cache_append": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_size_t, C.c_size_t, C.c_size_t,
+                                     C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "maivs_cache_read": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_size_t, C.c_void_p, C.c_void_p,
+                                   C.c_void_p]),
+    "maivs_cache_attend": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_size_t, C.c_size_t, C.c_size_t, C.c_void_p,
+                                     C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_size_t, C.c_void_p, C.c_void_p,
+                                     C.c_void_p, C.c_void_p, C.c_float, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "maivs_cache_attend_workspace": (C.c_int, [C.c_void_p, C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t, C.c_int,
+                                               C.POINTER(C.c_size_t)]),
+    "maivs_cache_attend_found": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_size_t, C.c_size_t, C.c_size_t,
+                                           C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_int, C.c_float,
+                                           C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "maivs_cache_attend_found_workspace": (C.c_int, [C.c_void_p, C.c_size_t, C.c_size_t, C.c_size_t, C.c_int,
+                                                     C.POINTER(C.c_size_t)]),
+    "maivs_cache_evict": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                    C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "maivs_cache_evict_workspace": (C.c_int, [C.c_void_p, C.POINTER(C.c_size_t)]),
+    "maivs_cache_flags": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(C.c_uint32)]),
     "maivs_profile": (C.c_int, [C.c_int]),
     "maivs_profile_read": (C.c_int, [C.c_int, C.POINTER(C.c_char_p), C.POINTER(C.c_double), C.c_size_t,
                                      C.POINTER(C.c_size_t)]),

@@ -33,6 +33,7 @@ SOURCES = [
     ("host/persist.cpp", "cxx"),
     ("capi.cpp", "cxx"),
     ("concurrent.cpp", "cxx"),
+    ("cache.cpp", "cxx"),
     ("cuda/clock.cu", "nvcc"),
     ("cuda/k_route.cu", "nvcc"),
     ("cuda/k_cellmajor.cu", "nvcc"),
@@ -44,9 +45,11 @@ SOURCES = [
     ("cuda/shard.cu", "nvcc"),
     ("cuda/build.cu", "nvcc"),
     ("cuda/k_merge.cu", "nvcc"),
+    ("cuda/k_cache.cu", "nvcc"),
+    ("cuda/k_cache_attend.cu", "nvcc"),
 ]
 HEADERS = ["handle.h", "host/hostmath.h", "host/index_host.h", "cuda/common.cuh", "cuda/kernels.cuh", "cuda/dev_common.cuh",
-           "cuda/umma.cuh", "cuda/engine.h"]
+           "cuda/umma.cuh", "cuda/engine.h", "cuda/cache.h", "cuda/cache_dev.cuh"]
 
 
 def _cmd(src: str, kind: str, obj: str) -> list[str]:

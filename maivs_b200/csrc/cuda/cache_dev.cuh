@@ -1,0 +1,78 @@
+// Device helpers of the attention cache's kernels: the row format and the types' conversions.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+namespace maivs {
+namespace dev {
+
+// Places of a row's code words (see cache.h).
+__host__ __device__ __forceinline__ int key_word(int G, int j, int t) {
+    return G == 1 ? t * 2 + j : (j >> 2) * 16 + t * 4 + (j & 3);
+}
+__host__ __device__ __forceinline__ int value_word(int G, int g, int e) {
+    return G == 1 ? e : (g >> 1) * 16 + e * 2 + (g & 1);
+}
+
+__device__ __forceinline__ float par_step(uint32_t p) { return __uint_as_float(p << 16); }
+__device__ __forceinline__ float par_low(uint32_t p) { return __uint_as_float(p & 0xFFFF0000u); }
+
+__device__ __forceinline__ float bf16_round(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
+
+// 16-bit patterns to and from f32
+template <typename T>
+__device__ __forceinline__ float to_f32(uint32_t bits);
+template <>
+__device__ __forceinline__ float to_f32<__half>(uint32_t bits) {
+    return __half2float(__ushort_as_half((unsigned short)bits));
+}
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(uint32_t bits) {
+    return __uint_as_float(bits << 16);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t from_f32(float x);
+template <>
+__device__ __forceinline__ uint32_t from_f32<__half>(float x) {
+    return __half_as_ushort(__float2half_rn(x));
+}
+template <>
+__device__ __forceinline__ uint32_t from_f32<__nv_bfloat16>(float x) {
+    return __bfloat16_as_ushort(__float2bfloat16_rn(x));
+}
+
+// The sequence of packed token `tok`: offsets[s] <= tok < offsets[s + 1], or -1 for a token before
+// the first or behind the last sequence. Called by an aligned group of 8 lanes (lane8, mask), which
+// count the starts at or below tok together: one round of loads per 8 sequences, none dependent;
+// above 512 sequences every lane bisects instead.
+__device__ __forceinline__ int find_sequence(const int32_t* __restrict__ off, int n_seqs, int tok, int lane8,
+                                             unsigned mask) {
+    int s;
+    if (n_seqs <= 512) {
+        int n = 0;
+        for (int i = lane8; i <= n_seqs; i += 8) n += __ldg(off + i) <= tok;
+        n += __shfl_xor_sync(mask, n, 1);
+        n += __shfl_xor_sync(mask, n, 2);
+        n += __shfl_xor_sync(mask, n, 4);
+        s = n - 1;
+    } else {
+        int lo = 0, hi = n_seqs + 1;  // the first start above tok
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (__ldg(off + mid) <= tok)
+                lo = mid + 1;
+            else
+                hi = mid;
+        }
+        s = lo - 1;
+    }
+    if (s < 0 || s >= n_seqs) return -1;
+    // offsets that do not ascend map a token nowhere rather than to a wrong row
+    return __ldg(off + s) <= tok && tok < __ldg(off + s + 1) ? s : -1;
+}
+
+}  // namespace dev
+}  // namespace maivs

@@ -21,7 +21,7 @@ std::atomic<unsigned long long> g_launches{0};
 
 bool tick_begin(int id, cudaStream_t st) {
     g_launches.fetch_add(1, std::memory_order_relaxed);
-    const bool timed = t_clock && t_clock->wants(id);
+    const bool timed = t_clock && id < kNumKernels && t_clock->wants(id);
     if (timed) t_clock->begin(id, st);
     return timed;
 }
@@ -44,13 +44,15 @@ cudaError_t take_launch_error(int* kernel) {
 }
 
 const char* kernel_name(int id) {
-    static const char* names[kNumKernels] = {"k_encode", "k_route_flat", "k_route_tree", "k_rescore_select",
+    static const char* names[kNumNamed] = {"k_encode", "k_route_flat", "k_route_tree", "k_rescore_select",
                                              "k_seed",   "k_inv_count",  "k_inv_scan",   "k_inv_scatter",
                                              "k_scan_cm", "k_final_cm",  "k_pq_prep",    "k_pq_scan",
                                              "k_pq_fold", "k_rerank",    "k_topk",       "k_rerank_items",
                                              "k_seed_finish", "k_local_list", "k_merge_topk", "k_scan_mma",
-                                             "k_seed_scan", "nccl_all_gather", "k_segment_merge", "k_rescore_dots", "k_probe_select"};
-    return id >= 0 && id < kNumKernels ? names[id] : "?";
+                                             "k_seed_scan", "nccl_all_gather", "k_segment_merge", "k_rescore_dots", "k_probe_select",
+                                             "k_cache_append", "k_cache_read", "k_cache_attend", "k_cache_join",
+                                             "k_cache_weights", "k_cache_select", "k_cache_move"};
+    return id >= 0 && id < kNumNamed ? names[id] : "?";
 }
 
 KernelClock::~KernelClock() {

@@ -1,0 +1,843 @@
+// Softmax attention over the attention cache's 4-bit rows.
+//
+// For a query column (a token's query head) with visible rows r and z_r = scale * q . k_r:
+// out = sum_r p_r v_r, p = softmax(z), in one pass over the rows with a running maximum and sum.
+//
+// The rows are streamed from HBM into registers, and stay there: a warp takes tiles of 16 rows, and a
+// 4-bit code becomes an f16 operand of mma.m16n8k16 by one mask. A nibble in the low four bits of a
+// half is the subnormal c * 2^-24, in the next four c * 2^-20; both are exact, the tensor core takes
+// subnormals as they are, and the powers of two are taken out of the f32 accumulators (or folded
+// into the query operand) afterwards. No operand goes through shared memory, so the tile loop has no
+// barrier, and two of the format's properties come for free: a group's step and low multiply sums
+// of its codes, not the codes.
+//
+//   keys    S^T = Q K^T: A = queries (M: columns, scaled by a power of two to f16's upper range),
+//           B = codes (N: 8 rows). Per group g: s += step_g * acc_g + low_g * sum(q in g).
+//   values  O^T = V^T P^T: A = codes (M: 16 dimensions of one group, K: 16 rows), B = p * step_g
+//           rounded to f16 (N: columns); the low terms p * low_g are summed in f32.
+//
+// S^T's accumulator layout (row = column of the query, columns = two rows of the cache) is the B
+// operand's layout of O^T, so p never leaves its thread.
+//
+// Rounding: codes are exact, 16-bit queries are exact in f16 down to 2^-24 of their row's largest
+// element, p * step is rounded to f16 (2^-12 relative, below the output's own rounding). f32 calls
+// split query and p * step into two f16 halves each (22 bits).
+#include <algorithm>
+
+#include "cache.h"
+#include "cache_dev.cuh"
+#include "common.cuh"
+#include "dev_common.cuh"
+
+namespace maivs {
+namespace dev {
+
+namespace {
+
+constexpr int kAttWarps = 4;
+constexpr int kAttBS = kAttWarps * 32;
+constexpr int kTile = 16;
+constexpr float kNoMax = -3.0e38f;
+constexpr float kLog2e = 1.4426950408889634f;
+// p * step goes into f16 scaled so that the group's largest step becomes 2^12: an old maximum may
+// be exceeded by 2^kLag before the accumulators are rescaled, and 2^12 * 2^kLag is below 65504.
+constexpr float kLag = 3.0f;
+constexpr float kPScale = 4096.0f;
+
+struct AttendPlan {
+    int nc;         // columns per tile
+    int col_tiles;  // of one sequence and head (or token and head)
+    int n_split;    // blocks that share one sequence's rows
+    size_t off_o, off_lse, off_logit, bytes;
+    int logit_rows;
+};
+
+struct AttendKernel {
+    AttendArgs a;
+    float2* part_ml;  // [split][token][q_head]: running maximum (log2) and sum
+    float* part_o;    // [split][token][q_head][dim]
+    float* lse2;      // [token][q_head], log2; null without weights
+    float* logits;    // [token][q_head][logit_rows], log2; null without weights
+    int logit_rows;
+    int n_split, col_tiles;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Codes as f16 operands: of each half of w, nibble kOdd (of the low two). 16-bit calls take them as
+// the subnormals above. f32 calls take c - 8 (16 (c - 8) for the odd nibble), by the exponent of 1024
+// and one exact subtraction: centred codes keep the sums small, so that the tensor core's truncated
+// additions and the cancellation against the low terms cost no f32 digits (measured on long rows:
+// error 2e-5 of the output's size with codes from 0).
+template <bool F32, bool kOdd>
+__device__ __forceinline__ uint32_t operand(uint32_t w) {
+    const uint32_t mask = kOdd ? 0x00F000F0u : 0x000F000Fu;
+    if (!F32) return w & mask;
+    const uint32_t up = (w & mask) | 0x64006400u, mid = kOdd ? 0x64806480u : 0x64086408u;
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&up), *reinterpret_cast<const __half2*>(&mid));
+    return *reinterpret_cast<const uint32_t*>(&d);
+}
+// The low of a group for codes as operand() gives them.
+template <bool F32>
+__device__ __forceinline__ float low_of(uint32_t par) {
+    return F32 ? __fmaf_rn(8.0f, par_step(par), par_low(par)) : par_low(par);
+}
+
+__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// The part of x that its f16 rounding (in packed pair p, half i) leaves over.
+__device__ __forceinline__ float left_over(float x, uint32_t p, int i) {
+    return __fsub_rn(x, to_f32<__half>(i ? p >> 16 : p & 0xFFFFu));
+}
+
+template <int N>
+__device__ __forceinline__ void load_words(const uint32_t* __restrict__ p, uint32_t (&w)[N]) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
+            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+        }
+    } else if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            const uint2 v = __ldg(reinterpret_cast<const uint2*>(p) + i);
+            w[2 * i] = v.x, w[2 * i + 1] = v.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = __ldg(p + i);
+    }
+}
+
+__device__ __forceinline__ float read_q(const void* q, int type, size_t i) {
+    if (type == kF32) return __ldg(static_cast<const float*>(q) + i);
+    const uint32_t b = __ldg(static_cast<const unsigned short*>(q) + i);
+    return type == kF16 ? to_f32<__half>(b) : to_f32<__nv_bfloat16>(b);
+}
+
+__device__ __forceinline__ void write_out(void* out, int type, size_t i, float x) {
+    if (type == kF32)
+        static_cast<float*>(out)[i] = x;
+    else
+        static_cast<unsigned short*>(out)[i] =
+            (unsigned short)(type == kF16 ? from_f32<__half>(x) : from_f32<__nv_bfloat16>(x));
+}
+
+// Rows of a sequence that its last token sees, and the number of its tokens.
+struct Span {
+    int first, count, len;
+};
+__device__ __forceinline__ Span span_of(const CacheView& c, const AttendArgs& a, int s) {
+    Span p;
+    const int lo = __ldg(a.tok.offsets + s), hi = __ldg(a.tok.offsets + s + 1);
+    const bool good = lo >= 0 && hi >= lo && hi <= a.tok.n_tokens;
+    p.first = lo;
+    p.count = good ? hi - lo : 0;
+    p.len = min(max(__ldg(a.tok.lengths + s), 0), c.capacity);
+    return p;
+}
+__device__ __forceinline__ int visible(const CacheView& c, const AttendArgs& a, int len, int i) {
+    return min(min(len + (a.causal ? i + 1 : 0), c.capacity), a.max_rows);
+}
+// Rows per split: an equal share, in whole passes of the block's warps.
+__device__ __forceinline__ int share_of(int rows, int n_split) {
+    const int step = kAttWarps * kTile;
+    return max((rows + n_split * step - 1) / (n_split * step), 1) * step;
+}
+
+template <int G, int NC, bool F32, bool FOUND>
+struct Shape {
+    static constexpr bool kTwo = NC == 16 || F32;    // both halves of the query operand's M are used
+    static constexpr int kQ = kTwo ? 8 : 4;          // query registers per 32 dimensions
+    static constexpr int kCols = NC / 8;             // columns per thread
+    static constexpr float kUnit = F32 ? 1.0f : 16777216.0f;  // 1 / what a code of 1 is as an operand
+    static constexpr bool kQShared = G * kQ > 16;    // wide queries wait in shared memory
+    static_assert(!(kQShared && NC == 16), "sixteen columns keep their queries in registers");
+};
+
+template <int G, int NC, bool F32, bool FOUND>
+__global__ void __launch_bounds__(kAttBS) k_cache_attend(CacheView c, AttendKernel kk) {
+    using S = Shape<G, NC, F32, FOUND>;
+    constexpr int kCols = S::kCols, kQ = S::kQ;
+    const AttendArgs& a = kk.a;
+    __shared__ float s_o[NC][G * kCacheGroup + 4];
+    __shared__ float s_m[kAttWarps][NC], s_l[kAttWarps][NC], s_low[kAttWarps][NC][G];
+    __shared__ uint4 s_q[S::kQShared ? 2 * G * (kQ / 4) : 1][32];
+
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gid = lane >> 2, t = lane & 3;
+    unsigned b = blockIdx.x;
+    const int ct0 = b % kk.col_tiles;
+    b /= kk.col_tiles;
+    const int sp = b % kk.n_split;
+    b /= kk.n_split;
+    const int h = b % c.heads;
+    const int item = b / c.heads;  // sequence, or token of a found list
+
+    Span sn;
+    int s, cols, rows_all;
+    if (FOUND) {
+        const unsigned m8 = 0xFFu << (lane / 8 * 8);
+        s = find_sequence(a.tok.offsets, c.n_seqs, item, lane & 7, m8);
+        if (s < 0) return;
+        sn = span_of(c, a, s);
+        cols = a.group;
+        rows_all = a.k;
+    } else {
+        s = item;
+        sn = span_of(c, a, s);
+        cols = sn.count * a.group;
+        rows_all = sn.count ? visible(c, a, sn.len, sn.count - 1) : 0;
+        if (threadIdx.x == 0 && h == 0 && sp == 0 && ct0 == 0) {
+            const int lo = __ldg(a.tok.offsets + s), hi = __ldg(a.tok.offsets + s + 1);
+            if (lo < 0 || hi < lo || hi > a.tok.n_tokens) atomicOr(c.flags, kCacheOffsets);
+            if (sn.count && min(sn.len + (a.causal ? sn.count : 0), c.capacity) > a.max_rows)
+                atomicOr(c.flags, kCacheTooLong);
+        }
+    }
+    const int share = share_of(rows_all, kk.n_split);
+    const int start = sp * share;
+    if (start >= rows_all && sp > 0) return;
+
+    const size_t head_row = ((size_t)s * c.heads + h) * c.rows;
+    const uint32_t* kc = c.kc + head_row * 8 * G;
+    const uint32_t* vc = c.vc + head_row * 8 * G;
+    const uint32_t* kp = c.kp + head_row * G;
+    const uint32_t* vp = c.vp + head_row * G;
+
+    for (int ct = ct0; ct * NC < cols; ct += kk.col_tiles) {
+        // ---- the columns of this thread (of the S^T layout: gid, and gid + 8) ----
+        int lim[kCols], tok[kCols], head[kCols];
+        float fac[kCols], qsum[kCols][G];
+        uint32_t q[S::kQShared ? 1 : 2 * G][kQ];
+        uint32_t qtmp[kQ];
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) {
+            const int col = ct * NC + gid + 8 * j;
+            const int i = col / a.group;
+            const bool in = col < cols;
+            tok[j] = FOUND ? item : sn.first + i;
+            head[j] = h * a.group + (col - i * a.group);
+            // a found list: entries must lie below the rows the token sees; rows of the list: k
+            lim[j] = !in ? 0 : FOUND ? a.k : visible(c, a, sn.len, i);
+            const size_t qi = (size_t)tok[j] * a.q_stride + (size_t)head[j] * c.dim;
+            float top = 0.0f;
+            bool bad = false;
+            for (int w = 0; w < 2 * G; ++w)
+                for (int n = 0; n < 8; ++n) {
+                    const int d = 32 * w + 8 * t + n;
+                    const float x = in && d < c.dim ? read_q(a.q, a.type, qi + d) : 0.0f;
+                    top = fmaxf(top, fabsf(x));
+                    bad |= !(fabsf(x) < INFINITY);
+                }
+            top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+            bad = (__ballot_sync(~0u, bad) >> (lane & ~3)) & 15u;
+            // 2^e brings the largest element to [2^14, 2^15)
+            const int e = top > 0.0f ? min(141 - (int)(__float_as_uint(top) >> 23), 126) : 0;
+            const float up = __uint_as_float((uint32_t)max(e + 127, 1) << 23);
+            // s = (sum of step * acc + low * qsum) * fac, with acc and qsum in units of 2^e / kUnit
+            fac[j] = bad ? __uint_as_float(0x7FC00000u)
+                         : __fmul_rn(__fmul_rn(__fdiv_rn(S::kUnit, up), a.scale), kLog2e);
+#pragma unroll
+            for (int g = 0; g < G; ++g) qsum[j][g] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 2 * G; ++w) {
+                float x[8];
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    const int d = 32 * w + 8 * t + n;
+                    x[n] = in && d < c.dim && !bad ? __fmul_rn(read_q(a.q, a.type, qi + d), up) : 0.0f;
+                    qsum[j][w / 2] = __fadd_rn(qsum[j][w / 2], x[n]);
+                }
+                // step s of word w takes nibbles (2 s, 2 s + 4) and, 16 times as large, (2 s + 1, 2 s + 5)
+#pragma unroll
+                for (int st = 0; st < 2; ++st) {
+                    const float y0 = x[2 * st], y1 = x[2 * st + 4];
+                    const float z0 = 0.0625f * x[2 * st + 1], z1 = 0.0625f * x[2 * st + 5];
+                    const uint32_t r0 = pack_h2(y0, y1), r2 = pack_h2(z0, z1);
+                    uint32_t* dst = S::kQShared ? qtmp : q[S::kQShared ? 0 : w];
+                    if (F32) {
+                        dst[4 * st] = r0, dst[4 * st + 2] = r2;
+                        dst[4 * st + 1] = pack_h2(left_over(y0, r0, 0), left_over(y1, r0, 1));
+                        dst[4 * st + 3] = pack_h2(left_over(z0, r2, 0), left_over(z1, r2, 1));
+                    } else if (NC == 16) {
+                        dst[4 * st + j] = r0, dst[4 * st + 2 + j] = r2;
+                    } else {
+                        dst[2 * st] = r0, dst[2 * st + 1] = r2;
+                    }
+                }
+                if constexpr (S::kQShared) {
+                    if (warp == 0) {
+                        if (kQ == 8) {
+                            s_q[2 * w][lane] = make_uint4(qtmp[0], qtmp[1], qtmp[2], qtmp[3]);
+                            s_q[2 * w + 1][lane] = make_uint4(qtmp[4], qtmp[5], qtmp[6], qtmp[7]);
+                        } else {
+                            s_q[w][lane] = make_uint4(qtmp[0], qtmp[1], qtmp[2], qtmp[3]);
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                qsum[j][g] = __fadd_rn(qsum[j][g], __shfl_xor_sync(~0u, qsum[j][g], 1));
+                qsum[j][g] = __fadd_rn(qsum[j][g], __shfl_xor_sync(~0u, qsum[j][g], 2));
+                qsum[j][g] = __fmul_rn(qsum[j][g], 1.0f / S::kUnit);
+            }
+        }
+        if constexpr (S::kQShared) __syncthreads();
+
+        const int col_last = min(ct * NC + NC, cols) - 1;
+        const int lim_first = FOUND ? 0 : visible(c, a, sn.len, ct * NC / a.group);
+        const int lim_last = FOUND ? a.k : visible(c, a, sn.len, col_last / a.group);
+        const int row_limit = FOUND ? visible(c, a, sn.len, item - sn.first) : 0;
+        const int end = min(min(start + share, rows_all), lim_last);
+
+        float m[kCols], l[kCols], low[kCols][G], norm[G];
+        float o[G][4][kCols][4];
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) {
+            m[j] = kNoMax;
+            l[j] = 0.0f;
+#pragma unroll
+            for (int g = 0; g < G; ++g) low[j][g] = 0.0f;
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            norm[g] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < kCols; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[g][i][j][r] = 0.0f;
+        }
+
+        for (int r0 = start + warp * kTile; r0 < end; r0 += kAttWarps * kTile) {
+            // ---- rows of the tile: gid and gid + 8 as keys, 2t, 2t + 1, 2t + 8, 2t + 9 as values ----
+            size_t krow[2], vrow[4];
+            bool ok[4];
+            if constexpr (FOUND) {
+                const uint64_t* list = a.rows + (size_t)item * a.k;
+                auto entry = [&](int e, bool& good) -> size_t {
+                    const uint64_t id = e < a.k ? __ldg(list + e) : ~0ull;
+                    good = id < (uint64_t)row_limit;
+                    return good ? (size_t)id : 0;
+                };
+                bool dummy;
+                krow[0] = entry(r0 + gid, dummy);
+                krow[1] = entry(r0 + gid + 8, dummy);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) vrow[i] = entry(r0 + 2 * t + (i & 1) + 8 * (i >> 1), ok[i]);
+            } else {
+                krow[0] = r0 + gid;
+                krow[1] = r0 + gid + 8;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) vrow[i] = r0 + 2 * t + (i & 1) + 8 * (i >> 1);
+            }
+            const bool edge = FOUND || r0 + kTile > lim_first;
+
+            uint32_t kpw[4][G], vpw[4][G];
+            if constexpr (FOUND) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    load_words<G>(kp + vrow[i] * G, kpw[i]);
+                    load_words<G>(vp + vrow[i] * G, vpw[i]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    load_words<2 * G>(kp + vrow[2 * i] * G, *reinterpret_cast<uint32_t(*)[2 * G]>(&kpw[2 * i]));
+                    load_words<2 * G>(vp + vrow[2 * i] * G, *reinterpret_cast<uint32_t(*)[2 * G]>(&vpw[2 * i]));
+                }
+            }
+
+            // ---- scores: sc[j][i] of column j and value row i ----
+            float sc[kCols][4];
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt) {
+                uint32_t w[2 * G];
+                const uint32_t* kr = kc + krow[nt] * 8 * G;
+                if constexpr (G == 1) {
+                    load_words<2>(kr + t * 2, w);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < G / 2; ++i)
+                        load_words<4>(kr + i * 16 + t * 4, *reinterpret_cast<uint32_t(*)[4]>(&w[4 * i]));
+                }
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int x = 2 * g; x < 2 * g + 2; ++x) {
+                        uint32_t qq[kQ];
+                        if constexpr (S::kQShared) {
+#pragma unroll
+                            for (int i = 0; i < kQ / 4; ++i) {
+                                const uint4 v = s_q[(kQ / 4) * x + i][lane];
+                                qq[4 * i] = v.x, qq[4 * i + 1] = v.y, qq[4 * i + 2] = v.z, qq[4 * i + 3] = v.w;
+                            }
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < kQ; ++i) qq[i] = q[x][i];
+                        }
+                        const uint32_t w0 = w[x], w1 = w0 >> 8;
+                        if constexpr (S::kTwo) {
+                            mma(acc, qq[0], qq[1], qq[2], qq[3], operand<F32, false>(w0), operand<F32, true>(w0));
+                            mma(acc, qq[4], qq[5], qq[6], qq[7], operand<F32, false>(w1), operand<F32, true>(w1));
+                        } else {
+                            mma(acc, qq[0], 0u, qq[1], 0u, operand<F32, false>(w0), operand<F32, true>(w0));
+                            mma(acc, qq[2], 0u, qq[3], 0u, operand<F32, false>(w1), operand<F32, true>(w1));
+                        }
+                    }
+                    const float st0 = par_step(kpw[2 * nt][g]), st1 = par_step(kpw[2 * nt + 1][g]);
+                    const float lo0 = low_of<F32>(kpw[2 * nt][g]), lo1 = low_of<F32>(kpw[2 * nt + 1][g]);
+                    if (F32) {  // the query's low halves
+                        acc[0] = __fadd_rn(acc[0], acc[2]);
+                        acc[1] = __fadd_rn(acc[1], acc[3]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < kCols; ++j) {
+                        sum[2 * j] = __fmaf_rn(st0, acc[2 * j], __fmaf_rn(lo0, qsum[j][g], sum[2 * j]));
+                        sum[2 * j + 1] = __fmaf_rn(st1, acc[2 * j + 1], __fmaf_rn(lo1, qsum[j][g], sum[2 * j + 1]));
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < kCols; ++j) {
+                    sc[j][2 * nt] = __fmul_rn(sum[2 * j], fac[j]);
+                    sc[j][2 * nt + 1] = __fmul_rn(sum[2 * j + 1], fac[j]);
+                }
+            }
+            if (edge) {
+#pragma unroll
+                for (int j = 0; j < kCols; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = r0 + 2 * t + (i & 1) + 8 * (i >> 1);
+                        if (r >= lim[j] || (FOUND && !ok[i])) sc[j][i] = -INFINITY;
+                    }
+            }
+            if (kk.logits) {
+#pragma unroll
+                for (int j = 0; j < kCols; ++j) {
+                    if (lim[j] <= 0) continue;
+                    float* lg = kk.logits + ((size_t)tok[j] * a.q_heads + head[j]) * kk.logit_rows + r0 + 2 * t;
+                    *reinterpret_cast<float2*>(lg) = make_float2(sc[j][0], sc[j][1]);
+                    *reinterpret_cast<float2*>(lg + 8) = make_float2(sc[j][2], sc[j][3]);
+                }
+            }
+
+            // ---- running maximum and the groups' power of two: rescaled only where they grow ----
+            float top[kCols], big[G];
+            bool grow = false;
+#pragma unroll
+            for (int j = 0; j < kCols; ++j) {
+                top[j] = fmaxf(fmaxf(sc[j][0], sc[j][1]), fmaxf(sc[j][2], sc[j][3]));
+                grow |= top[j] > m[j] + kLag;
+            }
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                big[g] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float x = par_step(vpw[i][g]);
+                    // rows that no column of the tile sees may hold anything
+                    const bool in = FOUND ? ok[i] : !edge || (int)vrow[i] < lim_last;
+                    if (in && x < INFINITY) big[g] = fmaxf(big[g], x);
+                }
+                grow |= big[g] > norm[g];
+            }
+            if (__any_sync(~0u, grow)) {
+                float f[kCols];
+#pragma unroll
+                for (int j = 0; j < kCols; ++j) {
+                    float x = top[j];
+                    x = fmaxf(x, __shfl_xor_sync(~0u, x, 1));
+                    x = fmaxf(x, __shfl_xor_sync(~0u, x, 2));
+                    const float mn = fmaxf(m[j], x);
+                    f[j] = ex2(m[j] - mn);
+                    m[j] = mn;
+                    l[j] = __fmul_rn(l[j], f[j]);
+#pragma unroll
+                    for (int g = 0; g < G; ++g) low[j][g] = __fmul_rn(low[j][g], f[j]);
+                }
+                // the O^T layout holds columns 2t and 2t + 1
+                float fo[kCols][2];
+#pragma unroll
+                for (int j = 0; j < kCols; ++j) {
+                    fo[j][0] = __shfl_sync(~0u, f[j], 8 * t);
+                    fo[j][1] = __shfl_sync(~0u, f[j], 8 * t + 4);
+                }
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    float x = big[g];
+                    x = fmaxf(x, __shfl_xor_sync(~0u, x, 1));
+                    x = fmaxf(x, __shfl_xor_sync(~0u, x, 2));
+                    float ratio = 1.0f;
+                    if (x > norm[g]) {
+                        // a power of two at or above the step, at least 2^-100
+                        const float n = fmaxf(2.0f * __uint_as_float(__float_as_uint(x) & 0x7F800000u), 7.8886e-31f);
+                        ratio = __fdiv_rn(norm[g], n);
+                        norm[g] = n;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int j = 0; j < kCols; ++j)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                o[g][i][j][r] = __fmul_rn(o[g][i][j][r], __fmul_rn(fo[j][r & 1], ratio));
+                }
+            }
+
+            float p[kCols][4];
+#pragma unroll
+            for (int j = 0; j < kCols; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    p[j][i] = ex2(__fsub_rn(sc[j][i], m[j]));
+                    l[j] = __fadd_rn(l[j], p[j][i]);
+                }
+
+            // ---- values ----
+            uint32_t vw[4][G];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t* vr = vc + vrow[i] * 8 * G;
+                if constexpr (G == 1) {
+                    load_words<1>(vr + gid, vw[i]);
+                } else {
+#pragma unroll
+                    for (int x = 0; x < G / 2; ++x)
+                        load_words<2>(vr + x * 16 + gid * 2, *reinterpret_cast<uint32_t(*)[2]>(&vw[i][2 * x]));
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const float inv = norm[g] > 0.0f ? __fdiv_rn(kPScale, norm[g]) : 0.0f;
+                float ps[kCols][4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float st = __fmul_rn(par_step(vpw[i][g]), inv), lo = low_of<F32>(vpw[i][g]);
+#pragma unroll
+                    for (int j = 0; j < kCols; ++j) {
+                        ps[j][i] = __fmul_rn(p[j][i], st);
+                        float add = __fmul_rn(p[j][i], lo);
+                        if (edge) {
+                            // a row the column does not see adds nothing, whatever it holds
+                            const bool seen = FOUND ? ok[i] : (int)vrow[i] < lim[j];
+                            ps[j][i] = seen ? ps[j][i] : 0.0f;
+                            add = seen ? add : 0.0f;
+                        }
+                        low[j][g] = __fadd_rn(low[j][g], add);
+                    }
+                }
+                const uint32_t u0 = __byte_perm(vw[0][g], vw[1][g], 0x5410), h0 = __byte_perm(vw[0][g], vw[1][g], 0x7632);
+                const uint32_t u8 = __byte_perm(vw[2][g], vw[3][g], 0x5410), h8 = __byte_perm(vw[2][g], vw[3][g], 0x7632);
+#pragma unroll
+                for (int j = 0; j < kCols; ++j) {
+                    const uint32_t b0 = pack_h2(ps[j][0], ps[j][1]), b1 = pack_h2(ps[j][2], ps[j][3]);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int sh = 8 * i;
+                        mma(o[g][2 * i][j], operand<F32, false>(u0 >> sh), operand<F32, false>(h0 >> sh),
+                            operand<F32, false>(u8 >> sh), operand<F32, false>(h8 >> sh), b0, b1);
+                        mma(o[g][2 * i + 1][j], operand<F32, true>(u0 >> sh), operand<F32, true>(h0 >> sh),
+                            operand<F32, true>(u8 >> sh), operand<F32, true>(h8 >> sh), b0, b1);
+                    }
+                    if (F32) {
+                        const uint32_t c0 = pack_h2(left_over(ps[j][0], b0, 0), left_over(ps[j][1], b0, 1));
+                        const uint32_t c1 = pack_h2(left_over(ps[j][2], b1, 0), left_over(ps[j][3], b1, 1));
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const int sh = 8 * i;
+                            mma(o[g][2 * i][j], operand<F32, false>(u0 >> sh), operand<F32, false>(h0 >> sh),
+                                operand<F32, false>(u8 >> sh), operand<F32, false>(h8 >> sh), c0, c1);
+                            mma(o[g][2 * i + 1][j], operand<F32, true>(u0 >> sh), operand<F32, true>(h0 >> sh),
+                                operand<F32, true>(u8 >> sh), operand<F32, true>(h8 >> sh), c0, c1);
+                        }
+                    }
+                }
+            }
+        }
+
+        // ---- the block's warps joined ----
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) {
+            l[j] = __fadd_rn(l[j], __shfl_xor_sync(~0u, l[j], 1));
+            l[j] = __fadd_rn(l[j], __shfl_xor_sync(~0u, l[j], 2));
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                low[j][g] = __fadd_rn(low[j][g], __shfl_xor_sync(~0u, low[j][g], 1));
+                low[j][g] = __fadd_rn(low[j][g], __shfl_xor_sync(~0u, low[j][g], 2));
+                if (t == 0) s_low[warp][gid + 8 * j][g] = low[j][g];
+            }
+            if (t == 0) s_m[warp][gid + 8 * j] = m[j], s_l[warp][gid + 8 * j] = l[j];
+        }
+        __syncthreads();
+        for (int w = 0; w < kAttWarps; ++w) {
+            if (warp == w) {
+#pragma unroll
+                for (int j = 0; j < kCols; ++j)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int col = 8 * j + 2 * t + x;
+                        float mx = s_m[0][col];
+#pragma unroll
+                        for (int y = 1; y < kAttWarps; ++y) mx = fmaxf(mx, s_m[y][col]);
+                        const float f = ex2(s_m[w][col] - mx);
+#pragma unroll
+                        for (int g = 0; g < G; ++g) {
+                            const float lw = s_low[w][col][g];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                                for (int y = 0; y < 2; ++y) {
+                                    // undo the operand's unit (16 for odd i) and kPScale / norm
+                                    const float un = (i & 1 ? S::kUnit / 16.0f : S::kUnit) / kPScale;
+                                    const float v = __fmul_rn(
+                                        __fadd_rn(__fmul_rn(__fmul_rn(o[g][i][j][2 * y + x], un), norm[g]), lw), f);
+                                    float* at = &s_o[col][g * kCacheGroup + 16 * i + gid + 8 * y];
+                                    *at = w == 0 ? v : __fadd_rn(*at, v);
+                                }
+                        }
+                    }
+            }
+            __syncthreads();
+        }
+        // ---- out, or this split's part ----
+        for (int col = warp; col < NC; col += kAttWarps) {
+            const int cc = ct * NC + col;
+            if (cc >= cols) break;
+            const int i = cc / a.group;
+            const int tk = FOUND ? item : sn.first + i;
+            const int hd = h * a.group + (cc - i * a.group);
+            float mx = s_m[0][col], sum = 0.0f;
+#pragma unroll
+            for (int y = 1; y < kAttWarps; ++y) mx = fmaxf(mx, s_m[y][col]);
+#pragma unroll
+            for (int y = 0; y < kAttWarps; ++y) sum = __fmaf_rn(s_l[y][col], ex2(s_m[y][col] - mx), sum);
+            const size_t th = (size_t)tk * a.q_heads + hd;
+            if (kk.n_split == 1) {
+                // no visible row: 0 and -inf
+                const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+                for (int d = lane; d < c.dim; d += 32)
+                    write_out(a.out, a.type, th * c.dim + d, sum == 0.0f ? 0.0f : __fmul_rn(s_o[col][d], inv));
+                if (lane == 0) {
+                    const float l2 = sum == 0.0f ? -INFINITY : __fadd_rn(mx, log2f(sum));
+                    if (a.lse) a.lse[th] = __fmul_rn(l2, 0.69314718055994531f);
+                    if (kk.lse2) kk.lse2[th] = l2;
+                }
+            } else {
+                const size_t at = (size_t)sp * a.tok.n_tokens * a.q_heads + th;
+                for (int d = lane; d < c.dim; d += 32) kk.part_o[at * c.dim + d] = s_o[col][d];
+                if (lane == 0) kk.part_ml[at] = make_float2(mx, sum);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// Joins the splits of one token's query head; a warp each.
+template <bool FOUND>
+__global__ void __launch_bounds__(128) k_cache_join(CacheView c, AttendKernel kk) {
+    const AttendArgs& a = kk.a;
+    const int lane = threadIdx.x & 31;
+    const long long th = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int tk = (int)(th / a.q_heads);
+    if (tk >= a.tok.n_tokens) return;
+    const int s = find_sequence(a.tok.offsets, c.n_seqs, tk, lane & 7, 0xFFu << (lane / 8 * 8));
+    if (s < 0) return;
+    const Span sn = span_of(c, a, s);
+    if (sn.count == 0) return;
+    const int rows = FOUND ? a.k : visible(c, a, sn.len, sn.count - 1);
+    const int share = share_of(rows, kk.n_split);
+    const int used = max(1, (rows + share - 1) / share);
+    const size_t step = (size_t)a.tok.n_tokens * a.q_heads;
+    float m = kNoMax, l = 0.0f;
+    for (int i = lane; i < used; i += 32) m = fmaxf(m, kk.part_ml[i * step + th].x);
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    for (int i = lane; i < used; i += 32) {
+        const float2 v = kk.part_ml[i * step + th];
+        l = __fmaf_rn(v.y, ex2(v.x - m), l);
+    }
+    for (int o = 16; o; o >>= 1) l = __fadd_rn(l, __shfl_xor_sync(~0u, l, o));
+    const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+    for (int d = lane; d < c.dim; d += 32) {
+        float acc = 0.0f;
+        for (int i = 0; i < used; ++i)
+            acc = __fmaf_rn(kk.part_o[(i * step + th) * c.dim + d], ex2(kk.part_ml[i * step + th].x - m), acc);
+        write_out(a.out, a.type, (size_t)th * c.dim + d, l == 0.0f ? 0.0f : __fmul_rn(acc, inv));
+    }
+    if (lane == 0) {
+        const float l2 = l == 0.0f ? -INFINITY : __fadd_rn(m, log2f(l));
+        if (a.lse) a.lse[th] = __fmul_rn(l2, 0.69314718055994531f);
+        if (kk.lse2) kk.lse2[th] = l2;
+    }
+}
+
+// Accumulated weights of a sequence's rows: decay * old + every softmax weight of the call, token by
+// token and head by head, so that the sum does not depend on the launch.
+__global__ void __launch_bounds__(256) k_cache_weights(CacheView c, AttendKernel kk) {
+    const AttendArgs& a = kk.a;
+    const int s = blockIdx.y;
+    const Span sn = span_of(c, a, s);
+    const int rows = min(sn.len + (a.causal ? sn.count : 0), c.capacity);
+    for (int r = blockIdx.x * 256 + threadIdx.x; r < rows; r += gridDim.x * 256) {
+        float sum = 0.0f;
+        for (int i = 0; i < sn.count; ++i) {
+            if (r >= visible(c, a, sn.len, i)) continue;
+            const size_t th = (size_t)(sn.first + i) * a.q_heads;
+            for (int h = 0; h < a.q_heads; ++h)
+                sum = __fadd_rn(sum, ex2(__fsub_rn(kk.logits[(th + h) * kk.logit_rows + r], kk.lse2[th + h])));
+        }
+        const size_t at = (size_t)s * c.capacity + r;
+        a.w_out[at] = __fadd_rn(__fmul_rn(a.decay, a.w_in[at]), sum);
+    }
+}
+
+// Softmax weights of a found list's entries, summed over the query heads.
+__global__ void __launch_bounds__(128) k_cache_found_weights(CacheView c, AttendKernel kk) {
+    const AttendArgs& a = kk.a;
+    const int blocks = (a.k + 127) / 128;  // of one token
+    const int tk = blockIdx.x / blocks, lane = threadIdx.x & 31;
+    const int s = find_sequence(a.tok.offsets, c.n_seqs, tk, lane & 7, 0xFFu << (lane / 8 * 8));
+    if (s < 0) return;
+    const size_t th = (size_t)tk * a.q_heads;
+    const int e = (blockIdx.x - tk * blocks) * 128 + threadIdx.x;
+    if (e < a.k) {
+        float sum = 0.0f;
+        for (int h = 0; h < a.q_heads; ++h) {
+            const float z = kk.logits[(th + h) * kk.logit_rows + e];
+            if (z != -INFINITY) sum = __fadd_rn(sum, ex2(__fsub_rn(z, kk.lse2[th + h])));
+        }
+        a.w_out[(size_t)tk * a.k + e] = sum;
+    }
+}
+
+size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
+
+AttendPlan make_plan(const CacheView& c, const AttendArgs& a) {
+    AttendPlan p{};
+    const bool found = a.k > 0;
+    const long long cols = found ? a.group : (long long)std::max(1, a.max_tokens) * a.group;
+    // sixteen columns fill the query operand's M; wide rows leave no registers for them
+    p.nc = a.type != kF32 && c.G <= 2 && cols > 8 ? 16 : 8;
+    p.col_tiles = (int)((cols + p.nc - 1) / p.nc);
+    const long long items = (long long)(found ? a.tok.n_tokens : c.n_seqs) * c.heads * p.col_tiles;
+    const int rows = std::max(1, found ? a.k : std::min(a.max_rows, c.capacity));
+    const int most = (rows + kAttWarps * kTile - 1) / (kAttWarps * kTile);
+    const long long want = 4ll * sm_count();
+    p.n_split = (int)std::max<long long>(1, std::min<long long>(most, (want + items - 1) / std::max(1ll, items)));
+    const size_t th = (size_t)a.tok.n_tokens * a.q_heads;
+    size_t off = 0;
+    if (p.n_split > 1) {
+        off += up256(th * p.n_split * sizeof(float2));
+        p.off_o = off;
+        off += up256(th * p.n_split * c.dim * sizeof(float));
+    }
+    p.logit_rows = (rows + kAttWarps * kTile - 1) / (kAttWarps * kTile) * (kAttWarps * kTile);
+    if (a.w_out) {
+        p.off_lse = off;
+        off += up256(th * sizeof(float));
+        p.off_logit = off;
+        off += up256(th * p.logit_rows * sizeof(float));
+    }
+    p.bytes = off;
+    return p;
+}
+
+template <int G, int NC, bool F32>
+void start(const CacheView& c, const AttendKernel& k, bool found, unsigned grid, cudaStream_t st) {
+    if (found)
+        k_cache_attend<G, NC, F32, true><<<grid, kAttBS, 0, st>>>(c, k);
+    else
+        k_cache_attend<G, NC, F32, false><<<grid, kAttBS, 0, st>>>(c, k);
+}
+
+template <int G>
+void start_g(const CacheView& c, const AttendKernel& k, int nc, bool found, unsigned grid, cudaStream_t st) {
+    if (k.a.type == kF32)
+        start<G, 8, true>(c, k, found, grid, st);
+    else if (nc == 8)
+        start<G, 8, false>(c, k, found, grid, st);
+    else if constexpr (G <= 2)
+        start<G, 16, false>(c, k, found, grid, st);
+}
+
+}  // namespace
+
+size_t cache_attend_workspace(const CacheView& c, const AttendArgs& a) { return make_plan(c, a).bytes; }
+
+long long cache_attend_blocks(const CacheView& c, const AttendArgs& a) {
+    const AttendPlan p = make_plan(c, a);
+    return (long long)(a.k > 0 ? a.tok.n_tokens : c.n_seqs) * c.heads * p.n_split * p.col_tiles;
+}
+
+void launch_cache_attend(const CacheView& c, const AttendArgs& a, cudaStream_t st) {
+    if (a.tok.n_tokens <= 0 && !a.w_out) return;
+    const bool found = a.k > 0;
+    if (found && a.tok.n_tokens <= 0) return;
+    const AttendPlan p = make_plan(c, a);
+    char* ws = static_cast<char*>(a.workspace);
+    AttendKernel k{};
+    k.a = a;
+    k.part_ml = reinterpret_cast<float2*>(ws);
+    k.part_o = reinterpret_cast<float*>(ws + p.off_o);
+    if (a.w_out) {
+        k.lse2 = reinterpret_cast<float*>(ws + p.off_lse);
+        k.logits = reinterpret_cast<float*>(ws + p.off_logit);
+        k.logit_rows = p.logit_rows;
+    }
+    k.n_split = p.n_split;
+    k.col_tiles = p.col_tiles;
+    if (a.tok.n_tokens > 0) {
+        const unsigned grid =
+            (unsigned)((long long)(found ? a.tok.n_tokens : c.n_seqs) * c.heads * p.n_split * p.col_tiles);
+        {
+            Tick tk(kKCacheAttend, st);
+            if (c.G == 1)
+                start_g<1>(c, k, p.nc, found, grid, st);
+            else if (c.G == 2)
+                start_g<2>(c, k, p.nc, found, grid, st);
+            else if (c.G == 4)
+                start_g<4>(c, k, p.nc, found, grid, st);
+            else
+                start_g<6>(c, k, p.nc, found, grid, st);
+        }
+        if (p.n_split > 1) {
+            Tick tk(kKCacheJoin, st);
+            const unsigned jg = (unsigned)(((long long)a.tok.n_tokens * a.q_heads + 3) / 4);
+            if (found)
+                k_cache_join<true><<<jg, 128, 0, st>>>(c, k);
+            else
+                k_cache_join<false><<<jg, 128, 0, st>>>(c, k);
+        }
+    }
+    if (a.w_out) {
+        Tick tk(kKCacheWeights, st);
+        if (found)
+            k_cache_found_weights<<<(unsigned)((a.k + 127) / 128 * (long long)a.tok.n_tokens), 128, 0, st>>>(c, k);
+        else
+            k_cache_weights<<<dim3((std::min(a.max_rows, c.capacity) + 255) / 256, c.n_seqs), 256, 0, st>>>(c, k);
+    }
+}
+
+}  // namespace dev
+}  // namespace maivs

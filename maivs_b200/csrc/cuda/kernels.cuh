@@ -64,7 +64,10 @@ struct IndexView {
 enum KernelId : int {
     kKEncode = 0, kKRouteFlat, kKRouteTree, kKRescore, kKSeed, kKInvCount, kKInvScan, kKInvScatter,
     kKScanCm, kKFinalCm, kKPqPrep, kKPqScan, kKPqFold, kKRerank, kKTopk, kKRerankItems, kKSeedFinish, kKLocalList, kKMergeTopk,
-    kKScanMma, kKSeedScan, kKAllGather, kKSegMerge, kKRescoreDots, kKProbeSelect, kNumKernels
+    kKScanMma, kKSeedScan, kKAllGather, kKSegMerge, kKRescoreDots, kKProbeSelect, kNumKernels,
+    // the attention cache's kernels: named and counted, but no index's clock times them
+    kKCacheAppend = kNumKernels, kKCacheRead, kKCacheAttend, kKCacheJoin, kKCacheWeights, kKCacheSelect, kKCacheMove,
+    kNumNamed
 };
 const char* kernel_name(int id);
 // Brackets a step that is not one of this library's kernels (an NCCL collective) on the thread's

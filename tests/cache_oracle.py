@@ -1,0 +1,111 @@
+"""The attention cache's operators from their definitions, in 64 bits on the CPU, for the tests.
+
+Everything is numpy and written row by row; inputs are what the calls get (already rounded to the
+call's type). The error bounds beside the values are derived here from the kernels' roundings, before
+any comparison: see attend_bounds.
+"""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+
+GROUP = 64
+
+
+def bf16(x):
+    """f32 array rounded to bf16 (nearest, ties to even), as f32."""
+    b = np.asarray(x, np.float32).view(np.uint32).astype(np.uint64)
+    out = ((b + 0x7FFF + ((b >> 16) & 1)) & 0xFFFF0000).astype(np.uint32).view(np.float32).copy()
+    nan = np.isnan(x)
+    out[nan] = np.nan
+    return out
+
+
+def quantise(x):
+    """Rows [..., dim] (f32) -> (values, low, step) as f64 [..., dim] each (low and step per element)."""
+    x = np.asarray(x, np.float32)
+    dim = x.shape[-1]
+    val, low_e, step_e = (np.zeros(x.shape) for _ in range(3))
+    for g in range(0, dim, GROUP):
+        part = x[..., g:g + GROUP]
+        hi, lo = part.max(axis=-1, keepdims=True), part.min(axis=-1, keepdims=True)
+        with np.errstate(all="ignore"):
+            step = bf16((hi - lo) * (np.float32(1.0) / np.float32(15.0))).astype(np.float64)
+            low = bf16(lo).astype(np.float64)
+            at = (part.astype(np.float64) - low) / np.where(step == 0, 1.0, step)
+            code = np.where(step == 0, 0.0, np.clip(np.rint(at), 0, 15))
+            v = (low + step * code).astype(np.float32).astype(np.float64)
+        bad = np.broadcast_to(~np.isfinite(part.astype(np.float64)).all(axis=-1, keepdims=True) | ~np.isfinite(step),
+                              v.shape)
+        val[..., g:g + GROUP] = np.where(bad, np.nan, v)
+        low_e[..., g:g + GROUP] = np.where(bad, np.nan, np.broadcast_to(low, v.shape))
+        step_e[..., g:g + GROUP] = np.where(bad, np.nan, np.broadcast_to(step, v.shape))
+    return val, low_e, step_e
+
+
+UNIT = {"bf16": 2.0 ** -8, "f16": 2.0 ** -11, "f32": 2.0 ** -24}  # half a step, relative
+TINY = {"bf16": 2.0 ** -134, "f16": 2.0 ** -25, "f32": 2.0 ** -150}  # half a step of the subnormals
+
+
+class Rows:
+    """The quantised rows of one head: keys and values with their low and step."""
+
+    def __init__(self, keys, values):
+        self.k, self.k_low, self.k_step = quantise(keys)
+        self.v, self.v_low, self.v_step = quantise(values)
+
+
+def attend_head(q, rows, which, scale, dtype):
+    """One query of one head over the rows `which` (a list, repeats count): out, lse, p and bounds on
+    the kernels' error in each.
+
+    z = scale * q . k is summed in f32 over dim products and their low terms (at most dim + 16
+    roundings of 2^-23 relative to the sum of magnitudes; the tensor core's additions truncate). The
+    query itself is exact in f16 for 16-bit types, and 2^-22 off for f32 (two halves). ex2 is off by
+    2^-22 relative, its argument by 2^-24 of |z - max| (in log2). p * step is rounded to f16 (2^-12
+    relative) in 16-bit calls, to two halves (2^-22) in f32 ones; half a subnormal step of f16 in units
+    where the largest step is 4096 adds 2^-37 of it per row, times the code. Sums over n rows add n
+    roundings of 2^-23. The result is rounded to the call's type.
+    """
+    d = len(q)
+    n = len(which)
+    if n == 0:
+        return np.zeros(d), -math.inf, np.zeros(0), np.zeros(d), 0.0, np.zeros(0)
+    q = np.asarray(q, np.float64)
+    k, v = rows.k[which], rows.v[which]
+    z = scale * (k @ q)
+    mag = abs(scale) * ((np.abs(rows.k_low[which]) + 15 * rows.k_step[which]) @ np.abs(q))
+    dz = ((d + 16) * 2.0 ** -23 + (2.0 ** -22 if dtype == "f32" else 2.0 ** -30)) * mag.max()
+    top = z.max()
+    e = np.exp(z - top)
+    total = e.sum()
+    p = e / total
+    lse = top + math.log(total)
+    # relative error of one p: exponent's argument, ex2, sum and division
+    spread = min((top - z).max() / math.log(2.0), 160.0)
+    dp = 2.0 * dz + (spread + 8) * 2.0 ** -23 + (n + 32) * 2.0 ** -23
+    out = p @ v
+    level = 15 * rows.v_step[which] + np.abs(rows.v_low[which])
+    a = p @ level
+    round_p = 2.0 ** -22 if dtype == "f32" else 2.0 ** -12
+    # a subnormal p * step: half of 2^-24 in units of (step's power of two, at most 2 * step) / 4096
+    tiny = n * 15 * 2.0 ** -25 / 4096 * 2 * rows.v_step[which].max(axis=0) * 8 if dtype != "f32" else 0.0
+    err = a * (round_p + dp + (n + 64) * 2.0 ** -23) + tiny
+    err = err + UNIT[dtype] * (np.abs(out) + err) + TINY[dtype]
+    return out, lse, p, err, dz + (n + 32) * 2.0 ** -23 + abs(lse) * 2.0 ** -22, p * dp + 2.0 ** -126
+
+
+def evict(length, keep, w, ids=None, protect=None):
+    """(new length, source row of every new row, rows that leave)."""
+    rank = []
+    for r in range(length):
+        x = float(w[r])
+        top = x != x or (protect is not None and int(ids[r]) >= int(protect))
+        rank.append(math.inf if top else x)
+    order = sorted(range(length), key=lambda r: (-rank[r], r))
+    m = min(length, keep)
+    kept = set(order[:m])
+    movers = iter(sorted(r for r in kept if r >= m))
+    src = [r if r in kept else next(movers) for r in range(m)]
+    return m, src, [r for r in range(length) if r not in kept]
