@@ -3,13 +3,12 @@
 // For a query column (a token's query head) with visible rows r and z_r = scale * q . k_r:
 // out = sum_r p_r v_r, p = softmax(z), in one pass over the rows with a running maximum and sum.
 //
-// The rows are streamed from HBM into registers, and stay there: a warp takes tiles of 16 rows, and a
-// 4-bit code becomes an f16 operand of mma.m16n8k16 by one mask. A nibble in the low four bits of a
+// A warp streams tiles of 16 rows through a ring of its own in shared memory (cp.async, no barrier of the
+// block in the loop), and a 4-bit code becomes an f16 operand of mma.m16n8k16 by one mask. A nibble in the low four bits of a
 // half is the subnormal c * 2^-24, in the next four c * 2^-20; both are exact, the tensor core takes
 // subnormals as they are, and the powers of two are taken out of the f32 accumulators (or folded
-// into the query operand) afterwards. No operand goes through shared memory, so the tile loop has no
-// barrier, and two of the format's properties come for free: a group's step and low multiply sums
-// of its codes, not the codes.
+// into the query operand) afterwards. A group's step and low multiply sums of its codes, not the
+// codes.
 //
 //   keys    S^T = Q K^T: A = queries (M: columns, scaled by a power of two to f16's upper range),
 //           B = codes (N: 8 rows). Per group g: s += step_g * acc_g + low_g * sum(q in g).
@@ -37,6 +36,8 @@ namespace {
 constexpr int kAttWarps = 4;
 constexpr int kAttBS = kAttWarps * 32;
 constexpr int kTile = 16;
+constexpr int kJoinBS = 128;
+constexpr int kMaxSplit = 1024;
 constexpr float kNoMax = -3.0e38f;
 constexpr float kLog2e = 1.4426950408889634f;
 // p * step goes into f16 scaled so that the group's largest step becomes 2^12: an old maximum may
@@ -125,6 +126,22 @@ __device__ __forceinline__ void load_words(const uint32_t* __restrict__ p, uint3
     }
 }
 
+// The same from the tile in shared memory.
+template <int N>
+__device__ __forceinline__ void tile_words(const uint32_t* p, uint32_t (&w)[N]) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+        }
+    } else {
+        static_assert(N == 2, "two words or fours");
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        w[0] = v.x, w[1] = v.y;
+    }
+}
+
 __device__ __forceinline__ float read_q(const void* q, int type, size_t i) {
     if (type == kF32) return __ldg(static_cast<const float*>(q) + i);
     const uint32_t b = __ldg(static_cast<const unsigned short*>(q) + i);
@@ -168,17 +185,64 @@ struct Shape {
     static constexpr int kCols = NC / 8;             // columns per thread
     static constexpr float kUnit = F32 ? 1.0f : 16777216.0f;  // 1 / what a code of 1 is as an operand
     static constexpr bool kQShared = G * kQ > 16;    // wide queries wait in shared memory
+    // A warp's ring of tiles in flight. Stages x warps per SM x 1152 G bytes cover HBM's latency.
+    static constexpr int kStages = FOUND ? 0 : G <= 2 ? 4 : 3;
+    static constexpr int kTileBytes = kTile * 72 * G;
+    static constexpr int kRingBytes = kAttWarps * kStages * kTileBytes;
+    static constexpr int kBlocks = G == 1 && NC == 8 ? 5 : G <= 2 && NC == 8 ? 4 : G <= 2 ? 3 : 2;  // per SM
     static_assert(!(kQShared && NC == 16), "sixteen columns keep their queries in registers");
 };
 
+// A tile in the ring: 16 rows of key codes, value codes, key parameters, value parameters. Sixteen-byte
+// pieces are placed so that a warp's reads meet no bank twice: key piece p of row r at p, but two
+// rows of 128 bytes swap halves; value piece p at p with two bits flipped by the row, since the
+// four rows a quad reads at once lie 128 bytes (or a multiple) apart.
+template <int G>
+__device__ __forceinline__ int key_piece(int p) {
+    return G == 4 ? p ^ (((p >> 3) & 1) << 2) : p;
+}
+template <int G>
+__device__ __forceinline__ int value_piece(int p) {
+    const int r = p / (2 * G);
+    return p ^ (G == 1 ? ((r >> 2) & 1) << 1 : ((r >> 1) & 3) << 1);
+}
+
+__device__ __forceinline__ void copy16(char* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
+                 : "memory");
+}
+
+template <int G>
+__device__ __forceinline__ void fetch_tile(char* tile, const uint32_t* kc, const uint32_t* vc, const uint32_t* kp,
+                                           const uint32_t* vp, int r0, int lane) {
+    const char* ks = reinterpret_cast<const char*>(kc + (size_t)r0 * 8 * G);
+    const char* vs = reinterpret_cast<const char*>(vc + (size_t)r0 * 8 * G);
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+        const int p = lane + 32 * i;
+        copy16(tile + key_piece<G>(p) * 16, ks + p * 16);
+        copy16(tile + 512 * G + value_piece<G>(p) * 16, vs + p * 16);
+    }
+#pragma unroll
+    for (int p = 0; p < 8 * G; p += 32) {
+        const int q = p + lane;
+        if (q < 8 * G) {
+            const char* src = q < 4 * G ? reinterpret_cast<const char*>(kp + (size_t)r0 * G) + q * 16
+                                        : reinterpret_cast<const char*>(vp + (size_t)r0 * G) + (q - 4 * G) * 16;
+            copy16(tile + 1024 * G + q * 16, src);
+        }
+    }
+}
+
 template <int G, int NC, bool F32, bool FOUND>
-__global__ void __launch_bounds__(kAttBS) k_cache_attend(CacheView c, AttendKernel kk) {
+__global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, FOUND>::kBlocks) k_cache_attend(CacheView c, AttendKernel kk) {
     using S = Shape<G, NC, F32, FOUND>;
     constexpr int kCols = S::kCols, kQ = S::kQ;
     const AttendArgs& a = kk.a;
     __shared__ float s_o[NC][G * kCacheGroup + 4];
     __shared__ float s_m[kAttWarps][NC], s_l[kAttWarps][NC], s_low[kAttWarps][NC][G];
     __shared__ uint4 s_q[S::kQShared ? 2 * G * (kQ / 4) : 1][32];
+    extern __shared__ __align__(128) char s_ring[];
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gid = lane >> 2, t = lane & 3;
     unsigned b = blockIdx.x;
@@ -328,7 +392,28 @@ __global__ void __launch_bounds__(kAttBS) k_cache_attend(CacheView c, AttendKern
                     for (int r = 0; r < 4; ++r) o[g][i][j][r] = 0.0f;
         }
 
+        char* ring = s_ring + warp * S::kStages * S::kTileBytes;
+        int stage = 0;
+        if constexpr (!FOUND) {
+#pragma unroll
+            for (int i = 0; i < S::kStages - 1; ++i) {
+                const int r = start + (warp + i * kAttWarps) * kTile;
+                if (r < end) fetch_tile<G>(ring + i * S::kTileBytes, kc, vc, kp, vp, r, lane);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            }
+        }
         for (int r0 = start + warp * kTile; r0 < end; r0 += kAttWarps * kTile) {
+            const char* tile = ring + stage * S::kTileBytes;
+            if constexpr (!FOUND) {
+                // this tile is there, and every lane is done with the one before, whose place the next takes
+                asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
+                __syncwarp();
+                const int r = r0 + (S::kStages - 1) * kAttWarps * kTile;
+                const int last = stage == 0 ? S::kStages - 1 : stage - 1;
+                if (r < end) fetch_tile<G>(ring + last * S::kTileBytes, kc, vc, kp, vp, r, lane);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                stage = stage == S::kStages - 1 ? 0 : stage + 1;
+            }
             // ---- rows of the tile: gid and gid + 8 as keys, 2t, 2t + 1, 2t + 8, 2t + 9 as values ----
             size_t krow[2], vrow[4];
             bool ok[4];
@@ -345,10 +430,10 @@ __global__ void __launch_bounds__(kAttBS) k_cache_attend(CacheView c, AttendKern
 #pragma unroll
                 for (int i = 0; i < 4; ++i) vrow[i] = entry(r0 + 2 * t + (i & 1) + 8 * (i >> 1), ok[i]);
             } else {
-                krow[0] = r0 + gid;
-                krow[1] = r0 + gid + 8;
+                krow[0] = gid;  // within the tile
+                krow[1] = gid + 8;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) vrow[i] = r0 + 2 * t + (i & 1) + 8 * (i >> 1);
+                for (int i = 0; i < 4; ++i) vrow[i] = 2 * t + (i & 1) + 8 * (i >> 1);
             }
             const bool edge = FOUND || r0 + kTile > lim_first;
 
@@ -362,8 +447,10 @@ __global__ void __launch_bounds__(kAttBS) k_cache_attend(CacheView c, AttendKern
             } else {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    load_words<2 * G>(kp + vrow[2 * i] * G, *reinterpret_cast<uint32_t(*)[2 * G]>(&kpw[2 * i]));
-                    load_words<2 * G>(vp + vrow[2 * i] * G, *reinterpret_cast<uint32_t(*)[2 * G]>(&vpw[2 * i]));
+                    const uint32_t* par = reinterpret_cast<const uint32_t*>(tile + 1024 * G);
+                    tile_words<2 * G>(par + vrow[2 * i] * G, *reinterpret_cast<uint32_t(*)[2 * G]>(&kpw[2 * i]));
+                    tile_words<2 * G>(par + (kTile + vrow[2 * i]) * G,
+                                      *reinterpret_cast<uint32_t(*)[2 * G]>(&vpw[2 * i]));
                 }
             }
 
@@ -372,13 +459,23 @@ __global__ void __launch_bounds__(kAttBS) k_cache_attend(CacheView c, AttendKern
 #pragma unroll
             for (int nt = 0; nt < 2; ++nt) {
                 uint32_t w[2 * G];
-                const uint32_t* kr = kc + krow[nt] * 8 * G;
-                if constexpr (G == 1) {
-                    load_words<2>(kr + t * 2, w);
+                if constexpr (FOUND) {
+                    const uint32_t* kr = kc + krow[nt] * 8 * G;
+                    if constexpr (G == 1) {
+                        load_words<2>(kr + t * 2, w);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < G / 2; ++i)
+                            load_words<4>(kr + i * 16 + t * 4, *reinterpret_cast<uint32_t(*)[4]>(&w[4 * i]));
+                    }
+                } else if constexpr (G == 1) {
+                    tile_words<2>(reinterpret_cast<const uint32_t*>(tile) + krow[nt] * 8 + t * 2, w);
                 } else {
 #pragma unroll
                     for (int i = 0; i < G / 2; ++i)
-                        load_words<4>(kr + i * 16 + t * 4, *reinterpret_cast<uint32_t(*)[4]>(&w[4 * i]));
+                        tile_words<4>(reinterpret_cast<const uint32_t*>(
+                                          tile + key_piece<G>((int)krow[nt] * 2 * G + i * 4 + t) * 16),
+                                      *reinterpret_cast<uint32_t(*)[4]>(&w[4 * i]));
                 }
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -458,7 +555,7 @@ __global__ void __launch_bounds__(kAttBS) k_cache_attend(CacheView c, AttendKern
                 for (int i = 0; i < 4; ++i) {
                     const float x = par_step(vpw[i][g]);
                     // rows that no column of the tile sees may hold anything
-                    const bool in = FOUND ? ok[i] : !edge || (int)vrow[i] < lim_last;
+                    const bool in = FOUND ? ok[i] : !edge || r0 + (int)vrow[i] < lim_last;
                     if (in && x < INFINITY) big[g] = fmaxf(big[g], x);
                 }
                 grow |= big[g] > norm[g];
@@ -519,13 +616,28 @@ __global__ void __launch_bounds__(kAttBS) k_cache_attend(CacheView c, AttendKern
             uint32_t vw[4][G];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint32_t* vr = vc + vrow[i] * 8 * G;
-                if constexpr (G == 1) {
-                    load_words<1>(vr + gid, vw[i]);
-                } else {
+                if constexpr (FOUND) {
+                    const uint32_t* vr = vc + vrow[i] * 8 * G;
+                    if constexpr (G == 1) {
+                        load_words<1>(vr + gid, vw[i]);
+                    } else {
 #pragma unroll
-                    for (int x = 0; x < G / 2; ++x)
-                        load_words<2>(vr + x * 16 + gid * 2, *reinterpret_cast<uint32_t(*)[2]>(&vw[i][2 * x]));
+                        for (int x = 0; x < G / 2; ++x)
+                            load_words<2>(vr + x * 16 + gid * 2, *reinterpret_cast<uint32_t(*)[2]>(&vw[i][2 * x]));
+                    }
+                } else {
+                    const char* vt = tile + 512 * G;
+                    if constexpr (G == 1) {
+                        vw[i][0] = *reinterpret_cast<const uint32_t*>(
+                            vt + value_piece<G>((int)vrow[i] * 2 + (gid >> 2)) * 16 + (gid & 3) * 4);
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < G / 2; ++x)
+                            tile_words<2>(reinterpret_cast<const uint32_t*>(
+                                              vt + value_piece<G>((int)vrow[i] * 2 * G + 4 * x + (gid >> 1)) * 16 +
+                                              (gid & 1) * 8),
+                                          *reinterpret_cast<uint32_t(*)[2]>(&vw[i][2 * x]));
+                    }
                 }
             }
 #pragma unroll
@@ -541,7 +653,7 @@ __global__ void __launch_bounds__(kAttBS) k_cache_attend(CacheView c, AttendKern
                         float add = __fmul_rn(p[j][i], lo);
                         if (edge) {
                             // a row the column does not see adds nothing, whatever it holds
-                            const bool seen = FOUND ? ok[i] : (int)vrow[i] < lim[j];
+                            const bool seen = FOUND ? ok[i] : r0 + (int)vrow[i] < lim[j];
                             ps[j][i] = seen ? ps[j][i] : 0.0f;
                             add = seen ? add : 0.0f;
                         }
@@ -654,14 +766,18 @@ __global__ void __launch_bounds__(kAttBS) k_cache_attend(CacheView c, AttendKern
     }
 }
 
-// Joins the splits of one token's query head; a warp each.
+// Joins the splits of one token's query head: a block each. Its warps take every fourth split, lanes the
+// dimensions; the warps' sums are added in order.
 template <bool FOUND>
-__global__ void __launch_bounds__(128) k_cache_join(CacheView c, AttendKernel kk) {
+__global__ void __launch_bounds__(kJoinBS) k_cache_join(CacheView c, AttendKernel kk) {
     const AttendArgs& a = kk.a;
-    const int lane = threadIdx.x & 31;
-    const long long th = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    constexpr int kWarps = kJoinBS / 32;
+    __shared__ float s_w[kMaxSplit];
+    __shared__ float s_red[kWarps];
+    __shared__ float s_acc[kWarps][kCacheMaxDim];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const size_t th = blockIdx.x;
     const int tk = (int)(th / a.q_heads);
-    if (tk >= a.tok.n_tokens) return;
     const int s = find_sequence(a.tok.offsets, c.n_seqs, tk, lane & 7, 0xFFu << (lane / 8 * 8));
     if (s < 0) return;
     const Span sn = span_of(c, a, s);
@@ -671,21 +787,50 @@ __global__ void __launch_bounds__(128) k_cache_join(CacheView c, AttendKernel kk
     const int used = max(1, (rows + share - 1) / share);
     const size_t step = (size_t)a.tok.n_tokens * a.q_heads;
     float m = kNoMax, l = 0.0f;
-    for (int i = lane; i < used; i += 32) m = fmaxf(m, kk.part_ml[i * step + th].x);
+    for (int i = threadIdx.x; i < used; i += kJoinBS) m = fmaxf(m, kk.part_ml[i * step + th].x);
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-    for (int i = lane; i < used; i += 32) {
+    if (lane == 0) s_red[warp] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_red[w]);
+    __syncthreads();
+    for (int i = threadIdx.x; i < used; i += kJoinBS) {
         const float2 v = kk.part_ml[i * step + th];
-        l = __fmaf_rn(v.y, ex2(v.x - m), l);
+        const float f = ex2(v.x - m);
+        s_w[i] = f;
+        l = __fmaf_rn(v.y, f, l);
     }
     for (int o = 16; o; o >>= 1) l = __fadd_rn(l, __shfl_xor_sync(~0u, l, o));
-    const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
-    for (int d = lane; d < c.dim; d += 32) {
-        float acc = 0.0f;
-        for (int i = 0; i < used; ++i)
-            acc = __fmaf_rn(kk.part_o[(i * step + th) * c.dim + d], ex2(kk.part_ml[i * step + th].x - m), acc);
-        write_out(a.out, a.type, (size_t)th * c.dim + d, l == 0.0f ? 0.0f : __fmul_rn(acc, inv));
+    if (lane == 0) s_red[warp] = l;
+    __syncthreads();
+    l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) l = __fadd_rn(l, s_red[w]);
+    constexpr int kLoads = kCacheMaxDim / 32;
+    float acc[kLoads];
+#pragma unroll
+    for (int x = 0; x < kLoads; ++x) acc[x] = 0.0f;
+    const int n = (c.dim + 31) / 32;
+#pragma unroll 4
+    for (int i = warp; i < used; i += kWarps) {
+        const float* part = kk.part_o + (i * step + th) * c.dim;
+        const float f = s_w[i];
+#pragma unroll
+        for (int x = 0; x < kLoads; ++x)
+            if (x < n && lane + 32 * x < c.dim) acc[x] = __fmaf_rn(part[lane + 32 * x], f, acc[x]);
     }
-    if (lane == 0) {
+#pragma unroll
+    for (int x = 0; x < kLoads; ++x)
+        if (x < n) s_acc[warp][lane + 32 * x] = acc[x];
+    __syncthreads();
+    const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+    for (int d = threadIdx.x; d < c.dim; d += kJoinBS) {
+        float v = s_acc[0][d];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) v = __fadd_rn(v, s_acc[w][d]);
+        write_out(a.out, a.type, th * c.dim + d, l == 0.0f ? 0.0f : __fmul_rn(v, inv));
+    }
+    if (threadIdx.x == 0) {
         const float l2 = l == 0.0f ? -INFINITY : __fadd_rn(m, log2f(l));
         if (a.lse) a.lse[th] = __fmul_rn(l2, 0.69314718055994531f);
         if (kk.lse2) kk.lse2[th] = l2;
@@ -744,7 +889,7 @@ AttendPlan make_plan(const CacheView& c, const AttendArgs& a) {
     const int rows = std::max(1, found ? a.k : std::min(a.max_rows, c.capacity));
     const int most = (rows + kAttWarps * kTile - 1) / (kAttWarps * kTile);
     const long long want = 4ll * sm_count();
-    p.n_split = (int)std::max<long long>(1, std::min<long long>(most, (want + items - 1) / std::max(1ll, items)));
+    p.n_split = (int)std::max<long long>(1, std::min<long long>(std::min(most, kMaxSplit), (want + items - 1) / std::max(1ll, items)));
     const size_t th = (size_t)a.tok.n_tokens * a.q_heads;
     size_t off = 0;
     if (p.n_split > 1) {
@@ -765,10 +910,13 @@ AttendPlan make_plan(const CacheView& c, const AttendArgs& a) {
 
 template <int G, int NC, bool F32>
 void start(const CacheView& c, const AttendKernel& k, bool found, unsigned grid, cudaStream_t st) {
-    if (found)
+    if (found) {
         k_cache_attend<G, NC, F32, true><<<grid, kAttBS, 0, st>>>(c, k);
-    else
-        k_cache_attend<G, NC, F32, false><<<grid, kAttBS, 0, st>>>(c, k);
+    } else {
+        constexpr int smem = Shape<G, NC, F32, false>::kRingBytes;
+        set_smem((const void*)k_cache_attend<G, NC, F32, false>, smem);
+        k_cache_attend<G, NC, F32, false><<<grid, kAttBS, smem, st>>>(c, k);
+    }
 }
 
 template <int G>
@@ -823,11 +971,11 @@ void launch_cache_attend(const CacheView& c, const AttendArgs& a, cudaStream_t s
         }
         if (p.n_split > 1) {
             Tick tk(kKCacheJoin, st);
-            const unsigned jg = (unsigned)(((long long)a.tok.n_tokens * a.q_heads + 3) / 4);
+            const unsigned jg = (unsigned)((long long)a.tok.n_tokens * a.q_heads);
             if (found)
-                k_cache_join<true><<<jg, 128, 0, st>>>(c, k);
+                k_cache_join<true><<<jg, kJoinBS, 0, st>>>(c, k);
             else
-                k_cache_join<false><<<jg, 128, 0, st>>>(c, k);
+                k_cache_join<false><<<jg, kJoinBS, 0, st>>>(c, k);
         }
     }
     if (a.w_out) {
