@@ -22,6 +22,7 @@
 // element, p * step is rounded to f16 (2^-12 relative, below the output's own rounding). f32 calls
 // split query and p * step into two f16 halves each (22 bits).
 #include <algorithm>
+#include <type_traits>
 
 #include "cache.h"
 #include "cache_dev.cuh"
@@ -106,27 +107,7 @@ __device__ __forceinline__ float left_over(float x, uint32_t p, int i) {
     return __fsub_rn(x, to_f32<__half>(i ? p >> 16 : p & 0xFFFFu));
 }
 
-template <int N>
-__device__ __forceinline__ void load_words(const uint32_t* __restrict__ p, uint32_t (&w)[N]) {
-    if constexpr (N % 4 == 0) {
-#pragma unroll
-        for (int i = 0; i < N / 4; ++i) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
-            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
-        }
-    } else if constexpr (N % 2 == 0) {
-#pragma unroll
-        for (int i = 0; i < N / 2; ++i) {
-            const uint2 v = __ldg(reinterpret_cast<const uint2*>(p) + i);
-            w[2 * i] = v.x, w[2 * i + 1] = v.y;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) w[i] = __ldg(p + i);
-    }
-}
-
-// The same from the tile in shared memory.
+// Words of a tile in shared memory.
 template <int N>
 __device__ __forceinline__ void tile_words(const uint32_t* p, uint32_t (&w)[N]) {
     if constexpr (N % 4 == 0) {
@@ -186,7 +167,7 @@ struct Shape {
     static constexpr float kUnit = F32 ? 1.0f : 16777216.0f;  // 1 / what a code of 1 is as an operand
     static constexpr bool kQShared = G * kQ > 16;    // wide queries wait in shared memory
     // A warp's ring of tiles in flight. Stages x warps per SM x 1152 G bytes cover HBM's latency.
-    static constexpr int kStages = FOUND ? 0 : G <= 2 ? 4 : 3;
+    static constexpr int kStages = G <= 2 ? 4 : 3;
     static constexpr int kTileBytes = kTile * 72 * G;
     static constexpr int kRingBytes = kAttWarps * kStages * kTileBytes;
     static constexpr int kBlocks = G == 1 && NC == 8 ? 5 : G <= 2 && NC == 8 ? 4 : G <= 2 ? 3 : 2;  // per SM
@@ -207,32 +188,81 @@ __device__ __forceinline__ int value_piece(int p) {
     return p ^ (G == 1 ? ((r >> 2) & 1) << 1 : ((r >> 1) & 3) << 1);
 }
 
-__device__ __forceinline__ void copy16(char* dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
-                 : "memory");
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 
-template <int G>
-__device__ __forceinline__ void fetch_tile(char* tile, const uint32_t* kc, const uint32_t* vc, const uint32_t* kp,
-                                           const uint32_t* vp, int r0, int lane) {
-    const char* ks = reinterpret_cast<const char*>(kc + (size_t)r0 * 8 * G);
-    const char* vs = reinterpret_cast<const char*>(vc + (size_t)r0 * 8 * G);
+// Brings tiles of one head into a warp's ring. Rows in order: a lane's pieces lie at fixed places of the
+// tile, so its three source addresses only advance. Found rows: the list names each piece's row.
+template <int G, bool FOUND>
+struct Fetch {
+    static constexpr int kParams = (8 * G + 31) / 32;  // rounds of parameter pieces (keys' then values')
+    const char *ks, *vs, *ps[kParams];
+    uint32_t kd[G], vd[G];
+    const uint64_t* list;
+    int k, row_limit, lane;
+
+    __device__ __forceinline__ void init(const uint32_t* kc, const uint32_t* vc, const uint32_t* kp, const uint32_t* vp,
+                                         int r0, int ln, const uint64_t* l, int k_, int limit) {
+        lane = ln;
+        list = l, k = k_, row_limit = limit;
+        if constexpr (FOUND) {
+            ks = reinterpret_cast<const char*>(kc), vs = reinterpret_cast<const char*>(vc);
+            ps[0] = reinterpret_cast<const char*>(kp);
+            if constexpr (kParams > 1) ps[1] = reinterpret_cast<const char*>(vp);
+        } else {
+            ks = reinterpret_cast<const char*>(kc) + ((size_t)r0 * 2 * G + lane) * 16;
+            vs = reinterpret_cast<const char*>(vc) + ((size_t)r0 * 2 * G + lane) * 16;
 #pragma unroll
-    for (int i = 0; i < G; ++i) {
-        const int p = lane + 32 * i;
-        copy16(tile + key_piece<G>(p) * 16, ks + p * 16);
-        copy16(tile + 512 * G + value_piece<G>(p) * 16, vs + p * 16);
-    }
+            for (int i = 0; i < kParams; ++i) {
+                const int q = lane + 32 * i;
+                ps[i] = q < 4 * G ? reinterpret_cast<const char*>(kp + (size_t)r0 * G) + q * 16
+                                  : reinterpret_cast<const char*>(vp + (size_t)r0 * G) + (q - 4 * G) * 16;
+            }
+        }
 #pragma unroll
-    for (int p = 0; p < 8 * G; p += 32) {
-        const int q = p + lane;
-        if (q < 8 * G) {
-            const char* src = q < 4 * G ? reinterpret_cast<const char*>(kp + (size_t)r0 * G) + q * 16
-                                        : reinterpret_cast<const char*>(vp + (size_t)r0 * G) + (q - 4 * G) * 16;
-            copy16(tile + 1024 * G + q * 16, src);
+        for (int i = 0; i < G; ++i) {
+            kd[i] = key_piece<G>(lane + 32 * i) * 16;
+            vd[i] = 512 * G + value_piece<G>(lane + 32 * i) * 16;
         }
     }
-}
+    __device__ __forceinline__ size_t row(int e) const {
+        const uint64_t id = e < k ? __ldg(list + e) : ~0ull;
+        return id < (uint64_t)row_limit ? (size_t)id : 0;
+    }
+    // The tile of rows (or list entries) r0 ..; pointers move on by the warps' stride.
+    __device__ __forceinline__ void next(uint32_t tile, int r0, const uint32_t* kp, const uint32_t* vp) {
+        if constexpr (FOUND) {
+#pragma unroll
+            for (int i = 0; i < G; ++i) {
+                const int p = lane + 32 * i, r = p / (2 * G);
+                const size_t at = (row(r0 + r) * 2 * G + (p - r * 2 * G)) * 16;
+                copy16(tile + kd[i], ks + at);
+                copy16(tile + vd[i], vs + at);
+            }
+            // a row's parameters are 4 G bytes: lane r brings row r's of the keys, lane r + 16 of the values
+            const uint32_t* src = (lane < 16 ? kp : vp) + row(r0 + (lane & 15)) * G;
+#pragma unroll
+            for (int i = 0; i < G; ++i) copy4(tile + 1024 * G + (lane * G + i) * 4, src + i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < G; ++i) {
+                copy16(tile + kd[i], ks + 512 * i);
+                copy16(tile + vd[i], vs + 512 * i);
+            }
+#pragma unroll
+            for (int i = 0; i < kParams; ++i) {
+                if (lane + 32 * i < 8 * G) copy16(tile + 1024 * G + (lane + 32 * i) * 16, ps[i]);
+                ps[i] += kAttWarps * kTile * 4 * G;
+            }
+            ks += kAttWarps * kTile * 32 * G;
+            vs += kAttWarps * kTile * 32 * G;
+        }
+    }
+};
 
 template <int G, int NC, bool F32, bool FOUND>
 __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, FOUND>::kBlocks) k_cache_attend(CacheView c, AttendKernel kk) {
@@ -371,8 +401,10 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, FOUND>::kBlocks) k_c
         const int lim_last = FOUND ? a.k : visible(c, a, sn.len, col_last / a.group);
         const int row_limit = FOUND ? visible(c, a, sn.len, item - sn.first) : 0;
         const int end = min(min(start + share, rows_all), lim_last);
+        const uint64_t* list = FOUND ? a.rows + (size_t)item * a.k : nullptr;
 
-        float m[kCols], l[kCols], low[kCols][G], norm[G];
+        // inv: what brings a step into f16's upper range, kPScale / norm, norm a power of two
+        float m[kCols], l[kCols], low[kCols][G], norm[G], inv[G];
         float o[G][4][kCols][4];
 #pragma unroll
         for (int j = 0; j < kCols; ++j) {
@@ -383,7 +415,7 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, FOUND>::kBlocks) k_c
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            norm[g] = 0.0f;
+            norm[g] = inv[g] = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -392,66 +424,32 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, FOUND>::kBlocks) k_c
                     for (int r = 0; r < 4; ++r) o[g][i][j][r] = 0.0f;
         }
 
-        char* ring = s_ring + warp * S::kStages * S::kTileBytes;
-        int stage = 0;
-        if constexpr (!FOUND) {
-#pragma unroll
-            for (int i = 0; i < S::kStages - 1; ++i) {
-                const int r = start + (warp + i * kAttWarps) * kTile;
-                if (r < end) fetch_tile<G>(ring + i * S::kTileBytes, kc, vc, kp, vp, r, lane);
-                asm volatile("cp.async.commit_group;" ::: "memory");
-            }
-        }
-        for (int r0 = start + warp * kTile; r0 < end; r0 += kAttWarps * kTile) {
-            const char* tile = ring + stage * S::kTileBytes;
-            if constexpr (!FOUND) {
-                // this tile is there, and every lane is done with the one before, whose place the next takes
-                asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
-                __syncwarp();
-                const int r = r0 + (S::kStages - 1) * kAttWarps * kTile;
-                const int last = stage == 0 ? S::kStages - 1 : stage - 1;
-                if (r < end) fetch_tile<G>(ring + last * S::kTileBytes, kc, vc, kp, vp, r, lane);
-                asm volatile("cp.async.commit_group;" ::: "memory");
-                stage = stage == S::kStages - 1 ? 0 : stage + 1;
-            }
-            // ---- rows of the tile: gid and gid + 8 as keys, 2t, 2t + 1, 2t + 8, 2t + 9 as values ----
-            size_t krow[2], vrow[4];
-            bool ok[4];
-            if constexpr (FOUND) {
-                const uint64_t* list = a.rows + (size_t)item * a.k;
-                auto entry = [&](int e, bool& good) -> size_t {
-                    const uint64_t id = e < a.k ? __ldg(list + e) : ~0ull;
-                    good = id < (uint64_t)row_limit;
-                    return good ? (size_t)id : 0;
-                };
-                bool dummy;
-                krow[0] = entry(r0 + gid, dummy);
-                krow[1] = entry(r0 + gid + 8, dummy);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) vrow[i] = entry(r0 + 2 * t + (i & 1) + 8 * (i >> 1), ok[i]);
-            } else {
-                krow[0] = gid;  // within the tile
-                krow[1] = gid + 8;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) vrow[i] = 2 * t + (i & 1) + 8 * (i >> 1);
-            }
-            const bool edge = FOUND || r0 + kTile > lim_first;
-
-            uint32_t kpw[4][G], vpw[4][G];
-            if constexpr (FOUND) {
+        // One tile of rows (or list entries) r0 ..: the scores' fragment has columns gid (and gid + 8) and
+        // rows 2t, 2t + 1, 2t + 8, 2t + 9. kEdge: some column does not see some row.
+        auto tile_step = [&](const char* tile, int r0, auto edge) {
+            constexpr bool kEdge = decltype(edge)::value;
+            bool ok[4];  // rows that some column sees
+            if constexpr (kEdge) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    load_words<G>(kp + vrow[i] * G, kpw[i]);
-                    load_words<G>(vp + vrow[i] * G, vpw[i]);
+                    const int r = r0 + 2 * t + (i & 1) + 8 * (i >> 1);
+                    ok[i] = r < lim_last;
+                    if (FOUND && ok[i]) ok[i] = __ldg(list + r) < (uint64_t)row_limit;
                 }
-            } else {
+            }
+            uint32_t kpw[4][G], vpw[4][G];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint32_t* par = reinterpret_cast<const uint32_t*>(tile + 1024 * G);
-                    tile_words<2 * G>(par + vrow[2 * i] * G, *reinterpret_cast<uint32_t(*)[2 * G]>(&kpw[2 * i]));
-                    tile_words<2 * G>(par + (kTile + vrow[2 * i]) * G,
-                                      *reinterpret_cast<uint32_t(*)[2 * G]>(&vpw[2 * i]));
-                }
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t* par = reinterpret_cast<const uint32_t*>(tile + 1024 * G) + (2 * t + 8 * i) * G;
+                tile_words<2 * G>(par, *reinterpret_cast<uint32_t(*)[2 * G]>(&kpw[2 * i]));
+                tile_words<2 * G>(par + kTile * G, *reinterpret_cast<uint32_t(*)[2 * G]>(&vpw[2 * i]));
+            }
+            if constexpr (kEdge) {
+                // rows that no column sees may hold anything
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int g = 0; g < G; ++g) vpw[i][g] = ok[i] ? vpw[i][g] : 0u;
             }
 
             // ---- scores: sc[j][i] of column j and value row i ----
@@ -459,22 +457,13 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, FOUND>::kBlocks) k_c
 #pragma unroll
             for (int nt = 0; nt < 2; ++nt) {
                 uint32_t w[2 * G];
-                if constexpr (FOUND) {
-                    const uint32_t* kr = kc + krow[nt] * 8 * G;
-                    if constexpr (G == 1) {
-                        load_words<2>(kr + t * 2, w);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < G / 2; ++i)
-                            load_words<4>(kr + i * 16 + t * 4, *reinterpret_cast<uint32_t(*)[4]>(&w[4 * i]));
-                    }
-                } else if constexpr (G == 1) {
-                    tile_words<2>(reinterpret_cast<const uint32_t*>(tile) + krow[nt] * 8 + t * 2, w);
+                if constexpr (G == 1) {
+                    tile_words<2>(reinterpret_cast<const uint32_t*>(tile) + (gid + 8 * nt) * 8 + t * 2, w);
                 } else {
 #pragma unroll
                     for (int i = 0; i < G / 2; ++i)
                         tile_words<4>(reinterpret_cast<const uint32_t*>(
-                                          tile + key_piece<G>((int)krow[nt] * 2 * G + i * 4 + t) * 16),
+                                          tile + key_piece<G>((gid + 8 * nt) * 2 * G + i * 4 + t) * 16),
                                       *reinterpret_cast<uint32_t(*)[4]>(&w[4 * i]));
                 }
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -521,13 +510,14 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, FOUND>::kBlocks) k_c
                     sc[j][2 * nt + 1] = __fmul_rn(sum[2 * j + 1], fac[j]);
                 }
             }
-            if (edge) {
+            bool see[kCols][4];
+            if constexpr (kEdge) {
 #pragma unroll
                 for (int j = 0; j < kCols; ++j)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int r = r0 + 2 * t + (i & 1) + 8 * (i >> 1);
-                        if (r >= lim[j] || (FOUND && !ok[i])) sc[j][i] = -INFINITY;
+                        see[j][i] = ok[i] && r0 + 2 * t + (i & 1) + 8 * (i >> 1) < lim[j];
+                        sc[j][i] = see[j][i] ? sc[j][i] : -INFINITY;
                     }
             }
             if (kk.logits) {
@@ -541,7 +531,7 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, FOUND>::kBlocks) k_c
             }
 
             // ---- running maximum and the groups' power of two: rescaled only where they grow ----
-            float top[kCols], big[G];
+            float top[kCols];
             bool grow = false;
 #pragma unroll
             for (int j = 0; j < kCols; ++j) {
@@ -549,17 +539,9 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, FOUND>::kBlocks) k_c
                 grow |= top[j] > m[j] + kLag;
             }
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-                big[g] = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float x = par_step(vpw[i][g]);
-                    // rows that no column of the tile sees may hold anything
-                    const bool in = FOUND ? ok[i] : !edge || r0 + (int)vrow[i] < lim_last;
-                    if (in && x < INFINITY) big[g] = fmaxf(big[g], x);
-                }
-                grow |= big[g] > norm[g];
-            }
+            for (int g = 0; g < G; ++g)
+                grow |= fmaxf(fmaxf(par_step(vpw[0][g]), par_step(vpw[1][g])),
+                              fmaxf(par_step(vpw[2][g]), par_step(vpw[3][g]))) > norm[g];
             if (__any_sync(~0u, grow)) {
                 float f[kCols];
 #pragma unroll
@@ -583,7 +565,12 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, FOUND>::kBlocks) k_c
                 }
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    float x = big[g];
+                    float x = 0.0f;  // a row with an infinite step is NaN whatever its scale
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float st = par_step(vpw[i][g]);
+                        x = st < INFINITY ? fmaxf(x, st) : x;
+                    }
                     x = fmaxf(x, __shfl_xor_sync(~0u, x, 1));
                     x = fmaxf(x, __shfl_xor_sync(~0u, x, 2));
                     float ratio = 1.0f;
@@ -592,6 +579,7 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, FOUND>::kBlocks) k_c
                         const float n = fmaxf(2.0f * __uint_as_float(__float_as_uint(x) & 0x7F800000u), 7.8886e-31f);
                         ratio = __fdiv_rn(norm[g], n);
                         norm[g] = n;
+                        inv[g] = __fdiv_rn(kPScale, n);
                     }
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
@@ -614,79 +602,91 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, FOUND>::kBlocks) k_c
 
             // ---- values ----
             uint32_t vw[4][G];
+            const char* vt = tile + 512 * G;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if constexpr (FOUND) {
-                    const uint32_t* vr = vc + vrow[i] * 8 * G;
-                    if constexpr (G == 1) {
-                        load_words<1>(vr + gid, vw[i]);
-                    } else {
-#pragma unroll
-                        for (int x = 0; x < G / 2; ++x)
-                            load_words<2>(vr + x * 16 + gid * 2, *reinterpret_cast<uint32_t(*)[2]>(&vw[i][2 * x]));
-                    }
+                const int r = 2 * t + (i & 1) + 8 * (i >> 1);
+                if constexpr (G == 1) {
+                    vw[i][0] = *reinterpret_cast<const uint32_t*>(vt + value_piece<G>(r * 2 + (gid >> 2)) * 16 +
+                                                                  (gid & 3) * 4);
                 } else {
-                    const char* vt = tile + 512 * G;
-                    if constexpr (G == 1) {
-                        vw[i][0] = *reinterpret_cast<const uint32_t*>(
-                            vt + value_piece<G>((int)vrow[i] * 2 + (gid >> 2)) * 16 + (gid & 3) * 4);
-                    } else {
 #pragma unroll
-                        for (int x = 0; x < G / 2; ++x)
-                            tile_words<2>(reinterpret_cast<const uint32_t*>(
-                                              vt + value_piece<G>((int)vrow[i] * 2 * G + 4 * x + (gid >> 1)) * 16 +
-                                              (gid & 1) * 8),
-                                          *reinterpret_cast<uint32_t(*)[2]>(&vw[i][2 * x]));
-                    }
+                    for (int x = 0; x < G / 2; ++x)
+                        tile_words<2>(reinterpret_cast<const uint32_t*>(
+                                          vt + value_piece<G>(r * 2 * G + 4 * x + (gid >> 1)) * 16 + (gid & 1) * 8),
+                                      *reinterpret_cast<uint32_t(*)[2]>(&vw[i][2 * x]));
                 }
             }
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                const float inv = norm[g] > 0.0f ? __fdiv_rn(kPScale, norm[g]) : 0.0f;
                 float ps[kCols][4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float st = __fmul_rn(par_step(vpw[i][g]), inv), lo = low_of<F32>(vpw[i][g]);
+                    const float st = __fmul_rn(par_step(vpw[i][g]), inv[g]), lo = low_of<F32>(vpw[i][g]);
 #pragma unroll
                     for (int j = 0; j < kCols; ++j) {
                         ps[j][i] = __fmul_rn(p[j][i], st);
-                        float add = __fmul_rn(p[j][i], lo);
-                        if (edge) {
+                        if constexpr (kEdge) {
                             // a row the column does not see adds nothing, whatever it holds
-                            const bool seen = FOUND ? ok[i] : r0 + (int)vrow[i] < lim[j];
-                            ps[j][i] = seen ? ps[j][i] : 0.0f;
-                            add = seen ? add : 0.0f;
+                            ps[j][i] = see[j][i] ? ps[j][i] : 0.0f;
+                            if (see[j][i]) low[j][g] = __fmaf_rn(p[j][i], lo, low[j][g]);
+                        } else {
+                            low[j][g] = __fmaf_rn(p[j][i], lo, low[j][g]);
                         }
-                        low[j][g] = __fadd_rn(low[j][g], add);
                     }
                 }
                 const uint32_t u0 = __byte_perm(vw[0][g], vw[1][g], 0x5410), h0 = __byte_perm(vw[0][g], vw[1][g], 0x7632);
                 const uint32_t u8 = __byte_perm(vw[2][g], vw[3][g], 0x5410), h8 = __byte_perm(vw[2][g], vw[3][g], 0x7632);
+                uint32_t b0[kCols], b1[kCols];
 #pragma unroll
-                for (int j = 0; j < kCols; ++j) {
-                    const uint32_t b0 = pack_h2(ps[j][0], ps[j][1]), b1 = pack_h2(ps[j][2], ps[j][3]);
+                for (int j = 0; j < kCols; ++j) b0[j] = pack_h2(ps[j][0], ps[j][1]), b1[j] = pack_h2(ps[j][2], ps[j][3]);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int sh = 8 * i;
-                        mma(o[g][2 * i][j], operand<F32, false>(u0 >> sh), operand<F32, false>(h0 >> sh),
-                            operand<F32, false>(u8 >> sh), operand<F32, false>(h8 >> sh), b0, b1);
-                        mma(o[g][2 * i + 1][j], operand<F32, true>(u0 >> sh), operand<F32, true>(h0 >> sh),
-                            operand<F32, true>(u8 >> sh), operand<F32, true>(h8 >> sh), b0, b1);
-                    }
-                    if (F32) {
-                        const uint32_t c0 = pack_h2(left_over(ps[j][0], b0, 0), left_over(ps[j][1], b0, 1));
-                        const uint32_t c1 = pack_h2(left_over(ps[j][2], b1, 0), left_over(ps[j][3], b1, 1));
+                for (int i = 0; i < 2; ++i) {
+                    const int sh = 8 * i;
+                    const uint32_t e0 = operand<F32, false>(u0 >> sh), e1 = operand<F32, false>(h0 >> sh),
+                                   e2 = operand<F32, false>(u8 >> sh), e3 = operand<F32, false>(h8 >> sh);
+                    const uint32_t d0 = operand<F32, true>(u0 >> sh), d1 = operand<F32, true>(h0 >> sh),
+                                   d2 = operand<F32, true>(u8 >> sh), d3 = operand<F32, true>(h8 >> sh);
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const int sh = 8 * i;
-                            mma(o[g][2 * i][j], operand<F32, false>(u0 >> sh), operand<F32, false>(h0 >> sh),
-                                operand<F32, false>(u8 >> sh), operand<F32, false>(h8 >> sh), c0, c1);
-                            mma(o[g][2 * i + 1][j], operand<F32, true>(u0 >> sh), operand<F32, true>(h0 >> sh),
-                                operand<F32, true>(u8 >> sh), operand<F32, true>(h8 >> sh), c0, c1);
+                    for (int j = 0; j < kCols; ++j) {
+                        mma(o[g][2 * i][j], e0, e1, e2, e3, b0[j], b1[j]);
+                        mma(o[g][2 * i + 1][j], d0, d1, d2, d3, b0[j], b1[j]);
+                        if (F32) {
+                            const uint32_t c0 = pack_h2(left_over(ps[j][0], b0[j], 0), left_over(ps[j][1], b0[j], 1));
+                            const uint32_t c1 = pack_h2(left_over(ps[j][2], b1[j], 0), left_over(ps[j][3], b1[j], 1));
+                            mma(o[g][2 * i][j], e0, e1, e2, e3, c0, c1);
+                            mma(o[g][2 * i + 1][j], d0, d1, d2, d3, c0, c1);
                         }
                     }
                 }
             }
+        };
+
+        char* ring = s_ring + warp * S::kStages * S::kTileBytes;
+        const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+        constexpr int kStride = kAttWarps * kTile;
+        Fetch<G, FOUND> fetch;
+        fetch.init(kc, vc, kp, vp, start + warp * kTile, lane, list, a.k, row_limit);
+#pragma unroll
+        for (int i = 0; i < S::kStages - 1; ++i) {
+            const int r = start + warp * kTile + i * kStride;
+            if (r < end) fetch.next(ring_at + i * S::kTileBytes, r, kp, vp);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+        int at = 0, to = (S::kStages - 1) * S::kTileBytes;  // this tile's place, and that of the one to fetch
+        for (int r0 = start + warp * kTile; r0 < end; r0 += kStride) {
+            // the tile is there, and every lane is done with the one before, whose place is filled next
+            asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
+            __syncwarp();
+            const int r = r0 + (S::kStages - 1) * kStride;
+            if (r < end) fetch.next(ring_at + to, r, kp, vp);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (FOUND || r0 + kTile > lim_first)
+                tile_step(ring + at, r0, std::true_type());
+            else
+                tile_step(ring + at, r0, std::integral_constant<bool, FOUND>());
+            to = at;
+            at = at == (S::kStages - 1) * S::kTileBytes ? 0 : at + S::kTileBytes;
         }
 
         // ---- the block's warps joined ----
@@ -910,13 +910,10 @@ AttendPlan make_plan(const CacheView& c, const AttendArgs& a) {
 
 template <int G, int NC, bool F32>
 void start(const CacheView& c, const AttendKernel& k, bool found, unsigned grid, cudaStream_t st) {
-    if (found) {
-        k_cache_attend<G, NC, F32, true><<<grid, kAttBS, 0, st>>>(c, k);
-    } else {
-        constexpr int smem = Shape<G, NC, F32, false>::kRingBytes;
-        set_smem((const void*)k_cache_attend<G, NC, F32, false>, smem);
-        k_cache_attend<G, NC, F32, false><<<grid, kAttBS, smem, st>>>(c, k);
-    }
+    constexpr int smem = Shape<G, NC, F32, false>::kRingBytes;
+    const auto kernel = found ? k_cache_attend<G, NC, F32, true> : k_cache_attend<G, NC, F32, false>;
+    set_smem((const void*)kernel, smem);
+    kernel<<<grid, kAttBS, smem, st>>>(c, k);
 }
 
 template <int G>
