@@ -10,13 +10,14 @@
 // into the query operand) afterwards. A group's step and low multiply sums of its codes, not the
 // codes.
 //
-//   keys    S^T = Q K^T: A = queries (M: columns, scaled by a power of two to f16's upper range),
-//           B = codes (N: 8 rows). Per group g: s += step_g * acc_g + low_g * sum(q in g).
+//   keys    S = K Q^T: A = codes (M: 16 rows), B = queries (N: 8 columns, scaled by a power of two to
+//           f16's upper range). Per group g: s += step_g * acc_g + low_g * sum(q in g).
 //   values  O^T = V^T P^T: A = codes (M: 16 dimensions of one group, K: 16 rows), B = p * step_g
 //           rounded to f16 (N: columns); the low terms p * low_g are summed in f32.
 //
-// S^T's accumulator layout (row = column of the query, columns = two rows of the cache) is the B
-// operand's layout of O^T, so p never leaves its thread.
+// The codes are the A operand of both, so that every register of both fragments is in use whatever
+// the number of columns, and a row's step and low are needed by one lane of every quad only. S's
+// accumulators become O^T's B operand by a transposition of 8 x 8 halves in registers.
 //
 // Rounding: codes are exact, 16-bit queries are exact in f16 down to 2^-24 of their row's largest
 // element, p * step is rounded to f16 (2^-12 relative, below the output's own rounding). f32 calls
@@ -116,17 +117,53 @@ __device__ __forceinline__ void tile_words(const uint32_t* p, uint32_t (&w)[N]) 
             const uint4 v = reinterpret_cast<const uint4*>(p)[i];
             w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
         }
+    } else if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            const uint2 v = reinterpret_cast<const uint2*>(p)[i];
+            w[2 * i] = v.x, w[2 * i + 1] = v.y;
+        }
     } else {
-        static_assert(N == 2, "two words or fours");
-        const uint2 v = *reinterpret_cast<const uint2*>(p);
-        w[0] = v.x, w[1] = v.y;
+        static_assert(N == 1, "one word, or an even number");
+        w[0] = *p;
     }
 }
 
-__device__ __forceinline__ float read_q(const void* q, int type, size_t i) {
-    if (type == kF32) return __ldg(static_cast<const float*>(q) + i);
-    const uint32_t b = __ldg(static_cast<const unsigned short*>(q) + i);
-    return type == kF16 ? to_f32<__half>(b) : to_f32<__nv_bfloat16>(b);
+// n <= 8 elements of a query from element i on; the others are 0.
+__device__ __forceinline__ void load_query8(const void* q, int type, size_t i, int n, float (&x)[8]) {
+    if (type == kF32) {
+        const float* p = static_cast<const float*>(q) + i;
+        if (n == 8 && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+            const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = e < n ? __ldg(p + e) : 0.0f;
+        }
+        return;
+    }
+    const unsigned short* p = static_cast<const unsigned short*>(q) + i;
+    uint32_t w[4];
+    if (n == 8 && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+        const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+        w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            w[e] = (2 * e < n ? __ldg(p + 2 * e) : 0u) | (2 * e + 1 < n ? (uint32_t)__ldg(p + 2 * e + 1) << 16 : 0u);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const uint32_t b = (w[e / 2] >> (16 * (e & 1))) & 0xFFFFu;
+        x[e] = type == kF16 ? to_f32<__half>(b) : to_f32<__nv_bfloat16>(b);
+    }
+}
+
+// An 8 x 8 matrix of halves, two columns of row lane / 4 per lane, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 
 __device__ __forceinline__ void write_out(void* out, int type, size_t i, float x) {
@@ -159,19 +196,18 @@ __device__ __forceinline__ int share_of(int rows, int n_split) {
     return max((rows + n_split * step - 1) / (n_split * step), 1) * step;
 }
 
-template <int G, int NC, bool F32, bool FOUND>
+template <int G, int NC, bool F32>
 struct Shape {
-    static constexpr bool kTwo = NC == 16 || F32;    // both halves of the query operand's M are used
-    static constexpr int kQ = kTwo ? 8 : 4;          // query registers per 32 dimensions
-    static constexpr int kCols = NC / 8;             // columns per thread
+    static constexpr int kNt = NC / 8;    // the MMA's N is eight columns
+    static constexpr int kCols = NC / 4;  // columns per thread
+    static constexpr int kQ = F32 ? 8 : 4;                    // query registers per 32 dimensions and eight columns
+    static constexpr bool kQShared = 2 * G * kNt * kQ > 32;   // wide queries wait in shared memory
     static constexpr float kUnit = F32 ? 1.0f : 16777216.0f;  // 1 / what a code of 1 is as an operand
-    static constexpr bool kQShared = G * kQ > 16;    // wide queries wait in shared memory
     // A warp's ring of tiles in flight. Stages x warps per SM x 1152 G bytes cover HBM's latency.
     static constexpr int kStages = G <= 2 ? 4 : 3;
     static constexpr int kTileBytes = kTile * 72 * G;
     static constexpr int kRingBytes = kAttWarps * kStages * kTileBytes;
     static constexpr int kBlocks = G == 1 && NC == 8 ? 5 : G <= 2 && NC == 8 ? 4 : G <= 2 ? 3 : 2;  // per SM
-    static_assert(!(kQShared && NC == 16), "sixteen columns keep their queries in registers");
 };
 
 // A tile in the ring: 16 rows of key codes, value codes, key parameters, value parameters. Sixteen-byte
@@ -265,13 +301,13 @@ struct Fetch {
 };
 
 template <int G, int NC, bool F32, bool FOUND>
-__global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, FOUND>::kBlocks) k_cache_attend(CacheView c, AttendKernel kk) {
-    using S = Shape<G, NC, F32, FOUND>;
-    constexpr int kCols = S::kCols, kQ = S::kQ;
+__global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_attend(CacheView c, AttendKernel kk) {
+    using S = Shape<G, NC, F32>;
+    constexpr int kNt = S::kNt, kCols = S::kCols, kQ = S::kQ;
     const AttendArgs& a = kk.a;
     __shared__ float s_o[NC][G * kCacheGroup + 4];
-    __shared__ float s_m[kAttWarps][NC], s_l[kAttWarps][NC], s_low[kAttWarps][NC][G];
-    __shared__ uint4 s_q[S::kQShared ? 2 * G * (kQ / 4) : 1][32];
+    __shared__ float s_m[kAttWarps][NC], s_l[kAttWarps][NC];
+    __shared__ uint4 s_q[S::kQShared ? 2 * G * kNt * (kQ / 4) : 1][32];
     extern __shared__ __align__(128) char s_ring[];
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gid = lane >> 2, t = lane & 3;
@@ -315,87 +351,101 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, FOUND>::kBlocks) k_c
     const uint32_t* vp = c.vp + head_row * G;
 
     for (int ct = ct0; ct * NC < cols; ct += kk.col_tiles) {
-        // ---- the columns of this thread (of the S^T layout: gid, and gid + 8) ----
-        int lim[kCols], tok[kCols], head[kCols];
+        // ---- queries: column gid of every eight, as B operands ----
+        // 2^e brings a column's largest element to [2^14, 2^15). Then
+        // score = (sum of step * acc + low * qsum) * fac, with acc and qsum in units of 2^e / kUnit.
         float fac[kCols], qsum[kCols][G];
-        uint32_t q[S::kQShared ? 1 : 2 * G][kQ];
-        uint32_t qtmp[kQ];
+        uint32_t q[S::kQShared ? 1 : kNt * 2 * G][kQ];
 #pragma unroll
-        for (int j = 0; j < kCols; ++j) {
+        for (int j = 0; j < kNt; ++j) {
             const int col = ct * NC + gid + 8 * j;
             const int i = col / a.group;
             const bool in = col < cols;
-            tok[j] = FOUND ? item : sn.first + i;
-            head[j] = h * a.group + (col - i * a.group);
-            // a found list: entries must lie below the rows the token sees; rows of the list: k
-            lim[j] = !in ? 0 : FOUND ? a.k : visible(c, a, sn.len, i);
-            const size_t qi = (size_t)tok[j] * a.q_stride + (size_t)head[j] * c.dim;
+            const size_t qi = (size_t)(FOUND ? item : sn.first + i) * a.q_stride +
+                              (size_t)(h * a.group + (col - i * a.group)) * c.dim;
             float top = 0.0f;
             bool bad = false;
-            for (int w = 0; w < 2 * G; ++w)
+            float x[2 * G][8];
+#pragma unroll
+            for (int w = 0; w < 2 * G; ++w) {
+                const int d = 32 * w + 8 * t;
+                load_query8(a.q, a.type, qi + d, in ? min(max(c.dim - d, 0), 8) : 0, x[w]);
+#pragma unroll
                 for (int n = 0; n < 8; ++n) {
-                    const int d = 32 * w + 8 * t + n;
-                    const float x = in && d < c.dim ? read_q(a.q, a.type, qi + d) : 0.0f;
-                    top = fmaxf(top, fabsf(x));
-                    bad |= !(fabsf(x) < INFINITY);
+                    top = fmaxf(top, fabsf(x[w][n]));
+                    bad |= !(fabsf(x[w][n]) < INFINITY);
                 }
+            }
             top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
             top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
             bad = (__ballot_sync(~0u, bad) >> (lane & ~3)) & 15u;
-            // 2^e brings the largest element to [2^14, 2^15)
             const int e = top > 0.0f ? min(141 - (int)(__float_as_uint(top) >> 23), 126) : 0;
-            const float up = __uint_as_float((uint32_t)max(e + 127, 1) << 23);
-            // s = (sum of step * acc + low * qsum) * fac, with acc and qsum in units of 2^e / kUnit
-            fac[j] = bad ? __uint_as_float(0x7FC00000u)
-                         : __fmul_rn(__fmul_rn(__fdiv_rn(S::kUnit, up), a.scale), kLog2e);
+            const float up = bad ? 0.0f : __uint_as_float((uint32_t)max(e + 127, 1) << 23);
+            const float f = bad ? __uint_as_float(0x7FC00000u)
+                                : __fmul_rn(__fmul_rn(__fdiv_rn(S::kUnit, up), a.scale), kLog2e);
+            float qs[G];
 #pragma unroll
-            for (int g = 0; g < G; ++g) qsum[j][g] = 0.0f;
+            for (int g = 0; g < G; ++g) qs[g] = 0.0f;
 #pragma unroll
             for (int w = 0; w < 2 * G; ++w) {
-                float x[8];
 #pragma unroll
                 for (int n = 0; n < 8; ++n) {
-                    const int d = 32 * w + 8 * t + n;
-                    x[n] = in && d < c.dim && !bad ? __fmul_rn(read_q(a.q, a.type, qi + d), up) : 0.0f;
-                    qsum[j][w / 2] = __fadd_rn(qsum[j][w / 2], x[n]);
+                    x[w][n] = bad ? 0.0f : __fmul_rn(x[w][n], up);
+                    qs[w / 2] = __fadd_rn(qs[w / 2], x[w][n]);
                 }
                 // step s of word w takes nibbles (2 s, 2 s + 4) and, 16 times as large, (2 s + 1, 2 s + 5)
+                uint32_t r[kQ];
 #pragma unroll
                 for (int st = 0; st < 2; ++st) {
-                    const float y0 = x[2 * st], y1 = x[2 * st + 4];
-                    const float z0 = 0.0625f * x[2 * st + 1], z1 = 0.0625f * x[2 * st + 5];
-                    const uint32_t r0 = pack_h2(y0, y1), r2 = pack_h2(z0, z1);
-                    uint32_t* dst = S::kQShared ? qtmp : q[S::kQShared ? 0 : w];
-                    if (F32) {
-                        dst[4 * st] = r0, dst[4 * st + 2] = r2;
-                        dst[4 * st + 1] = pack_h2(left_over(y0, r0, 0), left_over(y1, r0, 1));
-                        dst[4 * st + 3] = pack_h2(left_over(z0, r2, 0), left_over(z1, r2, 1));
-                    } else if (NC == 16) {
-                        dst[4 * st + j] = r0, dst[4 * st + 2 + j] = r2;
-                    } else {
-                        dst[2 * st] = r0, dst[2 * st + 1] = r2;
+                    const float y0 = x[w][2 * st], y1 = x[w][2 * st + 4];
+                    const float z0 = 0.0625f * x[w][2 * st + 1], z1 = 0.0625f * x[w][2 * st + 5];
+                    const uint32_t b0 = pack_h2(y0, y1), b1 = pack_h2(z0, z1);
+                    r[2 * st] = b0, r[2 * st + 1] = b1;
+                    if constexpr (F32) {
+                        r[4 + 2 * st] = pack_h2(left_over(y0, b0, 0), left_over(y1, b0, 1));
+                        r[5 + 2 * st] = pack_h2(left_over(z0, b1, 0), left_over(z1, b1, 1));
                     }
                 }
                 if constexpr (S::kQShared) {
-                    if (warp == 0) {
-                        if (kQ == 8) {
-                            s_q[2 * w][lane] = make_uint4(qtmp[0], qtmp[1], qtmp[2], qtmp[3]);
-                            s_q[2 * w + 1][lane] = make_uint4(qtmp[4], qtmp[5], qtmp[6], qtmp[7]);
-                        } else {
-                            s_q[w][lane] = make_uint4(qtmp[0], qtmp[1], qtmp[2], qtmp[3]);
-                        }
-                    }
+                    if (warp == 0)
+#pragma unroll
+                        for (int n = 0; n < kQ / 4; ++n)
+                            s_q[(w * kNt + j) * (kQ / 4) + n][lane] =
+                                make_uint4(r[4 * n], r[4 * n + 1], r[4 * n + 2], r[4 * n + 3]);
+                } else {
+#pragma unroll
+                    for (int n = 0; n < kQ; ++n) q[S::kQShared ? 0 : w * kNt + j][n] = r[n];
                 }
             }
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                qsum[j][g] = __fadd_rn(qsum[j][g], __shfl_xor_sync(~0u, qsum[j][g], 1));
-                qsum[j][g] = __fadd_rn(qsum[j][g], __shfl_xor_sync(~0u, qsum[j][g], 2));
-                qsum[j][g] = __fmul_rn(qsum[j][g], 1.0f / S::kUnit);
+                qs[g] = __fadd_rn(qs[g], __shfl_xor_sync(~0u, qs[g], 1));
+                qs[g] = __fadd_rn(qs[g], __shfl_xor_sync(~0u, qs[g], 2));
+                qs[g] = __fmul_rn(qs[g], 1.0f / S::kUnit);
+            }
+            // the scores' fragment holds columns 2t and 2t + 1
+#pragma unroll
+            for (int x2 = 0; x2 < 2; ++x2) {
+                const int from = 8 * t + 4 * x2;
+                fac[2 * j + x2] = __shfl_sync(~0u, f, from);
+#pragma unroll
+                for (int g = 0; g < G; ++g) qsum[2 * j + x2][g] = __shfl_sync(~0u, qs[g], from);
             }
         }
         if constexpr (S::kQShared) __syncthreads();
 
+        // ---- this thread's columns 8 (j / 2) + 2t + j % 2 ----
+        int lim[kCols];
+        size_t logit_at[kCols];
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) {
+            const int col = ct * NC + 8 * (j >> 1) + 2 * t + (j & 1);
+            const int i = col / a.group;
+            // of a found list every entry counts whose row the token sees
+            lim[j] = col >= cols ? 0 : FOUND ? a.k : visible(c, a, sn.len, i);
+            logit_at[j] = ((size_t)(FOUND ? item : sn.first + i) * a.q_heads + h * a.group + (col - i * a.group)) *
+                          kk.logit_rows;
+        }
         const int col_last = min(ct * NC + NC, cols) - 1;
         const int lim_first = FOUND ? 0 : visible(c, a, sn.len, ct * NC / a.group);
         const int lim_last = FOUND ? a.k : visible(c, a, sn.len, col_last / a.group);
@@ -405,7 +455,7 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, FOUND>::kBlocks) k_c
 
         // inv: what brings a step into f16's upper range, kPScale / norm, norm a power of two
         float m[kCols], l[kCols], low[kCols][G], norm[G], inv[G];
-        float o[G][4][kCols][4];
+        float o[G][4][kNt][4];
 #pragma unroll
         for (int j = 0; j < kCols; ++j) {
             m[j] = kNoMax;
@@ -419,136 +469,126 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, FOUND>::kBlocks) k_c
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int j = 0; j < kCols; ++j)
+                for (int j = 0; j < kNt; ++j)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) o[g][i][j][r] = 0.0f;
         }
 
-        // One tile of rows (or list entries) r0 ..: the scores' fragment has columns gid (and gid + 8) and
-        // rows 2t, 2t + 1, 2t + 8, 2t + 9. kEdge: some column does not see some row.
+        // One tile of rows (or list entries) r0 ..: the scores' fragment has rows gid and gid + 8 and this
+        // thread's columns. kEdge: some column does not see some row.
         auto tile_step = [&](const char* tile, int r0, auto edge) {
             constexpr bool kEdge = decltype(edge)::value;
-            bool ok[4];  // rows that some column sees
-            if constexpr (kEdge) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = r0 + 2 * t + (i & 1) + 8 * (i >> 1);
-                    ok[i] = r < lim_last;
-                    if (FOUND && ok[i]) ok[i] = __ldg(list + r) < (uint64_t)row_limit;
-                }
-            }
-            uint32_t kpw[4][G], vpw[4][G];
+            const uint32_t* par = reinterpret_cast<const uint32_t*>(tile + 1024 * G);
+            uint32_t vpw[2][G];
+            bool ok[2];  // rows that some column sees; others may hold anything
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const uint32_t* par = reinterpret_cast<const uint32_t*>(tile + 1024 * G) + (2 * t + 8 * i) * G;
-                tile_words<2 * G>(par, *reinterpret_cast<uint32_t(*)[2 * G]>(&kpw[2 * i]));
-                tile_words<2 * G>(par + kTile * G, *reinterpret_cast<uint32_t(*)[2 * G]>(&vpw[2 * i]));
-            }
-            if constexpr (kEdge) {
-                // rows that no column sees may hold anything
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
+                tile_words<G>(par + (kTile + gid + 8 * i) * G, vpw[i]);
+                if constexpr (kEdge) {
+                    const int r = r0 + gid + 8 * i;
+                    ok[i] = r < lim_last;
+                    if constexpr (FOUND) ok[i] = ok[i] && __ldg(list + r) < (uint64_t)row_limit;
 #pragma unroll
                     for (int g = 0; g < G; ++g) vpw[i][g] = ok[i] ? vpw[i][g] : 0u;
+                }
             }
 
-            // ---- scores: sc[j][i] of column j and value row i ----
-            float sc[kCols][4];
+            // ---- scores: sc[j][i] of column j and row gid + 8 i ----
+            float sc[kCols][2];
+            {
+                uint32_t w[2][2 * G], kpw[2][G];
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt) {
-                uint32_t w[2 * G];
-                if constexpr (G == 1) {
-                    tile_words<2>(reinterpret_cast<const uint32_t*>(tile) + (gid + 8 * nt) * 8 + t * 2, w);
-                } else {
+                for (int i = 0; i < 2; ++i) {
+                    tile_words<G>(par + (gid + 8 * i) * G, kpw[i]);
+                    if constexpr (G == 1) {
+                        tile_words<2>(reinterpret_cast<const uint32_t*>(tile) + (gid + 8 * i) * 8 + t * 2, w[i]);
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < G / 2; ++i)
-                        tile_words<4>(reinterpret_cast<const uint32_t*>(
-                                          tile + key_piece<G>((gid + 8 * nt) * 2 * G + i * 4 + t) * 16),
-                                      *reinterpret_cast<uint32_t(*)[4]>(&w[4 * i]));
+                        for (int x = 0; x < G / 2; ++x)
+                            tile_words<4>(reinterpret_cast<const uint32_t*>(
+                                              tile + key_piece<G>((gid + 8 * i) * 2 * G + x * 4 + t) * 16),
+                                          *reinterpret_cast<uint32_t(*)[4]>(&w[i][4 * x]));
+                    }
                 }
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int j = 0; j < kCols; ++j) sc[j][0] = sc[j][1] = 0.0f;
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    float acc[kNt][4];
+#pragma unroll
+                    for (int j = 0; j < kNt; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
 #pragma unroll
                     for (int x = 2 * g; x < 2 * g + 2; ++x) {
-                        uint32_t qq[kQ];
-                        if constexpr (S::kQShared) {
+                        uint32_t qq[kNt][kQ];
 #pragma unroll
-                            for (int i = 0; i < kQ / 4; ++i) {
-                                const uint4 v = s_q[(kQ / 4) * x + i][lane];
-                                qq[4 * i] = v.x, qq[4 * i + 1] = v.y, qq[4 * i + 2] = v.z, qq[4 * i + 3] = v.w;
+                        for (int j = 0; j < kNt; ++j) {
+                            if constexpr (S::kQShared) {
+#pragma unroll
+                                for (int n = 0; n < kQ / 4; ++n) {
+                                    const uint4 v = s_q[(x * kNt + j) * (kQ / 4) + n][lane];
+                                    qq[j][4 * n] = v.x, qq[j][4 * n + 1] = v.y;
+                                    qq[j][4 * n + 2] = v.z, qq[j][4 * n + 3] = v.w;
+                                }
+                            } else {
+#pragma unroll
+                                for (int n = 0; n < kQ; ++n) qq[j][n] = q[S::kQShared ? 0 : x * kNt + j][n];
                             }
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < kQ; ++i) qq[i] = q[x][i];
                         }
-                        const uint32_t w0 = w[x], w1 = w0 >> 8;
-                        if constexpr (S::kTwo) {
-                            mma(acc, qq[0], qq[1], qq[2], qq[3], operand<F32, false>(w0), operand<F32, true>(w0));
-                            mma(acc, qq[4], qq[5], qq[6], qq[7], operand<F32, false>(w1), operand<F32, true>(w1));
-                        } else {
-                            mma(acc, qq[0], 0u, qq[1], 0u, operand<F32, false>(w0), operand<F32, true>(w0));
-                            mma(acc, qq[2], 0u, qq[3], 0u, operand<F32, false>(w1), operand<F32, true>(w1));
+#pragma unroll
+                        for (int st = 0; st < 2; ++st) {
+                            const uint32_t w0 = w[0][x] >> (8 * st), w8 = w[1][x] >> (8 * st);
+                            const uint32_t a0 = operand<F32, false>(w0), a1 = operand<F32, false>(w8),
+                                           a2 = operand<F32, true>(w0), a3 = operand<F32, true>(w8);
+#pragma unroll
+                            for (int j = 0; j < kNt; ++j) {
+                                mma(acc[j], a0, a1, a2, a3, qq[j][2 * st], qq[j][2 * st + 1]);
+                                if constexpr (F32) mma(acc[j], a0, a1, a2, a3, qq[j][4 + 2 * st], qq[j][5 + 2 * st]);
+                            }
                         }
                     }
-                    const float st0 = par_step(kpw[2 * nt][g]), st1 = par_step(kpw[2 * nt + 1][g]);
-                    const float lo0 = low_of<F32>(kpw[2 * nt][g]), lo1 = low_of<F32>(kpw[2 * nt + 1][g]);
-                    if (F32) {  // the query's low halves
-                        acc[0] = __fadd_rn(acc[0], acc[2]);
-                        acc[1] = __fadd_rn(acc[1], acc[3]);
-                    }
 #pragma unroll
-                    for (int j = 0; j < kCols; ++j) {
-                        sum[2 * j] = __fmaf_rn(st0, acc[2 * j], __fmaf_rn(lo0, qsum[j][g], sum[2 * j]));
-                        sum[2 * j + 1] = __fmaf_rn(st1, acc[2 * j + 1], __fmaf_rn(lo1, qsum[j][g], sum[2 * j + 1]));
-                    }
-                }
+                    for (int i = 0; i < 2; ++i) {
+                        const float st = par_step(kpw[i][g]), lo = low_of<F32>(kpw[i][g]);
 #pragma unroll
-                for (int j = 0; j < kCols; ++j) {
-                    sc[j][2 * nt] = __fmul_rn(sum[2 * j], fac[j]);
-                    sc[j][2 * nt + 1] = __fmul_rn(sum[2 * j + 1], fac[j]);
+                        for (int j = 0; j < kCols; ++j)
+                            sc[j][i] = __fmaf_rn(st, acc[j >> 1][2 * i + (j & 1)], __fmaf_rn(lo, qsum[j][g], sc[j][i]));
+                    }
                 }
             }
-            bool see[kCols][4];
-            if constexpr (kEdge) {
+            bool see[kCols][2];
 #pragma unroll
-                for (int j = 0; j < kCols; ++j)
+            for (int j = 0; j < kCols; ++j)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        see[j][i] = ok[i] && r0 + 2 * t + (i & 1) + 8 * (i >> 1) < lim[j];
+                for (int i = 0; i < 2; ++i) {
+                    sc[j][i] = __fmul_rn(sc[j][i], fac[j]);
+                    if constexpr (kEdge) {
+                        see[j][i] = ok[i] && r0 + gid + 8 * i < lim[j];
                         sc[j][i] = see[j][i] ? sc[j][i] : -INFINITY;
                     }
-            }
+                }
             if (kk.logits) {
 #pragma unroll
-                for (int j = 0; j < kCols; ++j) {
-                    if (lim[j] <= 0) continue;
-                    float* lg = kk.logits + ((size_t)tok[j] * a.q_heads + head[j]) * kk.logit_rows + r0 + 2 * t;
-                    *reinterpret_cast<float2*>(lg) = make_float2(sc[j][0], sc[j][1]);
-                    *reinterpret_cast<float2*>(lg + 8) = make_float2(sc[j][2], sc[j][3]);
-                }
+                for (int j = 0; j < kCols; ++j)
+                    if (lim[j] > 0) {
+                        float* lg = kk.logits + logit_at[j] + r0 + gid;
+                        lg[0] = sc[j][0];
+                        lg[8] = sc[j][1];
+                    }
             }
 
             // ---- running maximum and the groups' power of two: rescaled only where they grow ----
-            float top[kCols];
             bool grow = false;
 #pragma unroll
-            for (int j = 0; j < kCols; ++j) {
-                top[j] = fmaxf(fmaxf(sc[j][0], sc[j][1]), fmaxf(sc[j][2], sc[j][3]));
-                grow |= top[j] > m[j] + kLag;
-            }
+            for (int j = 0; j < kCols; ++j) grow |= fmaxf(sc[j][0], sc[j][1]) > m[j] + kLag;
 #pragma unroll
-            for (int g = 0; g < G; ++g)
-                grow |= fmaxf(fmaxf(par_step(vpw[0][g]), par_step(vpw[1][g])),
-                              fmaxf(par_step(vpw[2][g]), par_step(vpw[3][g]))) > norm[g];
+            for (int g = 0; g < G; ++g) grow |= fmaxf(par_step(vpw[0][g]), par_step(vpw[1][g])) > norm[g];
             if (__any_sync(~0u, grow)) {
                 float f[kCols];
 #pragma unroll
                 for (int j = 0; j < kCols; ++j) {
-                    float x = top[j];
-                    x = fmaxf(x, __shfl_xor_sync(~0u, x, 1));
-                    x = fmaxf(x, __shfl_xor_sync(~0u, x, 2));
+                    float x = fmaxf(sc[j][0], sc[j][1]);
+#pragma unroll
+                    for (int d = 4; d < 32; d *= 2) x = fmaxf(x, __shfl_xor_sync(~0u, x, d));
                     const float mn = fmaxf(m[j], x);
                     f[j] = ex2(m[j] - mn);
                     m[j] = mn;
@@ -556,23 +596,13 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, FOUND>::kBlocks) k_c
 #pragma unroll
                     for (int g = 0; g < G; ++g) low[j][g] = __fmul_rn(low[j][g], f[j]);
                 }
-                // the O^T layout holds columns 2t and 2t + 1
-                float fo[kCols][2];
-#pragma unroll
-                for (int j = 0; j < kCols; ++j) {
-                    fo[j][0] = __shfl_sync(~0u, f[j], 8 * t);
-                    fo[j][1] = __shfl_sync(~0u, f[j], 8 * t + 4);
-                }
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    float x = 0.0f;  // a row with an infinite step is NaN whatever its scale
+                    // a row with an infinite step is NaN whatever its scale
+                    const float s0 = par_step(vpw[0][g]), s1 = par_step(vpw[1][g]);
+                    float x = fmaxf(s0 < INFINITY ? s0 : 0.0f, s1 < INFINITY ? s1 : 0.0f);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float st = par_step(vpw[i][g]);
-                        x = st < INFINITY ? fmaxf(x, st) : x;
-                    }
-                    x = fmaxf(x, __shfl_xor_sync(~0u, x, 1));
-                    x = fmaxf(x, __shfl_xor_sync(~0u, x, 2));
+                    for (int d = 4; d < 32; d *= 2) x = fmaxf(x, __shfl_xor_sync(~0u, x, d));
                     float ratio = 1.0f;
                     if (x > norm[g]) {
                         // a power of two at or above the step, at least 2^-100
@@ -584,23 +614,23 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, FOUND>::kBlocks) k_c
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
-                        for (int j = 0; j < kCols; ++j)
+                        for (int j = 0; j < kNt; ++j)
 #pragma unroll
                             for (int r = 0; r < 4; ++r)
-                                o[g][i][j][r] = __fmul_rn(o[g][i][j][r], __fmul_rn(fo[j][r & 1], ratio));
+                                o[g][i][j][r] = __fmul_rn(o[g][i][j][r], __fmul_rn(f[2 * j + (r & 1)], ratio));
                 }
             }
 
-            float p[kCols][4];
+            float p[kCols][2];
 #pragma unroll
             for (int j = 0; j < kCols; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < 2; ++i) {
                     p[j][i] = ex2(__fsub_rn(sc[j][i], m[j]));
                     l[j] = __fadd_rn(l[j], p[j][i]);
                 }
 
-            // ---- values ----
+            // ---- values: rows 2t, 2t + 1, 2t + 8, 2t + 9, words gid of every group ----
             uint32_t vw[4][G];
             const char* vt = tile + 512 * G;
 #pragma unroll
@@ -619,27 +649,33 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, FOUND>::kBlocks) k_c
             }
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                float ps[kCols][4];
+                // p * step of (row, columns 2t, 2t + 1), then transposed: (column gid, rows 2t, 2t + 1)
+                uint32_t b[kNt][2], c2[kNt][2];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < 2; ++i) {
                     const float st = __fmul_rn(par_step(vpw[i][g]), inv[g]), lo = low_of<F32>(vpw[i][g]);
 #pragma unroll
-                    for (int j = 0; j < kCols; ++j) {
-                        ps[j][i] = __fmul_rn(p[j][i], st);
-                        if constexpr (kEdge) {
-                            // a row the column does not see adds nothing, whatever it holds
-                            ps[j][i] = see[j][i] ? ps[j][i] : 0.0f;
-                            if (see[j][i]) low[j][g] = __fmaf_rn(p[j][i], lo, low[j][g]);
-                        } else {
-                            low[j][g] = __fmaf_rn(p[j][i], lo, low[j][g]);
+                    for (int j = 0; j < kNt; ++j) {
+                        float ps[2];
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            ps[x] = __fmul_rn(p[2 * j + x][i], st);
+                            float& lw = low[2 * j + x][g];
+                            if constexpr (kEdge) {
+                                // a row the column does not see adds nothing, whatever it holds
+                                ps[x] = see[2 * j + x][i] ? ps[x] : 0.0f;
+                                lw = see[2 * j + x][i] ? __fmaf_rn(p[2 * j + x][i], lo, lw) : lw;
+                            } else {
+                                lw = __fmaf_rn(p[2 * j + x][i], lo, lw);
+                            }
                         }
+                        b[j][i] = pack_h2(ps[0], ps[1]);
+                        if constexpr (F32) c2[j][i] = transpose8(pack_h2(left_over(ps[0], b[j][i], 0), left_over(ps[1], b[j][i], 1)));
+                        b[j][i] = transpose8(b[j][i]);
                     }
                 }
                 const uint32_t u0 = __byte_perm(vw[0][g], vw[1][g], 0x5410), h0 = __byte_perm(vw[0][g], vw[1][g], 0x7632);
                 const uint32_t u8 = __byte_perm(vw[2][g], vw[3][g], 0x5410), h8 = __byte_perm(vw[2][g], vw[3][g], 0x7632);
-                uint32_t b0[kCols], b1[kCols];
-#pragma unroll
-                for (int j = 0; j < kCols; ++j) b0[j] = pack_h2(ps[j][0], ps[j][1]), b1[j] = pack_h2(ps[j][2], ps[j][3]);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int sh = 8 * i;
@@ -648,14 +684,12 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, FOUND>::kBlocks) k_c
                     const uint32_t d0 = operand<F32, true>(u0 >> sh), d1 = operand<F32, true>(h0 >> sh),
                                    d2 = operand<F32, true>(u8 >> sh), d3 = operand<F32, true>(h8 >> sh);
 #pragma unroll
-                    for (int j = 0; j < kCols; ++j) {
-                        mma(o[g][2 * i][j], e0, e1, e2, e3, b0[j], b1[j]);
-                        mma(o[g][2 * i + 1][j], d0, d1, d2, d3, b0[j], b1[j]);
-                        if (F32) {
-                            const uint32_t c0 = pack_h2(left_over(ps[j][0], b0[j], 0), left_over(ps[j][1], b0[j], 1));
-                            const uint32_t c1 = pack_h2(left_over(ps[j][2], b1[j], 0), left_over(ps[j][3], b1[j], 1));
-                            mma(o[g][2 * i][j], e0, e1, e2, e3, c0, c1);
-                            mma(o[g][2 * i + 1][j], d0, d1, d2, d3, c0, c1);
+                    for (int j = 0; j < kNt; ++j) {
+                        mma(o[g][2 * i][j], e0, e1, e2, e3, b[j][0], b[j][1]);
+                        mma(o[g][2 * i + 1][j], d0, d1, d2, d3, b[j][0], b[j][1]);
+                        if constexpr (F32) {
+                            mma(o[g][2 * i][j], e0, e1, e2, e3, c2[j][0], c2[j][1]);
+                            mma(o[g][2 * i + 1][j], d0, d1, d2, d3, c2[j][0], c2[j][1]);
                         }
                     }
                 }
@@ -692,21 +726,21 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, FOUND>::kBlocks) k_c
         // ---- the block's warps joined ----
 #pragma unroll
         for (int j = 0; j < kCols; ++j) {
-            l[j] = __fadd_rn(l[j], __shfl_xor_sync(~0u, l[j], 1));
-            l[j] = __fadd_rn(l[j], __shfl_xor_sync(~0u, l[j], 2));
+            const int col = 8 * (j >> 1) + 2 * t + (j & 1);
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-                low[j][g] = __fadd_rn(low[j][g], __shfl_xor_sync(~0u, low[j][g], 1));
-                low[j][g] = __fadd_rn(low[j][g], __shfl_xor_sync(~0u, low[j][g], 2));
-                if (t == 0) s_low[warp][gid + 8 * j][g] = low[j][g];
-            }
-            if (t == 0) s_m[warp][gid + 8 * j] = m[j], s_l[warp][gid + 8 * j] = l[j];
+            for (int d = 4; d < 32; d *= 2) l[j] = __fadd_rn(l[j], __shfl_xor_sync(~0u, l[j], d));
+            if (gid == 0) s_m[warp][col] = m[j], s_l[warp][col] = l[j];
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int d = 4; d < 32; d *= 2)
+                    low[j][g] = __fadd_rn(low[j][g], __shfl_xor_sync(~0u, low[j][g], d));
         }
         __syncthreads();
         for (int w = 0; w < kAttWarps; ++w) {
             if (warp == w) {
 #pragma unroll
-                for (int j = 0; j < kCols; ++j)
+                for (int j = 0; j < kNt; ++j)
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         const int col = 8 * j + 2 * t + x;
@@ -716,7 +750,7 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, FOUND>::kBlocks) k_c
                         const float f = ex2(s_m[w][col] - mx);
 #pragma unroll
                         for (int g = 0; g < G; ++g) {
-                            const float lw = s_low[w][col][g];
+                            const float lw = low[2 * j + x][g];
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -910,7 +944,7 @@ AttendPlan make_plan(const CacheView& c, const AttendArgs& a) {
 
 template <int G, int NC, bool F32>
 void start(const CacheView& c, const AttendKernel& k, bool found, unsigned grid, cudaStream_t st) {
-    constexpr int smem = Shape<G, NC, F32, false>::kRingBytes;
+    constexpr int smem = Shape<G, NC, F32>::kRingBytes;
     const auto kernel = found ? k_cache_attend<G, NC, F32, true> : k_cache_attend<G, NC, F32, false>;
     set_smem((const void*)kernel, smem);
     kernel<<<grid, kAttBS, smem, st>>>(c, k);
