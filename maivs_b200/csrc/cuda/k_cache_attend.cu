@@ -73,10 +73,16 @@ __device__ __forceinline__ float ex2(float x) {
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                     uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same onto zeros.
+__device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                          uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 // Codes as f16 operands: of each half of w, nibble kOdd (of the low two). 16-bit calls take them as
@@ -516,8 +522,6 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
                 for (int g = 0; g < G; ++g) {
                     float acc[kNt][4];
 #pragma unroll
-                    for (int j = 0; j < kNt; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
-#pragma unroll
                     for (int x = 2 * g; x < 2 * g + 2; ++x) {
                         uint32_t qq[kNt][kQ];
 #pragma unroll
@@ -541,7 +545,10 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
                                            a2 = operand<F32, true>(w0), a3 = operand<F32, true>(w8);
 #pragma unroll
                             for (int j = 0; j < kNt; ++j) {
-                                mma(acc[j], a0, a1, a2, a3, qq[j][2 * st], qq[j][2 * st + 1]);
+                                if (x == 2 * g && st == 0)
+                                    mma_first(acc[j], a0, a1, a2, a3, qq[j][0], qq[j][1]);
+                                else
+                                    mma(acc[j], a0, a1, a2, a3, qq[j][2 * st], qq[j][2 * st + 1]);
                                 if constexpr (F32) mma(acc[j], a0, a1, a2, a3, qq[j][4 + 2 * st], qq[j][5 + 2 * st]);
                             }
                         }
