@@ -167,7 +167,7 @@ int maivs_cache_new(size_t n_seqs, size_t capacity, size_t n_heads, size_t dim, 
         v.dim = (int)dim;
         v.G = maivs::dev::cache_groups((int)dim);
         v.capacity = (int)capacity;
-        v.rows = (int)((capacity + 15) / 16 * 16);
+        v.rows = (int)((capacity + 31) / 32 * 32);
         const size_t rows = n_seqs * n_heads * (size_t)v.rows;
         if (rows > (size_t(1) << 40)) return cfail(cx, MAIVS_BAD_ARG, "the cache would have more than 2^40 rows");
         const size_t codes = rows * 32 * v.G, params = rows * 4 * v.G;

@@ -31,7 +31,7 @@ struct CacheView {
     uint32_t* flags;
     int n_seqs, heads, dim, G;
     int capacity;  // rows a sequence may hold
-    int rows;      // capacity rounded up to 16: rows allocated
+    int rows;      // capacity rounded up to 32: rows allocated, since tiles are read whole
 };
 
 // bits of the device flags

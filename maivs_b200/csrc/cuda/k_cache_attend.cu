@@ -37,7 +37,9 @@ namespace {
 
 constexpr int kAttWarps = 4;
 constexpr int kAttBS = kAttWarps * 32;
-constexpr int kTile = 16;
+constexpr int kTile = 16;       // rows of one MMA
+// Tiles of 16 rows that a warp takes together.
+__host__ __device__ constexpr int sub_tiles(int G) { return G <= 2 ? 2 : 1; }
 constexpr int kJoinBS = 128;
 constexpr int kMaxSplit = 1024;
 constexpr float kNoMax = -3.0e38f;
@@ -197,8 +199,8 @@ __device__ __forceinline__ int visible(const CacheView& c, const AttendArgs& a, 
     return min(min(len + (a.causal ? i + 1 : 0), c.capacity), a.max_rows);
 }
 // Rows per split: an equal share, in whole passes of the block's warps.
-__device__ __forceinline__ int share_of(int rows, int n_split) {
-    const int step = kAttWarps * kTile;
+__device__ __forceinline__ int share_of(int rows, int n_split, int G) {
+    const int step = kAttWarps * kTile * sub_tiles(G);
     return max((rows + n_split * step - 1) / (n_split * step), 1) * step;
 }
 
@@ -210,8 +212,10 @@ struct Shape {
     static constexpr bool kQShared = 2 * G * kNt * kQ > 32;   // wide queries wait in shared memory
     static constexpr float kUnit = F32 ? 1.0f : 16777216.0f;  // 1 / what a code of 1 is as an operand
     // A warp's ring of tiles in flight. Stages x warps per SM x 1152 G bytes cover HBM's latency.
-    static constexpr int kStages = G <= 2 ? 4 : 3;
-    static constexpr int kTileBytes = kTile * 72 * G;
+    static constexpr int kSub = sub_tiles(G);  // tiles of 16 rows that go through a step together
+    static constexpr int kRows = kSub * kTile;
+    static constexpr int kStages = G <= 2 ? 2 : 3;
+    static constexpr int kTileBytes = kRows * 72 * G;
     static constexpr int kRingBytes = kAttWarps * kStages * kTileBytes;
     static constexpr int kBlocks = G == 1 && NC == 8 ? 5 : G <= 2 && NC == 8 ? 4 : G <= 2 ? 3 : 2;  // per SM
 };
@@ -241,9 +245,11 @@ __device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
 // tile, so its three source addresses only advance. Found rows: the list names each piece's row.
 template <int G, bool FOUND>
 struct Fetch {
-    static constexpr int kParams = (8 * G + 31) / 32;  // rounds of parameter pieces (keys' then values')
+    static constexpr int kSub = sub_tiles(G), kRows = kSub * kTile;
+    static constexpr int kCodes = kSub * G;                   // rounds of 32 code pieces
+    static constexpr int kParams = (8 * G * kSub + 31) / 32;  // rounds of parameter pieces (keys' then values')
+    static constexpr int kHalf = 4 * G * kSub;                // parameter pieces of the keys
     const char *ks, *vs, *ps[kParams];
-    uint32_t kd[G], vd[G];
     const uint64_t* list;
     int k, row_limit, lane;
 
@@ -253,22 +259,15 @@ struct Fetch {
         list = l, k = k_, row_limit = limit;
         if constexpr (FOUND) {
             ks = reinterpret_cast<const char*>(kc), vs = reinterpret_cast<const char*>(vc);
-            ps[0] = reinterpret_cast<const char*>(kp);
-            if constexpr (kParams > 1) ps[1] = reinterpret_cast<const char*>(vp);
         } else {
             ks = reinterpret_cast<const char*>(kc) + ((size_t)r0 * 2 * G + lane) * 16;
             vs = reinterpret_cast<const char*>(vc) + ((size_t)r0 * 2 * G + lane) * 16;
 #pragma unroll
             for (int i = 0; i < kParams; ++i) {
                 const int q = lane + 32 * i;
-                ps[i] = q < 4 * G ? reinterpret_cast<const char*>(kp + (size_t)r0 * G) + q * 16
-                                  : reinterpret_cast<const char*>(vp + (size_t)r0 * G) + (q - 4 * G) * 16;
+                ps[i] = q < kHalf ? reinterpret_cast<const char*>(kp + (size_t)r0 * G) + q * 16
+                                  : reinterpret_cast<const char*>(vp + (size_t)r0 * G) + (q - kHalf) * 16;
             }
-        }
-#pragma unroll
-        for (int i = 0; i < G; ++i) {
-            kd[i] = key_piece<G>(lane + 32 * i) * 16;
-            vd[i] = 512 * G + value_piece<G>(lane + 32 * i) * 16;
         }
     }
     __device__ __forceinline__ size_t row(int e) const {
@@ -277,31 +276,34 @@ struct Fetch {
     }
     // The tile of rows (or list entries) r0 ..; pointers move on by the warps' stride.
     __device__ __forceinline__ void next(uint32_t tile, int r0, const uint32_t* kp, const uint32_t* vp) {
-        if constexpr (FOUND) {
 #pragma unroll
-            for (int i = 0; i < G; ++i) {
-                const int p = lane + 32 * i, r = p / (2 * G);
-                const size_t at = (row(r0 + r) * 2 * G + (p - r * 2 * G)) * 16;
-                copy16(tile + kd[i], ks + at);
-                copy16(tile + vd[i], vs + at);
+        for (int i = 0; i < kCodes; ++i) {
+            const int p = lane + 32 * i;
+            size_t at = 512 * i;
+            if constexpr (FOUND) {
+                const int r = p / (2 * G);
+                at = (row(r0 + r) * 2 * G + (p - r * 2 * G)) * 16;
             }
-            // a row's parameters are 4 G bytes: lane r brings row r's of the keys, lane r + 16 of the values
-            const uint32_t* src = (lane < 16 ? kp : vp) + row(r0 + (lane & 15)) * G;
+            copy16(tile + key_piece<G>(p) * 16, ks + at);
+            copy16(tile + 32 * G * kRows + value_piece<G>(p) * 16, vs + at);
+        }
+        if constexpr (FOUND) {
+            // a row's parameters are 4 G bytes of the keys and as many of the values
 #pragma unroll
-            for (int i = 0; i < G; ++i) copy4(tile + 1024 * G + (lane * G + i) * 4, src + i);
+            for (int y = 0; y < kSub; ++y) {
+                const int r = lane + 32 * y;  // the keys' rows, then the values'
+                const uint32_t* src = (r < kRows ? kp : vp) + row(r0 + (r < kRows ? r : r - kRows)) * G;
+#pragma unroll
+                for (int i = 0; i < G; ++i) copy4(tile + 64 * G * kRows + (r * G + i) * 4, src + i);
+            }
         } else {
 #pragma unroll
-            for (int i = 0; i < G; ++i) {
-                copy16(tile + kd[i], ks + 512 * i);
-                copy16(tile + vd[i], vs + 512 * i);
-            }
-#pragma unroll
             for (int i = 0; i < kParams; ++i) {
-                if (lane + 32 * i < 8 * G) copy16(tile + 1024 * G + (lane + 32 * i) * 16, ps[i]);
-                ps[i] += kAttWarps * kTile * 4 * G;
+                if (lane + 32 * i < 2 * kHalf) copy16(tile + 64 * G * kRows + (lane + 32 * i) * 16, ps[i]);
+                ps[i] += kAttWarps * kRows * 4 * G;
             }
-            ks += kAttWarps * kTile * 32 * G;
-            vs += kAttWarps * kTile * 32 * G;
+            ks += kAttWarps * kRows * 32 * G;
+            vs += kAttWarps * kRows * 32 * G;
         }
     }
 };
@@ -309,7 +311,7 @@ struct Fetch {
 template <int G, int NC, bool F32, bool FOUND>
 __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_attend(CacheView c, AttendKernel kk) {
     using S = Shape<G, NC, F32>;
-    constexpr int kNt = S::kNt, kCols = S::kCols, kQ = S::kQ;
+    constexpr int kNt = S::kNt, kCols = S::kCols, kQ = S::kQ, kR = 2 * S::kSub;
     const AttendArgs& a = kk.a;
     __shared__ float s_o[NC][G * kCacheGroup + 4];
     __shared__ float s_m[kAttWarps][NC], s_l[kAttWarps][NC];
@@ -346,7 +348,7 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
                 atomicOr(c.flags, kCacheTooLong);
         }
     }
-    const int share = share_of(rows_all, kk.n_split);
+    const int share = share_of(rows_all, kk.n_split, G);
     const int start = sp * share;
     if (start >= rows_all && sp > 0) return;
 
@@ -480,16 +482,16 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
                     for (int r = 0; r < 4; ++r) o[g][i][j][r] = 0.0f;
         }
 
-        // One tile of rows (or list entries) r0 ..: the scores' fragment has rows gid and gid + 8 and this
-        // thread's columns. kEdge: some column does not see some row.
+        // One step of rows (or list entries) r0 ..: kSub times 16 of them. The scores' fragments have rows
+        // gid + 8 i (i < 2 kSub) and this thread's columns. kEdge: some column does not see some row.
         auto tile_step = [&](const char* tile, int r0, auto edge) {
             constexpr bool kEdge = decltype(edge)::value;
-            const uint32_t* par = reinterpret_cast<const uint32_t*>(tile + 1024 * G);
-            uint32_t vpw[2][G];
-            bool ok[2];  // rows that some column sees; others may hold anything
+            const uint32_t* par = reinterpret_cast<const uint32_t*>(tile + 64 * G * S::kRows);
+            uint32_t vpw[kR][G];
+            bool ok[kR];  // rows that some column sees; others may hold anything
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                tile_words<G>(par + (kTile + gid + 8 * i) * G, vpw[i]);
+            for (int i = 0; i < kR; ++i) {
+                tile_words<G>(par + (S::kRows + gid + 8 * i) * G, vpw[i]);
                 if constexpr (kEdge) {
                     const int r = r0 + gid + 8 * i;
                     ok[i] = r < lim_last;
@@ -500,24 +502,26 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
             }
 
             // ---- scores: sc[j][i] of column j and row gid + 8 i ----
-            float sc[kCols][2];
-            {
+            float sc[kCols][kR];
+#pragma unroll
+            for (int u = 0; u < S::kSub; ++u) {
                 uint32_t w[2][2 * G], kpw[2][G];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    tile_words<G>(par + (gid + 8 * i) * G, kpw[i]);
+                    const int r = gid + 16 * u + 8 * i;
+                    tile_words<G>(par + r * G, kpw[i]);
                     if constexpr (G == 1) {
-                        tile_words<2>(reinterpret_cast<const uint32_t*>(tile) + (gid + 8 * i) * 8 + t * 2, w[i]);
+                        tile_words<2>(reinterpret_cast<const uint32_t*>(tile) + r * 8 + t * 2, w[i]);
                     } else {
 #pragma unroll
                         for (int x = 0; x < G / 2; ++x)
                             tile_words<4>(reinterpret_cast<const uint32_t*>(
-                                              tile + key_piece<G>((gid + 8 * i) * 2 * G + x * 4 + t) * 16),
+                                              tile + key_piece<G>(r * 2 * G + x * 4 + t) * 16),
                                           *reinterpret_cast<uint32_t(*)[4]>(&w[i][4 * x]));
                     }
                 }
 #pragma unroll
-                for (int j = 0; j < kCols; ++j) sc[j][0] = sc[j][1] = 0.0f;
+                for (int j = 0; j < kCols; ++j) sc[j][2 * u] = sc[j][2 * u + 1] = 0.0f;
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
                     float acc[kNt][4];
@@ -558,15 +562,16 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
                         const float st = par_step(kpw[i][g]), lo = low_of<F32>(kpw[i][g]);
 #pragma unroll
                         for (int j = 0; j < kCols; ++j)
-                            sc[j][i] = __fmaf_rn(st, acc[j >> 1][2 * i + (j & 1)], __fmaf_rn(lo, qsum[j][g], sc[j][i]));
+                            sc[j][2 * u + i] = __fmaf_rn(st, acc[j >> 1][2 * i + (j & 1)],
+                                                         __fmaf_rn(lo, qsum[j][g], sc[j][2 * u + i]));
                     }
                 }
             }
-            bool see[kCols][2];
+            bool see[kCols][kR];
 #pragma unroll
             for (int j = 0; j < kCols; ++j)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
+                for (int i = 0; i < kR; ++i) {
                     sc[j][i] = __fmul_rn(sc[j][i], fac[j]);
                     if constexpr (kEdge) {
                         see[j][i] = ok[i] && r0 + gid + 8 * i < lim[j];
@@ -578,22 +583,33 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
                 for (int j = 0; j < kCols; ++j)
                     if (lim[j] > 0) {
                         float* lg = kk.logits + logit_at[j] + r0 + gid;
-                        lg[0] = sc[j][0];
-                        lg[8] = sc[j][1];
+#pragma unroll
+                        for (int i = 0; i < kR; ++i) lg[8 * i] = sc[j][i];
                     }
             }
 
             // ---- running maximum and the groups' power of two: rescaled only where they grow ----
+            float top[kCols], big[G];
             bool grow = false;
 #pragma unroll
-            for (int j = 0; j < kCols; ++j) grow |= fmaxf(sc[j][0], sc[j][1]) > m[j] + kLag;
+            for (int j = 0; j < kCols; ++j) {
+                top[j] = sc[j][0];
 #pragma unroll
-            for (int g = 0; g < G; ++g) grow |= fmaxf(par_step(vpw[0][g]), par_step(vpw[1][g])) > norm[g];
+                for (int i = 1; i < kR; ++i) top[j] = fmaxf(top[j], sc[j][i]);
+                grow |= top[j] > m[j] + kLag;
+            }
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                big[g] = par_step(vpw[0][g]);
+#pragma unroll
+                for (int i = 1; i < kR; ++i) big[g] = fmaxf(big[g], par_step(vpw[i][g]));
+                grow |= big[g] > norm[g];
+            }
             if (__any_sync(~0u, grow)) {
                 float f[kCols];
 #pragma unroll
                 for (int j = 0; j < kCols; ++j) {
-                    float x = fmaxf(sc[j][0], sc[j][1]);
+                    float x = top[j];
 #pragma unroll
                     for (int d = 4; d < 32; d *= 2) x = fmaxf(x, __shfl_xor_sync(~0u, x, d));
                     const float mn = fmaxf(m[j], x);
@@ -606,8 +622,12 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
                     // a row with an infinite step is NaN whatever its scale
-                    const float s0 = par_step(vpw[0][g]), s1 = par_step(vpw[1][g]);
-                    float x = fmaxf(s0 < INFINITY ? s0 : 0.0f, s1 < INFINITY ? s1 : 0.0f);
+                    float x = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < kR; ++i) {
+                        const float st = par_step(vpw[i][g]);
+                        x = st < INFINITY ? fmaxf(x, st) : x;
+                    }
 #pragma unroll
                     for (int d = 4; d < 32; d *= 2) x = fmaxf(x, __shfl_xor_sync(~0u, x, d));
                     float ratio = 1.0f;
@@ -628,21 +648,23 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
                 }
             }
 
-            float p[kCols][2];
+            float p[kCols][kR];
 #pragma unroll
             for (int j = 0; j < kCols; ++j)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
+                for (int i = 0; i < kR; ++i) {
                     p[j][i] = ex2(__fsub_rn(sc[j][i], m[j]));
                     l[j] = __fadd_rn(l[j], p[j][i]);
                 }
 
-            // ---- values: rows 2t, 2t + 1, 2t + 8, 2t + 9, words gid of every group ----
+            // ---- values: rows 2t, 2t + 1, 2t + 8, 2t + 9 of every 16, words gid of every group ----
+#pragma unroll
+            for (int u = 0; u < S::kSub; ++u) {
             uint32_t vw[4][G];
-            const char* vt = tile + 512 * G;
+            const char* vt = tile + 32 * G * S::kRows;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int r = 2 * t + (i & 1) + 8 * (i >> 1);
+                const int r = 16 * u + 2 * t + (i & 1) + 8 * (i >> 1);
                 if constexpr (G == 1) {
                     vw[i][0] = *reinterpret_cast<const uint32_t*>(vt + value_piece<G>(r * 2 + (gid >> 2)) * 16 +
                                                                   (gid & 3) * 4);
@@ -660,20 +682,20 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
                 uint32_t b[kNt][2], c2[kNt][2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const float st = __fmul_rn(par_step(vpw[i][g]), inv[g]), lo = low_of<F32>(vpw[i][g]);
+                    const float st = __fmul_rn(par_step(vpw[2 * u + i][g]), inv[g]), lo = low_of<F32>(vpw[2 * u + i][g]);
 #pragma unroll
                     for (int j = 0; j < kNt; ++j) {
                         float ps[2];
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
-                            ps[x] = __fmul_rn(p[2 * j + x][i], st);
+                            ps[x] = __fmul_rn(p[2 * j + x][2 * u + i], st);
                             float& lw = low[2 * j + x][g];
                             if constexpr (kEdge) {
                                 // a row the column does not see adds nothing, whatever it holds
-                                ps[x] = see[2 * j + x][i] ? ps[x] : 0.0f;
-                                lw = see[2 * j + x][i] ? __fmaf_rn(p[2 * j + x][i], lo, lw) : lw;
+                                ps[x] = see[2 * j + x][2 * u + i] ? ps[x] : 0.0f;
+                                lw = see[2 * j + x][2 * u + i] ? __fmaf_rn(p[2 * j + x][2 * u + i], lo, lw) : lw;
                             } else {
-                                lw = __fmaf_rn(p[2 * j + x][i], lo, lw);
+                                lw = __fmaf_rn(p[2 * j + x][2 * u + i], lo, lw);
                             }
                         }
                         b[j][i] = pack_h2(ps[0], ps[1]);
@@ -701,28 +723,30 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
                     }
                 }
             }
+            }
         };
 
         char* ring = s_ring + warp * S::kStages * S::kTileBytes;
         const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
-        constexpr int kStride = kAttWarps * kTile;
+        constexpr int kStride = kAttWarps * S::kRows;
+        const int mine = start + warp * S::kRows;
         Fetch<G, FOUND> fetch;
-        fetch.init(kc, vc, kp, vp, start + warp * kTile, lane, list, a.k, row_limit);
+        fetch.init(kc, vc, kp, vp, mine, lane, list, a.k, row_limit);
 #pragma unroll
         for (int i = 0; i < S::kStages - 1; ++i) {
-            const int r = start + warp * kTile + i * kStride;
+            const int r = mine + i * kStride;
             if (r < end) fetch.next(ring_at + i * S::kTileBytes, r, kp, vp);
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
         int at = 0, to = (S::kStages - 1) * S::kTileBytes;  // this tile's place, and that of the one to fetch
-        for (int r0 = start + warp * kTile; r0 < end; r0 += kStride) {
+        for (int r0 = mine; r0 < end; r0 += kStride) {
             // the tile is there, and every lane is done with the one before, whose place is filled next
             asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
             __syncwarp();
             const int r = r0 + (S::kStages - 1) * kStride;
             if (r < end) fetch.next(ring_at + to, r, kp, vp);
             asm volatile("cp.async.commit_group;" ::: "memory");
-            if (FOUND || r0 + kTile > lim_first)
+            if (FOUND || r0 + S::kRows > lim_first)
                 tile_step(ring + at, r0, std::true_type());
             else
                 tile_step(ring + at, r0, std::integral_constant<bool, FOUND>());
@@ -824,7 +848,7 @@ __global__ void __launch_bounds__(kJoinBS) k_cache_join(CacheView c, AttendKerne
     const Span sn = span_of(c, a, s);
     if (sn.count == 0) return;
     const int rows = FOUND ? a.k : visible(c, a, sn.len, sn.count - 1);
-    const int share = share_of(rows, kk.n_split);
+    const int share = share_of(rows, kk.n_split, c.G);
     const int used = max(1, (rows + share - 1) / share);
     const size_t step = (size_t)a.tok.n_tokens * a.q_heads;
     float m = kNoMax, l = 0.0f;
@@ -928,7 +952,7 @@ AttendPlan make_plan(const CacheView& c, const AttendArgs& a) {
     p.col_tiles = (int)((cols + p.nc - 1) / p.nc);
     const long long items = (long long)(found ? a.tok.n_tokens : c.n_seqs) * c.heads * p.col_tiles;
     const int rows = std::max(1, found ? a.k : std::min(a.max_rows, c.capacity));
-    const int most = (rows + kAttWarps * kTile - 1) / (kAttWarps * kTile);
+    const int step = kAttWarps * kTile * sub_tiles(c.G), most = (rows + step - 1) / step;
     const long long want = 4ll * sm_count();
     p.n_split = (int)std::max<long long>(1, std::min<long long>(std::min(most, kMaxSplit), (want + items - 1) / std::max(1ll, items)));
     const size_t th = (size_t)a.tok.n_tokens * a.q_heads;
@@ -938,7 +962,7 @@ AttendPlan make_plan(const CacheView& c, const AttendArgs& a) {
         p.off_o = off;
         off += up256(th * p.n_split * c.dim * sizeof(float));
     }
-    p.logit_rows = (rows + kAttWarps * kTile - 1) / (kAttWarps * kTile) * (kAttWarps * kTile);
+    p.logit_rows = most * step;
     if (a.w_out) {
         p.off_lse = off;
         off += up256(th * sizeof(float));

@@ -21,8 +21,8 @@ def cache():
 def test_sizes(cache):
     st = cache.stats()
     assert st["row_bytes"] == 144.0 and st["capacity"] == 100.0 and st["device"] == -1.0
-    # 112 rows (capacity rounded up to 16) of 3 sequences and 2 heads
-    assert st["device_bytes"] == 3 * 2 * 112 * 144 + 256
+    # 128 rows (capacity rounded up to 32) of 3 sequences and 2 heads
+    assert st["device_bytes"] == 3 * 2 * 128 * 144 + 256
     one = cache.attend_workspace(3, 4)
     assert cache.attend_workspace(3, 4, weights=True) > one
     assert cache.attend_found_workspace(3, 4, 10) > 0
