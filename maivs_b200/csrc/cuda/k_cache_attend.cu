@@ -42,6 +42,7 @@ constexpr int kTile = 16;       // rows of one MMA
 __host__ __device__ constexpr int sub_tiles(int G) { return G <= 2 ? 2 : 1; }
 constexpr int kJoinBS = 128;
 constexpr int kMaxSplit = 1024;
+constexpr int kWaves = 4;
 constexpr float kNoMax = -3.0e38f;
 constexpr float kLog2e = 1.4426950408889634f;
 // p * step goes into f16 scaled so that the group's largest step becomes 2^12: an old maximum may
@@ -52,7 +53,8 @@ constexpr float kPScale = 4096.0f;
 struct AttendPlan {
     int nc;         // columns per tile
     int col_tiles;  // of one sequence and head (or token and head)
-    int n_split;    // blocks that share one sequence's rows
+    int share;      // rows of one block
+    int n_split;    // blocks that share the longest sequence's rows
     size_t off_o, off_lse, off_logit, bytes;
     int logit_rows;
 };
@@ -64,7 +66,7 @@ struct AttendKernel {
     float* lse2;      // [token][q_head], log2; null without weights
     float* logits;    // [token][q_head][logit_rows], log2; null without weights
     int logit_rows;
-    int n_split, col_tiles;
+    int share, n_split, col_tiles;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -198,11 +200,8 @@ __device__ __forceinline__ Span span_of(const CacheView& c, const AttendArgs& a,
 __device__ __forceinline__ int visible(const CacheView& c, const AttendArgs& a, int len, int i) {
     return min(min(len + (a.causal ? i + 1 : 0), c.capacity), a.max_rows);
 }
-// Rows per split: an equal share, in whole passes of the block's warps.
-__device__ __forceinline__ int share_of(int rows, int n_split, int G) {
-    const int step = kAttWarps * kTile * sub_tiles(G);
-    return max((rows + n_split * step - 1) / (n_split * step), 1) * step;
-}
+// Blocks per SM that the registers of a variant are held to.
+__host__ __device__ constexpr int blocks_of(int G, int nc) { return nc == 16 || G > 2 ? 2 : G == 2 ? 3 : 5; }
 
 template <int G, int NC, bool F32>
 struct Shape {
@@ -214,10 +213,10 @@ struct Shape {
     // A warp's ring of tiles in flight. Stages x warps per SM x 1152 G bytes cover HBM's latency.
     static constexpr int kSub = sub_tiles(G);  // tiles of 16 rows that go through a step together
     static constexpr int kRows = kSub * kTile;
-    static constexpr int kStages = G <= 2 ? 2 : 3;
+    static constexpr int kStages = G <= 2 && NC == 8 ? 2 : 3;
     static constexpr int kTileBytes = kRows * 72 * G;
     static constexpr int kRingBytes = kAttWarps * kStages * kTileBytes;
-    static constexpr int kBlocks = G == 1 && NC == 8 ? 5 : G <= 2 && NC == 8 ? 4 : G <= 2 ? 3 : 2;  // per SM
+    static constexpr int kBlocks = blocks_of(G, NC);
 };
 
 // A tile in the ring: 16 rows of key codes, value codes, key parameters, value parameters. Sixteen-byte
@@ -348,8 +347,7 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
                 atomicOr(c.flags, kCacheTooLong);
         }
     }
-    const int share = share_of(rows_all, kk.n_split, G);
-    const int start = sp * share;
+    const int start = sp * kk.share;
     if (start >= rows_all && sp > 0) return;
 
     const size_t head_row = ((size_t)s * c.heads + h) * c.rows;
@@ -458,7 +456,7 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
         const int lim_first = FOUND ? 0 : visible(c, a, sn.len, ct * NC / a.group);
         const int lim_last = FOUND ? a.k : visible(c, a, sn.len, col_last / a.group);
         const int row_limit = FOUND ? visible(c, a, sn.len, item - sn.first) : 0;
-        const int end = min(min(start + share, rows_all), lim_last);
+        const int end = min(min(start + kk.share, rows_all), lim_last);
         const uint64_t* list = FOUND ? a.rows + (size_t)item * a.k : nullptr;
 
         // inv: what brings a step into f16's upper range, kPScale / norm, norm a power of two
@@ -848,8 +846,7 @@ __global__ void __launch_bounds__(kJoinBS) k_cache_join(CacheView c, AttendKerne
     const Span sn = span_of(c, a, s);
     if (sn.count == 0) return;
     const int rows = FOUND ? a.k : visible(c, a, sn.len, sn.count - 1);
-    const int share = share_of(rows, kk.n_split, c.G);
-    const int used = max(1, (rows + share - 1) / share);
+    const int used = max(1, (rows + kk.share - 1) / kk.share);
     const size_t step = (size_t)a.tok.n_tokens * a.q_heads;
     float m = kNoMax, l = 0.0f;
     for (int i = threadIdx.x; i < used; i += kJoinBS) m = fmaxf(m, kk.part_ml[i * step + th].x);
@@ -952,9 +949,13 @@ AttendPlan make_plan(const CacheView& c, const AttendArgs& a) {
     p.col_tiles = (int)((cols + p.nc - 1) / p.nc);
     const long long items = (long long)(found ? a.tok.n_tokens : c.n_seqs) * c.heads * p.col_tiles;
     const int rows = std::max(1, found ? a.k : std::min(a.max_rows, c.capacity));
-    const int step = kAttWarps * kTile * sub_tiles(c.G), most = (rows + step - 1) / step;
-    const long long want = 4ll * sm_count();
-    p.n_split = (int)std::max<long long>(1, std::min<long long>(std::min(most, kMaxSplit), (want + items - 1) / std::max(1ll, items)));
+    const int step = kAttWarps * kTile * sub_tiles(c.G);
+    const long long slots = (long long)blocks_of(c.G, p.nc) * sm_count();
+    const bool ragged = !found && c.n_seqs > 1;
+    const long long want = std::max(1ll, (ragged ? kWaves * slots : slots) / std::max(1ll, items));
+    const int least = std::max(1, (rows + kMaxSplit - 1) / kMaxSplit);
+    p.share = (std::max((int)std::min<long long>(rows, (rows + want - 1) / want), least) + step - 1) / step * step;
+    p.n_split = (rows + p.share - 1) / p.share;
     const size_t th = (size_t)a.tok.n_tokens * a.q_heads;
     size_t off = 0;
     if (p.n_split > 1) {
@@ -962,7 +963,7 @@ AttendPlan make_plan(const CacheView& c, const AttendArgs& a) {
         p.off_o = off;
         off += up256(th * p.n_split * c.dim * sizeof(float));
     }
-    p.logit_rows = most * step;
+    p.logit_rows = p.n_split * p.share;
     if (a.w_out) {
         p.off_lse = off;
         off += up256(th * sizeof(float));
@@ -1015,6 +1016,7 @@ void launch_cache_attend(const CacheView& c, const AttendArgs& a, cudaStream_t s
         k.logits = reinterpret_cast<float*>(ws + p.off_logit);
         k.logit_rows = p.logit_rows;
     }
+    k.share = p.share;
     k.n_split = p.n_split;
     k.col_tiles = p.col_tiles;
     if (a.tok.n_tokens > 0) {
