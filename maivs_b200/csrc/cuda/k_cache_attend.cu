@@ -216,6 +216,8 @@ struct Shape {
     static constexpr int kStages = G <= 2 && NC == 8 ? 2 : 3;
     static constexpr int kTileBytes = kRows * 72 * G;
     static constexpr int kRingBytes = kAttWarps * kStages * kTileBytes;
+    static constexpr int kPitch = G * kCacheGroup + 4;  // floats of one column's sums; a warp's writes meet no bank twice
+    static_assert(kRingBytes >= kAttWarps * NC * kPitch * 4, "the sums fit in the ring");
     static constexpr int kBlocks = blocks_of(G, NC);
 };
 
@@ -312,7 +314,6 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
     using S = Shape<G, NC, F32>;
     constexpr int kNt = S::kNt, kCols = S::kCols, kQ = S::kQ, kR = 2 * S::kSub;
     const AttendArgs& a = kk.a;
-    __shared__ float s_o[NC][G * kCacheGroup + 4];
     __shared__ float s_m[kAttWarps][NC], s_l[kAttWarps][NC];
     __shared__ uint4 s_q[S::kQShared ? 2 * G * kNt * (kQ / 4) : 1][32];
     extern __shared__ __align__(128) char s_ring[];
@@ -357,6 +358,27 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
     const uint32_t* vp = c.vp + head_row * G;
 
     for (int ct = ct0; ct * NC < cols; ct += kk.col_tiles) {
+        const int col_last = min(ct * NC + NC, cols) - 1;
+        const int lim_first = FOUND ? 0 : visible(c, a, sn.len, ct * NC / a.group);
+        const int lim_last = FOUND ? a.k : visible(c, a, sn.len, col_last / a.group);
+        const int row_limit = FOUND ? visible(c, a, sn.len, item - sn.first) : 0;
+        const int end = min(min(start + kk.share, rows_all), lim_last);
+        const uint64_t* list = FOUND ? a.rows + (size_t)item * a.k : nullptr;
+
+        // ---- the first tiles are on their way while the queries are prepared ----
+        char* ring = s_ring + warp * S::kStages * S::kTileBytes;
+        const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+        constexpr int kStride = kAttWarps * S::kRows;
+        const int mine = start + warp * S::kRows;
+        Fetch<G, FOUND> fetch;
+        fetch.init(kc, vc, kp, vp, mine, lane, list, a.k, row_limit);
+#pragma unroll
+        for (int i = 0; i < S::kStages - 1; ++i) {
+            const int r = mine + i * kStride;
+            if (r < end) fetch.next(ring_at + i * S::kTileBytes, r, kp, vp);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+
         // ---- queries: column gid of every eight, as B operands ----
         // 2^e brings a column's largest element to [2^14, 2^15). Then
         // score = (sum of step * acc + low * qsum) * fac, with acc and qsum in units of 2^e / kUnit.
@@ -452,13 +474,6 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
             logit_at[j] = ((size_t)(FOUND ? item : sn.first + i) * a.q_heads + h * a.group + (col - i * a.group)) *
                           kk.logit_rows;
         }
-        const int col_last = min(ct * NC + NC, cols) - 1;
-        const int lim_first = FOUND ? 0 : visible(c, a, sn.len, ct * NC / a.group);
-        const int lim_last = FOUND ? a.k : visible(c, a, sn.len, col_last / a.group);
-        const int row_limit = FOUND ? visible(c, a, sn.len, item - sn.first) : 0;
-        const int end = min(min(start + kk.share, rows_all), lim_last);
-        const uint64_t* list = FOUND ? a.rows + (size_t)item * a.k : nullptr;
-
         // inv: what brings a step into f16's upper range, kPScale / norm, norm a power of two
         float m[kCols], l[kCols], low[kCols][G], norm[G], inv[G];
         float o[G][4][kNt][4];
@@ -724,18 +739,6 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
             }
         };
 
-        char* ring = s_ring + warp * S::kStages * S::kTileBytes;
-        const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
-        constexpr int kStride = kAttWarps * S::kRows;
-        const int mine = start + warp * S::kRows;
-        Fetch<G, FOUND> fetch;
-        fetch.init(kc, vc, kp, vp, mine, lane, list, a.k, row_limit);
-#pragma unroll
-        for (int i = 0; i < S::kStages - 1; ++i) {
-            const int r = mine + i * kStride;
-            if (r < end) fetch.next(ring_at + i * S::kTileBytes, r, kp, vp);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        }
         int at = 0, to = (S::kStages - 1) * S::kTileBytes;  // this tile's place, and that of the one to fetch
         for (int r0 = mine; r0 < end; r0 += kStride) {
             // the tile is there, and every lane is done with the one before, whose place is filled next
@@ -752,7 +755,9 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
             at = at == (S::kStages - 1) * S::kTileBytes ? 0 : at + S::kTileBytes;
         }
 
-        // ---- the block's warps joined ----
+        // ---- the block's warps joined: each leaves its sums, relative to the block's maximum, where its
+        // ring was ----
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
         for (int j = 0; j < kCols; ++j) {
             const int col = 8 * (j >> 1) + 2 * t + (j & 1);
@@ -766,36 +771,27 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
                     low[j][g] = __fadd_rn(low[j][g], __shfl_xor_sync(~0u, low[j][g], d));
         }
         __syncthreads();
-        for (int w = 0; w < kAttWarps; ++w) {
-            if (warp == w) {
+        float* s_o = reinterpret_cast<float*>(s_ring);  // [warp][column][S::kPitch]
 #pragma unroll
-                for (int j = 0; j < kNt; ++j)
+        for (int j = 0; j < kCols; ++j) {
+            const int col = 8 * (j >> 1) + 2 * t + (j & 1);
+            float mx = s_m[0][col];
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const int col = 8 * j + 2 * t + x;
-                        float mx = s_m[0][col];
+            for (int y = 1; y < kAttWarps; ++y) mx = fmaxf(mx, s_m[y][col]);
+            const float f = ex2(m[j] - mx);
 #pragma unroll
-                        for (int y = 1; y < kAttWarps; ++y) mx = fmaxf(mx, s_m[y][col]);
-                        const float f = ex2(s_m[w][col] - mx);
+            for (int g = 0; g < G; ++g) {
+                // undo the operand's unit (16 for odd i) and kPScale / norm
+                const float n0 = __fmul_rn(S::kUnit / kPScale, norm[g]), n1 = __fmul_rn(S::kUnit / 16.0f / kPScale, norm[g]);
 #pragma unroll
-                        for (int g = 0; g < G; ++g) {
-                            const float lw = low[2 * j + x][g];
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                                for (int y = 0; y < 2; ++y) {
-                                    // undo the operand's unit (16 for odd i) and kPScale / norm
-                                    const float un = (i & 1 ? S::kUnit / 16.0f : S::kUnit) / kPScale;
-                                    const float v = __fmul_rn(
-                                        __fadd_rn(__fmul_rn(__fmul_rn(o[g][i][j][2 * y + x], un), norm[g]), lw), f);
-                                    float* at = &s_o[col][g * kCacheGroup + 16 * i + gid + 8 * y];
-                                    *at = w == 0 ? v : __fadd_rn(*at, v);
-                                }
-                        }
-                    }
+                    for (int y = 0; y < 2; ++y)
+                        s_o[(warp * NC + col) * S::kPitch + g * kCacheGroup + 16 * i + gid + 8 * y] =
+                            __fmul_rn(__fmaf_rn(o[g][i][j >> 1][2 * y + (j & 1)], i & 1 ? n1 : n0, low[j][g]), f);
             }
-            __syncthreads();
         }
+        __syncthreads();
         // ---- out, or this split's part ----
         for (int col = warp; col < NC; col += kAttWarps) {
             const int cc = ct * NC + col;
@@ -809,11 +805,18 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
 #pragma unroll
             for (int y = 0; y < kAttWarps; ++y) sum = __fmaf_rn(s_l[y][col], ex2(s_m[y][col] - mx), sum);
             const size_t th = (size_t)tk * a.q_heads + hd;
+            const float* so = s_o + col * S::kPitch;
+            auto value = [&](int d) -> float {
+                float v = so[d];
+#pragma unroll
+                for (int y = 1; y < kAttWarps; ++y) v = __fadd_rn(v, so[y * NC * S::kPitch + d]);
+                return v;
+            };
             if (kk.n_split == 1) {
                 // no visible row: 0 and -inf
                 const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
                 for (int d = lane; d < c.dim; d += 32)
-                    write_out(a.out, a.type, th * c.dim + d, sum == 0.0f ? 0.0f : __fmul_rn(s_o[col][d], inv));
+                    write_out(a.out, a.type, th * c.dim + d, sum == 0.0f ? 0.0f : __fmul_rn(value(d), inv));
                 if (lane == 0) {
                     const float l2 = sum == 0.0f ? -INFINITY : __fadd_rn(mx, log2f(sum));
                     if (a.lse) a.lse[th] = __fmul_rn(l2, 0.69314718055994531f);
@@ -821,7 +824,7 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
                 }
             } else {
                 const size_t at = (size_t)sp * a.tok.n_tokens * a.q_heads + th;
-                for (int d = lane; d < c.dim; d += 32) kk.part_o[at * c.dim + d] = s_o[col][d];
+                for (int d = lane; d < c.dim; d += 32) kk.part_o[at * c.dim + d] = value(d);
                 if (lane == 0) kk.part_ml[at] = make_float2(mx, sum);
             }
         }
