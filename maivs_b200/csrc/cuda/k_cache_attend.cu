@@ -22,6 +22,8 @@
 // Rounding: codes are exact, 16-bit queries are exact in f16 down to 2^-24 of their row's largest
 // element, p * step is rounded to f16 (2^-12 relative, below the output's own rounding). f32 calls
 // split query and p * step into two f16 halves each (22 bits).
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -41,8 +43,12 @@ constexpr int kTile = 16;       // rows of one MMA
 // Tiles of 16 rows that a warp takes together.
 __host__ __device__ constexpr int sub_tiles(int G) { return G <= 2 ? 2 : 1; }
 constexpr int kJoinBS = 128;
-constexpr int kMaxSplit = 1024;
+constexpr int kMaxCluster = 8;
+constexpr int kMaxParts = 1024;
 constexpr int kWaves = 4;
+// Up to so many rows a cluster of blocks reads them and joins in shared memory, in one launch; above, its
+// blocks would wait for the slowest and the SMs for a place for all of them.
+constexpr int kClusterRows = 2048;
 constexpr float kNoMax = -3.0e38f;
 constexpr float kLog2e = 1.4426950408889634f;
 // p * step goes into f16 scaled so that the group's largest step becomes 2^12: an old maximum may
@@ -53,20 +59,21 @@ constexpr float kPScale = 4096.0f;
 struct AttendPlan {
     int nc;         // columns per tile
     int col_tiles;  // of one sequence and head (or token and head)
-    int share;      // rows of one block
-    int n_split;    // blocks that share the longest sequence's rows
+    int cluster;    // blocks that share rows and join in shared memory
+    int parts;      // blocks (of no cluster) that share rows and are joined by k_cache_join
+    int share;      // rows of such a block
     size_t off_o, off_lse, off_logit, bytes;
     int logit_rows;
 };
 
 struct AttendKernel {
     AttendArgs a;
-    float2* part_ml;  // [split][token][q_head]: running maximum (log2) and sum
-    float* part_o;    // [split][token][q_head][dim]
+    float2* part_ml;  // [part][token][q_head]: running maximum (log2) and sum
+    float* part_o;    // [part][token][q_head][dim]
     float* lse2;      // [token][q_head], log2; null without weights
     float* logits;    // [token][q_head][logit_rows], log2; null without weights
     int logit_rows;
-    int share, n_split, col_tiles;
+    int cluster, parts, share, col_tiles;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -200,6 +207,12 @@ __device__ __forceinline__ Span span_of(const CacheView& c, const AttendArgs& a,
 __device__ __forceinline__ int visible(const CacheView& c, const AttendArgs& a, int len, int i) {
     return min(min(len + (a.causal ? i + 1 : 0), c.capacity), a.max_rows);
 }
+// Rows per block where n blocks share them: equal, in whole steps of the block's warps.
+__host__ __device__ __forceinline__ int share_of(int rows, int n, int G) {
+    const int step = kAttWarps * kTile * sub_tiles(G);
+    return max((int)(((long long)rows + (long long)n * step - 1) / ((long long)n * step)), 1) * step;
+}
+
 // Blocks per SM that the registers of a variant are held to.
 __host__ __device__ constexpr int blocks_of(int G, int nc) { return nc == 16 || G > 2 ? 2 : G == 2 ? 3 : 5; }
 
@@ -309,21 +322,32 @@ struct Fetch {
     }
 };
 
-template <int G, int NC, bool F32, bool FOUND>
+// kRows: rows in order. kClustered: the same, joined by a cluster of blocks. kFound: rows of a list.
+enum class Mode { kRows, kClustered, kFound };
+
+template <int G, int NC, bool F32, Mode MODE>
 __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_attend(CacheView c, AttendKernel kk) {
+    constexpr bool FOUND = MODE == Mode::kFound, kCluster = MODE == Mode::kClustered;
     using S = Shape<G, NC, F32>;
     constexpr int kNt = S::kNt, kCols = S::kCols, kQ = S::kQ, kR = 2 * S::kSub;
     const AttendArgs& a = kk.a;
     __shared__ float s_m[kAttWarps][NC], s_l[kAttWarps][NC];
+    __shared__ float2 s_blk[kCluster ? NC : 1], s_all[kCluster ? NC : 1];  // maximum and sum: of the block, of the cluster
+    __shared__ float s_f[kCluster ? kMaxCluster : 1][NC];  // what brings a block's sums to the cluster's maximum
     __shared__ uint4 s_q[S::kQShared ? 2 * G * kNt * (kQ / 4) : 1][32];
     extern __shared__ __align__(128) char s_ring[];
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gid = lane >> 2, t = lane & 3;
     unsigned b = blockIdx.x;
+    int rank = 0;
+    if constexpr (kCluster) {
+        rank = b % kk.cluster;
+        b /= kk.cluster;
+    }
     const int ct0 = b % kk.col_tiles;
     b /= kk.col_tiles;
-    const int sp = b % kk.n_split;
-    b /= kk.n_split;
+    const int part = b % kk.parts;
+    b /= kk.parts;
     const int h = b % c.heads;
     const int item = b / c.heads;  // sequence, or token of a found list
 
@@ -341,15 +365,18 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
         sn = span_of(c, a, s);
         cols = sn.count * a.group;
         rows_all = sn.count ? visible(c, a, sn.len, sn.count - 1) : 0;
-        if (threadIdx.x == 0 && h == 0 && sp == 0 && ct0 == 0) {
+        if (threadIdx.x == 0 && h == 0 && part == 0 && rank == 0 && ct0 == 0) {
             const int lo = __ldg(a.tok.offsets + s), hi = __ldg(a.tok.offsets + s + 1);
             if (lo < 0 || hi < lo || hi > a.tok.n_tokens) atomicOr(c.flags, kCacheOffsets);
             if (sn.count && min(sn.len + (a.causal ? sn.count : 0), c.capacity) > a.max_rows)
                 atomicOr(c.flags, kCacheTooLong);
         }
     }
-    const int start = sp * kk.share;
-    if (start >= rows_all && sp > 0) return;
+    const int share = kCluster ? share_of(rows_all, kk.cluster, G) : kk.share;
+    const int start = (part + rank) * share;
+    if (part > 0 && start >= rows_all) return;
+    namespace cg = cooperative_groups;
+    const cg::cluster_group cluster = cg::this_cluster();
 
     const size_t head_row = ((size_t)s * c.heads + h) * c.rows;
     const uint32_t* kc = c.kc + head_row * 8 * G;
@@ -362,7 +389,7 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
         const int lim_first = FOUND ? 0 : visible(c, a, sn.len, ct * NC / a.group);
         const int lim_last = FOUND ? a.k : visible(c, a, sn.len, col_last / a.group);
         const int row_limit = FOUND ? visible(c, a, sn.len, item - sn.first) : 0;
-        const int end = min(min(start + kk.share, rows_all), lim_last);
+        const int end = min(min(start + share, rows_all), lim_last);
         const uint64_t* list = FOUND ? a.rows + (size_t)item * a.k : nullptr;
 
         // ---- the first tiles are on their way while the queries are prepared ----
@@ -792,53 +819,111 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
             }
         }
         __syncthreads();
-        // ---- out, or this split's part ----
-        for (int col = warp; col < NC; col += kAttWarps) {
-            const int cc = ct * NC + col;
-            if (cc >= cols) break;
-            const int i = cc / a.group;
-            const int tk = FOUND ? item : sn.first + i;
-            const int hd = h * a.group + (cc - i * a.group);
-            float mx = s_m[0][col], sum = 0.0f;
+        if constexpr (kCluster) {
+            for (int e = threadIdx.x; e < NC * G * kCacheGroup; e += kAttBS) {
+                const int col = e / (G * kCacheGroup), d = e % (G * kCacheGroup);
+                float v = s_o[col * S::kPitch + d];
 #pragma unroll
-            for (int y = 1; y < kAttWarps; ++y) mx = fmaxf(mx, s_m[y][col]);
+                for (int y = 1; y < kAttWarps; ++y) v = __fadd_rn(v, s_o[(y * NC + col) * S::kPitch + d]);
+                s_o[col * S::kPitch + d] = v;
+            }
+            if (threadIdx.x < NC) {
+                const int col = threadIdx.x;
+                float mx = s_m[0][col], sum = 0.0f;
 #pragma unroll
-            for (int y = 0; y < kAttWarps; ++y) sum = __fmaf_rn(s_l[y][col], ex2(s_m[y][col] - mx), sum);
-            const size_t th = (size_t)tk * a.q_heads + hd;
-            const float* so = s_o + col * S::kPitch;
-            auto value = [&](int d) -> float {
-                float v = so[d];
+                for (int y = 1; y < kAttWarps; ++y) mx = fmaxf(mx, s_m[y][col]);
 #pragma unroll
-                for (int y = 1; y < kAttWarps; ++y) v = __fadd_rn(v, so[y * NC * S::kPitch + d]);
-                return v;
-            };
-            if (kk.n_split == 1) {
+                for (int y = 0; y < kAttWarps; ++y) sum = __fmaf_rn(s_l[y][col], ex2(s_m[y][col] - mx), sum);
+                s_blk[col] = make_float2(mx, sum);
+            }
+            // ---- the cluster's blocks joined: every block finishes a share of the elements ----
+            cluster.sync();
+            if (threadIdx.x < NC) {
+                const int col = threadIdx.x;
+                float mx = kNoMax, sum = 0.0f;
+                for (int r = 0; r < kk.cluster; ++r) {
+                    const float2 v = *cluster.map_shared_rank(&s_blk[col], r);
+                    mx = fmaxf(mx, v.x);
+                }
+                for (int r = 0; r < kk.cluster; ++r) {
+                    const float2 v = *cluster.map_shared_rank(&s_blk[col], r);
+                    const float f = ex2(v.x - mx);
+                    s_f[r][col] = f;
+                    sum = __fmaf_rn(v.y, f, sum);
+                }
+                s_all[col] = make_float2(mx, sum);
+            }
+            __syncthreads();
+            const int n_cols = min(NC, cols - ct * NC);
+            for (int e = rank * kAttBS + threadIdx.x; e < n_cols * G * kCacheGroup; e += kk.cluster * kAttBS) {
+                const int col = e / (G * kCacheGroup), d = e % (G * kCacheGroup);
+                if (d >= c.dim) continue;
+                const int cc = ct * NC + col, i = cc / a.group;
+                const size_t th = (size_t)(FOUND ? item : sn.first + i) * a.q_heads + h * a.group + (cc - i * a.group);
+                float v = 0.0f;
+                for (int r = 0; r < kk.cluster; ++r) {
+                    const float* src = cluster.map_shared_rank(s_o, r);
+                    v = __fmaf_rn(src[col * S::kPitch + d], s_f[r][col], v);
+                }
+                const float2 ml = s_all[col];
                 // no visible row: 0 and -inf
-                const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
-                for (int d = lane; d < c.dim; d += 32)
-                    write_out(a.out, a.type, th * c.dim + d, sum == 0.0f ? 0.0f : __fmul_rn(value(d), inv));
-                if (lane == 0) {
-                    const float l2 = sum == 0.0f ? -INFINITY : __fadd_rn(mx, log2f(sum));
+                write_out(a.out, a.type, th * c.dim + d, ml.y == 0.0f ? 0.0f : __fdiv_rn(v, ml.y));
+                if (d == 0) {
+                    const float l2 = ml.y == 0.0f ? -INFINITY : __fadd_rn(ml.x, log2f(ml.y));
                     if (a.lse) a.lse[th] = __fmul_rn(l2, 0.69314718055994531f);
                     if (kk.lse2) kk.lse2[th] = l2;
                 }
-            } else {
-                const size_t at = (size_t)sp * a.tok.n_tokens * a.q_heads + th;
-                for (int d = lane; d < c.dim; d += 32) kk.part_o[at * c.dim + d] = value(d);
-                if (lane == 0) kk.part_ml[at] = make_float2(mx, sum);
             }
+            cluster.sync();  // nobody reads this block's sums any more
+        } else {
+            // ---- out, or this block's part ----
+            for (int col = warp; col < NC; col += kAttWarps) {
+                const int cc = ct * NC + col;
+                if (cc >= cols) break;
+                const int i = cc / a.group;
+                const int tk = FOUND ? item : sn.first + i;
+                const int hd = h * a.group + (cc - i * a.group);
+                float mx = s_m[0][col], sum = 0.0f;
+#pragma unroll
+                for (int y = 1; y < kAttWarps; ++y) mx = fmaxf(mx, s_m[y][col]);
+#pragma unroll
+                for (int y = 0; y < kAttWarps; ++y) sum = __fmaf_rn(s_l[y][col], ex2(s_m[y][col] - mx), sum);
+                const size_t th = (size_t)tk * a.q_heads + hd;
+                const float* so = s_o + col * S::kPitch;
+                auto value = [&](int d) -> float {
+                    float v = so[d];
+#pragma unroll
+                    for (int y = 1; y < kAttWarps; ++y) v = __fadd_rn(v, so[y * NC * S::kPitch + d]);
+                    return v;
+                };
+                if (kk.parts == 1) {
+                    // no visible row: 0 and -inf
+                    const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+                    for (int d = lane; d < c.dim; d += 32)
+                        write_out(a.out, a.type, th * c.dim + d, sum == 0.0f ? 0.0f : __fmul_rn(value(d), inv));
+                    if (lane == 0) {
+                        const float l2 = sum == 0.0f ? -INFINITY : __fadd_rn(mx, log2f(sum));
+                        if (a.lse) a.lse[th] = __fmul_rn(l2, 0.69314718055994531f);
+                        if (kk.lse2) kk.lse2[th] = l2;
+                    }
+                } else {
+                    const size_t at = (size_t)part * a.tok.n_tokens * a.q_heads + th;
+                    for (int d = lane; d < c.dim; d += 32) kk.part_o[at * c.dim + d] = value(d);
+                    if (lane == 0) kk.part_ml[at] = make_float2(mx, sum);
+                }
+            }
+            __syncthreads();
         }
-        __syncthreads();
     }
 }
 
-// Joins the splits of one token's query head: a block each. Its warps take every fourth split, lanes the
+// Joins the parts of one token's query head: a block each. Its warps take every fourth part, lanes the
 // dimensions; the warps' sums are added in order.
 template <bool FOUND>
 __global__ void __launch_bounds__(kJoinBS) k_cache_join(CacheView c, AttendKernel kk) {
     const AttendArgs& a = kk.a;
     constexpr int kWarps = kJoinBS / 32;
-    __shared__ float s_w[kMaxSplit];
+    __shared__ float s_w[kMaxParts];
     __shared__ float s_red[kWarps];
     __shared__ float s_acc[kWarps][kCacheMaxDim];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -954,19 +1039,29 @@ AttendPlan make_plan(const CacheView& c, const AttendArgs& a) {
     const int rows = std::max(1, found ? a.k : std::min(a.max_rows, c.capacity));
     const int step = kAttWarps * kTile * sub_tiles(c.G);
     const long long slots = (long long)blocks_of(c.G, p.nc) * sm_count();
+    // Enough blocks to fill the GPU once; with sequences of different lengths kWaves times as many, of
+    // fixed rows, so that the longest do not run on alone.
+    const int most = (rows + step - 1) / step;
     const bool ragged = !found && c.n_seqs > 1;
-    const long long want = std::max(1ll, (ragged ? kWaves * slots : slots) / std::max(1ll, items));
-    const int least = std::max(1, (rows + kMaxSplit - 1) / kMaxSplit);
-    p.share = (std::max((int)std::min<long long>(rows, (rows + want - 1) / want), least) + step - 1) / step * step;
-    p.n_split = (rows + p.share - 1) / p.share;
+    const long long fill = std::max(1ll, slots / std::max(1ll, items));
+    p.cluster = p.parts = 1;
+    p.share = most * step;
+    if (!found && rows <= kClusterRows && fill >= 2) {
+        p.cluster = (int)std::min<long long>({kMaxCluster, fill, most});
+    } else {
+        const long long n = ragged ? std::max(1ll, kWaves * slots / std::max(1ll, items)) : fill;
+        const int least = (rows + kMaxParts - 1) / kMaxParts;
+        p.share = (std::max((int)std::min<long long>(rows, (rows + n - 1) / n), least) + step - 1) / step * step;
+        p.parts = (rows + p.share - 1) / p.share;
+    }
     const size_t th = (size_t)a.tok.n_tokens * a.q_heads;
     size_t off = 0;
-    if (p.n_split > 1) {
-        off += up256(th * p.n_split * sizeof(float2));
+    if (p.parts > 1) {
+        off += up256(th * p.parts * sizeof(float2));
         p.off_o = off;
-        off += up256(th * p.n_split * c.dim * sizeof(float));
+        off += up256(th * p.parts * c.dim * sizeof(float));
     }
-    p.logit_rows = p.n_split * p.share;
+    p.logit_rows = most * step;
     if (a.w_out) {
         p.off_lse = off;
         off += up256(th * sizeof(float));
@@ -980,9 +1075,21 @@ AttendPlan make_plan(const CacheView& c, const AttendArgs& a) {
 template <int G, int NC, bool F32>
 void start(const CacheView& c, const AttendKernel& k, bool found, unsigned grid, cudaStream_t st) {
     constexpr int smem = Shape<G, NC, F32>::kRingBytes;
-    const auto kernel = found ? k_cache_attend<G, NC, F32, true> : k_cache_attend<G, NC, F32, false>;
+    const auto kernel = found           ? k_cache_attend<G, NC, F32, Mode::kFound>
+                        : k.cluster > 1 ? k_cache_attend<G, NC, F32, Mode::kClustered>
+                                        : k_cache_attend<G, NC, F32, Mode::kRows>;
     set_smem((const void*)kernel, smem);
-    kernel<<<grid, kAttBS, smem, st>>>(c, k);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kAttBS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {(unsigned)k.cluster, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = k.cluster > 1 ? 1 : 0;
+    cudaLaunchKernelEx(&cfg, kernel, c, k);
 }
 
 template <int G>
@@ -1001,7 +1108,7 @@ size_t cache_attend_workspace(const CacheView& c, const AttendArgs& a) { return 
 
 long long cache_attend_blocks(const CacheView& c, const AttendArgs& a) {
     const AttendPlan p = make_plan(c, a);
-    return (long long)(a.k > 0 ? a.tok.n_tokens : c.n_seqs) * c.heads * p.n_split * p.col_tiles;
+    return (long long)(a.k > 0 ? a.tok.n_tokens : c.n_seqs) * c.heads * p.cluster * p.parts * p.col_tiles;
 }
 
 void launch_cache_attend(const CacheView& c, const AttendArgs& a, cudaStream_t st) {
@@ -1019,12 +1126,13 @@ void launch_cache_attend(const CacheView& c, const AttendArgs& a, cudaStream_t s
         k.logits = reinterpret_cast<float*>(ws + p.off_logit);
         k.logit_rows = p.logit_rows;
     }
+    k.cluster = p.cluster;
+    k.parts = p.parts;
     k.share = p.share;
-    k.n_split = p.n_split;
     k.col_tiles = p.col_tiles;
     if (a.tok.n_tokens > 0) {
         const unsigned grid =
-            (unsigned)((long long)(found ? a.tok.n_tokens : c.n_seqs) * c.heads * p.n_split * p.col_tiles);
+            (unsigned)((long long)(found ? a.tok.n_tokens : c.n_seqs) * c.heads * p.cluster * p.parts * p.col_tiles);
         {
             Tick tk(kKCacheAttend, st);
             if (c.G == 1)
@@ -1036,7 +1144,7 @@ void launch_cache_attend(const CacheView& c, const AttendArgs& a, cudaStream_t s
             else
                 start_g<6>(c, k, p.nc, found, grid, st);
         }
-        if (p.n_split > 1) {
+        if (p.parts > 1) {
             Tick tk(kKCacheJoin, st);
             const unsigned jg = (unsigned)((long long)a.tok.n_tokens * a.q_heads);
             if (found)
