@@ -1,5 +1,6 @@
 // The attention cache's storage: rows into 4 bits and back, and eviction by accumulated weight.
 #include <algorithm>
+#include <type_traits>
 
 #include "cache.h"
 #include "cache_dev.cuh"
@@ -13,84 +14,200 @@ namespace {
 
 constexpr int kUnit = 8;       // lanes per group of 64 dimensions, 8 dimensions each
 constexpr int kStoreBS = 256;  // threads of the append and read kernels
+constexpr int kUnits = kStoreBS / kUnit;
+// Units that a thread has in flight: one where the call is small and its latency counts, four where
+// HBM's bandwidth does.
+constexpr int kDeep = 4;
 
-// One unit's place: which token, head and group, and the cache row it maps to (-1: none).
-struct Unit {
-    int tok, head, group, seq, row;
-};
+// Lane l of a unit takes dimensions 8 c .. 8 c + 7 of its group, c = chunk_of(l). In this order an 8 x 8
+// transposition of nibbles over the unit's lanes turns the lanes' codes into value words and back.
+__device__ __forceinline__ int chunk_of(int l) { return 2 * (l & 3) + (l >> 2); }
 
-__device__ __forceinline__ bool find_unit(const CacheView& c, const CacheTokens& tk, long long unit, int lane8,
-                                          unsigned mask, Unit* u) {
-    const long long per_tok = (long long)c.heads * c.G;
-    u->tok = (int)(unit / per_tok);
-    const int rest = (int)(unit - (long long)u->tok * per_tok);
-    u->head = rest / c.G;
-    u->group = rest - u->head * c.G;
-    u->seq = -1;
-    u->row = -1;
-    if (u->tok >= tk.n_tokens) return false;
-    u->seq = find_sequence(tk.offsets, c.n_seqs, u->tok, lane8, mask);
-    if (u->seq < 0) return false;
-    const long long row = (long long)min(max(tk.lengths[u->seq], 0), c.capacity) + (u->tok - tk.offsets[u->seq]);
-    if (row >= c.capacity) return false;
-    u->row = (int)row;
-    return true;
+// Nibble k of lane l <-> nibble l of lane k, within aligned groups of 8 lanes: halves, bytes, nibbles.
+__device__ __forceinline__ uint32_t transpose_nibbles(uint32_t x, int l, unsigned mask) {
+    uint32_t y = __shfl_xor_sync(mask, x, 4);
+    x = __byte_perm(x, y, l & 4 ? 0x3276 : 0x5410);
+    y = __shfl_xor_sync(mask, x, 2);
+    x = __byte_perm(x, y, l & 2 ? 0x3715 : 0x6240);
+    y = __shfl_xor_sync(mask, x, 1);
+    return l & 1 ? (x & 0xF0F0F0F0u) | ((y >> 4) & 0x0F0F0F0Fu) : (x & 0x0F0F0F0Fu) | ((y << 4) & 0xF0F0F0F0u);
 }
 
-// The code of x among the levels low + step * 0..15: the nearest in real arithmetic, ties to the
-// even code. t = (x - low) / step in 32 bits is off by less than 1e-5 levels, so only an x that
-// close to the middle of two levels is decided by the exact sign of (x - low) - (k + 1/2) step:
-// the product is exact (8 x 5 bits), and the difference's own rounding error is added back.
-__device__ __forceinline__ uint32_t code_of(float x, float low, float step, float inv) {
-    const float d = __fsub_rn(x, low);
-    const float t = __fmul_rn(d, inv);
-    float c = rintf(t);
-    if (fabsf(__fsub_rn(t, c)) > 0.49998f && t < 15.0f) {
-        const float k = floorf(t);
-        const float b = __fmul_rn(k + 0.5f, step);
-        // error of d: x - low == d + e exactly
-        const float xb = __fadd_rn(d, low);
-        const float e = __fadd_rn(__fsub_rn(x, xb), __fsub_rn(__fsub_rn(xb, d), low));
-        const float z = __fadd_rn(__fsub_rn(d, b), e);
-        c = z > 0.0f || (z == 0.0f && ((int)k & 1)) ? k + 1.0f : k;
+// u / per for the small numbers of a block (u < 2^13, per < 2^13), by = ceil(2^32 / per), 0 for per = 1.
+__device__ __forceinline__ int quotient(int u, uint32_t by) { return by ? (int)__umulhi((uint32_t)u, by) : u; }
+
+// Where the tokens of a block go: the row of token i, or -1 (padding), or -2 (past the capacity).
+struct Place {
+    int seq, row;
+};
+
+__device__ __forceinline__ Place place_of(const CacheView& c, const CacheTokens& tk, int tok, int lane8, unsigned mask) {
+    Place p{-1, -1};
+    if (tok >= tk.n_tokens) return p;
+    p.seq = find_sequence(tk.offsets, c.n_seqs, tok, lane8, mask);
+    if (p.seq < 0) return p;
+    const long long row =
+        (long long)min(max(__ldg(tk.lengths + p.seq), 0), c.capacity) + (tok - __ldg(tk.offsets + p.seq));
+    p.row = row < c.capacity ? (int)row : -2;
+    return p;
+}
+
+// Codes of eight elements, element i in nibble i: the nearest of the levels low + step * 0..15, ties to the
+// even code, from the quotient in 64 bits. The rare way: see below for when it is needed.
+__device__ __noinline__ uint32_t codes_exact(float4 a, float4 b, float low, float step) {
+    const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    uint32_t code = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const double c = rint(((double)x[i] - low) / step);
+        code |= (uint32_t)fmin(fmax(c, 0.0), 15.0) << (4 * i);
     }
-    // max first: a NaN becomes 0
-    return (uint32_t)fminf(fmaxf(c, 0.0f), 15.0f);
+    return code;
+}
+
+// The same in 32 bits. t = (x - low) / step is the quotient after one correction by its residual, which is
+// exact: t is within half an ulp (2^-21) of the true quotient, and equal to it where that is k + 1/2.
+// Rounding to a whole number is an addition of 1.5 * 2^23 (ties to even), whose low bits are the code.
+// That decides wrongly only where the true quotient is within 2^-21 of k + 1/2 and not equal to it:
+//  - 16-bit elements: x - low and (k + 1/2) step are multiples of one power of two, and so is their
+//    difference, unless some element is below 2^-13 (bf16) or 2^-10 (f16) of the step: `fine` asks
+//    for the exact way there. x - low itself is exact under the same condition;
+//  - f32 elements: wherever t is that close to k + 1/2, which is asked here.
+template <typename T>
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float low, float step, bool fine) {
+    constexpr float kMagic = 12582912.0f;
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(step));
+    uint32_t code = 0;
+#pragma unroll
+    for (int i = 7; i >= 0; --i) {
+        const float d = __fsub_rn(x[i], low);
+        float t = __fmul_rn(d, inv);
+        t = __fmaf_rn(__fmaf_rn(-t, step, d), inv, t);
+        if constexpr (!std::is_same<T, __nv_bfloat16>::value) t = fminf(fmaxf(t, 0.0f), 15.0f);  // bf16: low is the smallest
+        const float r = __fadd_rn(t, kMagic);
+        if constexpr (sizeof(T) == 4) fine |= fabsf(__fsub_rn(t, __fsub_rn(r, kMagic))) > 0.499996f;
+        code = code * 16 + (__float_as_uint(r) & 15u);
+    }
+    // a subnormal step has no reciprocal here
+    if (fine || inv == INFINITY)
+        code = codes_exact(make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]), low, step);
+    return code;
+}
+
+// Eight elements of a row, n of them there. 16-bit types as they lie in memory, two to a word.
+template <typename T>
+struct Raw8 {
+    uint32_t w[2 * sizeof(T)];
+};
+
+template <typename T>
+__device__ __forceinline__ Raw8<T> load8(const T* __restrict__ p, int n, bool vec) {
+    Raw8<T> r;
+    if (vec && n == 8) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+            const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+            r.w[4 * i] = a.x, r.w[4 * i + 1] = a.y, r.w[4 * i + 2] = a.z, r.w[4 * i + 3] = a.w;
+        }
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r.w[i] = i < n ? __ldg(reinterpret_cast<const uint32_t*>(p) + i) : 0u;
+    } else {
+        const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            r.w[i] = (2 * i < n ? __ldg(q + 2 * i) : 0u) | (2 * i + 1 < n ? (uint32_t)__ldg(q + 2 * i + 1) << 16 : 0u);
+    }
+    return r;
 }
 
 template <typename T>
-__device__ __forceinline__ void load8(const T* __restrict__ p, int n, bool vec, float (&x)[8]) {
-    if (vec) {
-        if constexpr (sizeof(T) == 4) {
-            const float4 a = __ldcs(reinterpret_cast<const float4*>(p));
-            const float4 b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
-            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-        } else {
-            const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p));
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+__device__ __forceinline__ float element(const Raw8<T>& r, int i) {
+    if constexpr (sizeof(T) == 4)
+        return __uint_as_float(r.w[i]);
+    else
+        return to_f32<T>(i & 1 ? r.w[i / 2] >> 16 : r.w[i / 2] & 0xFFFFu);
+}
+
+// Largest and smallest of a unit's 64 elements (NaN if one is), and this lane's smallest magnitude. 16-bit
+// types by packed comparisons: the largest and the negated smallest go through the lanes as one word.
+__device__ __forceinline__ void extremes(const Raw8<float>& r, int n, unsigned mask, float* hi, float* lo, float* small) {
+    float h = -INFINITY, l = INFINITY;
+    bool nan = false;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[2 * i] = to_f32<T>(w[i] & 0xFFFFu);
-                x[2 * i + 1] = to_f32<T>(w[i] >> 16);
-            }
+    for (int e = 0; e < 8; ++e)
+        if (e < n) {
+            const float x = element(r, e);
+            h = fmaxf(h, x);
+            l = fminf(l, x);
+            nan |= x != x;
         }
-    } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = i < n ? (float)p[i] : 0.0f;
+    for (int o = 4; o; o >>= 1) {
+        h = fmaxf(h, __shfl_xor_sync(mask, h, o));
+        l = fminf(l, __shfl_xor_sync(mask, l, o));
     }
+    nan = (__ballot_sync(mask, nan) & mask) != 0;
+    *hi = nan ? __uint_as_float(0x7FC00000u) : h;
+    *lo = nan ? __uint_as_float(0x7FC00000u) : l;
+    *small = 0.0f;
+}
+template <typename T>
+struct Pair;
+template <>
+struct Pair<__half> {
+    using type = __half2;
+    static constexpr uint32_t kInf = 0x7C007C00u;
+};
+template <>
+struct Pair<__nv_bfloat16> {
+    using type = __nv_bfloat162;
+    static constexpr uint32_t kInf = 0x7F807F80u;
+};
+template <typename P>
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    const P m = __hmax2_nan(*reinterpret_cast<const P*>(&a), *reinterpret_cast<const P*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+}
+template <typename T>
+__device__ __forceinline__ void extremes(const Raw8<T>& r, int n, unsigned mask, float* hi, float* lo, float* small) {
+    using P = typename Pair<T>::type;
+    uint32_t up[4], down[4];  // the elements, and the elements negated; -inf where there is none
+#pragma unroll
+    for (int i = 0; i < 4; ++i) up[i] = r.w[i], down[i] = r.w[i] ^ 0x80008000u;
+    if (n < 8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t keep = 2 * i + 1 < n ? ~0u : 2 * i < n ? 0xFFFFu : 0u, none = (Pair<T>::kInf | 0x80008000u) & ~keep;
+            up[i] = (up[i] & keep) | none;
+            down[i] = (down[i] & keep) | none;
+        }
+    }
+    // magnitudes order as whole numbers
+    const uint32_t a = __vimin3_u16x2(up[0] & 0x7FFF7FFFu, up[1] & 0x7FFF7FFFu, up[2] & 0x7FFF7FFFu);
+    const uint32_t last = up[3] & 0x7FFF7FFFu, b = __vimin3_u16x2(a, last, last);
+    *small = to_f32<T>(min(b & 0xFFFFu, b >> 16));
+    const uint32_t u = max2<P>(max2<P>(up[0], up[1]), max2<P>(up[2], up[3]));
+    const uint32_t d = max2<P>(max2<P>(down[0], down[1]), max2<P>(down[2], down[3]));
+    uint32_t m = max2<P>(__byte_perm(u, d, 0x5410), __byte_perm(u, d, 0x7632));
+#pragma unroll
+    for (int o = 4; o; o >>= 1) m = max2<P>(m, __shfl_xor_sync(mask, m, o));
+    *hi = to_f32<T>(m & 0xFFFFu);
+    *lo = -to_f32<T>(m >> 16);
 }
 
 template <typename T>
 __device__ __forceinline__ void store8(T* __restrict__ p, int n, bool vec, const float (&x)[8]) {
-    if (vec) {
+    if (vec && n == 8) {
         if constexpr (sizeof(T) == 4) {
-            reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-            reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+            __stcs(reinterpret_cast<float4*>(p), make_float4(x[0], x[1], x[2], x[3]));
+            __stcs(reinterpret_cast<float4*>(p) + 1, make_float4(x[4], x[5], x[6], x[7]));
         } else {
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = from_f32<T>(x[2 * i]) | (from_f32<T>(x[2 * i + 1]) << 16);
-            *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+            __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
         }
     } else {
 #pragma unroll
@@ -99,123 +216,127 @@ __device__ __forceinline__ void store8(T* __restrict__ p, int n, bool vec, const
     }
 }
 
-// Nibble (n) of the value words <-> lane L of the unit: dimension 64 g + 8 L + e is nibble
-// L / 2 + 4 (L % 2) of word e.
-__device__ __forceinline__ int lane_of_nibble(int n) { return 2 * (n & 3) + (n >> 2); }
-__device__ __forceinline__ int nibble_of_lane(int l) { return (l >> 1) + 4 * (l & 1); }
-
-// Rows into the cache. Eight lanes take a group of 64 dimensions; blockIdx.y: 0 keys, 1 values.
-template <typename T>
-__global__ void __launch_bounds__(kStoreBS) k_cache_append(CacheView c, AppendArgs a, bool vec, long long units) {
-    const int lane8 = threadIdx.x % kUnit;
+// Rows into the cache. blockIdx.x: a run of `run` tokens, blockIdx.y: 0 keys, 1 values. Eight lanes take
+// a group of 64 dimensions of one head; a block's units go over its tokens' heads and groups in order,
+// U of a thread at a time. Bound by HBM (one read of the tokens, one write of the rows) with U = 4.
+template <typename T, int G, int U>
+__global__ void __launch_bounds__(kStoreBS) k_cache_append(CacheView c, AppendArgs a, bool vec, int run, uint32_t by) {
+    __shared__ Place s_place[kUnits * kDeep];
+    const int l8 = threadIdx.x % kUnit, unit = threadIdx.x / kUnit;
     const unsigned mask = 0xFFu << (threadIdx.x % 32 / kUnit * kUnit);
-    const long long unit = ((long long)blockIdx.x * kStoreBS + threadIdx.x) / kUnit;
-    if (unit >= units) return;
-    Unit u;
-    const bool have = find_unit(c, a.tok, unit, lane8, mask, &u);
-    const bool first = u.head == 0 && u.group == 0 && lane8 == 0 && blockIdx.y == 0;
-    if (!have) {
-        if (first && u.seq >= 0) atomicOr(c.flags, kCacheFull);
-        return;
-    }
     const bool is_key = blockIdx.y == 0;
-    const T* src = static_cast<const T*>(is_key ? a.keys : a.values) +
-                   (size_t)u.tok * (is_key ? a.key_stride : a.value_stride) + (size_t)u.head * c.dim;
-    const int d0 = u.group * kCacheGroup + lane8 * 8;
-    const int n = min(max(c.dim - d0, 0), 8);
-    float x[8];
-    load8(src + d0, n, vec && n == 8, x);
-    float hi = -INFINITY, lo = INFINITY;
-    bool nan = false;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (i < n) {
-            hi = fmaxf(hi, x[i]);
-            lo = fminf(lo, x[i]);
-            nan |= x[i] != x[i];
-        }
-#pragma unroll
-    for (int o = 4; o; o >>= 1) {
-        hi = fmaxf(hi, __shfl_xor_sync(mask, hi, o));
-        lo = fminf(lo, __shfl_xor_sync(mask, lo, o));
-    }
-    nan = (__ballot_sync(mask, nan) & mask) != 0;
-    float step, low;
-    if (u.group * kCacheGroup >= c.dim) {  // a group of padding
-        step = low = 0.0f;
-    } else if (nan) {
-        step = low = __uint_as_float(0x7FC00000u);
-    } else {
-        // the format's own roundings: f32, then bf16
-        step = bf16_round(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
-        low = bf16_round(lo);
-    }
-    uint32_t code = 0;
-    if (step > 0.0f && step < INFINITY) {
-        const float inv = __fdiv_rn(1.0f, step);
-        if (inv < INFINITY) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i < n) code |= code_of(x[i], low, step, inv) << (4 * i);
-        } else {  // a subnormal step whose reciprocal overflows
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i < n)
-                    code |= (uint32_t)fmin(fmax(rint(((double)x[i] - low) / step), 0.0), 15.0) << (4 * i);
+    const int tok0 = blockIdx.x * run, n_tok = min(run, a.tok.n_tokens - tok0);
+    for (int i = unit; i < n_tok; i += kUnits) {
+        const Place p = place_of(c, a.tok, tok0 + i, l8, mask);
+        if (l8 == 0) {
+            s_place[i] = p;
+            if (is_key && p.row == -2) atomicOr(c.flags, kCacheFull);
+            if (is_key && p.row >= 0) {
+                const size_t at = (size_t)p.seq * c.capacity + p.row;
+                if (a.weights) a.weights[at] = 0.0f;
+                if (a.ids) a.ids[at] = a.token_ids[tok0 + i];
+            }
         }
     }
-    const size_t row = ((size_t)u.seq * c.heads + u.head) * c.rows + u.row;
-    if (is_key) {
-        c.kc[row * 8 * c.G + key_word(c.G, 2 * u.group + (lane8 >> 2), lane8 & 3)] = code;
-    } else {
-        uint32_t w = 0;
+    __syncthreads();
+    const T* src = static_cast<const T*>(is_key ? a.keys : a.values);
+    const size_t stride = is_key ? a.key_stride : a.value_stride;
+    const int per = c.heads * G, units = n_tok * per;
+    for (int u0 = unit; u0 < units; u0 += kUnits * U) {
+        Raw8<T> raw[U];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t v = __shfl_sync(mask, code, lane_of_nibble(i), kUnit);
-            w |= ((v >> (4 * lane8)) & 15u) << (4 * i);
+        for (int i = 0; i < U; ++i) {
+            const int u = u0 + i * kUnits;
+            if (u >= units) continue;
+            const int tok = quotient(u, by), rest = u - tok * per, head = rest / G;
+            const int d = (rest - head * G) * kCacheGroup + 8 * chunk_of(l8);
+            const int n = s_place[tok].row >= 0 ? min(max(c.dim - d, 0), 8) : 0;
+            raw[i] = load8(src + (size_t)(tok0 + tok) * stride + (size_t)head * c.dim + d, n, vec);
         }
-        c.vc[row * 8 * c.G + value_word(c.G, u.group, lane8)] = w;
-    }
-    if (lane8 == 0)
-        (is_key ? c.kp : c.vp)[row * c.G + u.group] = (__float_as_uint(step) >> 16) | (__float_as_uint(low) & 0xFFFF0000u);
-    if (first) {
-        const size_t at = (size_t)u.seq * c.capacity + u.row;
-        if (a.weights) a.weights[at] = 0.0f;
-        if (a.ids) a.ids[at] = a.token_ids[u.tok];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int u = u0 + i * kUnits;
+            if (u >= units) continue;
+            const int tok = quotient(u, by), rest = u - tok * per, head = rest / G, g = rest - head * G;
+            const Place p = s_place[tok];
+            if (p.row < 0) continue;
+            const int chunk = chunk_of(l8), n = min(max(c.dim - g * kCacheGroup - 8 * chunk, 0), 8);
+            float hi, lo, small;
+            extremes(raw[i], n, mask, &hi, &lo, &small);
+            float step = 0.0f, low = 0.0f;
+            uint32_t code = 0;
+            if (g * kCacheGroup < c.dim) {  // not a group of padding
+                // the format's own roundings: f32, then bf16
+                step = bf16_round(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
+                low = bf16_round(lo);
+                if (step > 0.0f && step < INFINITY) {
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = element(raw[i], e);
+                    const float few = std::is_same<T, __half>::value ? 0x1p-10f : 0x1p-13f;
+                    code = codes_of<T>(x, low, step, sizeof(T) == 2 && small < few * step);
+                    if (n < 8) code &= (1u << (4 * n)) - 1;  // padding
+                }
+            }
+            const size_t row = ((size_t)p.seq * c.heads + head) * c.rows + p.row;
+            if (is_key)
+                c.kc[row * 8 * G + key_word(G, 2 * g + (chunk >> 2), chunk & 3)] = code;
+            else
+                c.vc[row * 8 * G + value_word(G, g, l8)] = transpose_nibbles(code, l8, mask);
+            if (l8 == 0)
+                (is_key ? c.kp : c.vp)[row * G + g] = (__float_as_uint(step) >> 16) | (__float_as_uint(low) & 0xFFFF0000u);
+        }
     }
 }
 
-// Rows back as values.
-template <typename T>
-__global__ void __launch_bounds__(kStoreBS) k_cache_read(CacheView c, ReadArgs a, bool vec, long long units) {
-    const int lane8 = threadIdx.x % kUnit;
+// Rows back as values, in the same order.
+template <typename T, int G, int U>
+__global__ void __launch_bounds__(kStoreBS) k_cache_read(CacheView c, ReadArgs a, bool vec, int run, uint32_t by) {
+    __shared__ Place s_place[kUnits * kDeep];
+    const int l8 = threadIdx.x % kUnit, unit = threadIdx.x / kUnit;
     const unsigned mask = 0xFFu << (threadIdx.x % 32 / kUnit * kUnit);
-    const long long unit = ((long long)blockIdx.x * kStoreBS + threadIdx.x) / kUnit;
-    if (unit >= units) return;
-    Unit u;
-    if (!find_unit(c, a.tok, unit, lane8, mask, &u)) return;
     const bool is_key = blockIdx.y == 0;
-    const size_t row = ((size_t)u.seq * c.heads + u.head) * c.rows + u.row;
-    uint32_t code;
-    if (is_key) {
-        code = c.kc[row * 8 * c.G + key_word(c.G, 2 * u.group + (lane8 >> 2), lane8 & 3)];
-    } else {
-        const uint32_t w = c.vc[row * 8 * c.G + value_word(c.G, u.group, lane8)];
-        const int sh = 4 * nibble_of_lane(lane8);
-        code = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) code |= ((__shfl_sync(mask, w, i, kUnit) >> sh) & 15u) << (4 * i);
+    const int tok0 = blockIdx.x * run, n_tok = min(run, a.tok.n_tokens - tok0);
+    for (int i = unit; i < n_tok; i += kUnits) {
+        const Place p = place_of(c, a.tok, tok0 + i, l8, mask);
+        if (l8 == 0) s_place[i] = p;
     }
-    const uint32_t par = (is_key ? c.kp : c.vp)[row * c.G + u.group];
-    const float step = par_step(par), low = par_low(par);
-    const int d0 = u.group * kCacheGroup + lane8 * 8;
-    const int n = min(max(c.dim - d0, 0), 8);
-    if (n == 0) return;
-    float x[8];
+    __syncthreads();
+    T* dst = static_cast<T*>(is_key ? a.keys : a.values);
+    const int per = c.heads * G, units = n_tok * per, chunk = chunk_of(l8);
+    for (int u0 = unit; u0 < units; u0 += kUnits * U) {
+        uint32_t code[U], par[U];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __fmaf_rn(step, (float)((code >> (4 * i)) & 15u), low);
-    T* dst = static_cast<T*>(is_key ? a.keys : a.values) + ((size_t)u.tok * c.heads + u.head) * c.dim + d0;
-    store8(dst, n, vec && n == 8, x);
+        for (int i = 0; i < U; ++i) {
+            const int u = u0 + i * kUnits;
+            if (u >= units) continue;
+            const int tok = quotient(u, by), rest = u - tok * per, head = rest / G, g = rest - head * G;
+            const Place p = s_place[tok];
+            if (p.row < 0) continue;
+            const size_t row = ((size_t)p.seq * c.heads + head) * c.rows + p.row;
+            code[i] = is_key ? c.kc[row * 8 * G + key_word(G, 2 * g + (chunk >> 2), chunk & 3)]
+                             : c.vc[row * 8 * G + value_word(G, g, l8)];
+            par[i] = (is_key ? c.kp : c.vp)[row * G + g];
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int u = u0 + i * kUnits;
+            if (u >= units) continue;
+            const int tok = quotient(u, by), rest = u - tok * per, head = rest / G, g = rest - head * G;
+            if (s_place[tok].row < 0) continue;
+            const uint32_t w = is_key ? code[i] : transpose_nibbles(code[i], l8, mask);
+            const float step = par_step(par[i]), low = par_low(par[i]);
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                // a whole number below 2^23 as the low bits of 2^23 + itself
+                const float v = __fsub_rn(__uint_as_float(0x4B000000u | ((w >> (4 * e)) & 15u)), 8388608.0f);
+                x[e] = __fmaf_rn(step, v, low);
+            }
+            const int d = g * kCacheGroup + 8 * chunk, n = min(max(c.dim - d, 0), 8);
+            store8(dst + ((size_t)(tok0 + tok) * c.heads + head) * c.dim + d, n, vec, x);
+        }
+    }
 }
 
 // ---- eviction -------------------------------------------------------------------------------------
@@ -421,35 +542,81 @@ bool aligned16(const void* p, size_t stride_bytes) {
 
 }  // namespace
 
+namespace {
+
+// Tokens per block and units in flight per thread: four where that still gives every SM its blocks.
+struct StorePlan {
+    int run;
+    uint32_t by;
+    bool deep;
+    dim3 grid;
+};
+StorePlan store_plan(const CacheView& c, int n_tokens) {
+    const int per = c.heads * c.G;
+    StorePlan p{};
+    p.deep = (long long)n_tokens * per >= (long long)kUnits * kDeep * 8 * sm_count();
+    p.run = std::max(1, kUnits * (p.deep ? kDeep : 1) / per);
+    p.by = per == 1 ? 0u : (uint32_t)(((1ull << 32) + per - 1) / per);
+    p.grid = dim3((unsigned)((n_tokens + p.run - 1) / p.run), 2);
+    return p;
+}
+
+template <typename T, int G>
+void start_append(const CacheView& c, const AppendArgs& a, bool vec, const StorePlan& p, cudaStream_t st) {
+    if (p.deep)
+        k_cache_append<T, G, kDeep><<<p.grid, kStoreBS, 0, st>>>(c, a, vec, p.run, p.by);
+    else
+        k_cache_append<T, G, 1><<<p.grid, kStoreBS, 0, st>>>(c, a, vec, p.run, p.by);
+}
+template <typename T, int G>
+void start_read(const CacheView& c, const ReadArgs& a, bool vec, const StorePlan& p, cudaStream_t st) {
+    if (p.deep)
+        k_cache_read<T, G, kDeep><<<p.grid, kStoreBS, 0, st>>>(c, a, vec, p.run, p.by);
+    else
+        k_cache_read<T, G, 1><<<p.grid, kStoreBS, 0, st>>>(c, a, vec, p.run, p.by);
+}
+
+// f with the type and the groups as constants
+template <typename F>
+void by_type_and_groups(int type, int G, F f) {
+    auto groups = [&](auto t) {
+        using T = decltype(t);
+        if (G == 1)
+            f(T(), std::integral_constant<int, 1>());
+        else if (G == 2)
+            f(T(), std::integral_constant<int, 2>());
+        else if (G == 4)
+            f(T(), std::integral_constant<int, 4>());
+        else
+            f(T(), std::integral_constant<int, 6>());
+    };
+    if (type == kF32)
+        groups(float());
+    else if (type == kF16)
+        groups(__half());
+    else
+        groups(__nv_bfloat16());
+}
+
+}  // namespace
+
 void launch_cache_append(const CacheView& c, const AppendArgs& a, cudaStream_t st) {
     if (a.tok.n_tokens <= 0) return;
-    const long long units = (long long)a.tok.n_tokens * c.heads * c.G;
-    const dim3 grid((unsigned)((units * kUnit + kStoreBS - 1) / kStoreBS), 2);
     const size_t es = a.type == kF32 ? 4 : 2;
     const bool vec = aligned16(a.keys, a.key_stride * es) && aligned16(a.values, a.value_stride * es) &&
                      (size_t)c.dim * es % 16 == 0;
+    const StorePlan p = store_plan(c, a.tok.n_tokens);
     Tick tk(kKCacheAppend, st);
-    if (a.type == kF32)
-        k_cache_append<float><<<grid, kStoreBS, 0, st>>>(c, a, vec, units);
-    else if (a.type == kF16)
-        k_cache_append<__half><<<grid, kStoreBS, 0, st>>>(c, a, vec, units);
-    else
-        k_cache_append<__nv_bfloat16><<<grid, kStoreBS, 0, st>>>(c, a, vec, units);
+    by_type_and_groups(a.type, c.G, [&](auto t, auto g) { start_append<decltype(t), decltype(g)::value>(c, a, vec, p, st); });
 }
 
 void launch_cache_read(const CacheView& c, const ReadArgs& a, cudaStream_t st) {
     if (a.tok.n_tokens <= 0) return;
-    const long long units = (long long)a.tok.n_tokens * c.heads * c.G;
-    const dim3 grid((unsigned)((units * kUnit + kStoreBS - 1) / kStoreBS), 2);
     const size_t es = a.type == kF32 ? 4 : 2;
     const bool vec = aligned16(a.keys, 0) && aligned16(a.values, 0) && (size_t)c.dim * es % 16 == 0;
+    const StorePlan p = store_plan(c, a.tok.n_tokens);
     Tick tk(kKCacheRead, st);
-    if (a.type == kF32)
-        k_cache_read<float><<<grid, kStoreBS, 0, st>>>(c, a, vec, units);
-    else if (a.type == kF16)
-        k_cache_read<__half><<<grid, kStoreBS, 0, st>>>(c, a, vec, units);
-    else
-        k_cache_read<__nv_bfloat16><<<grid, kStoreBS, 0, st>>>(c, a, vec, units);
+    by_type_and_groups(a.type, c.G, [&](auto t, auto g) { start_read<decltype(t), decltype(g)::value>(c, a, vec, p, st); });
 }
 
 size_t cache_evict_workspace(const CacheView& c) {
