@@ -24,17 +24,14 @@ constexpr int kDeep = 4;
 __device__ __forceinline__ int chunk_of(int l) { return 2 * (l & 3) + (l >> 2); }
 
 // Nibble k of lane l <-> nibble l of lane k, within aligned groups of 8 lanes: halves, bytes, nibbles.
-__device__ __forceinline__ uint32_t transpose_nibbles(uint32_t x, int l, unsigned mask) {
-    uint32_t y = __shfl_xor_sync(mask, x, 4);
+__device__ __forceinline__ uint32_t transpose_nibbles(uint32_t x, int l) {
+    uint32_t y = __shfl_xor_sync(~0u, x, 4);
     x = __byte_perm(x, y, l & 4 ? 0x3276 : 0x5410);
-    y = __shfl_xor_sync(mask, x, 2);
+    y = __shfl_xor_sync(~0u, x, 2);
     x = __byte_perm(x, y, l & 2 ? 0x3715 : 0x6240);
-    y = __shfl_xor_sync(mask, x, 1);
+    y = __shfl_xor_sync(~0u, x, 1);
     return l & 1 ? (x & 0xF0F0F0F0u) | ((y >> 4) & 0x0F0F0F0Fu) : (x & 0x0F0F0F0Fu) | ((y << 4) & 0xF0F0F0F0u);
 }
-
-// u / per for the small numbers of a block (u < 2^13, per < 2^13), by = ceil(2^32 / per), 0 for per = 1.
-__device__ __forceinline__ int quotient(int u, uint32_t by) { return by ? (int)__umulhi((uint32_t)u, by) : u; }
 
 // Where the tokens of a block go: the row of token i, or -1 (padding), or -2 (past the capacity).
 struct Place {
@@ -132,7 +129,7 @@ __device__ __forceinline__ float element(const Raw8<T>& r, int i) {
 
 // Largest and smallest of a unit's 64 elements (NaN if one is), and this lane's smallest magnitude. 16-bit
 // types by packed comparisons: the largest and the negated smallest go through the lanes as one word.
-__device__ __forceinline__ void extremes(const Raw8<float>& r, int n, unsigned mask, float* hi, float* lo, float* small) {
+__device__ __forceinline__ void extremes(const Raw8<float>& r, int n, float* hi, float* lo, float* small) {
     float h = -INFINITY, l = INFINITY;
     bool nan = false;
 #pragma unroll
@@ -145,10 +142,10 @@ __device__ __forceinline__ void extremes(const Raw8<float>& r, int n, unsigned m
         }
 #pragma unroll
     for (int o = 4; o; o >>= 1) {
-        h = fmaxf(h, __shfl_xor_sync(mask, h, o));
-        l = fminf(l, __shfl_xor_sync(mask, l, o));
+        h = fmaxf(h, __shfl_xor_sync(~0u, h, o));
+        l = fminf(l, __shfl_xor_sync(~0u, l, o));
+        nan |= __shfl_xor_sync(~0u, (int)nan, o) != 0;
     }
-    nan = (__ballot_sync(mask, nan) & mask) != 0;
     *hi = nan ? __uint_as_float(0x7FC00000u) : h;
     *lo = nan ? __uint_as_float(0x7FC00000u) : l;
     *small = 0.0f;
@@ -171,7 +168,7 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
     return *reinterpret_cast<const uint32_t*>(&m);
 }
 template <typename T>
-__device__ __forceinline__ void extremes(const Raw8<T>& r, int n, unsigned mask, float* hi, float* lo, float* small) {
+__device__ __forceinline__ void extremes(const Raw8<T>& r, int n, float* hi, float* lo, float* small) {
     using P = typename Pair<T>::type;
     uint32_t up[4], down[4];  // the elements, and the elements negated; -inf where there is none
 #pragma unroll
@@ -192,7 +189,7 @@ __device__ __forceinline__ void extremes(const Raw8<T>& r, int n, unsigned mask,
     const uint32_t d = max2<P>(max2<P>(down[0], down[1]), max2<P>(down[2], down[3]));
     uint32_t m = max2<P>(__byte_perm(u, d, 0x5410), __byte_perm(u, d, 0x7632));
 #pragma unroll
-    for (int o = 4; o; o >>= 1) m = max2<P>(m, __shfl_xor_sync(mask, m, o));
+    for (int o = 4; o; o >>= 1) m = max2<P>(m, __shfl_xor_sync(~0u, m, o));
     *hi = to_f32<T>(m & 0xFFFFu);
     *lo = -to_f32<T>(m >> 16);
 }
@@ -216,56 +213,78 @@ __device__ __forceinline__ void store8(T* __restrict__ p, int n, bool vec, const
     }
 }
 
-// Rows into the cache. blockIdx.x: a run of `run` tokens, blockIdx.y: 0 keys, 1 values. Eight lanes take
-// a group of 64 dimensions of one head; a block's units go over its tokens' heads and groups in order,
-// U of a thread at a time. Bound by HBM (one read of the tokens, one write of the rows) with U = 4.
-template <typename T, int G, int U>
-__global__ void __launch_bounds__(kStoreBS) k_cache_append(CacheView c, AppendArgs a, bool vec, int run, uint32_t by) {
-    __shared__ Place s_place[kUnits * kDeep];
-    const int l8 = threadIdx.x % kUnit, unit = threadIdx.x / kUnit;
+// How a block goes over its run of tokens. A pass takes `side` tokens next to each other; a unit keeps its
+// head and group through all passes, U of which a thread has in flight at a time.
+struct StoreShape {
+    int run;   // tokens of a block
+    int side;  // tokens of a pass
+    int wide;  // units of a token that a block takes (the grid's y covers the others)
+};
+
+// Places of a block's tokens, as row numbers of the first head (-1: none).
+constexpr int kMaxRun = kUnits * kDeep * 4;
+
+__device__ __forceinline__ void find_places(const CacheView& c, const CacheTokens& tk, int tok0, int n_tok,
+                                            long long* place, bool flag, float* weights, uint64_t* ids,
+                                            const uint64_t* token_ids) {
+    const int l8 = threadIdx.x % kUnit;
     const unsigned mask = 0xFFu << (threadIdx.x % 32 / kUnit * kUnit);
-    const bool is_key = blockIdx.y == 0;
-    const int tok0 = blockIdx.x * run, n_tok = min(run, a.tok.n_tokens - tok0);
-    for (int i = unit; i < n_tok; i += kUnits) {
-        const Place p = place_of(c, a.tok, tok0 + i, l8, mask);
+    for (int i = threadIdx.x / kUnit; i < n_tok; i += kUnits) {
+        const Place p = place_of(c, tk, tok0 + i, l8, mask);
         if (l8 == 0) {
-            s_place[i] = p;
-            if (is_key && p.row == -2) atomicOr(c.flags, kCacheFull);
-            if (is_key && p.row >= 0) {
-                const size_t at = (size_t)p.seq * c.capacity + p.row;
-                if (a.weights) a.weights[at] = 0.0f;
-                if (a.ids) a.ids[at] = a.token_ids[tok0 + i];
+            place[i] = p.row < 0 ? -1 : (long long)p.seq * c.heads * c.rows + p.row;
+            if (flag) {
+                if (p.row == -2) atomicOr(c.flags, kCacheFull);
+                if (p.row >= 0) {
+                    const size_t at = (size_t)p.seq * c.capacity + p.row;
+                    if (weights) weights[at] = 0.0f;
+                    if (ids) ids[at] = token_ids[tok0 + i];
+                }
             }
         }
     }
     __syncthreads();
-    const T* src = static_cast<const T*>(is_key ? a.keys : a.values);
+}
+
+// Rows into the cache. blockIdx.x: a run of tokens; blockIdx.y: even keys, odd values, times the slices of a
+// token's units. Eight lanes take a group of 64 dimensions of one head. Every lane goes through the same
+// passes; those without a unit, or whose token has no row, load and store nothing.
+template <typename T, int G, int U>
+__global__ void __launch_bounds__(kStoreBS) k_cache_append(CacheView c, AppendArgs a, bool vec, StoreShape sh) {
+    __shared__ long long s_place[kMaxRun];
+    const bool is_key = !(blockIdx.y & 1);
+    const int tok0 = blockIdx.x * sh.run, n_tok = min(sh.run, a.tok.n_tokens - tok0);
+    find_places(c, a.tok, tok0, n_tok, s_place, blockIdx.y == 0, a.weights, a.ids, a.token_ids);
+
+    const int l8 = threadIdx.x % kUnit, unit = threadIdx.x / kUnit, chunk = chunk_of(l8);
+    const int mine = unit / sh.wide, rest = (blockIdx.y >> 1) * kUnits + unit - mine * sh.wide;
+    const int head = rest / G, g = rest - head * G;
+    const int d = g * kCacheGroup + 8 * chunk;
+    const bool in = mine < sh.side && head < c.heads;
+    const int have = in ? min(max(c.dim - d, 0), 8) : 0;
+    const bool pad = g * kCacheGroup >= c.dim;  // a group of padding
     const size_t stride = is_key ? a.key_stride : a.value_stride;
-    const int per = c.heads * G, units = n_tok * per;
-    for (int u0 = unit; u0 < units; u0 += kUnits * U) {
+    const T* src = static_cast<const T*>(is_key ? a.keys : a.values) + (size_t)(tok0 + mine) * stride +
+                   (size_t)head * c.dim + d;
+    uint32_t* codes = (is_key ? c.kc : c.vc) + (size_t)head * c.rows * 8 * G +
+                      (is_key ? key_word(G, 2 * g + (chunk >> 2), chunk & 3) : value_word(G, g, l8));
+    uint32_t* params = (is_key ? c.kp : c.vp) + (size_t)head * c.rows * G + g;
+    for (int t0 = 0; t0 < n_tok; t0 += sh.side * U) {
         Raw8<T> raw[U];
+        long long row[U];
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            const int u = u0 + i * kUnits;
-            if (u >= units) continue;
-            const int tok = quotient(u, by), rest = u - tok * per, head = rest / G;
-            const int d = (rest - head * G) * kCacheGroup + 8 * chunk_of(l8);
-            const int n = s_place[tok].row >= 0 ? min(max(c.dim - d, 0), 8) : 0;
-            raw[i] = load8(src + (size_t)(tok0 + tok) * stride + (size_t)head * c.dim + d, n, vec);
+            const int t = t0 + i * sh.side + mine;
+            row[i] = in && t < n_tok ? s_place[t] : -1;
+            raw[i] = load8(src + (size_t)(t0 + i * sh.side) * stride, row[i] >= 0 ? have : 0, vec);
         }
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            const int u = u0 + i * kUnits;
-            if (u >= units) continue;
-            const int tok = quotient(u, by), rest = u - tok * per, head = rest / G, g = rest - head * G;
-            const Place p = s_place[tok];
-            if (p.row < 0) continue;
-            const int chunk = chunk_of(l8), n = min(max(c.dim - g * kCacheGroup - 8 * chunk, 0), 8);
             float hi, lo, small;
-            extremes(raw[i], n, mask, &hi, &lo, &small);
+            extremes(raw[i], have, &hi, &lo, &small);
             float step = 0.0f, low = 0.0f;
             uint32_t code = 0;
-            if (g * kCacheGroup < c.dim) {  // not a group of padding
+            if (!pad) {
                 // the format's own roundings: f32, then bf16
                 step = bf16_round(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
                 low = bf16_round(lo);
@@ -275,56 +294,51 @@ __global__ void __launch_bounds__(kStoreBS) k_cache_append(CacheView c, AppendAr
                     for (int e = 0; e < 8; ++e) x[e] = element(raw[i], e);
                     const float few = std::is_same<T, __half>::value ? 0x1p-10f : 0x1p-13f;
                     code = codes_of<T>(x, low, step, sizeof(T) == 2 && small < few * step);
-                    if (n < 8) code &= (1u << (4 * n)) - 1;  // padding
+                    if (have < 8) code &= (1u << (4 * have)) - 1;  // padding
                 }
             }
-            const size_t row = ((size_t)p.seq * c.heads + head) * c.rows + p.row;
-            if (is_key)
-                c.kc[row * 8 * G + key_word(G, 2 * g + (chunk >> 2), chunk & 3)] = code;
-            else
-                c.vc[row * 8 * G + value_word(G, g, l8)] = transpose_nibbles(code, l8, mask);
-            if (l8 == 0)
-                (is_key ? c.kp : c.vp)[row * G + g] = (__float_as_uint(step) >> 16) | (__float_as_uint(low) & 0xFFFF0000u);
+            if (!is_key) code = transpose_nibbles(code, l8);
+            if (row[i] >= 0) {
+                codes[row[i] * (8 * G)] = code;
+                if (l8 == 0) params[row[i] * G] = (__float_as_uint(step) >> 16) | (__float_as_uint(low) & 0xFFFF0000u);
+            }
         }
     }
 }
 
 // Rows back as values, in the same order.
 template <typename T, int G, int U>
-__global__ void __launch_bounds__(kStoreBS) k_cache_read(CacheView c, ReadArgs a, bool vec, int run, uint32_t by) {
-    __shared__ Place s_place[kUnits * kDeep];
-    const int l8 = threadIdx.x % kUnit, unit = threadIdx.x / kUnit;
-    const unsigned mask = 0xFFu << (threadIdx.x % 32 / kUnit * kUnit);
-    const bool is_key = blockIdx.y == 0;
-    const int tok0 = blockIdx.x * run, n_tok = min(run, a.tok.n_tokens - tok0);
-    for (int i = unit; i < n_tok; i += kUnits) {
-        const Place p = place_of(c, a.tok, tok0 + i, l8, mask);
-        if (l8 == 0) s_place[i] = p;
-    }
-    __syncthreads();
-    T* dst = static_cast<T*>(is_key ? a.keys : a.values);
-    const int per = c.heads * G, units = n_tok * per, chunk = chunk_of(l8);
-    for (int u0 = unit; u0 < units; u0 += kUnits * U) {
+__global__ void __launch_bounds__(kStoreBS) k_cache_read(CacheView c, ReadArgs a, bool vec, StoreShape sh) {
+    __shared__ long long s_place[kMaxRun];
+    const bool is_key = !(blockIdx.y & 1);
+    const int tok0 = blockIdx.x * sh.run, n_tok = min(sh.run, a.tok.n_tokens - tok0);
+    find_places(c, a.tok, tok0, n_tok, s_place, false, nullptr, nullptr, nullptr);
+
+    const int l8 = threadIdx.x % kUnit, unit = threadIdx.x / kUnit, chunk = chunk_of(l8);
+    const int mine = unit / sh.wide, rest = (blockIdx.y >> 1) * kUnits + unit - mine * sh.wide;
+    const int head = rest / G, g = rest - head * G;
+    const int d = g * kCacheGroup + 8 * chunk;
+    const bool in = mine < sh.side && head < c.heads;
+    const int have = min(max(c.dim - d, 0), 8);
+    const size_t stride = (size_t)c.heads * c.dim;
+    T* dst = static_cast<T*>(is_key ? a.keys : a.values) + (size_t)(tok0 + mine) * stride + (size_t)head * c.dim + d;
+    const uint32_t* codes = (is_key ? c.kc : c.vc) + (size_t)head * c.rows * 8 * G +
+                            (is_key ? key_word(G, 2 * g + (chunk >> 2), chunk & 3) : value_word(G, g, l8));
+    const uint32_t* params = (is_key ? c.kp : c.vp) + (size_t)head * c.rows * G + g;
+    for (int t0 = 0; t0 < n_tok; t0 += sh.side * U) {
         uint32_t code[U], par[U];
+        bool there[U];
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            const int u = u0 + i * kUnits;
-            if (u >= units) continue;
-            const int tok = quotient(u, by), rest = u - tok * per, head = rest / G, g = rest - head * G;
-            const Place p = s_place[tok];
-            if (p.row < 0) continue;
-            const size_t row = ((size_t)p.seq * c.heads + head) * c.rows + p.row;
-            code[i] = is_key ? c.kc[row * 8 * G + key_word(G, 2 * g + (chunk >> 2), chunk & 3)]
-                             : c.vc[row * 8 * G + value_word(G, g, l8)];
-            par[i] = (is_key ? c.kp : c.vp)[row * G + g];
+            const int t = t0 + i * sh.side + mine;
+            const long long row = in && t < n_tok ? s_place[t] : -1;
+            there[i] = row >= 0;
+            code[i] = there[i] ? codes[row * (8 * G)] : 0u;
+            par[i] = there[i] ? params[row * G] : 0u;
         }
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            const int u = u0 + i * kUnits;
-            if (u >= units) continue;
-            const int tok = quotient(u, by), rest = u - tok * per, head = rest / G, g = rest - head * G;
-            if (s_place[tok].row < 0) continue;
-            const uint32_t w = is_key ? code[i] : transpose_nibbles(code[i], l8, mask);
+            const uint32_t w = is_key ? code[i] : transpose_nibbles(code[i], l8);
             const float step = par_step(par[i]), low = par_low(par[i]);
             float x[8];
 #pragma unroll
@@ -333,8 +347,7 @@ __global__ void __launch_bounds__(kStoreBS) k_cache_read(CacheView c, ReadArgs a
                 const float v = __fsub_rn(__uint_as_float(0x4B000000u | ((w >> (4 * e)) & 15u)), 8388608.0f);
                 x[e] = __fmaf_rn(step, v, low);
             }
-            const int d = g * kCacheGroup + 8 * chunk, n = min(max(c.dim - d, 0), 8);
-            store8(dst + ((size_t)(tok0 + tok) * c.heads + head) * c.dim + d, n, vec, x);
+            if (there[i]) store8(dst + (size_t)(t0 + i * sh.side) * stride, have, vec, x);
         }
     }
 }
@@ -544,36 +557,38 @@ bool aligned16(const void* p, size_t stride_bytes) {
 
 namespace {
 
-// Tokens per block and units in flight per thread: four where that still gives every SM its blocks.
+// Passes in flight per thread and tokens per block: four and four times that many where it still gives
+// every SM its blocks.
 struct StorePlan {
-    int run;
-    uint32_t by;
+    StoreShape shape;
     bool deep;
     dim3 grid;
 };
 StorePlan store_plan(const CacheView& c, int n_tokens) {
-    const int per = c.heads * c.G;
+    const int per = c.heads * c.G, slices = (per + kUnits - 1) / kUnits;
     StorePlan p{};
-    p.deep = (long long)n_tokens * per >= (long long)kUnits * kDeep * 8 * sm_count();
-    p.run = std::max(1, kUnits * (p.deep ? kDeep : 1) / per);
-    p.by = per == 1 ? 0u : (uint32_t)(((1ull << 32) + per - 1) / per);
-    p.grid = dim3((unsigned)((n_tokens + p.run - 1) / p.run), 2);
+    p.shape.wide = std::min(per, kUnits);
+    p.shape.side = kUnits / p.shape.wide;
+    const long long tokens_all = 4ll * sm_count() * p.shape.side * kDeep * 4;
+    p.deep = (long long)n_tokens * slices * 2 >= tokens_all;
+    p.shape.run = p.shape.side * (p.deep ? kDeep * 4 : 1);
+    p.grid = dim3((unsigned)((n_tokens + p.shape.run - 1) / p.shape.run), (unsigned)(2 * slices));
     return p;
 }
 
 template <typename T, int G>
 void start_append(const CacheView& c, const AppendArgs& a, bool vec, const StorePlan& p, cudaStream_t st) {
     if (p.deep)
-        k_cache_append<T, G, kDeep><<<p.grid, kStoreBS, 0, st>>>(c, a, vec, p.run, p.by);
+        k_cache_append<T, G, kDeep><<<p.grid, kStoreBS, 0, st>>>(c, a, vec, p.shape);
     else
-        k_cache_append<T, G, 1><<<p.grid, kStoreBS, 0, st>>>(c, a, vec, p.run, p.by);
+        k_cache_append<T, G, 1><<<p.grid, kStoreBS, 0, st>>>(c, a, vec, p.shape);
 }
 template <typename T, int G>
 void start_read(const CacheView& c, const ReadArgs& a, bool vec, const StorePlan& p, cudaStream_t st) {
     if (p.deep)
-        k_cache_read<T, G, kDeep><<<p.grid, kStoreBS, 0, st>>>(c, a, vec, p.run, p.by);
+        k_cache_read<T, G, kDeep><<<p.grid, kStoreBS, 0, st>>>(c, a, vec, p.shape);
     else
-        k_cache_read<T, G, 1><<<p.grid, kStoreBS, 0, st>>>(c, a, vec, p.run, p.by);
+        k_cache_read<T, G, 1><<<p.grid, kStoreBS, 0, st>>>(c, a, vec, p.shape);
 }
 
 // f with the type and the groups as constants
