@@ -1,4 +1,6 @@
 // The attention cache's storage: rows into 4 bits and back, and eviction by accumulated weight.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -355,6 +357,10 @@ __global__ void __launch_bounds__(kStoreBS) k_cache_read(CacheView c, ReadArgs a
 // ---- eviction -------------------------------------------------------------------------------------
 constexpr int kSelBS = 1024;
 constexpr int kSelWarps = kSelBS / 32;
+constexpr int kSelCluster = 8;
+constexpr int kDigit = 11;  // bits of a round
+constexpr int kBuckets = 1 << kDigit;
+constexpr int kSelKeys = 40 * 1024;  // keys that fit beside the counters
 
 struct EvictWork {
     int32_t* n_move;  // [n_seqs]
@@ -370,106 +376,162 @@ __host__ __device__ inline EvictWork evict_work(void* ws, int n_seqs, int capaci
     return w;
 }
 
-// Block-wide exclusive sums of three counts per warp; total in the last entry.
-__device__ __forceinline__ void scan_warps(int (*cnt)[3], int warp, int lane) {
-    __syncthreads();
-    if (warp == 0) {
-        for (int q = 0; q < 3; ++q) {
-            const int v = cnt[lane][q];
-            int s = v;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int t = __shfl_up_sync(~0u, s, o);
-                if (lane >= o) s += t;
-            }
-            cnt[lane][q] = s - v;
-            if (lane == 31) cnt[32][q] = s;
-        }
-    }
-    __syncthreads();
+// The barrier of a cluster of N blocks.
+template <int N>
+__device__ __forceinline__ void sync_blocks() {
+    if constexpr (N == 1)
+        __syncthreads();
+    else
+        cooperative_groups::this_cluster().sync();
 }
 
-// One CTA per sequence: the keep-th largest weight by four rounds of 256-bucket counting over the
-// order-preserving keys, then which rows stay, which leave and which move where.
+// Sums of the counts before this warp (all three), over the cluster's blocks in order; total in `all`.
+// s_cnt: [kSelWarps + 1][3], the last entry the block's sum.
+template <int N>
+__device__ __forceinline__ void scan_counts(int (*s_cnt)[3], int warp, int lane, int (&before)[3], int (&all)[3]) {
+    const auto cl = cooperative_groups::this_cluster();
+    __syncthreads();
+    if (warp < 3) {
+        const int v = s_cnt[lane][warp];
+        int s = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(~0u, s, o);
+            if (lane >= o) s += t;
+        }
+        __syncwarp();
+        s_cnt[lane][warp] = s - v;
+        if (lane == 31) s_cnt[kSelWarps][warp] = s;
+    }
+    sync_blocks<N>();
+    int v[N][3];
+#pragma unroll
+    for (int r = 0; r < N; ++r)
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+            v[r][q] = N == 1 ? s_cnt[kSelWarps][q] : *cl.map_shared_rank(&s_cnt[kSelWarps][q], r);
+    const int rank = N == 1 ? 0 : (int)cl.block_rank();
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+        before[q] = s_cnt[warp][q];
+        all[q] = 0;
+#pragma unroll
+        for (int r = 0; r < N; ++r) {
+            all[q] += v[r][q];
+            before[q] += r < rank ? v[r][q] : 0;
+        }
+    }
+    sync_blocks<N>();  // the counters may be written again
+}
+
+// A cluster per sequence: the keep-th largest weight by three rounds of counting over the
+// order-preserving keys (11, 11 and 10 bits from the top), then which rows stay, which leave and which
+// move where. A block takes one stretch of the rows and keeps their keys in shared memory; counts are
+// gathered over the cluster, ranks follow the rows' order. Bound by the latency of its dozen
+// barriers; one block took 57 us for 31,000 rows where eight take a few.
+template <int N>
 __global__ void __launch_bounds__(kSelBS) k_cache_select(CacheView c, EvictArgs a, int key_cap) {
+    const auto cl = cooperative_groups::this_cluster();
     extern __shared__ uint32_t s_key[];
-    __shared__ int s_hist[256];
+    __shared__ __align__(8) int s_hist[kBuckets];
     __shared__ int s_cnt[kSelWarps + 1][3];
+    __shared__ int s_sum[kSelWarps];
     __shared__ int s_pick[2];
-    const int s = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int rank = N == 1 ? 0 : (int)cl.block_rank();
+    const int s = blockIdx.x / N, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int L = min(max(a.lengths[s], 0), c.capacity), m = min(L, a.keep);
-    const float* w = a.w_in + (size_t)s * c.capacity;
-    const uint64_t* ids = a.ids_in ? a.ids_in + (size_t)s * c.capacity : nullptr;
-    const uint64_t from = a.protect_from && ids ? a.protect_from[s] : ~0ull;
+    const size_t base = (size_t)s * c.capacity;
+    const float* w = a.w_in + base;
+    const uint64_t* ids = a.ids_in ? a.ids_in + base : nullptr;
     const bool guard = a.protect_from && ids;
+    const uint64_t from = guard ? a.protect_from[s] : 0;
+    // every warp takes one stretch of rows
+    const int per = (L + N * kSelBS - 1) / (N * kSelBS) * 32;
+    const int b0 = min(L, rank * kSelWarps * per), b1 = min(L, b0 + kSelWarps * per);
+    const int r0 = min(b1, b0 + warp * per), r1 = min(b1, r0 + per);
     auto make_key = [&](int r) -> uint32_t {
         const float x = w[r];
         // ids from protect_from on and NaN rank as +inf; -0 as 0
         const bool top = (guard && ids[r] >= from) || x != x;
         return float_key(top ? INFINITY : __fadd_rn(x, 0.0f));
     };
-    auto key = [&](int r) -> uint32_t { return r < key_cap ? s_key[r] : make_key(r); };
-    for (int r = threadIdx.x; r < min(L, key_cap); r += kSelBS) s_key[r] = make_key(r);
-    // the m-th largest key T and how many rows equal to it stay (the lowest rows of them)
+    auto key = [&](int r) -> uint32_t { return r - b0 < key_cap ? s_key[r - b0] : make_key(r); };
+    const bool all_stay = m >= L, cut = !all_stay && m > 0;
+    if (cut) {
+#pragma unroll 4
+        for (int r = b0 + threadIdx.x; r < min(b1, b0 + key_cap); r += kSelBS) s_key[r - b0] = make_key(r);
+    }
+    // the m-th largest key T, and how many rows equal to it stay (the lowest rows of them)
     uint32_t T = 0;
-    int need = m;  // rank from the top still to be placed among the keys with T's prefix
-    if (m < L && m > 0) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = threadIdx.x; i < 256; i += kSelBS) s_hist[i] = 0;
-            __syncthreads();
-            for (int r = threadIdx.x; r < L; r += kSelBS) {
-                const uint32_t k = key(r);
-                if (shift == 24 || (k >> (shift + 8)) == (T >> (shift + 8))) atomicAdd(&s_hist[(k >> shift) & 255], 1);
+    int need = m;
+    if (cut) {
+        int high = 32;  // bits of T below `high` are still unknown
+#pragma unroll 1
+        for (int round = 0; round < 3; ++round) {
+            const int bits = round < 2 ? kDigit : 32 - 2 * kDigit, shift = high - bits;
+            for (int i = threadIdx.x; i < kBuckets; i += kSelBS) s_hist[i] = 0;
+            sync_blocks<N>();  // and the keys are there
+            for (int r = b0 + warp * 32; r < b1; r += kSelBS) {
+                const uint32_t k = r + lane < b1 ? key(r + lane) : 0u;
+                const bool in = r + lane < b1 && (round == 0 || (k >> high) == (T >> high));
+                const uint32_t d = in ? (k >> shift) & ((1u << bits) - 1) : ~0u;
+                // one addition per distinct digit of the warp: weights crowd in a few buckets
+                const unsigned same = __match_any_sync(~0u, d);
+                if (in && lane == __ffs(same) - 1) atomicAdd(&s_hist[d], __popc(same));
             }
-            __syncthreads();
-            if (warp == 0) {
-                // lane l holds buckets 255 - 8 l .. 248 - 8 l, from the top
-                int sum = 0;
-                for (int i = 0; i < 8; ++i) sum += s_hist[255 - 8 * lane - i];
-                int incl = sum;
+            sync_blocks<N>();
+            // buckets from the top, two a thread
+            const int top = kBuckets - 2 - 2 * (int)threadIdx.x;
+            int2 part[N];
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int t = __shfl_up_sync(~0u, incl, o);
-                    if (lane >= o) incl += t;
-                }
-                int before = incl - sum;
-                if (before < need && incl >= need) {
-                    for (int i = 0; i < 8; ++i) {
-                        const int h = s_hist[255 - 8 * lane - i];
-                        if (before + h >= need) {
-                            s_pick[0] = 255 - 8 * lane - i;
-                            s_pick[1] = need - before;
-                            break;
-                        }
-                        before += h;
-                    }
-                }
+            for (int r = 0; r < N; ++r)
+                part[r] = *reinterpret_cast<const int2*>(N == 1 ? &s_hist[top] : cl.map_shared_rank(&s_hist[top], r));
+            int h[2] = {0, 0};
+#pragma unroll
+            for (int r = 0; r < N; ++r) h[0] += part[r].y, h[1] += part[r].x;
+            const int sum = h[0] + h[1];
+            int incl = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int t = __shfl_up_sync(~0u, incl, o);
+                if (lane >= o) incl += t;
             }
+            if (lane == 31) s_sum[warp] = incl;
             __syncthreads();
+            int earlier = lane < warp ? s_sum[lane] : 0;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) earlier += __shfl_xor_sync(~0u, earlier, o);
+            int before = incl - sum + earlier;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (before < need && before + h[i] >= need) {
+                    s_pick[0] = kBuckets - 1 - 2 * (int)threadIdx.x - i;
+                    s_pick[1] = need - before;
+                }
+                before += h[i];
+            }
+            sync_blocks<N>();  // everyone has read the histograms
             T |= (uint32_t)s_pick[0] << shift;
             need = s_pick[1];
+            high = shift;
         }
     }
-    const bool all = m >= L;
-    // every warp takes one stretch of rows, so that ranks follow the rows' order
-    const int per = (L + kSelWarps * 32 - 1) / (kSelWarps * 32) * 32;
-    const int r0 = warp * per, r1 = min(L, r0 + per);
-    int eq = 0;
-    __syncthreads();
-    if (!all && m > 0)
-        for (int r = r0 + lane; r < r1; r += 32) eq += key(r) == T;
-    for (int o = 16; o; o >>= 1) eq += __shfl_xor_sync(~0u, eq, o);
-    if (lane == 0) s_cnt[warp][0] = eq, s_cnt[warp][1] = s_cnt[warp][2] = 0;
-    scan_warps(s_cnt, warp, lane);
-    const int eq0 = s_cnt[warp][0];
+    // how many equal rows lie before this warp's
     const unsigned below = (1u << lane) - 1;
-    auto kept_row = [&](int r, int& eq_seen) -> bool {
+    int before[3], all[3];
+    int eq = 0;
+    if (cut)
+        for (int r = r0; r < r1; r += 32) eq += __popc(__ballot_sync(~0u, r + lane < r1 && key(min(r + lane, r1 - 1)) == T));
+    if (lane == 0) s_cnt[warp][0] = eq, s_cnt[warp][1] = s_cnt[warp][2] = 0;
+    scan_counts<N>(s_cnt, warp, lane, before, all);
+    const int eq0 = before[0];
+    auto kept_row = [&](int r, int& seen) -> bool {
         const bool in = r < r1;
-        const uint32_t k = in && !all && m > 0 ? key(r) : 0u;
-        const bool is_eq = in && !all && m > 0 && k == T;
+        const uint32_t k = in && cut ? key(r) : 0u;
+        const bool is_eq = in && cut && k == T;
         const unsigned b = __ballot_sync(~0u, is_eq);
-        const bool keep = in && (all || (m > 0 && (k > T || (is_eq && eq_seen + __popc(b & below) < need))));
-        eq_seen += __popc(b);
+        const bool keep = in && (all_stay || (cut && (k > T || (is_eq && seen + __popc(b & below) < need))));
+        seen += __popc(b);
         return keep;
     };
     int n_hole = 0, n_src = 0, n_gone = 0, seen = eq0;
@@ -480,16 +542,14 @@ __global__ void __launch_bounds__(kSelBS) k_cache_select(CacheView c, EvictArgs 
         n_src += __popc(__ballot_sync(~0u, x < r1 && x >= m && k));
         n_gone += __popc(__ballot_sync(~0u, x < r1 && !k));
     }
-    __syncthreads();
     if (lane == 0) s_cnt[warp][0] = n_hole, s_cnt[warp][1] = n_src, s_cnt[warp][2] = n_gone;
-    scan_warps(s_cnt, warp, lane);
-    int at_hole = s_cnt[warp][0], at_src = s_cnt[warp][1], at_gone = s_cnt[warp][2];
+    scan_counts<N>(s_cnt, warp, lane, before, all);
     const EvictWork wk = evict_work(a.workspace, c.n_seqs, c.capacity);
-    if (threadIdx.x == 0) {
-        wk.n_move[s] = s_cnt[kSelWarps][0];
+    if (threadIdx.x == 0 && rank == 0) {
+        wk.n_move[s] = all[0];
         a.new_lengths[s] = m;
     }
-    const size_t base = (size_t)s * c.capacity;
+    int at_hole = before[0], at_src = before[1], at_gone = before[2];
     seen = eq0;
     for (int r = r0; r < r1; r += 32) {
         const int x = r + lane;
@@ -511,40 +571,66 @@ __global__ void __launch_bounds__(kSelBS) k_cache_select(CacheView c, EvictArgs 
 }
 
 // Move i of a sequence takes row src[i] (at or past the new length) to row hole[i] (below it), so no
-// row is both read and written. A warp moves one row of one head.
+// row is both read and written. A thread moves one of a row's pieces of one head (16 bytes of codes, or the
+// parameters of its keys or values), four at a time.
+template <int G>
 __global__ void __launch_bounds__(256) k_cache_move(CacheView c, EvictArgs a) {
+    constexpr int kPieces = 4 * G + 2, kDeepMove = 4;
     const EvictWork wk = evict_work(a.workspace, c.n_seqs, c.capacity);
-    const int s = blockIdx.y, lane = threadIdx.x & 31;
-    const int n = wk.n_move[s];
-    const int warps = gridDim.x * (blockDim.x >> 5);
+    const int s = blockIdx.y;
     const size_t base = (size_t)s * c.capacity;
-    const int code16 = 2 * c.G;  // 16-byte pieces of a row's codes
-    for (long long i = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i < (long long)n * c.heads; i += warps) {
-        const int p = (int)(i / c.heads), h = (int)(i - (long long)p * c.heads);
-        const int to = wk.hole[base + p], fr = wk.src[base + p];
-        const size_t rb = ((size_t)s * c.heads + h) * c.rows;
-        if (lane < 2 * code16) {
-            const int q = lane < code16 ? lane : lane - code16;
-            uint32_t* codes = lane < code16 ? c.kc : c.vc;
-            reinterpret_cast<uint4*>(codes + (rb + to) * 8 * c.G)[q] =
-                reinterpret_cast<const uint4*>(codes + (rb + fr) * 8 * c.G)[q];
-        } else if (lane - 2 * code16 < 2 * c.G) {
-            const int q = lane - 2 * code16;
-            uint32_t* par = q < c.G ? c.kp : c.vp;
-            const int g = q < c.G ? q : q - c.G;
-            par[(rb + to) * c.G + g] = par[(rb + fr) * c.G + g];
-        }
-        if (c.G == 6) {  // 24 + 24 pieces and words: the lanes above took 32 of the 36
-            if (lane < 4) {
-                const int q = lane + 8;
-                uint32_t* par = q < c.G ? c.kp : c.vp;
-                const int g = q < c.G ? q : q - c.G;
-                par[(rb + to) * c.G + g] = par[(rb + fr) * c.G + g];
+    const int32_t* hole = wk.hole + base;
+    const int32_t* src = wk.src + base;
+    const int n = wk.n_move[s];
+    const long long todo = (long long)n * c.heads * kPieces, threads = (long long)gridDim.x * blockDim.x;
+    for (long long w0 = blockIdx.x * blockDim.x + threadIdx.x; w0 < todo; w0 += threads * kDeepMove) {
+        uint4 v[kDeepMove];
+        char* dst[kDeepMove];
+        int piece[kDeepMove];
+#pragma unroll
+        for (int i = 0; i < kDeepMove; ++i) {
+            const long long x = w0 + i * threads;
+            piece[i] = -1;
+            if (x >= todo) continue;
+            const long long pair_head = x / kPieces;
+            piece[i] = (int)(x - pair_head * kPieces);
+            // head by head, so that neighbouring threads move neighbouring rows of one head
+            const int h = (int)(pair_head / n), p = (int)(pair_head - (long long)h * n);
+            const size_t rb = ((size_t)s * c.heads + h) * c.rows;
+            const size_t to = rb + hole[p], fr = rb + src[p];
+            if (piece[i] < 4 * G) {
+                uint32_t* codes = piece[i] < 2 * G ? c.kc : c.vc;
+                const int q = (piece[i] < 2 * G ? piece[i] : piece[i] - 2 * G) * 4;
+                v[i] = *reinterpret_cast<const uint4*>(codes + fr * 8 * G + q);
+                dst[i] = reinterpret_cast<char*>(codes + to * 8 * G + q);
+            } else {
+                uint32_t* par = piece[i] == 4 * G ? c.kp : c.vp;
+                const uint32_t* f = par + fr * G;
+                dst[i] = reinterpret_cast<char*>(par + to * G);
+                v[i].x = f[0];
+                if (G > 1) v[i].y = f[1];
+                if (G > 2) v[i].z = f[2], v[i].w = f[3];
+                if (G > 4) {
+                    reinterpret_cast<uint32_t*>(dst[i])[4] = f[4];
+                    reinterpret_cast<uint32_t*>(dst[i])[5] = f[5];
+                }
+                if (piece[i] == 4 * G && h == 0) {
+                    a.w_out[base + hole[p]] = a.w_in[base + src[p]];
+                    if (a.ids_out) a.ids_out[base + hole[p]] = a.ids_in[base + src[p]];
+                }
             }
         }
-        if (h == 0 && lane == 0) {
-            a.w_out[base + to] = a.w_in[base + fr];
-            if (a.ids_out) a.ids_out[base + to] = a.ids_in[base + fr];
+#pragma unroll
+        for (int i = 0; i < kDeepMove; ++i) {
+            if (piece[i] < 0) continue;
+            if (piece[i] < 4 * G) {
+                *reinterpret_cast<uint4*>(dst[i]) = v[i];
+            } else {
+                uint32_t* d = reinterpret_cast<uint32_t*>(dst[i]);
+                d[0] = v[i].x;
+                if (G > 1) d[1] = v[i].y;
+                if (G > 2) d[2] = v[i].z, d[3] = v[i].w;
+            }
         }
     }
 }
@@ -639,18 +725,40 @@ size_t cache_evict_workspace(const CacheView& c) {
 }
 
 void launch_cache_evict(const CacheView& c, const EvictArgs& a, cudaStream_t st) {
-    const int key_cap = std::min(c.capacity, 48 * 1024);  // keys of 192 KiB fit beside the counters
-    const size_t smem = (size_t)key_cap * sizeof(uint32_t);
-    set_smem((const void*)k_cache_select, smem);
+    // Eight blocks per sequence where one would go over its keys several times: 8192 rows in one block took
+    // as long as in a cluster, with its slower barriers.
+    const int n_blocks = c.capacity > 8192 ? kSelCluster : 1;
+    const int per = (c.capacity + n_blocks * kSelBS - 1) / (n_blocks * kSelBS) * kSelBS;
+    const int key_cap = std::min(per, kSelKeys);
     {
+        const size_t smem = (size_t)key_cap * sizeof(uint32_t);
+        const auto kernel = n_blocks > 1 ? k_cache_select<kSelCluster> : k_cache_select<1>;
+        set_smem((const void*)kernel, smem);
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)(c.n_seqs * n_blocks));
+        cfg.blockDim = dim3(kSelBS);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim = {(unsigned)n_blocks, 1, 1};
+        cfg.attrs = attr;
+        cfg.numAttrs = n_blocks > 1 ? 1 : 0;
         Tick tk(kKCacheSelect, st);
-        k_cache_select<<<c.n_seqs, kSelBS, smem, st>>>(c, a, key_cap);
+        cudaLaunchKernelEx(&cfg, kernel, c, a, key_cap);
     }
-    const long long most = (long long)std::max(0, std::min(a.keep, c.capacity - a.keep)) * c.heads;
+    const long long most = (long long)std::max(0, std::min(a.keep, c.capacity - a.keep)) * c.heads * (4 * c.G + 2);
     if (most == 0) return;
-    const unsigned gx = (unsigned)std::min<long long>((most + 7) / 8, std::max(1, 8 * sm_count() / c.n_seqs));
+    const dim3 grid((unsigned)std::min<long long>((most + 1023) / 1024, std::max(1, 16 * sm_count() / c.n_seqs)), c.n_seqs);
     Tick tk(kKCacheMove, st);
-    k_cache_move<<<dim3(gx, c.n_seqs), 256, 0, st>>>(c, a);
+    if (c.G == 1)
+        k_cache_move<1><<<grid, 256, 0, st>>>(c, a);
+    else if (c.G == 2)
+        k_cache_move<2><<<grid, 256, 0, st>>>(c, a);
+    else if (c.G == 4)
+        k_cache_move<4><<<grid, 256, 0, st>>>(c, a);
+    else
+        k_cache_move<6><<<grid, 256, 0, st>>>(c, a);
 }
 
 }  // namespace dev
