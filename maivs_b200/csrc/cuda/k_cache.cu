@@ -385,13 +385,15 @@ __device__ __forceinline__ void sync_blocks() {
         cooperative_groups::this_cluster().sync();
 }
 
-// Sums of the counts before this warp (all three), over the cluster's blocks in order; total in `all`.
-// s_cnt: [kSelWarps + 1][3], the last entry the block's sum.
+// Sums of the counts before this warp (all four), over the cluster's blocks in order; totals in `all`.
+// s_cnt: one entry per warp, the last one the block's sum.
+constexpr int kCounts = 4;
 template <int N>
-__device__ __forceinline__ void scan_counts(int (*s_cnt)[3], int warp, int lane, int (&before)[3], int (&all)[3]) {
+__device__ __forceinline__ void scan_counts(int (*s_cnt)[kCounts], int warp, int lane, int (&before)[kCounts],
+                                            int (&all)[kCounts]) {
     const auto cl = cooperative_groups::this_cluster();
     __syncthreads();
-    if (warp < 3) {
+    if (warp < kCounts) {
         const int v = s_cnt[lane][warp];
         int s = v;
 #pragma unroll
@@ -404,39 +406,37 @@ __device__ __forceinline__ void scan_counts(int (*s_cnt)[3], int warp, int lane,
         if (lane == 31) s_cnt[kSelWarps][warp] = s;
     }
     sync_blocks<N>();
-    int v[N][3];
+    int4 v[N];
 #pragma unroll
     for (int r = 0; r < N; ++r)
-#pragma unroll
-        for (int q = 0; q < 3; ++q)
-            v[r][q] = N == 1 ? s_cnt[kSelWarps][q] : *cl.map_shared_rank(&s_cnt[kSelWarps][q], r);
+        v[r] = *reinterpret_cast<const int4*>(N == 1 ? s_cnt[kSelWarps] : cl.map_shared_rank(s_cnt[kSelWarps], r));
     const int rank = N == 1 ? 0 : (int)cl.block_rank();
 #pragma unroll
-    for (int q = 0; q < 3; ++q) {
-        before[q] = s_cnt[warp][q];
-        all[q] = 0;
+    for (int q = 0; q < kCounts; ++q) before[q] = s_cnt[warp][q], all[q] = 0;
 #pragma unroll
-        for (int r = 0; r < N; ++r) {
-            all[q] += v[r][q];
-            before[q] += r < rank ? v[r][q] : 0;
+    for (int r = 0; r < N; ++r) {
+        const int x[kCounts] = {v[r].x, v[r].y, v[r].z, v[r].w};
+#pragma unroll
+        for (int q = 0; q < kCounts; ++q) {
+            all[q] += x[q];
+            before[q] += r < rank ? x[q] : 0;
         }
     }
-    sync_blocks<N>();  // the counters may be written again
 }
 
 // A cluster per sequence: the keep-th largest weight by three rounds of counting over the
 // order-preserving keys (11, 11 and 10 bits from the top), then which rows stay, which leave and which
 // move where. A block takes one stretch of the rows and keeps their keys in shared memory; counts are
-// gathered over the cluster, ranks follow the rows' order. Bound by the latency of its dozen
-// barriers; one block took 57 us for 31,000 rows where eight take a few.
+// gathered over the cluster, ranks follow the rows' order. Bound by the latency of its five barriers
+// of the cluster and of the loads between them.
 template <int N>
 __global__ void __launch_bounds__(kSelBS) k_cache_select(CacheView c, EvictArgs a, int key_cap) {
     const auto cl = cooperative_groups::this_cluster();
     extern __shared__ uint32_t s_key[];
-    __shared__ __align__(8) int s_hist[kBuckets];
-    __shared__ int s_cnt[kSelWarps + 1][3];
+    __shared__ __align__(8) int s_hist[3][kBuckets];  // one a round, so that a round needs one barrier
+    __shared__ __align__(16) int s_cnt[kSelWarps + 1][kCounts];
     __shared__ int s_sum[kSelWarps];
-    __shared__ int s_pick[2];
+    __shared__ int s_pick[3][2];
     const int rank = N == 1 ? 0 : (int)cl.block_rank();
     const int s = blockIdx.x / N, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int L = min(max(a.lengths[s], 0), c.capacity), m = min(L, a.keep);
@@ -460,6 +460,8 @@ __global__ void __launch_bounds__(kSelBS) k_cache_select(CacheView c, EvictArgs 
     if (cut) {
 #pragma unroll 4
         for (int r = b0 + threadIdx.x; r < min(b1, b0 + key_cap); r += kSelBS) s_key[r - b0] = make_key(r);
+        for (int i = threadIdx.x; i < 3 * kBuckets; i += kSelBS) s_hist[0][i] = 0;
+        __syncthreads();
     }
     // the m-th largest key T, and how many rows equal to it stay (the lowest rows of them)
     uint32_t T = 0;
@@ -469,15 +471,13 @@ __global__ void __launch_bounds__(kSelBS) k_cache_select(CacheView c, EvictArgs 
 #pragma unroll 1
         for (int round = 0; round < 3; ++round) {
             const int bits = round < 2 ? kDigit : 32 - 2 * kDigit, shift = high - bits;
-            for (int i = threadIdx.x; i < kBuckets; i += kSelBS) s_hist[i] = 0;
-            sync_blocks<N>();  // and the keys are there
             for (int r = b0 + warp * 32; r < b1; r += kSelBS) {
                 const uint32_t k = r + lane < b1 ? key(r + lane) : 0u;
                 const bool in = r + lane < b1 && (round == 0 || (k >> high) == (T >> high));
                 const uint32_t d = in ? (k >> shift) & ((1u << bits) - 1) : ~0u;
                 // one addition per distinct digit of the warp: weights crowd in a few buckets
                 const unsigned same = __match_any_sync(~0u, d);
-                if (in && lane == __ffs(same) - 1) atomicAdd(&s_hist[d], __popc(same));
+                if (in && lane == __ffs(same) - 1) atomicAdd(&s_hist[round][d], __popc(same));
             }
             sync_blocks<N>();
             // buckets from the top, two a thread
@@ -485,7 +485,8 @@ __global__ void __launch_bounds__(kSelBS) k_cache_select(CacheView c, EvictArgs 
             int2 part[N];
 #pragma unroll
             for (int r = 0; r < N; ++r)
-                part[r] = *reinterpret_cast<const int2*>(N == 1 ? &s_hist[top] : cl.map_shared_rank(&s_hist[top], r));
+                part[r] = *reinterpret_cast<const int2*>(N == 1 ? &s_hist[round][top]
+                                                                : cl.map_shared_rank(&s_hist[round][top], r));
             int h[2] = {0, 0};
 #pragma unroll
             for (int r = 0; r < N; ++r) h[0] += part[r].y, h[1] += part[r].x;
@@ -505,26 +506,36 @@ __global__ void __launch_bounds__(kSelBS) k_cache_select(CacheView c, EvictArgs 
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 if (before < need && before + h[i] >= need) {
-                    s_pick[0] = kBuckets - 1 - 2 * (int)threadIdx.x - i;
-                    s_pick[1] = need - before;
+                    s_pick[round][0] = kBuckets - 1 - 2 * (int)threadIdx.x - i;
+                    s_pick[round][1] = need - before;
                 }
                 before += h[i];
             }
-            sync_blocks<N>();  // everyone has read the histograms
-            T |= (uint32_t)s_pick[0] << shift;
-            need = s_pick[1];
+            __syncthreads();
+            T |= (uint32_t)s_pick[round][0] << shift;
+            need = s_pick[round][1];
             high = shift;
         }
     }
-    // how many equal rows lie before this warp's
+    // Rows above T and equal to T, below the new length (low) and not: low rows come first, so the
+    // equal rows that stay are the first `need`, low ones first, and one scan gives every rank.
     const unsigned below = (1u << lane) - 1;
-    int before[3], all[3];
-    int eq = 0;
-    if (cut)
-        for (int r = r0; r < r1; r += 32) eq += __popc(__ballot_sync(~0u, r + lane < r1 && key(min(r + lane, r1 - 1)) == T));
-    if (lane == 0) s_cnt[warp][0] = eq, s_cnt[warp][1] = s_cnt[warp][2] = 0;
+    int cnt[kCounts] = {0, 0, 0, 0}, before[kCounts], all[kCounts];
+    for (int r = r0; r < r1; r += 32) {
+        const int x = r + lane;
+        const uint32_t k = x < r1 && cut ? key(x) : 0u;
+        const bool above = x < r1 && (all_stay || (cut && k > T)), same = x < r1 && cut && k == T;
+        const unsigned ba = __ballot_sync(~0u, above), bs = __ballot_sync(~0u, same);
+        const unsigned low = m - r >= 32 ? ~0u : m - r <= 0 ? 0u : (1u << (m - r)) - 1;
+        cnt[0] += __popc(ba & low), cnt[1] += __popc(bs & low);
+        cnt[2] += __popc(ba & ~low), cnt[3] += __popc(bs & ~low);
+    }
+    if (lane == 0) *reinterpret_cast<int4*>(s_cnt[warp]) = make_int4(cnt[0], cnt[1], cnt[2], cnt[3]);
     scan_counts<N>(s_cnt, warp, lane, before, all);
-    const int eq0 = before[0];
+    const int stay_low = before[0] + min(need, before[1]);
+    const int stay_high = before[2] + min(need, before[1] + before[3]) - min(need, before[1]);
+    const int stay_low_all = all[0] + min(need, all[1]);
+    int seen = before[1] + before[3];
     auto kept_row = [&](int r, int& seen) -> bool {
         const bool in = r < r1;
         const uint32_t k = in && cut ? key(r) : 0u;
@@ -534,23 +545,12 @@ __global__ void __launch_bounds__(kSelBS) k_cache_select(CacheView c, EvictArgs 
         seen += __popc(b);
         return keep;
     };
-    int n_hole = 0, n_src = 0, n_gone = 0, seen = eq0;
-    for (int r = r0; r < r1; r += 32) {
-        const int x = r + lane;
-        const bool k = kept_row(x, seen);
-        n_hole += __popc(__ballot_sync(~0u, x < r1 && x < m && !k));
-        n_src += __popc(__ballot_sync(~0u, x < r1 && x >= m && k));
-        n_gone += __popc(__ballot_sync(~0u, x < r1 && !k));
-    }
-    if (lane == 0) s_cnt[warp][0] = n_hole, s_cnt[warp][1] = n_src, s_cnt[warp][2] = n_gone;
-    scan_counts<N>(s_cnt, warp, lane, before, all);
     const EvictWork wk = evict_work(a.workspace, c.n_seqs, c.capacity);
     if (threadIdx.x == 0 && rank == 0) {
-        wk.n_move[s] = all[0];
+        wk.n_move[s] = m - stay_low_all;
         a.new_lengths[s] = m;
     }
-    int at_hole = before[0], at_src = before[1], at_gone = before[2];
-    seen = eq0;
+    int at_hole = min(r0, m) - stay_low, at_src = stay_high, at_gone = r0 - stay_low - stay_high;
     for (int r = r0; r < r1; r += 32) {
         const int x = r + lane;
         const bool in = x < r1;
@@ -568,6 +568,7 @@ __global__ void __launch_bounds__(kSelBS) k_cache_select(CacheView c, EvictArgs 
         at_src += __popc(bs);
         at_gone += __popc(bg);
     }
+    sync_blocks<N>();  // nobody reads this block's counters any more
 }
 
 // Move i of a sequence takes row src[i] (at or past the new length) to row hole[i] (below it), so no
