@@ -46,6 +46,7 @@ constexpr int kJoinBS = 128;
 constexpr int kMaxCluster = 8;
 constexpr int kMaxParts = 1024;
 constexpr int kWaves = 4;
+constexpr int kSoloLists = 2;
 // Up to so many rows a cluster of blocks reads them and joins in shared memory, in one launch; above, its
 // blocks would wait for the slowest and the SMs for a place for all of them.
 constexpr int kClusterRows = 2048;
@@ -62,6 +63,7 @@ struct AttendPlan {
     int cluster;    // blocks that share rows and join in shared memory
     int parts;      // blocks (of no cluster) that share rows and are joined by k_cache_join
     int share;      // rows of such a block
+    bool solo;      // a warp per list and head
     size_t off_o, off_lse, off_logit, bytes;
     int logit_rows;
 };
@@ -74,6 +76,7 @@ struct AttendKernel {
     float* logits;    // [token][q_head][logit_rows], log2; null without weights
     int logit_rows;
     int cluster, parts, share, col_tiles;
+    bool solo;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -216,7 +219,7 @@ __host__ __device__ __forceinline__ int share_of(int rows, int n, int G) {
 // Blocks per SM that the registers of a variant are held to.
 __host__ __device__ constexpr int blocks_of(int G, int nc) { return nc == 16 || G > 2 ? 2 : G == 2 ? 3 : 5; }
 
-template <int G, int NC, bool F32>
+template <int G, int NC, bool F32, bool FOUND>
 struct Shape {
     static constexpr int kNt = NC / 8;    // the MMA's N is eight columns
     static constexpr int kCols = NC / 4;  // columns per thread
@@ -226,7 +229,8 @@ struct Shape {
     // A warp's ring of tiles in flight. Stages x warps per SM x 1152 G bytes cover HBM's latency.
     static constexpr int kSub = sub_tiles(G);  // tiles of 16 rows that go through a step together
     static constexpr int kRows = kSub * kTile;
-    static constexpr int kStages = G <= 2 && NC == 8 ? 2 : 3;
+    // Found rows take two trips (the list, then the rows), so more of them are under way.
+    static constexpr int kStages = FOUND && G <= 2 ? 3 : G <= 2 && NC == 8 ? 2 : 3;
     static constexpr int kTileBytes = kRows * 72 * G;
     static constexpr int kRingBytes = kAttWarps * kStages * kTileBytes;
     static constexpr int kPitch = G * kCacheGroup + 4;  // floats of one column's sums; a warp's writes meet no bank twice
@@ -266,6 +270,7 @@ struct Fetch {
     const char *ks, *vs, *ps[kParams];
     const uint64_t* list;
     int k, row_limit, lane;
+    int entry;  // row that lane's entry of the next tile names, -1: none that the token sees
 
     __device__ __forceinline__ void init(const uint32_t* kc, const uint32_t* vc, const uint32_t* kp, const uint32_t* vp,
                                          int r0, int ln, const uint64_t* l, int k_, int limit) {
@@ -273,6 +278,7 @@ struct Fetch {
         list = l, k = k_, row_limit = limit;
         if constexpr (FOUND) {
             ks = reinterpret_cast<const char*>(kc), vs = reinterpret_cast<const char*>(vc);
+            entry = row(r0 + lane);
         } else {
             ks = reinterpret_cast<const char*>(kc) + ((size_t)r0 * 2 * G + lane) * 16;
             vs = reinterpret_cast<const char*>(vc) + ((size_t)r0 * 2 * G + lane) * 16;
@@ -284,19 +290,28 @@ struct Fetch {
             }
         }
     }
-    __device__ __forceinline__ size_t row(int e) const {
-        const uint64_t id = e < k ? __ldg(list + e) : ~0ull;
-        return id < (uint64_t)row_limit ? (size_t)id : 0;
+    __device__ __forceinline__ int row(int e) const {
+        const uint64_t id = lane < kRows && e < k ? __ldg(list + e) : ~0ull;
+        return id < (uint64_t)row_limit ? (int)id : -1;
     }
-    // The tile of rows (or list entries) r0 ..; pointers move on by the warps' stride.
-    __device__ __forceinline__ void next(uint32_t tile, int r0, const uint32_t* kp, const uint32_t* vp) {
+    // The tile of rows (or list entries) r0 ..; pointers, or the entries, move on by `stride` rows. The tile's
+    // entries that name a row are set in *seen.
+    __device__ __forceinline__ void next(uint32_t tile, uint32_t* seen, int r0, int stride, const uint32_t* kp,
+                                         const uint32_t* vp) {
+        int mine = 0;
+        if constexpr (FOUND) {
+            const unsigned have = __ballot_sync(~0u, entry >= 0);
+            if (lane == 0) *seen = have;
+            mine = max(entry, 0);  // entries without a row bring row 0, and are masked
+            entry = row(r0 + stride + lane);
+        }
 #pragma unroll
         for (int i = 0; i < kCodes; ++i) {
             const int p = lane + 32 * i;
             size_t at = 512 * i;
             if constexpr (FOUND) {
                 const int r = p / (2 * G);
-                at = (row(r0 + r) * 2 * G + (p - r * 2 * G)) * 16;
+                at = ((size_t)__shfl_sync(~0u, mine, r) * 2 * G + (p - r * 2 * G)) * 16;
             }
             copy16(tile + key_piece<G>(p) * 16, ks + at);
             copy16(tile + 32 * G * kRows + value_piece<G>(p) * 16, vs + at);
@@ -306,7 +321,7 @@ struct Fetch {
 #pragma unroll
             for (int y = 0; y < kSub; ++y) {
                 const int r = lane + 32 * y;  // the keys' rows, then the values'
-                const uint32_t* src = (r < kRows ? kp : vp) + row(r0 + (r < kRows ? r : r - kRows)) * G;
+                const uint32_t* src = (r < kRows ? kp : vp) + (size_t)__shfl_sync(~0u, mine, r < kRows ? r : r - kRows) * G;
 #pragma unroll
                 for (int i = 0; i < G; ++i) copy4(tile + 64 * G * kRows + (r * G + i) * 4, src + i);
             }
@@ -323,22 +338,34 @@ struct Fetch {
 };
 
 // kRows: rows in order. kClustered: the same, joined by a cluster of blocks. kFound: rows of a list.
-enum class Mode { kRows, kClustered, kFound };
+// kFoundSolo: the same, a list and head per warp.
+enum class Mode { kRows, kClustered, kFound, kFoundSolo };
 
 template <int G, int NC, bool F32, Mode MODE>
-__global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_attend(CacheView c, AttendKernel kk) {
-    constexpr bool FOUND = MODE == Mode::kFound, kCluster = MODE == Mode::kClustered;
-    using S = Shape<G, NC, F32>;
+__global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, (MODE >= Mode::kFound)>::kBlocks) k_cache_attend(CacheView c, AttendKernel kk) {
+    constexpr bool kSolo = MODE == Mode::kFoundSolo, FOUND = MODE == Mode::kFound || kSolo;
+    constexpr bool kCluster = MODE == Mode::kClustered;
+    constexpr int kTeam = kSolo ? 1 : kAttWarps;  // warps that share rows
+    using S = Shape<G, NC, F32, (MODE >= Mode::kFound)>;
     constexpr int kNt = S::kNt, kCols = S::kCols, kQ = S::kQ, kR = 2 * S::kSub;
     const AttendArgs& a = kk.a;
     __shared__ float s_m[kAttWarps][NC], s_l[kAttWarps][NC];
     __shared__ float2 s_blk[kCluster ? NC : 1], s_all[kCluster ? NC : 1];  // maximum and sum: of the block, of the cluster
     __shared__ float s_f[kCluster ? kMaxCluster : 1][NC];  // what brings a block's sums to the cluster's maximum
     __shared__ uint4 s_q[S::kQShared ? 2 * G * kNt * (kQ / 4) : 1][32];
+    __shared__ uint32_t s_seen[FOUND ? kAttWarps : 1][S::kStages];
     extern __shared__ __align__(128) char s_ring[];
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gid = lane >> 2, t = lane & 3;
-    unsigned b = blockIdx.x;
+    const int first = kSolo ? warp : 0;  // of the team
+    unsigned b = kSolo ? blockIdx.x * kAttWarps + warp : blockIdx.x;
+    auto team_sync = [] {
+        if constexpr (kSolo)
+            __syncwarp();
+        else
+            __syncthreads();
+    };
+    static_assert(!(kSolo && S::kQShared), "a solo warp keeps its queries in registers");
     int rank = 0;
     if constexpr (kCluster) {
         rank = b % kk.cluster;
@@ -350,6 +377,7 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
     b /= kk.parts;
     const int h = b % c.heads;
     const int item = b / c.heads;  // sequence, or token of a found list
+    if (kSolo && item >= a.tok.n_tokens) return;
 
     Span sn;
     int s, cols, rows_all;
@@ -395,14 +423,14 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
         // ---- the first tiles are on their way while the queries are prepared ----
         char* ring = s_ring + warp * S::kStages * S::kTileBytes;
         const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
-        constexpr int kStride = kAttWarps * S::kRows;
-        const int mine = start + warp * S::kRows;
+        constexpr int kStride = kTeam * S::kRows;
+        const int mine = start + (kSolo ? 0 : warp) * S::kRows;
         Fetch<G, FOUND> fetch;
         fetch.init(kc, vc, kp, vp, mine, lane, list, a.k, row_limit);
 #pragma unroll
         for (int i = 0; i < S::kStages - 1; ++i) {
             const int r = mine + i * kStride;
-            if (r < end) fetch.next(ring_at + i * S::kTileBytes, r, kp, vp);
+            if (r < end) fetch.next(ring_at + i * S::kTileBytes, &s_seen[FOUND ? warp : 0][i], r, kStride, kp, vp);
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
 
@@ -524,7 +552,7 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
 
         // One step of rows (or list entries) r0 ..: kSub times 16 of them. The scores' fragments have rows
         // gid + 8 i (i < 2 kSub) and this thread's columns. kEdge: some column does not see some row.
-        auto tile_step = [&](const char* tile, int r0, auto edge) {
+        auto tile_step = [&](const char* tile, uint32_t seen, int r0, auto edge) {
             constexpr bool kEdge = decltype(edge)::value;
             const uint32_t* par = reinterpret_cast<const uint32_t*>(tile + 64 * G * S::kRows);
             uint32_t vpw[kR][G];
@@ -534,8 +562,7 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
                 tile_words<G>(par + (S::kRows + gid + 8 * i) * G, vpw[i]);
                 if constexpr (kEdge) {
                     const int r = r0 + gid + 8 * i;
-                    ok[i] = r < lim_last;
-                    if constexpr (FOUND) ok[i] = ok[i] && __ldg(list + r) < (uint64_t)row_limit;
+                    ok[i] = FOUND ? (seen >> (r - r0)) & 1 : r < lim_last;
 #pragma unroll
                     for (int g = 0; g < G; ++g) vpw[i][g] = ok[i] ? vpw[i][g] : 0u;
                 }
@@ -772,12 +799,12 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
             asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
             __syncwarp();
             const int r = r0 + (S::kStages - 1) * kStride;
-            if (r < end) fetch.next(ring_at + to, r, kp, vp);
+            if (r < end) fetch.next(ring_at + to, &s_seen[FOUND ? warp : 0][to / S::kTileBytes], r, kStride, kp, vp);
             asm volatile("cp.async.commit_group;" ::: "memory");
             if (FOUND || r0 + S::kRows > lim_first)
-                tile_step(ring + at, r0, std::true_type());
+                tile_step(ring + at, FOUND ? s_seen[warp][at / S::kTileBytes] : 0u, r0, std::true_type());
             else
-                tile_step(ring + at, r0, std::integral_constant<bool, FOUND>());
+                tile_step(ring + at, 0u, r0, std::integral_constant<bool, FOUND>());
             to = at;
             at = at == (S::kStages - 1) * S::kTileBytes ? 0 : at + S::kTileBytes;
         }
@@ -797,14 +824,14 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
                 for (int d = 4; d < 32; d *= 2)
                     low[j][g] = __fadd_rn(low[j][g], __shfl_xor_sync(~0u, low[j][g], d));
         }
-        __syncthreads();
+        team_sync();
         float* s_o = reinterpret_cast<float*>(s_ring);  // [warp][column][S::kPitch]
 #pragma unroll
         for (int j = 0; j < kCols; ++j) {
             const int col = 8 * (j >> 1) + 2 * t + (j & 1);
-            float mx = s_m[0][col];
+            float mx = s_m[first][col];
 #pragma unroll
-            for (int y = 1; y < kAttWarps; ++y) mx = fmaxf(mx, s_m[y][col]);
+            for (int y = 1; y < kTeam; ++y) mx = fmaxf(mx, s_m[first + y][col]);
             const float f = ex2(m[j] - mx);
 #pragma unroll
             for (int g = 0; g < G; ++g) {
@@ -818,7 +845,7 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
                             __fmul_rn(__fmaf_rn(o[g][i][j >> 1][2 * y + (j & 1)], i & 1 ? n1 : n0, low[j][g]), f);
             }
         }
-        __syncthreads();
+        team_sync();
         if constexpr (kCluster) {
             for (int e = threadIdx.x; e < NC * G * kCacheGroup; e += kAttBS) {
                 const int col = e / (G * kCacheGroup), d = e % (G * kCacheGroup);
@@ -877,23 +904,24 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
             cluster.sync();  // nobody reads this block's sums any more
         } else {
             // ---- out, or this block's part ----
-            for (int col = warp; col < NC; col += kAttWarps) {
+            for (int col = kSolo ? 0 : warp; col < NC; col += kTeam) {
                 const int cc = ct * NC + col;
                 if (cc >= cols) break;
                 const int i = cc / a.group;
                 const int tk = FOUND ? item : sn.first + i;
                 const int hd = h * a.group + (cc - i * a.group);
-                float mx = s_m[0][col], sum = 0.0f;
+                float mx = s_m[first][col], sum = 0.0f;
 #pragma unroll
-                for (int y = 1; y < kAttWarps; ++y) mx = fmaxf(mx, s_m[y][col]);
+                for (int y = 1; y < kTeam; ++y) mx = fmaxf(mx, s_m[first + y][col]);
 #pragma unroll
-                for (int y = 0; y < kAttWarps; ++y) sum = __fmaf_rn(s_l[y][col], ex2(s_m[y][col] - mx), sum);
+                for (int y = 0; y < kTeam; ++y)
+                    sum = __fmaf_rn(s_l[first + y][col], ex2(s_m[first + y][col] - mx), sum);
                 const size_t th = (size_t)tk * a.q_heads + hd;
-                const float* so = s_o + col * S::kPitch;
+                const float* so = s_o + (first * NC + col) * S::kPitch;
                 auto value = [&](int d) -> float {
                     float v = so[d];
 #pragma unroll
-                    for (int y = 1; y < kAttWarps; ++y) v = __fadd_rn(v, so[y * NC * S::kPitch + d]);
+                    for (int y = 1; y < kTeam; ++y) v = __fadd_rn(v, so[y * NC * S::kPitch + d]);
                     return v;
                 };
                 if (kk.parts == 1) {
@@ -912,7 +940,7 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32>::kBlocks) k_cache_at
                     if (lane == 0) kk.part_ml[at] = make_float2(mx, sum);
                 }
             }
-            __syncthreads();
+            team_sync();
         }
     }
 }
@@ -1046,6 +1074,8 @@ AttendPlan make_plan(const CacheView& c, const AttendArgs& a) {
     const long long fill = std::max(1ll, slots / std::max(1ll, items));
     p.cluster = p.parts = 1;
     p.share = most * step;
+    // Lists enough to fill the GPU by warps: none waits for a block's barriers.
+    p.solo = found && c.G <= 2 && p.nc == 8 && items * kSoloLists >= slots * kAttWarps;
     if (!found && rows <= kClusterRows && fill >= 2) {
         p.cluster = (int)std::min<long long>({kMaxCluster, fill, most});
     } else {
@@ -1074,10 +1104,17 @@ AttendPlan make_plan(const CacheView& c, const AttendArgs& a) {
 
 template <int G, int NC, bool F32>
 void start(const CacheView& c, const AttendKernel& k, bool found, unsigned grid, cudaStream_t st) {
-    constexpr int smem = Shape<G, NC, F32>::kRingBytes;
-    const auto kernel = found           ? k_cache_attend<G, NC, F32, Mode::kFound>
-                        : k.cluster > 1 ? k_cache_attend<G, NC, F32, Mode::kClustered>
-                                        : k_cache_attend<G, NC, F32, Mode::kRows>;
+    const int smem = found ? Shape<G, NC, F32, true>::kRingBytes : Shape<G, NC, F32, false>::kRingBytes;
+    auto kernel = k_cache_attend<G, NC, F32, Mode::kRows>;
+    if (found)
+        kernel = k_cache_attend<G, NC, F32, Mode::kFound>;
+    else if (k.cluster > 1)
+        kernel = k_cache_attend<G, NC, F32, Mode::kClustered>;
+    if constexpr (G <= 2 && NC == 8)
+        if (k.solo) {
+            kernel = k_cache_attend<G, NC, F32, Mode::kFoundSolo>;
+            grid = (grid + kAttWarps - 1) / kAttWarps;
+        }
     set_smem((const void*)kernel, smem);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid);
@@ -1129,6 +1166,7 @@ void launch_cache_attend(const CacheView& c, const AttendArgs& a, cudaStream_t s
     k.cluster = p.cluster;
     k.parts = p.parts;
     k.share = p.share;
+    k.solo = p.solo;
     k.col_tiles = p.col_tiles;
     if (a.tok.n_tokens > 0) {
         const unsigned grid =
