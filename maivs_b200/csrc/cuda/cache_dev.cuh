@@ -74,5 +74,22 @@ __device__ __forceinline__ int find_sequence(const int32_t* __restrict__ off, in
     return __ldg(off + s) <= tok && tok < __ldg(off + s + 1) ? s : -1;
 }
 
+// Launches the second kernel of a pair: its blocks may be set up while the first still runs (the first says
+// so by cudaTriggerProgrammaticLaunchCompletion), and it waits by cudaGridDependencySynchronize before it
+// touches anything.
+template <typename... P, typename... A>
+inline void launch_after(void (*kernel)(P...), dim3 grid, int threads, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 }  // namespace dev
 }  // namespace maivs

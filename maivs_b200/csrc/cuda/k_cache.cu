@@ -432,6 +432,7 @@ __device__ __forceinline__ void scan_counts(int (*s_cnt)[kCounts], int warp, int
 template <int N>
 __global__ void __launch_bounds__(kSelBS) k_cache_select(CacheView c, EvictArgs a, int key_cap) {
     const auto cl = cooperative_groups::this_cluster();
+    cudaTriggerProgrammaticLaunchCompletion();  // the moves wait for this grid's end
     extern __shared__ uint32_t s_key[];
     __shared__ __align__(8) int s_hist[3][kBuckets];  // one a round, so that a round needs one barrier
     __shared__ __align__(16) int s_cnt[kSelWarps + 1][kCounts];
@@ -578,6 +579,7 @@ template <int G>
 __global__ void __launch_bounds__(256) k_cache_move(CacheView c, EvictArgs a) {
     constexpr int kPieces = 4 * G + 2, kDeepMove = 4;
     const EvictWork wk = evict_work(a.workspace, c.n_seqs, c.capacity);
+    cudaGridDependencySynchronize();
     const int s = blockIdx.y;
     const size_t base = (size_t)s * c.capacity;
     const int32_t* hole = wk.hole + base;
@@ -753,13 +755,13 @@ void launch_cache_evict(const CacheView& c, const EvictArgs& a, cudaStream_t st)
     const dim3 grid((unsigned)std::min<long long>((most + 1023) / 1024, std::max(1, 16 * sm_count() / c.n_seqs)), c.n_seqs);
     Tick tk(kKCacheMove, st);
     if (c.G == 1)
-        k_cache_move<1><<<grid, 256, 0, st>>>(c, a);
+        launch_after(k_cache_move<1>, grid, 256, st, c, a);
     else if (c.G == 2)
-        k_cache_move<2><<<grid, 256, 0, st>>>(c, a);
+        launch_after(k_cache_move<2>, grid, 256, st, c, a);
     else if (c.G == 4)
-        k_cache_move<4><<<grid, 256, 0, st>>>(c, a);
+        launch_after(k_cache_move<4>, grid, 256, st, c, a);
     else
-        k_cache_move<6><<<grid, 256, 0, st>>>(c, a);
+        launch_after(k_cache_move<6>, grid, 256, st, c, a);
 }
 
 }  // namespace dev

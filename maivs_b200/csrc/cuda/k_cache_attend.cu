@@ -356,6 +356,7 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, (MODE >= Mode::kFoun
     __shared__ uint32_t s_seen[FOUND ? kAttWarps : 1][S::kStages];
     extern __shared__ __align__(128) char s_ring[];
 
+    cudaTriggerProgrammaticLaunchCompletion();  // the join's blocks wait for this grid's end
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gid = lane >> 2, t = lane & 3;
     const int first = kSolo ? warp : 0;  // of the team
     unsigned b = kSolo ? blockIdx.x * kAttWarps + warp : blockIdx.x;
@@ -957,6 +958,8 @@ __global__ void __launch_bounds__(kJoinBS) k_cache_join(CacheView c, AttendKerne
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const size_t th = blockIdx.x;
     const int tk = (int)(th / a.q_heads);
+    cudaTriggerProgrammaticLaunchCompletion();
+    cudaGridDependencySynchronize();
     const int s = find_sequence(a.tok.offsets, c.n_seqs, tk, lane & 7, 0xFFu << (lane / 8 * 8));
     if (s < 0) return;
     const Span sn = span_of(c, a, s);
@@ -1019,6 +1022,7 @@ __global__ void __launch_bounds__(kJoinBS) k_cache_join(CacheView c, AttendKerne
 // token and head by head, so that the sum does not depend on the launch.
 __global__ void __launch_bounds__(256) k_cache_weights(CacheView c, AttendKernel kk) {
     const AttendArgs& a = kk.a;
+    cudaGridDependencySynchronize();
     const int s = blockIdx.y;
     const Span sn = span_of(c, a, s);
     const int rows = min(sn.len + (a.causal ? sn.count : 0), c.capacity);
@@ -1038,6 +1042,7 @@ __global__ void __launch_bounds__(256) k_cache_weights(CacheView c, AttendKernel
 // Softmax weights of a found list's entries, summed over the query heads.
 __global__ void __launch_bounds__(128) k_cache_found_weights(CacheView c, AttendKernel kk) {
     const AttendArgs& a = kk.a;
+    cudaGridDependencySynchronize();
     const int blocks = (a.k + 127) / 128;  // of one token
     const int tk = blockIdx.x / blocks, lane = threadIdx.x & 31;
     const int s = find_sequence(a.tok.offsets, c.n_seqs, tk, lane & 7, 0xFFu << (lane / 8 * 8));
@@ -1186,17 +1191,17 @@ void launch_cache_attend(const CacheView& c, const AttendArgs& a, cudaStream_t s
             Tick tk(kKCacheJoin, st);
             const unsigned jg = (unsigned)((long long)a.tok.n_tokens * a.q_heads);
             if (found)
-                k_cache_join<true><<<jg, kJoinBS, 0, st>>>(c, k);
+                launch_after(k_cache_join<true>, dim3(jg), kJoinBS, st, c, k);
             else
-                k_cache_join<false><<<jg, kJoinBS, 0, st>>>(c, k);
+                launch_after(k_cache_join<false>, dim3(jg), kJoinBS, st, c, k);
         }
     }
     if (a.w_out) {
         Tick tk(kKCacheWeights, st);
         if (found)
-            k_cache_found_weights<<<(unsigned)((a.k + 127) / 128 * (long long)a.tok.n_tokens), 128, 0, st>>>(c, k);
+            launch_after(k_cache_found_weights, dim3((unsigned)((a.k + 127) / 128 * (long long)a.tok.n_tokens)), 128, st, c, k);
         else
-            k_cache_weights<<<dim3((std::min(a.max_rows, c.capacity) + 255) / 256, c.n_seqs), 256, 0, st>>>(c, k);
+            launch_after(k_cache_weights, dim3((std::min(a.max_rows, c.capacity) + 255) / 256, c.n_seqs), 256, st, c, k);
     }
 }
 
