@@ -47,9 +47,11 @@ SOURCES = [
     ("cuda/k_merge.cu", "nvcc"),
     ("cuda/k_cache.cu", "nvcc"),
     ("cuda/k_cache_attend.cu", "nvcc"),
+    ("cuda/k_cache_wide.cu", "nvcc"),
 ]
 HEADERS = ["handle.h", "host/hostmath.h", "host/index_host.h", "cuda/common.cuh", "cuda/kernels.cuh", "cuda/dev_common.cuh",
-           "cuda/umma.cuh", "cuda/engine.h", "cuda/cache.h", "cuda/cache_dev.cuh"]
+           "cuda/umma.cuh", "cuda/engine.h", "cuda/cache.h", "cuda/cache_dev.cuh",
+           "cuda/cache_attend.cuh"]
 
 
 def _cmd(src: str, kind: str, obj: str) -> list[str]:

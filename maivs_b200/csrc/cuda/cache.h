@@ -38,6 +38,7 @@ struct CacheView {
 constexpr uint32_t kCacheFull = 1;      // append: tokens past the capacity were left out
 constexpr uint32_t kCacheTooLong = 2;   // attend: a sequence has more rows than max_rows
 constexpr uint32_t kCacheOffsets = 4;   // offsets not ascending within [0, n_tokens]
+constexpr uint32_t kCacheWait = 8;      // attend: a bounded wait ran out; the call's results are invalid
 
 // Instantiated group counts; a dimension takes the smallest that holds it.
 inline int cache_groups(int dim) { return dim <= 64 ? 1 : dim <= 128 ? 2 : dim <= 256 ? 4 : 6; }

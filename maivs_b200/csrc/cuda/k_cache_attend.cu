@@ -27,8 +27,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "cache.h"
-#include "cache_dev.cuh"
+#include "cache_attend.cuh"
 #include "common.cuh"
 #include "dev_common.cuh"
 
@@ -47,16 +46,10 @@ constexpr int kMaxCluster = 8;
 constexpr int kMaxParts = 1024;
 constexpr int kWaves = 4;
 constexpr int kSoloLists = 2;
+constexpr int kWideLeast = 64;
 // Up to so many rows a cluster of blocks reads them and joins in shared memory, in one launch; above, its
 // blocks would wait for the slowest and the SMs for a place for all of them.
 constexpr int kClusterRows = 2048;
-constexpr float kNoMax = -3.0e38f;
-constexpr float kLog2e = 1.4426950408889634f;
-// p * step goes into f16 scaled so that the group's largest step becomes 2^12: an old maximum may
-// be exceeded by 2^kLag before the accumulators are rescaled, and 2^12 * 2^kLag is below 65504.
-constexpr float kLag = 3.0f;
-constexpr float kPScale = 4096.0f;
-
 struct AttendPlan {
     int nc;         // columns per tile
     int col_tiles;  // of one sequence and head (or token and head)
@@ -64,26 +57,10 @@ struct AttendPlan {
     int parts;      // blocks (of no cluster) that share rows and are joined by k_cache_join
     int share;      // rows of such a block
     bool solo;      // a warp per list and head
+    bool wide;      // blocks of 128 columns on the fifth-generation tensor cores
     size_t off_o, off_lse, off_logit, bytes;
     int logit_rows;
 };
-
-struct AttendKernel {
-    AttendArgs a;
-    float2* part_ml;  // [part][token][q_head]: running maximum (log2) and sum
-    float* part_o;    // [part][token][q_head][dim]
-    float* lse2;      // [token][q_head], log2; null without weights
-    float* logits;    // [token][q_head][logit_rows], log2; null without weights
-    int logit_rows;
-    int cluster, parts, share, col_tiles;
-    bool solo;
-};
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                     uint32_t b1) {
@@ -118,11 +95,6 @@ __device__ __forceinline__ float low_of(uint32_t par) {
     return F32 ? __fmaf_rn(8.0f, par_step(par), par_low(par)) : par_low(par);
 }
 
-__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 // The part of x that its f16 rounding (in packed pair p, half i) leaves over.
 __device__ __forceinline__ float left_over(float x, uint32_t p, int i) {
     return __fsub_rn(x, to_f32<__half>(i ? p >> 16 : p & 0xFFFFu));
@@ -149,36 +121,6 @@ __device__ __forceinline__ void tile_words(const uint32_t* p, uint32_t (&w)[N]) 
     }
 }
 
-// n <= 8 elements of a query from element i on; the others are 0.
-__device__ __forceinline__ void load_query8(const void* q, int type, size_t i, int n, float (&x)[8]) {
-    if (type == kF32) {
-        const float* p = static_cast<const float*>(q) + i;
-        if (n == 8 && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
-            const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = e < n ? __ldg(p + e) : 0.0f;
-        }
-        return;
-    }
-    const unsigned short* p = static_cast<const unsigned short*>(q) + i;
-    uint32_t w[4];
-    if (n == 8 && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-        w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            w[e] = (2 * e < n ? __ldg(p + 2 * e) : 0u) | (2 * e + 1 < n ? (uint32_t)__ldg(p + 2 * e + 1) << 16 : 0u);
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const uint32_t b = (w[e / 2] >> (16 * (e & 1))) & 0xFFFFu;
-        x[e] = type == kF16 ? to_f32<__half>(b) : to_f32<__nv_bfloat16>(b);
-    }
-}
-
 // An 8 x 8 matrix of halves, two columns of row lane / 4 per lane, transposed.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t y;
@@ -186,30 +128,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     return y;
 }
 
-__device__ __forceinline__ void write_out(void* out, int type, size_t i, float x) {
-    if (type == kF32)
-        static_cast<float*>(out)[i] = x;
-    else
-        static_cast<unsigned short*>(out)[i] =
-            (unsigned short)(type == kF16 ? from_f32<__half>(x) : from_f32<__nv_bfloat16>(x));
-}
-
-// Rows of a sequence that its last token sees, and the number of its tokens.
-struct Span {
-    int first, count, len;
-};
-__device__ __forceinline__ Span span_of(const CacheView& c, const AttendArgs& a, int s) {
-    Span p;
-    const int lo = __ldg(a.tok.offsets + s), hi = __ldg(a.tok.offsets + s + 1);
-    const bool good = lo >= 0 && hi >= lo && hi <= a.tok.n_tokens;
-    p.first = lo;
-    p.count = good ? hi - lo : 0;
-    p.len = min(max(__ldg(a.tok.lengths + s), 0), c.capacity);
-    return p;
-}
-__device__ __forceinline__ int visible(const CacheView& c, const AttendArgs& a, int len, int i) {
-    return min(min(len + (a.causal ? i + 1 : 0), c.capacity), a.max_rows);
-}
 // Rows per block where n blocks share them: equal, in whole steps of the block's warps.
 __host__ __device__ __forceinline__ int share_of(int rows, int n, int G) {
     const int step = kAttWarps * kTile * sub_tiles(G);
@@ -1065,13 +983,15 @@ AttendPlan make_plan(const CacheView& c, const AttendArgs& a) {
     AttendPlan p{};
     const bool found = a.k > 0;
     const long long cols = found ? a.group : (long long)std::max(1, a.max_tokens) * a.group;
-    // sixteen columns fill the query operand's M; wide rows leave no registers for them
-    p.nc = a.type != kF32 && c.G <= 2 && cols > 8 ? 16 : 8;
+    // Columns that fill half a block of 128 or more go to k_cache_wide; sixteen share a tile's codes where
+    // the registers hold them.
+    p.wide = !found && a.type != kF32 && c.G <= 2 && cols > kWideLeast;
+    p.nc = p.wide ? kWideCols : a.type != kF32 && c.G <= 2 && cols > 8 ? 16 : 8;
     p.col_tiles = (int)((cols + p.nc - 1) / p.nc);
     const long long items = (long long)(found ? a.tok.n_tokens : c.n_seqs) * c.heads * p.col_tiles;
     const int rows = std::max(1, found ? a.k : std::min(a.max_rows, c.capacity));
     const int step = kAttWarps * kTile * sub_tiles(c.G);
-    const long long slots = (long long)blocks_of(c.G, p.nc) * sm_count();
+    const long long slots = (long long)(p.wide ? 1 : blocks_of(c.G, p.nc)) * sm_count();
     // Enough blocks to fill the GPU once; with sequences of different lengths kWaves times as many, of
     // fixed rows, so that the longest do not run on alone.
     const int most = (rows + step - 1) / step;
@@ -1081,7 +1001,7 @@ AttendPlan make_plan(const CacheView& c, const AttendArgs& a) {
     p.share = most * step;
     // Lists enough to fill the GPU by warps: none waits for a block's barriers.
     p.solo = found && c.G <= 2 && p.nc == 8 && items * kSoloLists >= slots * kAttWarps;
-    if (!found && rows <= kClusterRows && fill >= 2) {
+    if (!found && !p.wide && rows <= kClusterRows && fill >= 2) {
         p.cluster = (int)std::min<long long>({kMaxCluster, fill, most});
     } else {
         const long long n = ragged ? std::max(1ll, kWaves * slots / std::max(1ll, items)) : fill;
@@ -1178,7 +1098,9 @@ void launch_cache_attend(const CacheView& c, const AttendArgs& a, cudaStream_t s
             (unsigned)((long long)(found ? a.tok.n_tokens : c.n_seqs) * c.heads * p.cluster * p.parts * p.col_tiles);
         {
             Tick tk(kKCacheAttend, st);
-            if (c.G == 1)
+            if (p.wide)
+                launch_cache_wide(c, k, grid, st);
+            else if (c.G == 1)
                 start_g<1>(c, k, p.nc, found, grid, st);
             else if (c.G == 2)
                 start_g<2>(c, k, p.nc, found, grid, st);

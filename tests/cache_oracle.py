@@ -66,7 +66,9 @@ def attend_head(q, rows, which, scale, dtype):
     2^-22 relative, its argument by 2^-24 of |z - max| (in log2). p * step is rounded to f16 (2^-12
     relative) in 16-bit calls, to two halves (2^-22) in f32 ones; half a subnormal step of f16 in units
     where the largest step is 4096 adds 2^-37 of it per row, times the code. Sums over n rows add n
-    roundings of 2^-23. The result is rounded to the call's type.
+    roundings of 2^-23. The result is rounded to the call's type. With many columns (16-bit types), the
+    values themselves are rounded to f16 as well (2^-12 more), in units of their row's power of two (at
+    most twice its largest level), whose subnormals add 2^-25 of it.
     """
     d = len(q)
     n = len(which)
@@ -88,9 +90,9 @@ def attend_head(q, rows, which, scale, dtype):
     out = p @ v
     level = 15 * rows.v_step[which] + np.abs(rows.v_low[which])
     a = p @ level
-    round_p = 2.0 ** -22 if dtype == "f32" else 2.0 ** -12
-    # a subnormal p * step: half of 2^-24 in units of (step's power of two, at most 2 * step) / 4096
-    tiny = n * 15 * 2.0 ** -25 / 4096 * 2 * rows.v_step[which].max(axis=0) * 8 if dtype != "f32" else 0.0
+    round_p = 2.0 ** -22 if dtype == "f32" else 2.0 ** -11
+    # a subnormal p * level: half of 2^-24 in units of (the level's power of two) / 4096, times 2^3 of lag
+    tiny = (n * 2.0 ** -25 / 4096 * 8 + 2.0 ** -25) * 2 * np.nanmax(level) if dtype != "f32" else 0.0
     err = a * (round_p + dp + (n + 64) * 2.0 ** -23) + tiny
     err = err + UNIT[dtype] * (np.abs(out) + err) + TINY[dtype]
     return out, lse, p, err, dz + (n + 32) * 2.0 ** -23 + abs(lse) * 2.0 ** -22, p * dp + 2.0 ** -126

@@ -133,6 +133,18 @@ def check_attend(rng, held, new, heads, group, dim, dtype, causal=True, weights=
     return got, got_l, got_w
 
 
+def check_attend_raw(f, q, held, new, dtype):
+    """One causal call without a comparison: outputs, log-sum-exps, flags."""
+    t, hq, dim = q.shape
+    qt, _ = rounded(q, dtype)
+    out, lse = torch.empty_like(qt), torch.empty(t, hq, device="cuda")
+    size = f.cache.attend_workspace(t, hq)
+    ws = torch.empty(max(size, 1), dtype=torch.uint8, device="cuda")
+    f.cache.attend(qt.data_ptr(), t, hq, offsets(new).data_ptr(), i32(held).data_ptr(), out.data_ptr(), dtype=dtype,
+                   d_lse=lse.data_ptr(), d_workspace=ws.data_ptr(), workspace_bytes=size, stream=stream())
+    return out.float().cpu().numpy(), lse.cpu().numpy(), f.cache.flags(stream())
+
+
 # ---- storage --------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("dim", [1, 32, 40, 64, 65, 80, 128, 192, 256, 377, 384])
@@ -270,6 +282,60 @@ def test_attend_padding_strides_and_empty_sequences(causal):
     rng = np.random.default_rng(11)
     check_attend(rng, [20, 0, 33, 0, 5], [2, 0, 1, 3, 0], 2, 2, 96, "f16", causal=causal, weights=True, front=3,
                  back=4, q_pad=5, capacity=50)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("dim", [40, 64, 80, 128])
+def test_attend_many_columns(dim, dtype):
+    """Blocks of 128 columns: full, ragged and several of them, rows in one part and in several."""
+    rng = np.random.default_rng(dim)
+    check_attend(rng, [300, 0, 127, 130], [33, 17, 1, 50], 1, 4, dim, dtype, weights=dim == 80)
+    check_attend(rng, [1500], [9], 2, 8, dim, dtype, weights=dim == 64, front=2, back=1, q_pad=3)
+    check_attend(rng, [130, 60], [24, 0], 1, 3, dim, dtype, causal=False, weights=True, capacity=200)
+
+
+def test_attend_many_columns_wide_ranges():
+    """Rising maxima, rows of very different magnitude (their powers of two grow from tile to tile)."""
+    rng = np.random.default_rng(31)
+    n, dim = 700, 128
+    q = rng.standard_normal((20, 4, dim)).astype(np.float32)
+    keys = tokens(rng, n, 1, dim)
+    keys[:, 0] += q[3, 0] * np.linspace(-2, 4, n)[:, None]
+    for mag in (np.ones(n), 10.0 ** np.linspace(-3, 3, n), 10.0 ** rng.uniform(-3, 3, n), np.full(n, 1e-20),
+                np.full(n, 1e20)):
+        values = (tokens(rng, n, 1, dim) * mag[:, None, None]).astype(np.float32)
+        f = Filled(rng, [n], n, 1, dim, "bf16", keys, values)
+        check_attend(rng, [n - 20], [20], 1, 4, dim, "bf16", fill=f, qs=q, capacity=n, weights=True)
+
+
+def test_attend_many_columns_ignore_what_they_cannot_see():
+    rng = np.random.default_rng(32)
+    held, new, cap = [200, 90], [40, 30], 256
+    k, v = tokens(rng, 2 * cap, 1, 128), tokens(rng, 2 * cap, 1, 128)
+    for s in range(2):
+        k[s * cap + held[s] + new[s]:(s + 1) * cap] = np.nan
+        v[s * cap + held[s] + new[s]:(s + 1) * cap] = np.inf
+    f = Filled(rng, [cap, cap], cap, 1, 128, "bf16", k, v)
+    got, _, _ = check_attend(rng, held, new, 1, 4, 128, "bf16", fill=f, capacity=cap, weights=True)
+    assert np.isfinite(got).all()
+    # a NaN value row of the step: the tokens before it do not see it, those from it on do
+    v[held[0] + 11] = np.nan
+    k[cap + held[1] + 7] = np.inf
+    f = Filled(rng, [cap, cap], cap, 1, 128, "bf16", k, v)
+    got, lse, _ = check_attend(rng, held, new, 1, 4, 128, "bf16", fill=f, capacity=cap)
+    assert np.isfinite(got[:11]).all() and np.isnan(got[11:40]).all() and np.isfinite(lse[:40]).all()
+    assert np.isfinite(got[40:47]).all() and np.isnan(got[47:]).all() and np.isnan(lse[47:]).all()
+
+
+def test_attend_many_columns_non_finite_queries():
+    rng = np.random.default_rng(33)
+    q = rng.standard_normal((30, 4, 64)).astype(np.float32)
+    q[3, 1, 5], q[20, 0, 9] = np.nan, -np.inf
+    f = Filled(rng, [70], 70, 1, 64, "f16")
+    got, lse, _ = check_attend_raw(f, q, [40], [30], "f16")
+    bad = np.zeros((30, 4), bool)
+    bad[3, 1] = bad[20, 0] = True
+    assert np.isnan(got[bad]).all() and np.isfinite(got[~bad]).all() and np.isnan(lse[bad]).all()
 
 
 def test_attend_hints_do_not_change_results():
