@@ -20,8 +20,9 @@
 // accumulators become O^T's B operand by a transposition of 8 x 8 halves in registers.
 //
 // Rounding: codes are exact, 16-bit queries are exact in f16 down to 2^-24 of their row's largest
-// element, p * step is rounded to f16 (2^-12 relative, below the output's own rounding). f32 calls
-// split query and p * step into two f16 halves each (22 bits).
+// element. p * step is rounded to f16 in bf16 calls (2^-12 relative, below the output's own rounding) and
+// split into two halves (22 bits) in f16 and f32 calls; one half doubled an f16 output's error where few rows
+// carry the weight. f32 calls split the query as well.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -46,7 +47,6 @@ constexpr int kMaxCluster = 8;
 constexpr int kMaxParts = 1024;
 constexpr int kWaves = 4;
 constexpr int kSoloLists = 2;
-constexpr int kWideLeast = 64;
 // Up to so many rows a cluster of blocks reads them and joins in shared memory, in one launch; above, its
 // blocks would wait for the slowest and the SMs for a place for all of them.
 constexpr int kClusterRows = 2048;
@@ -152,7 +152,7 @@ struct Shape {
     static constexpr int kTileBytes = kRows * 72 * G;
     static constexpr int kRingBytes = kAttWarps * kStages * kTileBytes;
     static constexpr int kPitch = G * kCacheGroup + 4;  // floats of one column's sums; a warp's writes meet no bank twice
-    static_assert(kRingBytes >= kAttWarps * NC * kPitch * 4, "the sums fit in the ring");
+    static_assert(kStages * kTileBytes >= NC * kPitch * 4, "a warp's sums fit in its ring");
     static constexpr int kBlocks = blocks_of(G, NC);
 };
 
@@ -259,8 +259,11 @@ struct Fetch {
 // kFoundSolo: the same, a list and head per warp.
 enum class Mode { kRows, kClustered, kFound, kFoundSolo };
 
-template <int G, int NC, bool F32, Mode MODE>
-__global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, (MODE >= Mode::kFound)>::kBlocks) k_cache_attend(CacheView c, AttendKernel kk) {
+template <int G, int NC, int TYPE, Mode MODE>
+__global__ void __launch_bounds__(kAttBS, Shape<G, NC, TYPE == kF32, (MODE >= Mode::kFound)>::kBlocks)
+    k_cache_attend(CacheView c, AttendKernel kk) {
+    constexpr bool F32 = TYPE == kF32;
+    constexpr bool kTwoHalves = TYPE != kBF16;  // p * step as two halves
     constexpr bool kSolo = MODE == Mode::kFoundSolo, FOUND = MODE == Mode::kFound || kSolo;
     constexpr bool kCluster = MODE == Mode::kClustered;
     constexpr int kTeam = kSolo ? 1 : kAttWarps;  // warps that share rows
@@ -685,7 +688,8 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, (MODE >= Mode::kFoun
                             }
                         }
                         b[j][i] = pack_h2(ps[0], ps[1]);
-                        if constexpr (F32) c2[j][i] = transpose8(pack_h2(left_over(ps[0], b[j][i], 0), left_over(ps[1], b[j][i], 1)));
+                        if constexpr (kTwoHalves)
+                            c2[j][i] = transpose8(pack_h2(left_over(ps[0], b[j][i], 0), left_over(ps[1], b[j][i], 1)));
                         b[j][i] = transpose8(b[j][i]);
                     }
                 }
@@ -702,7 +706,7 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, (MODE >= Mode::kFoun
                     for (int j = 0; j < kNt; ++j) {
                         mma(o[g][2 * i][j], e0, e1, e2, e3, b[j][0], b[j][1]);
                         mma(o[g][2 * i + 1][j], d0, d1, d2, d3, b[j][0], b[j][1]);
-                        if constexpr (F32) {
+                        if constexpr (kTwoHalves) {
                             mma(o[g][2 * i][j], e0, e1, e2, e3, c2[j][0], c2[j][1]);
                             mma(o[g][2 * i + 1][j], d0, d1, d2, d3, c2[j][0], c2[j][1]);
                         }
@@ -744,7 +748,8 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, F32, (MODE >= Mode::kFoun
                     low[j][g] = __fadd_rn(low[j][g], __shfl_xor_sync(~0u, low[j][g], d));
         }
         team_sync();
-        float* s_o = reinterpret_cast<float*>(s_ring);  // [warp][column][S::kPitch]
+        // [warp][column][S::kPitch] from where every warp is done; a solo warp stays in its own ring
+        float* s_o = reinterpret_cast<float*>(s_ring) + (kSolo ? warp * (S::kStages * S::kTileBytes / 4 - NC * S::kPitch) : 0);
 #pragma unroll
         for (int j = 0; j < kCols; ++j) {
             const int col = 8 * (j >> 1) + 2 * t + (j & 1);
@@ -983,9 +988,12 @@ AttendPlan make_plan(const CacheView& c, const AttendArgs& a) {
     AttendPlan p{};
     const bool found = a.k > 0;
     const long long cols = found ? a.group : (long long)std::max(1, a.max_tokens) * a.group;
-    // Columns that fill half a block of 128 or more go to k_cache_wide; sixteen share a tile's codes where
-    // the registers hold them.
-    p.wide = !found && a.type != kF32 && c.G <= 2 && cols > kWideLeast;
+    // Columns that fill blocks of 128 to four fifths go to k_cache_wide (4 sequences of 20,000 rows, 8 heads of
+    // 128, wide against sixteen columns: 128 columns 236 and 229 us, 192 330 and 316, 256 348 and 406, 512 594
+    // and 741; one sequence, 2048 columns: 437 and 745). Below that, sixteen share a tile's codes where the
+    // registers hold them.
+    const long long full = (cols + kWideCols - 1) / kWideCols * kWideCols;
+    p.wide = !found && a.type == kBF16 && c.G <= 2 && cols >= kWideCols && 5 * cols >= 4 * full;
     p.nc = p.wide ? kWideCols : a.type != kF32 && c.G <= 2 && cols > 8 ? 16 : 8;
     p.col_tiles = (int)((cols + p.nc - 1) / p.nc);
     const long long items = (long long)(found ? a.tok.n_tokens : c.n_seqs) * c.heads * p.col_tiles;
@@ -1027,17 +1035,17 @@ AttendPlan make_plan(const CacheView& c, const AttendArgs& a) {
     return p;
 }
 
-template <int G, int NC, bool F32>
+template <int G, int NC, int TYPE>
 void start(const CacheView& c, const AttendKernel& k, bool found, unsigned grid, cudaStream_t st) {
-    const int smem = found ? Shape<G, NC, F32, true>::kRingBytes : Shape<G, NC, F32, false>::kRingBytes;
-    auto kernel = k_cache_attend<G, NC, F32, Mode::kRows>;
+    const int smem = found ? Shape<G, NC, TYPE == kF32, true>::kRingBytes : Shape<G, NC, TYPE == kF32, false>::kRingBytes;
+    auto kernel = k_cache_attend<G, NC, TYPE, Mode::kRows>;
     if (found)
-        kernel = k_cache_attend<G, NC, F32, Mode::kFound>;
+        kernel = k_cache_attend<G, NC, TYPE, Mode::kFound>;
     else if (k.cluster > 1)
-        kernel = k_cache_attend<G, NC, F32, Mode::kClustered>;
+        kernel = k_cache_attend<G, NC, TYPE, Mode::kClustered>;
     if constexpr (G <= 2 && NC == 8)
         if (k.solo) {
-            kernel = k_cache_attend<G, NC, F32, Mode::kFoundSolo>;
+            kernel = k_cache_attend<G, NC, TYPE, Mode::kFoundSolo>;
             grid = (grid + kAttWarps - 1) / kAttWarps;
         }
     set_smem((const void*)kernel, smem);
@@ -1054,14 +1062,21 @@ void start(const CacheView& c, const AttendKernel& k, bool found, unsigned grid,
     cudaLaunchKernelEx(&cfg, kernel, c, k);
 }
 
+template <int G, int TYPE>
+void start_16(const CacheView& c, const AttendKernel& k, int nc, bool found, unsigned grid, cudaStream_t st) {
+    if constexpr (G <= 2)
+        if (nc == 16) return start<G, 16, TYPE>(c, k, found, grid, st);
+    start<G, 8, TYPE>(c, k, found, grid, st);
+}
+
 template <int G>
 void start_g(const CacheView& c, const AttendKernel& k, int nc, bool found, unsigned grid, cudaStream_t st) {
     if (k.a.type == kF32)
-        start<G, 8, true>(c, k, found, grid, st);
-    else if (nc == 8)
-        start<G, 8, false>(c, k, found, grid, st);
-    else if constexpr (G <= 2)
-        start<G, 16, false>(c, k, found, grid, st);
+        start<G, 8, kF32>(c, k, found, grid, st);
+    else if (k.a.type == kF16)
+        start_16<G, kF16>(c, k, nc, found, grid, st);
+    else
+        start_16<G, kBF16>(c, k, nc, found, grid, st);
 }
 
 }  // namespace

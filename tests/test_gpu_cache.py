@@ -289,28 +289,28 @@ def test_attend_padding_strides_and_empty_sequences(causal):
 def test_attend_many_columns(dim, dtype):
     """Blocks of 128 columns: full, ragged and several of them, rows in one part and in several."""
     rng = np.random.default_rng(dim)
-    check_attend(rng, [300, 0, 127, 130], [33, 17, 1, 50], 1, 4, dim, dtype, weights=dim == 80)
-    check_attend(rng, [1500], [9], 2, 8, dim, dtype, weights=dim == 64, front=2, back=1, q_pad=3)
-    check_attend(rng, [130, 60], [24, 0], 1, 3, dim, dtype, causal=False, weights=True, capacity=200)
+    check_attend(rng, [300, 0, 127, 130], [33, 17, 1, 53], 1, 4, dim, dtype, weights=dim == 80)
+    check_attend(rng, [1500], [13], 2, 8, dim, dtype, weights=dim == 64, front=2, back=1, q_pad=3)
+    check_attend(rng, [130, 60], [32, 0], 1, 4, dim, dtype, causal=False, weights=True, capacity=200)
 
 
 def test_attend_many_columns_wide_ranges():
     """Rising maxima, rows of very different magnitude (their powers of two grow from tile to tile)."""
     rng = np.random.default_rng(31)
     n, dim = 700, 128
-    q = rng.standard_normal((20, 4, dim)).astype(np.float32)
+    q = rng.standard_normal((32, 4, dim)).astype(np.float32)
     keys = tokens(rng, n, 1, dim)
     keys[:, 0] += q[3, 0] * np.linspace(-2, 4, n)[:, None]
     for mag in (np.ones(n), 10.0 ** np.linspace(-3, 3, n), 10.0 ** rng.uniform(-3, 3, n), np.full(n, 1e-20),
                 np.full(n, 1e20)):
         values = (tokens(rng, n, 1, dim) * mag[:, None, None]).astype(np.float32)
         f = Filled(rng, [n], n, 1, dim, "bf16", keys, values)
-        check_attend(rng, [n - 20], [20], 1, 4, dim, "bf16", fill=f, qs=q, capacity=n, weights=True)
+        check_attend(rng, [n - 32], [32], 1, 4, dim, "bf16", fill=f, qs=q, capacity=n, weights=True)
 
 
 def test_attend_many_columns_ignore_what_they_cannot_see():
     rng = np.random.default_rng(32)
-    held, new, cap = [200, 90], [40, 30], 256
+    held, new, cap = [200, 90], [44, 36], 256
     k, v = tokens(rng, 2 * cap, 1, 128), tokens(rng, 2 * cap, 1, 128)
     for s in range(2):
         k[s * cap + held[s] + new[s]:(s + 1) * cap] = np.nan
@@ -323,17 +323,17 @@ def test_attend_many_columns_ignore_what_they_cannot_see():
     k[cap + held[1] + 7] = np.inf
     f = Filled(rng, [cap, cap], cap, 1, 128, "bf16", k, v)
     got, lse, _ = check_attend(rng, held, new, 1, 4, 128, "bf16", fill=f, capacity=cap)
-    assert np.isfinite(got[:11]).all() and np.isnan(got[11:40]).all() and np.isfinite(lse[:40]).all()
-    assert np.isfinite(got[40:47]).all() and np.isnan(got[47:]).all() and np.isnan(lse[47:]).all()
+    assert np.isfinite(got[:11]).all() and np.isnan(got[11:44]).all() and np.isfinite(lse[:44]).all()
+    assert np.isfinite(got[44:51]).all() and np.isnan(got[51:]).all() and np.isnan(lse[51:]).all()
 
 
 def test_attend_many_columns_non_finite_queries():
     rng = np.random.default_rng(33)
-    q = rng.standard_normal((30, 4, 64)).astype(np.float32)
+    q = rng.standard_normal((32, 4, 64)).astype(np.float32)
     q[3, 1, 5], q[20, 0, 9] = np.nan, -np.inf
-    f = Filled(rng, [70], 70, 1, 64, "f16")
-    got, lse, _ = check_attend_raw(f, q, [40], [30], "f16")
-    bad = np.zeros((30, 4), bool)
+    f = Filled(rng, [72], 72, 1, 64, "f16")
+    got, lse, _ = check_attend_raw(f, q, [40], [32], "f16")
+    bad = np.zeros((32, 4), bool)
     bad[3, 1] = bad[20, 0] = True
     assert np.isnan(got[bad]).all() and np.isfinite(got[~bad]).all() and np.isnan(lse[bad]).all()
 
@@ -496,6 +496,50 @@ def test_attend_found(dim, heads, group, k, dtype):
                          out2.data_ptr(), dtype=dtype, d_workspace=ws.data_ptr(), workspace_bytes=size,
                          stream=stream())
     assert torch.equal(out, out2)
+
+
+def test_attend_found_many_lists():
+    """More lists than the GPU has blocks for: a list and head per warp, against one list at a time."""
+    rng = np.random.default_rng(41)
+    for dim, heads, group, k, dtype in ((64, 2, 2, 70, "f32"), (128, 1, 8, 33, "bf16"), (64, 1, 5, 97, "f16")):
+        t, n = 3000, 4000
+        f = Filled(rng, [n], n, heads, dim, dtype)
+        hq = heads * group
+        q, qx = rounded((rng.standard_normal((t, hq, dim)) * 1.5).astype(np.float32), dtype)
+        lists = rng.integers(0, n + 200, (t, k)).astype(np.uint64)
+        lists[rng.random((t, k)) < 0.1] = PAD
+        rows = torch.tensor(lists.view(np.int64)).cuda()
+        out, lse = torch.empty_like(q), torch.empty(t, hq, device="cuda")
+        w = torch.empty(t, k, device="cuda")
+        size = f.cache.attend_found_workspace(t, hq, k)
+        ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+
+        def go(first, count, out, lse, w):
+            f.cache.attend_found(q[first:].data_ptr(), count, hq, offsets([count]).data_ptr(), i32([n]).data_ptr(),
+                                 rows[first:].data_ptr(), k, out.data_ptr(), dtype=dtype, d_lse=lse.data_ptr(),
+                                 d_weights=w.data_ptr(), d_workspace=ws.data_ptr(), workspace_bytes=size,
+                                 stream=stream())
+
+        go(0, t, out, lse, w)
+        torch.cuda.synchronize()
+        got, gl, gw = out.float().cpu().numpy(), lse.cpu().numpy(), w.cpu().numpy()
+        assert np.isfinite(got).all() and np.isfinite(gl).all() and np.allclose(gw.sum(axis=1), hq, rtol=1e-4)
+        for tok in range(0, t, 97):
+            at = [e for e in range(k) if int(lists[tok, e]) < n]
+            which = [int(lists[tok, e]) for e in at]
+            for hh in range(hq):
+                o, l, _, err, lerr, _ = O.attend_head(qx[tok, hh], f.rows[0][hh // group], which, dim ** -0.5, dtype)
+                close(got[tok, hh], o, err, f"out {tok} {hh}")
+                close(gl[tok, hh], l, lerr, f"lse {tok} {hh}")
+        # every list again in small calls: the same up to the order of the sums (twice the bound of one)
+        o2, l2, w2 = torch.empty_like(out), torch.empty_like(lse), torch.empty_like(w)
+        for first in range(0, t, 100):
+            go(first, 100, o2[first:], l2[first:], w2[first:])
+        torch.cuda.synchronize()
+        span = (k + 64) * 2.0 ** -22
+        assert ((w2 - w).abs().max() <= hq * span * 4) and ((l2 - lse).abs().max() <= span * 8)
+        top = torch.maximum(out.abs().float(), o2.abs().float()).amax()
+        assert (o2.float() - out.float()).abs().max() <= top * (2.0 ** -7 if dtype == "bf16" else 2.0 ** -10)
 
 
 # ---- eviction -------------------------------------------------------------------------------------
