@@ -44,6 +44,30 @@ __device__ __forceinline__ uint32_t from_f32<__nv_bfloat16>(float x) {
     return __bfloat16_as_ushort(__float2bfloat16_rn(x));
 }
 
+// Two f32 in one register pair.
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 pair(float a, float b) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(f2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+    f2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+    f2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 // The sequence of packed token `tok`: offsets[s] <= tok < offsets[s + 1], or -1 for a token before
 // the first or behind the last sequence. Called by an aligned group of 8 lanes (lane8, mask), which
 // count the starts at or below tok together: one round of loads per 8 sequences, none dependent;

@@ -72,22 +72,39 @@ __device__ __noinline__ uint32_t codes_exact(float4 a, float4 b, float low, floa
 //    difference, unless some element is below 2^-13 (bf16) or 2^-10 (f16) of the step: `fine` asks
 //    for the exact way there. x - low itself is exact under the same condition;
 //  - f32 elements: wherever t is that close to k + 1/2, which is asked here.
+// Elements i and i + 4 go together in packed f32 operations; the codes of four are summed as
+// c_0 + 16 c_1 + 256 c_2 + 4096 c_3, exact in f32.
 template <typename T>
 __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float low, float step, bool fine) {
     constexpr float kMagic = 12582912.0f;
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(step));
-    uint32_t code = 0;
+    const f2 lows = pair(-low, -low), steps = pair(-step, -step), invs = pair(inv, inv), magic = pair(kMagic, kMagic),
+             down = pair(-kMagic, -kMagic);
+    f2 sum = 0;
+    float scale = 1.0f;
 #pragma unroll
-    for (int i = 7; i >= 0; --i) {
-        const float d = __fsub_rn(x[i], low);
-        float t = __fmul_rn(d, inv);
-        t = __fmaf_rn(__fmaf_rn(-t, step, d), inv, t);
-        if constexpr (!std::is_same<T, __nv_bfloat16>::value) t = fminf(fmaxf(t, 0.0f), 15.0f);  // bf16: low is the smallest
-        const float r = __fadd_rn(t, kMagic);
-        if constexpr (sizeof(T) == 4) fine |= fabsf(__fsub_rn(t, __fsub_rn(r, kMagic))) > 0.499996f;
-        code = code * 16 + (__float_as_uint(r) & 15u);
+    for (int i = 0; i < 4; ++i) {
+        const f2 d = add2(pair(x[i], x[i + 4]), lows);
+        f2 t = mul2(d, invs);
+        t = fma2(fma2(t, steps, d), invs, t);
+        if constexpr (!std::is_same<T, __nv_bfloat16>::value) {  // bf16: low is the smallest
+            float a, b;
+            unpair(t, a, b);
+            t = pair(fminf(fmaxf(a, 0.0f), 15.0f), fminf(fmaxf(b, 0.0f), 15.0f));
+        }
+        const f2 c = add2(add2(t, magic), down);
+        if constexpr (sizeof(T) == 4) {
+            float a, b;
+            unpair(fma2(c, pair(-1.0f, -1.0f), t), a, b);
+            fine |= fmaxf(fabsf(a), fabsf(b)) > 0.499996f;
+        }
+        sum = fma2(c, pair(scale, scale), sum);
+        scale *= 16.0f;
     }
+    float lo, hi;
+    unpair(add2(sum, magic), lo, hi);
+    uint32_t code = __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x5410);
     // a subnormal step has no reciprocal here
     if (fine || inv == INFINITY)
         code = codes_exact(make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]), low, step);
@@ -100,10 +117,17 @@ struct Raw8 {
     uint32_t w[2 * sizeof(T)];
 };
 
-template <typename T>
+// kWhole: all eight are there, or none (n = 0: zeros).
+template <typename T, bool kWhole>
 __device__ __forceinline__ Raw8<T> load8(const T* __restrict__ p, int n, bool vec) {
     Raw8<T> r;
-    if (vec && n == 8) {
+    if constexpr (kWhole) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+            const uint4 a = n ? __ldcs(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0, 0, 0, 0);
+            r.w[4 * i] = a.x, r.w[4 * i + 1] = a.y, r.w[4 * i + 2] = a.z, r.w[4 * i + 3] = a.w;
+        }
+    } else if (vec && n == 8) {
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
             const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p) + i);
@@ -196,9 +220,9 @@ __device__ __forceinline__ void extremes(const Raw8<T>& r, int n, float* hi, flo
     *lo = -to_f32<T>(m >> 16);
 }
 
-template <typename T>
+template <typename T, bool kWhole>
 __device__ __forceinline__ void store8(T* __restrict__ p, int n, bool vec, const float (&x)[8]) {
-    if (vec && n == 8) {
+    if (kWhole || (vec && n == 8)) {
         if constexpr (sizeof(T) == 4) {
             __stcs(reinterpret_cast<float4*>(p), make_float4(x[0], x[1], x[2], x[3]));
             __stcs(reinterpret_cast<float4*>(p) + 1, make_float4(x[4], x[5], x[6], x[7]));
@@ -251,7 +275,7 @@ __device__ __forceinline__ void find_places(const CacheView& c, const CacheToken
 // Rows into the cache. blockIdx.x: a run of tokens; blockIdx.y: even keys, odd values, times the slices of a
 // token's units. Eight lanes take a group of 64 dimensions of one head. Every lane goes through the same
 // passes; those without a unit, or whose token has no row, load and store nothing.
-template <typename T, int G, int U>
+template <typename T, int G, int U, bool kWhole>
 __global__ void __launch_bounds__(kStoreBS) k_cache_append(CacheView c, AppendArgs a, bool vec, StoreShape sh) {
     __shared__ long long s_place[kMaxRun];
     const bool is_key = !(blockIdx.y & 1);
@@ -263,8 +287,8 @@ __global__ void __launch_bounds__(kStoreBS) k_cache_append(CacheView c, AppendAr
     const int head = rest / G, g = rest - head * G;
     const int d = g * kCacheGroup + 8 * chunk;
     const bool in = mine < sh.side && head < c.heads;
-    const int have = in ? min(max(c.dim - d, 0), 8) : 0;
-    const bool pad = g * kCacheGroup >= c.dim;  // a group of padding
+    const int have = kWhole ? 8 : in ? min(max(c.dim - d, 0), 8) : 0;
+    const bool pad = !kWhole && g * kCacheGroup >= c.dim;  // a group of padding
     const size_t stride = is_key ? a.key_stride : a.value_stride;
     const T* src = static_cast<const T*>(is_key ? a.keys : a.values) + (size_t)(tok0 + mine) * stride +
                    (size_t)head * c.dim + d;
@@ -278,7 +302,7 @@ __global__ void __launch_bounds__(kStoreBS) k_cache_append(CacheView c, AppendAr
         for (int i = 0; i < U; ++i) {
             const int t = t0 + i * sh.side + mine;
             row[i] = in && t < n_tok ? s_place[t] : -1;
-            raw[i] = load8(src + (size_t)(t0 + i * sh.side) * stride, row[i] >= 0 ? have : 0, vec);
+            raw[i] = load8<T, kWhole>(src + (size_t)(t0 + i * sh.side) * stride, row[i] >= 0 ? have : 0, vec);
         }
 #pragma unroll
         for (int i = 0; i < U; ++i) {
@@ -309,7 +333,7 @@ __global__ void __launch_bounds__(kStoreBS) k_cache_append(CacheView c, AppendAr
 }
 
 // Rows back as values, in the same order.
-template <typename T, int G, int U>
+template <typename T, int G, int U, bool kWhole>
 __global__ void __launch_bounds__(kStoreBS) k_cache_read(CacheView c, ReadArgs a, bool vec, StoreShape sh) {
     __shared__ long long s_place[kMaxRun];
     const bool is_key = !(blockIdx.y & 1);
@@ -321,7 +345,7 @@ __global__ void __launch_bounds__(kStoreBS) k_cache_read(CacheView c, ReadArgs a
     const int head = rest / G, g = rest - head * G;
     const int d = g * kCacheGroup + 8 * chunk;
     const bool in = mine < sh.side && head < c.heads;
-    const int have = min(max(c.dim - d, 0), 8);
+    const int have = kWhole ? 8 : min(max(c.dim - d, 0), 8);
     const size_t stride = (size_t)c.heads * c.dim;
     T* dst = static_cast<T*>(is_key ? a.keys : a.values) + (size_t)(tok0 + mine) * stride + (size_t)head * c.dim + d;
     const uint32_t* codes = (is_key ? c.kc : c.vc) + (size_t)head * c.rows * 8 * G +
@@ -342,14 +366,25 @@ __global__ void __launch_bounds__(kStoreBS) k_cache_read(CacheView c, ReadArgs a
         for (int i = 0; i < U; ++i) {
             const uint32_t w = is_key ? code[i] : transpose_nibbles(code[i], l8);
             const float step = par_step(par[i]), low = par_low(par[i]);
+            // A nibble where it lies, as the low bits of 2^23 + 16^e c, times step / 16^e: exact, so one rounding
             float x[8];
+            f2 s2 = pair(step, __fmul_rn(step, 0.0625f)), lows = pair(low, low);
+            const f2 down = pair(-8388608.0f, -8388608.0f), next = pair(0x1p-8f, 0x1p-8f);
+            const uint32_t up = w >> 16;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                // a whole number below 2^23 as the low bits of 2^23 + itself
-                const float v = __fsub_rn(__uint_as_float(0x4B000000u | ((w >> (4 * e)) & 15u)), 8388608.0f);
-                x[e] = __fmaf_rn(step, v, low);
+            for (int e = 0; e < 2; ++e) {
+                const uint32_t m0 = 15u << (8 * e), m1 = 15u << (8 * e + 4);
+                const f2 a = add2(pair(__uint_as_float((w & m0) | 0x4B000000u), __uint_as_float((w & m1) | 0x4B000000u)), down);
+                const f2 b = add2(pair(__uint_as_float((up & m0) | 0x4B000000u), __uint_as_float((up & m1) | 0x4B000000u)), down);
+                unpair(fma2(a, s2, lows), x[2 * e], x[2 * e + 1]);
+                unpair(fma2(b, s2, lows), x[2 * e + 4], x[2 * e + 5]);
+                s2 = mul2(s2, next);
             }
-            if (there[i]) store8(dst + (size_t)(t0 + i * sh.side) * stride, have, vec, x);
+            if (step < 0x1p-100f) {  // step / 16^e may not be exact there
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = __fmaf_rn(step, (float)((w >> (4 * e)) & 15u), low);
+            }
+            if (there[i]) store8<T, kWhole>(dst + (size_t)(t0 + i * sh.side) * stride, have, vec, x);
         }
     }
 }
@@ -665,19 +700,19 @@ StorePlan store_plan(const CacheView& c, int n_tokens) {
     return p;
 }
 
-template <typename T, int G>
+template <typename T, int G, bool kWhole>
 void start_append(const CacheView& c, const AppendArgs& a, bool vec, const StorePlan& p, cudaStream_t st) {
     if (p.deep)
-        k_cache_append<T, G, kDeep><<<p.grid, kStoreBS, 0, st>>>(c, a, vec, p.shape);
+        k_cache_append<T, G, kDeep, kWhole><<<p.grid, kStoreBS, 0, st>>>(c, a, vec, p.shape);
     else
-        k_cache_append<T, G, 1><<<p.grid, kStoreBS, 0, st>>>(c, a, vec, p.shape);
+        k_cache_append<T, G, 1, kWhole><<<p.grid, kStoreBS, 0, st>>>(c, a, vec, p.shape);
 }
-template <typename T, int G>
+template <typename T, int G, bool kWhole>
 void start_read(const CacheView& c, const ReadArgs& a, bool vec, const StorePlan& p, cudaStream_t st) {
     if (p.deep)
-        k_cache_read<T, G, kDeep><<<p.grid, kStoreBS, 0, st>>>(c, a, vec, p.shape);
+        k_cache_read<T, G, kDeep, kWhole><<<p.grid, kStoreBS, 0, st>>>(c, a, vec, p.shape);
     else
-        k_cache_read<T, G, 1><<<p.grid, kStoreBS, 0, st>>>(c, a, vec, p.shape);
+        k_cache_read<T, G, 1, kWhole><<<p.grid, kStoreBS, 0, st>>>(c, a, vec, p.shape);
 }
 
 // f with the type and the groups as constants
@@ -711,7 +746,12 @@ void launch_cache_append(const CacheView& c, const AppendArgs& a, cudaStream_t s
                      (size_t)c.dim * es % 16 == 0;
     const StorePlan p = store_plan(c, a.tok.n_tokens);
     Tick tk(kKCacheAppend, st);
-    by_type_and_groups(a.type, c.G, [&](auto t, auto g) { start_append<decltype(t), decltype(g)::value>(c, a, vec, p, st); });
+    by_type_and_groups(a.type, c.G, [&](auto t, auto g) {
+        if (vec && c.dim == c.G * kCacheGroup)
+            start_append<decltype(t), decltype(g)::value, true>(c, a, vec, p, st);
+        else
+            start_append<decltype(t), decltype(g)::value, false>(c, a, vec, p, st);
+    });
 }
 
 void launch_cache_read(const CacheView& c, const ReadArgs& a, cudaStream_t st) {
@@ -720,7 +760,12 @@ void launch_cache_read(const CacheView& c, const ReadArgs& a, cudaStream_t st) {
     const bool vec = aligned16(a.keys, 0) && aligned16(a.values, 0) && (size_t)c.dim * es % 16 == 0;
     const StorePlan p = store_plan(c, a.tok.n_tokens);
     Tick tk(kKCacheRead, st);
-    by_type_and_groups(a.type, c.G, [&](auto t, auto g) { start_read<decltype(t), decltype(g)::value>(c, a, vec, p, st); });
+    by_type_and_groups(a.type, c.G, [&](auto t, auto g) {
+        if (vec && c.dim == c.G * kCacheGroup)
+            start_read<decltype(t), decltype(g)::value, true>(c, a, vec, p, st);
+        else
+            start_read<decltype(t), decltype(g)::value, false>(c, a, vec, p, st);
+    });
 }
 
 size_t cache_evict_workspace(const CacheView& c) {

@@ -157,6 +157,9 @@ def test_append_and_read_are_exact(dtype, dim):
     k[1, 0, :min(dim, 16)] = np.arange(16)[:dim]  # whole numbers: ties
     v[2, 1] = np.round(v[2, 1] * 4) / 4
     v[3, 2] *= 1e-30
+    v[4, 0] *= 3e-37  # (f16: zeros)
+    k[5, 1] *= 1e-39
+    v[6, 1] *= 1e37 if dtype != "f16" else 1e4
     kt, kx = rounded(k, dtype)
     vt, vx = rounded(v, dtype)
     c = M.AttentionCache(4, cap, heads, dim)
