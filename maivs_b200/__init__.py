@@ -4,6 +4,8 @@
 return types and errors (src/index.rs and src/concurrent.rs #[pymethods], src/lib.rs:32-39). The index is built on the host cores;
 `search` / `search_batch` run on the GPU through hand-written sm_100a kernels behind the C ABI of
 include/maivs_b200.h. There is no CPU search path: without a CUDA device, search raises.
+`AttentionCache` (no counterpart in the reference) is the read-out that follows a search: key and value
+rows in 4 bits, attention over them or over the rows found, eviction by the weight they gathered.
 """
 from __future__ import annotations
 
@@ -14,8 +16,8 @@ import numpy as np
 
 from . import _lib
 
-__all__ = ["FlatCellIndex", "ConcurrentIndex", "AttentionCache", "profile", "profile_read", "MaivsError", "nccl_unique_id",
-           "shard_over_torch"]
+__all__ = ["FlatCellIndex", "ConcurrentIndex", "AttentionCache", "profile", "profile_read", "MaivsError",
+           "nccl_unique_id", "shard_over_torch"]
 
 
 class MaivsError(RuntimeError):
@@ -628,6 +630,7 @@ class AttentionCache:
         L = _lib.lib()
         h = C.c_void_p()
         self._h = None
+        self._free = L.maivs_cache_free  # still there when the interpreter takes the module down
         rc = L.maivs_cache_new(_size(n_seqs, "n_seqs"), _size(capacity, "capacity"), _size(n_heads, "n_heads"),
                                _size(dim, "dim"), -1 if device is None else _size(device, "device"), C.byref(h))
         self._h = h
@@ -642,7 +645,7 @@ class AttentionCache:
     def __del__(self):
         h = getattr(self, "_h", None)
         if h:
-            _lib.lib().maivs_cache_free(h)
+            self._free(h)
             self._h = None
 
     def _check(self, rc: int) -> None:
@@ -728,7 +731,8 @@ class AttentionCache:
 
     def flags(self, stream: int = 0) -> int:
         """Flags set since the last call (1: append past the capacity, 2: a sequence longer than
-        max_rows, 4: offsets out of order); synchronises `stream`."""
+        max_rows, 4: offsets out of order, 8: a bounded wait ran out, results invalid); synchronises
+        `stream`."""
         f = C.c_uint32(0)
         self._check(_lib.lib().maivs_cache_flags(self._h, stream, C.byref(f)))
         return int(f.value)

@@ -110,6 +110,8 @@ std::string attend_args(const maivs_cache* cx, size_t n_tokens, size_t q_heads, 
         return "n_query_heads must be a multiple of the cache's heads";
     if (n_tokens > kMaxTokens) return "n_tokens must be at most 2^27";
     if (k > (size_t(1) << 27)) return "k must be at most 2^27";
+    if (n_tokens * q_heads > (size_t(1) << 30)) return "n_tokens x n_query_heads must be at most 2^30";
+    if ((k + 127) / 128 * n_tokens > 0x7FFFFFFF) return "n_tokens x k must be at most 2^38";
     a->tok.n_tokens = (int)n_tokens;
     a->q_heads = (int)q_heads;
     a->group = (int)(q_heads / cx->v.heads);
@@ -308,7 +310,8 @@ int check_attend(maivs_cache* cx, const AttendArgs* pa) {
         return cfail(cx, MAIVS_BAD_ARG, "d_queries and d_out must be given, aligned to their type");
     if (!aligned(a.lse, 4) || !aligned(a.w_in, 4) || !aligned(a.w_out, 4) || !aligned(a.rows, 8))
         return cfail(cx, MAIVS_BAD_ARG, "d_lse, weights and rows must be aligned to their type");
-    if (!std::isfinite(a.scale)) return cfail(cx, MAIVS_BAD_ARG, "scale must be finite");
+    // the kernels fold it into one f32 factor with the query's power of two and the codes' 2^24
+    if (!(std::fabs(a.scale) <= 0x1p100f)) return cfail(cx, MAIVS_BAD_ARG, "scale must be finite and at most 2^100 in magnitude");
     if (!std::isfinite(a.decay)) return cfail(cx, MAIVS_BAD_ARG, "decay must be finite");
     return 0;
 }

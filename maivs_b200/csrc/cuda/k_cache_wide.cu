@@ -185,10 +185,11 @@ __device__ __forceinline__ void decode_keys(const KeyCodes<G>& x, char* sk, int 
     }
     if (part == 0) {
         uint32_t ext[4] = {0, 0, 0, 0};
-        const float far = __fmul_rn(up, (float)(1 << kSumDown));
+        constexpr float kFar = 1 << kSumDown;
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            const float low = __fmul_rn(par_low(x.p[g]), far), mids = __fmul_rn(8.0f * par_step(x.p[g]), far);
+            // `up` first: up * kFar is past f32's range in a tile of zeros
+            const float low = __fmul_rn(par_low(x.p[g]), up) * kFar, mids = __fmul_rn(par_step(x.p[g]), up) * (8 * kFar);
             ext[2 * g] = pack_h2(low, low);
             ext[2 * g + 1] = pack_h2(mids, mids);
         }

@@ -107,7 +107,7 @@ def test_append_refuses(cache, kw):
 
 @pytest.mark.parametrize("kw", [dict(n_query_heads=3), dict(n_query_heads=0), dict(d_queries=0), dict(d_out=0),
                                 dict(d_out=P + 1), dict(dtype="int4"), dict(query_stride=319), dict(scale=float("nan")),
-                                dict(scale=float("inf")), dict(decay=float("nan")), dict(d_weights_in=P),
+                                dict(scale=float("inf")), dict(scale=-1.3e30), dict(decay=float("nan")), dict(d_weights_in=P),
                                 dict(d_weights_out=P), dict(d_lse=P + 1), dict(d_offsets=0), dict(n_tokens=-4),
                                 dict(d_workspace=P + 8, d_weights_in=P, d_weights_out=P),
                                 dict(d_weights_in=P, d_weights_out=P, workspace_bytes=8),
@@ -139,10 +139,14 @@ def test_workspace_refuses(cache):
         cache.attend_workspace(4, 3)
     with pytest.raises(ValueError):
         cache.attend_found_workspace(4, 4, 0)
+    with pytest.raises(ValueError, match="2\\^30"):
+        cache.attend_workspace(2**20, 2048)
+    with pytest.raises(ValueError, match="2\\^38"):
+        cache.attend_found_workspace(2**20, 2, 2**20)
     # a grid of more than 2^31 blocks
     big = M.AttentionCache(65535, 16, 1024, 64, device=None)
     with pytest.raises(ValueError, match="blocks"):
-        big.attend_workspace(1 << 20, 1024 * 8, max_tokens=1 << 20)
+        big.attend_workspace(1 << 17, 1024 * 8, max_tokens=1 << 17)
 
 
 def test_without_a_gpu_a_cache_fails_loudly():

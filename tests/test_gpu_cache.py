@@ -311,6 +311,25 @@ def test_attend_many_columns_wide_ranges():
         check_attend(rng, [n - 32], [32], 1, 4, dim, "bf16", fill=f, qs=q, capacity=n, weights=True)
 
 
+@pytest.mark.parametrize("new", [1, 32])
+@pytest.mark.parametrize("mag", [0.0, 1e-38, 1e-30, 1e30])
+def test_attend_tiles_of_zeros_and_of_extreme_keys(mag, new):
+    """Whole tiles of rows whose keys, and whose values, are zeros, tiny or huge."""
+    rng = np.random.default_rng(34)
+    n, dim = 400, 128
+    keys, values = tokens(rng, n, 1, dim), tokens(rng, n, 1, dim)
+    values[128:384] *= mag
+    q = rng.standard_normal((new, 4, dim)).astype(np.float32)
+    if mag != 1e30:
+        keys[:256] *= mag
+        f = Filled(rng, [n], n, 1, dim, "bf16", keys, values)
+        check_attend(rng, [n - new], [new], 1, 4, dim, "bf16", fill=f, qs=q, capacity=n, weights=True)
+    keys *= mag
+    f = Filled(rng, [n], n, 1, dim, "bf16", keys, np.zeros_like(values))
+    check_attend(rng, [n - new], [new], 1, 4, dim, "bf16", fill=f, qs=q, capacity=n, weights=True,
+                 scale=0.1 / mag if mag > 1e-37 else None)  # (a scale past 2^100 is refused)
+
+
 def test_attend_many_columns_ignore_what_they_cannot_see():
     rng = np.random.default_rng(32)
     held, new, cap = [200, 90], [44, 36], 256
@@ -610,6 +629,54 @@ def test_evict_long_sequences():
     n = 70_001
     w = np.round(rng.random((1, n)) * 5000).astype(np.float32)
     check_evict(rng, [n], n, 12_345, w, heads=1)
+    w = np.round(rng.random((5, 9_000)) * 50).astype(np.float32)
+    check_evict(rng, [9_000, 5, 0, 4_097, 8_999], 9_000, 4_096, w, heads=1, protect=[3 * 8_990 + 11] * 5)
+
+
+def test_rows_past_32_bits():
+    """20 million rows of 8 heads of 128: their words are counted past 2^31."""
+    n, heads, dim, tail = 20_000_000, 8, 128, 40
+    rng = np.random.default_rng(51)
+    c = M.AttentionCache(1, n, heads, dim)  # 23 GB; rows not written are zeros
+    k, v = tokens(rng, tail, heads, dim), tokens(rng, tail, heads, dim)
+    kt, kx = rounded(k, "bf16")
+    vt, vx = rounded(v, "bf16")
+    off, ln = offsets([tail]), i32([n - tail])
+    c.append(kt.data_ptr(), vt.data_ptr(), tail, off.data_ptr(), ln.data_ptr(), stream=stream())
+    ko, vo = torch.empty(tail, heads, dim, device="cuda"), torch.empty(tail, heads, dim, device="cuda")
+    c.read(ko.data_ptr(), vo.data_ptr(), tail, off.data_ptr(), ln.data_ptr(), dtype="f32", stream=stream())
+    torch.cuda.synchronize()
+    kq, vq = O.quantise(kx)[0], O.quantise(vx)[0]
+    assert np.array_equal(ko.cpu().numpy(), kq.astype(np.float32))
+    assert np.array_equal(vo.cpu().numpy(), vq.astype(np.float32))
+    # attention: the tail's rows against 2e7 rows of score 0; of one token, and of enough for blocks of 128 columns
+    for t in (1, 32):
+        q, qx = rounded(np.repeat(4 * k[-1:].repeat(4, axis=1), t, axis=0), "bf16")
+        out, lse = torch.empty_like(q), torch.empty(t, heads * 4, device="cuda")
+        size = c.attend_workspace(t, heads * 4)
+        ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+        c.attend(q.data_ptr(), t, heads * 4, offsets([t]).data_ptr(), i32([n]).data_ptr(), out.data_ptr(), causal=False,
+                 d_lse=lse.data_ptr(), d_workspace=ws.data_ptr(), workspace_bytes=size, stream=stream())
+        torch.cuda.synchronize()
+        for hh in (0, 13, 31):
+            z = kq[:, hh // 4] @ qx[0, hh].astype(np.float64) * dim ** -0.5
+            want = np.log(np.exp(z).sum() + (n - tail))
+            # the zero rows' sum has 2e7 terms of 1, in up to 1024 parts: 2e4 roundings of 2^-24 each and a join
+            assert np.abs(lse[:, hh].cpu().numpy() - want).max() < 3e4 * 2.0 ** -23
+            o = (np.exp(z - want) @ vq[:, hh // 4])
+            bound = np.exp(z - want) @ np.abs(vq[:, hh // 4]) * 0.01 + 1e-3
+            assert (np.abs(out[:, hh].float().cpu().numpy() - o) <= bound + 2.0 ** -8 * np.abs(o)).all()
+    # eviction moves the heaviest from the far end
+    w = torch.zeros(1, n, device="cuda")
+    w[0, n - tail:] = 1.0
+    nl = i32([0])
+    ws = torch.empty(c.evict_workspace(), dtype=torch.uint8, device="cuda")
+    c.evict(i32([n]).data_ptr(), tail, w.data_ptr(), w.data_ptr(), nl.data_ptr(), d_workspace=ws.data_ptr(),
+            workspace_bytes=ws.numel(), stream=stream())
+    c.read(ko.data_ptr(), vo.data_ptr(), tail, off.data_ptr(), i32([0]).data_ptr(), dtype="f32", stream=stream())
+    torch.cuda.synchronize()
+    assert nl.item() == tail and np.array_equal(ko.cpu().numpy(), kq.astype(np.float32))
+    assert np.array_equal(vo.cpu().numpy(), vq.astype(np.float32)) and c.flags(stream()) == 0
 
 
 # ---- streams, graphs, two calls at once -----------------------------------------------------------
