@@ -317,7 +317,7 @@ int maivs_cache_read(maivs_cache* cx, void* d_keys, void* d_values, int dtype, s
  * launch. Offsets that do not ascend within 0..n_tokens set flag 4; those sequences are skipped. Flag 8:
  * a bounded wait of the kernel for many columns ran out, and the call's results are invalid. A value row that
  * is not finite makes the outputs that see it NaN, at least in its groups of 64 dimensions. |scale| is at
- * most 2^100, and a query whose largest element times scale passes that gives NaN. */
+ * most 2^100, and a query whose largest element times scale passes that gives NaN. d_out overlaps no input. */
 int maivs_cache_attend(maivs_cache* cx, const void* d_queries, int dtype, size_t n_tokens, size_t query_stride,
                        size_t n_query_heads, const int32_t* d_offsets, const int32_t* d_lengths, int causal,
                        float scale, size_t max_rows, size_t max_tokens, void* d_out, float* d_lse,
@@ -329,7 +329,7 @@ int maivs_cache_attend_workspace(maivs_cache* cx, size_t n_tokens, size_t n_quer
 /* attend over the rows d_rows[token][0 .. k), as maivs_search_batch_device writes ids: an entry that
  * is not a row the token sees (UINT64_MAX padding among them) is left out, one that occurs twice
  * counts twice. d_weights ([n_tokens][k], may be NULL) receives each entry's softmax weight summed
- * over the query heads (0 for entries left out). */
+ * over the query heads (0 for entries left out). Tokens of no sequence are left as they are. */
 int maivs_cache_attend_found(maivs_cache* cx, const void* d_queries, int dtype, size_t n_tokens, size_t query_stride,
                              size_t n_query_heads, const int32_t* d_offsets, const int32_t* d_lengths,
                              const uint64_t* d_rows, size_t k, int causal, float scale, void* d_out, float* d_lse,

@@ -107,7 +107,7 @@ int on_device(maivs_cache* cx, F launch) {
 std::string attend_args(const maivs_cache* cx, size_t n_tokens, size_t q_heads, size_t max_rows, size_t max_tokens,
                         size_t k, bool weights, AttendArgs* a) {
     if (q_heads == 0 || q_heads % (size_t)cx->v.heads != 0 || q_heads > 65536)
-        return "n_query_heads must be a multiple of the cache's heads";
+        return "n_query_heads must be a multiple of the cache's heads, at most 65536";
     if (n_tokens > kMaxTokens) return "n_tokens must be at most 2^27";
     if (k > (size_t(1) << 27)) return "k must be at most 2^27";
     if (n_tokens * q_heads > (size_t(1) << 30)) return "n_tokens x n_query_heads must be at most 2^30";

@@ -677,10 +677,6 @@ bool aligned16(const void* p, size_t stride_bytes) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride_bytes % 16 == 0;
 }
 
-}  // namespace
-
-namespace {
-
 // Passes in flight per thread and tokens per block: four and four times that many where it still gives
 // every SM its blocks.
 struct StorePlan {

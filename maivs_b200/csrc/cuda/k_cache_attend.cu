@@ -4,11 +4,10 @@
 // out = sum_r p_r v_r, p = softmax(z), in one pass over the rows with a running maximum and sum.
 //
 // A warp streams tiles of 16 rows through a ring of its own in shared memory (cp.async, no barrier of the
-// block in the loop), and a 4-bit code becomes an f16 operand of mma.m16n8k16 by one mask. A nibble in the low four bits of a
-// half is the subnormal c * 2^-24, in the next four c * 2^-20; both are exact, the tensor core takes
-// subnormals as they are, and the powers of two are taken out of the f32 accumulators (or folded
-// into the query operand) afterwards. A group's step and low multiply sums of its codes, not the
-// codes.
+// block in the loop), and a 4-bit code becomes an f16 operand of mma.m16n8k16 by one mask. A nibble in the low
+// four bits of a half is the subnormal c * 2^-24, in the next four c * 2^-20; both are exact, the tensor core
+// takes subnormals as they are, and the powers of two are taken out of the f32 accumulators (or folded into the
+// query operand) afterwards. A group's step and low multiply sums of its codes, not the codes.
 //
 //   keys    S = K Q^T: A = codes (M: 16 rows), B = queries (N: 8 columns, scaled by a power of two to
 //           f16's upper range). Per group g: s += step_g * acc_g + low_g * sum(q in g).
@@ -23,6 +22,15 @@
 // element. p * step is rounded to f16 in bf16 calls (2^-12 relative, below the output's own rounding) and
 // split into two halves (22 bits) in f16 and f32 calls; one half doubled an f16 output's error where few rows
 // carry the weight. f32 calls split the query as well.
+//
+// Bound by instructions, close to HBM: two tiles of 16 rows (G = 2, eight columns) take some 520 of a warp, half
+// of them on the integer pipe (shifts and masks of codes, moves of halves), at 2304 bytes a tile. One token of
+// 8 query heads a head over 262,144 rows of 8 heads of 128, f16: 80 us, 302 MB (a copy's rate would be 46); with
+// one half for p * step, as in bf16, 69, of them 61 in this kernel, 4.9 TB/s. A token each of 64 sequences of 500
+// to 8,000 rows, 4 query heads a head, bf16: 97 us with the rows' weights (297 MB), 77 of them here.
+// Measured and not kept: a multiplication for the codes' shifts (86 us for 83), clusters that join long rows in
+// shared memory (98 for 69), four or two blocks of two groups a SM for three, three and six waves of ragged
+// parts for four.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -649,70 +657,70 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, TYPE == kF32, (MODE >= Mo
             // ---- values: rows 2t, 2t + 1, 2t + 8, 2t + 9 of every 16, words gid of every group ----
 #pragma unroll
             for (int u = 0; u < S::kSub; ++u) {
-            uint32_t vw[4][G];
-            const char* vt = tile + 32 * G * S::kRows;
+                uint32_t vw[4][G];
+                const char* vt = tile + 32 * G * S::kRows;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = 16 * u + 2 * t + (i & 1) + 8 * (i >> 1);
-                if constexpr (G == 1) {
-                    vw[i][0] = *reinterpret_cast<const uint32_t*>(vt + value_piece<G>(r * 2 + (gid >> 2)) * 16 +
-                                                                  (gid & 3) * 4);
-                } else {
+                for (int i = 0; i < 4; ++i) {
+                    const int r = 16 * u + 2 * t + (i & 1) + 8 * (i >> 1);
+                    if constexpr (G == 1) {
+                        vw[i][0] = *reinterpret_cast<const uint32_t*>(vt + value_piece<G>(r * 2 + (gid >> 2)) * 16 +
+                                                                      (gid & 3) * 4);
+                    } else {
 #pragma unroll
-                    for (int x = 0; x < G / 2; ++x)
-                        tile_words<2>(reinterpret_cast<const uint32_t*>(
-                                          vt + value_piece<G>(r * 2 * G + 4 * x + (gid >> 1)) * 16 + (gid & 1) * 8),
-                                      *reinterpret_cast<uint32_t(*)[2]>(&vw[i][2 * x]));
+                        for (int x = 0; x < G / 2; ++x)
+                            tile_words<2>(reinterpret_cast<const uint32_t*>(
+                                              vt + value_piece<G>(r * 2 * G + 4 * x + (gid >> 1)) * 16 + (gid & 1) * 8),
+                                          *reinterpret_cast<uint32_t(*)[2]>(&vw[i][2 * x]));
+                    }
                 }
-            }
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-                // p * step of (row, columns 2t, 2t + 1), then transposed: (column gid, rows 2t, 2t + 1)
-                uint32_t b[kNt][2], c2[kNt][2];
+                for (int g = 0; g < G; ++g) {
+                    // p * step of (row, columns 2t, 2t + 1), then transposed: (column gid, rows 2t, 2t + 1)
+                    uint32_t b[kNt][2], c2[kNt][2];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float st = __fmul_rn(par_step(vpw[2 * u + i][g]), inv[g]), lo = low_of<F32>(vpw[2 * u + i][g]);
+                    for (int i = 0; i < 2; ++i) {
+                        const float st = __fmul_rn(par_step(vpw[2 * u + i][g]), inv[g]), lo = low_of<F32>(vpw[2 * u + i][g]);
 #pragma unroll
-                    for (int j = 0; j < kNt; ++j) {
-                        float ps[2];
+                        for (int j = 0; j < kNt; ++j) {
+                            float ps[2];
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            ps[x] = __fmul_rn(p[2 * j + x][2 * u + i], st);
-                            float& lw = low[2 * j + x][g];
-                            if constexpr (kEdge) {
-                                // a row the column does not see adds nothing, whatever it holds
-                                ps[x] = see[2 * j + x][2 * u + i] ? ps[x] : 0.0f;
-                                lw = see[2 * j + x][2 * u + i] ? __fmaf_rn(p[2 * j + x][2 * u + i], lo, lw) : lw;
-                            } else {
-                                lw = __fmaf_rn(p[2 * j + x][2 * u + i], lo, lw);
+                            for (int x = 0; x < 2; ++x) {
+                                ps[x] = __fmul_rn(p[2 * j + x][2 * u + i], st);
+                                float& lw = low[2 * j + x][g];
+                                if constexpr (kEdge) {
+                                    // a row the column does not see adds nothing, whatever it holds
+                                    ps[x] = see[2 * j + x][2 * u + i] ? ps[x] : 0.0f;
+                                    lw = see[2 * j + x][2 * u + i] ? __fmaf_rn(p[2 * j + x][2 * u + i], lo, lw) : lw;
+                                } else {
+                                    lw = __fmaf_rn(p[2 * j + x][2 * u + i], lo, lw);
+                                }
+                            }
+                            b[j][i] = pack_h2(ps[0], ps[1]);
+                            if constexpr (kTwoHalves)
+                                c2[j][i] = transpose8(pack_h2(left_over(ps[0], b[j][i], 0), left_over(ps[1], b[j][i], 1)));
+                            b[j][i] = transpose8(b[j][i]);
+                        }
+                    }
+                    const uint32_t u0 = __byte_perm(vw[0][g], vw[1][g], 0x5410), h0 = __byte_perm(vw[0][g], vw[1][g], 0x7632);
+                    const uint32_t u8 = __byte_perm(vw[2][g], vw[3][g], 0x5410), h8 = __byte_perm(vw[2][g], vw[3][g], 0x7632);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int sh = 8 * i;
+                        const uint32_t e0 = operand<F32, false>(u0 >> sh), e1 = operand<F32, false>(h0 >> sh),
+                                       e2 = operand<F32, false>(u8 >> sh), e3 = operand<F32, false>(h8 >> sh);
+                        const uint32_t d0 = operand<F32, true>(u0 >> sh), d1 = operand<F32, true>(h0 >> sh),
+                                       d2 = operand<F32, true>(u8 >> sh), d3 = operand<F32, true>(h8 >> sh);
+#pragma unroll
+                        for (int j = 0; j < kNt; ++j) {
+                            mma(o[g][2 * i][j], e0, e1, e2, e3, b[j][0], b[j][1]);
+                            mma(o[g][2 * i + 1][j], d0, d1, d2, d3, b[j][0], b[j][1]);
+                            if constexpr (kTwoHalves) {
+                                mma(o[g][2 * i][j], e0, e1, e2, e3, c2[j][0], c2[j][1]);
+                                mma(o[g][2 * i + 1][j], d0, d1, d2, d3, c2[j][0], c2[j][1]);
                             }
                         }
-                        b[j][i] = pack_h2(ps[0], ps[1]);
-                        if constexpr (kTwoHalves)
-                            c2[j][i] = transpose8(pack_h2(left_over(ps[0], b[j][i], 0), left_over(ps[1], b[j][i], 1)));
-                        b[j][i] = transpose8(b[j][i]);
                     }
                 }
-                const uint32_t u0 = __byte_perm(vw[0][g], vw[1][g], 0x5410), h0 = __byte_perm(vw[0][g], vw[1][g], 0x7632);
-                const uint32_t u8 = __byte_perm(vw[2][g], vw[3][g], 0x5410), h8 = __byte_perm(vw[2][g], vw[3][g], 0x7632);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int sh = 8 * i;
-                    const uint32_t e0 = operand<F32, false>(u0 >> sh), e1 = operand<F32, false>(h0 >> sh),
-                                   e2 = operand<F32, false>(u8 >> sh), e3 = operand<F32, false>(h8 >> sh);
-                    const uint32_t d0 = operand<F32, true>(u0 >> sh), d1 = operand<F32, true>(h0 >> sh),
-                                   d2 = operand<F32, true>(u8 >> sh), d3 = operand<F32, true>(h8 >> sh);
-#pragma unroll
-                    for (int j = 0; j < kNt; ++j) {
-                        mma(o[g][2 * i][j], e0, e1, e2, e3, b[j][0], b[j][1]);
-                        mma(o[g][2 * i + 1][j], d0, d1, d2, d3, b[j][0], b[j][1]);
-                        if constexpr (kTwoHalves) {
-                            mma(o[g][2 * i][j], e0, e1, e2, e3, c2[j][0], c2[j][1]);
-                            mma(o[g][2 * i + 1][j], d0, d1, d2, d3, c2[j][0], c2[j][1]);
-                        }
-                    }
-                }
-            }
             }
         };
 

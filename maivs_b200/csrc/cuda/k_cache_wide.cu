@@ -16,6 +16,11 @@
 // tile i + 1 and the keys of tile i + 2. Thread 0 issues the products: S of tile i + 1 as soon as S of tile i is
 // in registers, P V of tile i at the end of the step, so both run beside the exponentials.
 //
+// Bound by the decoding warps: some 5,000 clocks a tile of G = 2, the columns' warps 3,300, the products' arithmetic 550.
+// Chunks of 32 to 64 tokens over 4 sequences of 20,000 to 32,000 rows, 8 heads of 128 with 4 query heads each: 394
+// us, 78 GFLOP, an eighth of the tensor cores' rate. Loads of codes in whole lines that were then exchanged in
+// shared memory took 447.
+//
 // Rounding: scores are as exact as the other kernel's (the log-sum-exp and the rows' weights come from
 // them); both are scaled by powers of two, the keys by one per tile. V = low + step c is rounded to f16, in
 // units where the largest level so far is 2^14; P is rounded to f16, in units where the running maximum's is
@@ -32,9 +37,9 @@ namespace dev {
 
 namespace {
 
-constexpr int kWideBS = 16 * 32;
+constexpr int kWideBS = 25 * 32;
 constexpr int kRowsTile = 128;
-constexpr uint32_t kColS = 0, kColO = 128, kColP = 256;  // tensor memory columns: S, O, P
+constexpr uint32_t kColS = 0, kColO = 256, kColP = 384;  // tensor memory columns: two of S, O, two of P
 constexpr uint32_t kTmemCols = 512;
 constexpr int kKeyUp = 6, kValueUp = 14, kSumDown = 8;   // powers of two of the largest key and value, of the query's sums
 constexpr int kNoExp = -200;
@@ -82,7 +87,50 @@ __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&v)[32]) 
                  "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(at)
                  : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(v[0]),
+        "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(at)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// A wait of a second at most; false when they ran out.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity) {
+    if (umma::bar_try(bar, parity)) return true;
+    uint64_t first, now;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(first));
+    do {
+        for (int i = 0; i < 64; ++i)
+            if (umma::bar_try(bar, parity)) return true;
+        asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+    } while (now - first < 1000000000ull);
+    return false;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+    return from_f32<__nv_bfloat16>(lo) | (from_f32<__nv_bfloat16>(hi) << 16);
+}
+
+// The kernel takes bf16 queries: n <= 8 elements from element i on, two to a word; the others are 0.
+__device__ __forceinline__ void load_query8_raw(const void* q, size_t i, int n, uint32_t (&w)[4]) {
+    const unsigned short* p = static_cast<const unsigned short*>(q) + i;
+    if (n == 8 && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+        const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+        w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            w[e] = (2 * e < n ? __ldg(p + 2 * e) : 0u) | (2 * e + 1 < n ? (uint32_t)__ldg(p + 2 * e + 1) << 16 : 0u);
+    }
+}
 
 template <int G>
 struct Wide {
@@ -91,6 +139,12 @@ struct Wide {
     static constexpr int kKBytes = kQBytes, kVBytes = 2 * G * kCacheGroup * 128;
     static constexpr int kSmem = kQBytes + 2 * kKBytes + 2 * kVBytes + 1024;
 };
+
+// The value word of eight rows that decoding thread p takes: eight threads' pieces meet no bank twice.
+template <int G>
+__device__ __forceinline__ int word_of(int p) {
+    return G == 1 ? p & 7 : (p & 7) * 2 + ((p >> 3) & 1);
+}
 
 // What the decoding warps leave for the columns' warps, for tile i at i % 4.
 template <int G>
@@ -117,28 +171,66 @@ struct ValueCodes {
     uint32_t p[G];
 };
 
+// Brings tile after tile of a decoding thread's codes and parameters: its addresses only advance. Whole tiles are
+// loaded without a bound: with one on every load, the loads of a tile took 2,000 clocks longer.
 template <int G>
-__device__ __forceinline__ void load_keys(KeyCodes<G>& x, const uint32_t* kc, const uint32_t* kp, int row0, int rows_end,
-                                          int p) {
-    const int r = row0 + (p & 127);
-    const bool in = r < rows_end;
+struct KeySource {
+    const uint4* codes;
+    const uint32_t* params;
+    int left;  // rows from the thread's row to the end
+    int whole; // rows from the tile's start to the end
+
+    __device__ __forceinline__ KeySource(const uint32_t* kc, const uint32_t* kp, int row0, int rows_end, int p) {
+        const int r = row0 + (p & 127);
+        codes = reinterpret_cast<const uint4*>(kc + (size_t)r * 8 * G) + (p >> 7) * G;
+        params = kp + (size_t)r * G;
+        left = rows_end - r, whole = rows_end - row0;
+    }
+    __device__ __forceinline__ void next(KeyCodes<G>& x) {
+        if (whole >= kRowsTile) {
 #pragma unroll
-    for (int i = 0; i < G; ++i)
-        x.c[i] = in ? __ldg(reinterpret_cast<const uint4*>(kc + (size_t)r * 8 * G) + (p >> 7) * G + i) : make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < G; ++i) x.c[i] = __ldg(codes + i);
 #pragma unroll
-    for (int g = 0; g < G; ++g) x.p[g] = in ? __ldg(kp + (size_t)r * G + g) : 0u;
-}
+            for (int g = 0; g < G; ++g) x.p[g] = __ldg(params + g);
+        } else {
+#pragma unroll
+            for (int i = 0; i < G; ++i) x.c[i] = left > 0 ? __ldg(codes + i) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int g = 0; g < G; ++g) x.p[g] = left > 0 ? __ldg(params + g) : 0u;
+        }
+        codes += kRowsTile * 2 * G, params += kRowsTile * G;
+        left -= kRowsTile, whole -= kRowsTile;
+    }
+};
 template <int G>
-__device__ __forceinline__ void load_values(ValueCodes<G>& x, const uint32_t* vc, const uint32_t* vp, int row0,
-                                            int rows_end, int p) {
-    const int r = row0 + (p & 127);
+struct ValueSource {
+    const uint32_t *codes, *params;
+    int left, whole;  // as above; the codes are those of eight rows
+    int left_codes;
+
+    __device__ __forceinline__ ValueSource(const uint32_t* vc, const uint32_t* vp, int row0, int rows_end, int p) {
+        const int r = row0 + (p & 127), rb = row0 + p / (8 * G) * 8;  // 8 G words times 16 blocks of rows
+        codes = vc + (size_t)rb * 8 * G + word_of<G>(p);
+        params = vp + (size_t)r * G;
+        left = rows_end - r, left_codes = rows_end - rb, whole = rows_end - row0;
+        if (p >= 128 * G) codes = vc, left_codes = whole = 0;  // (G = 1: half the threads bring parameters only)
+    }
+    __device__ __forceinline__ void next(ValueCodes<G>& x) {
+        if (whole >= kRowsTile) {
 #pragma unroll
-    for (int g = 0; g < G; ++g) x.p[g] = r < rows_end ? __ldg(vp + (size_t)r * G + g) : 0u;
-    const int word = p % (8 * G), rb = row0 + p / (8 * G) * 8;  // 8 G words times 16 blocks of rows
+            for (int g = 0; g < G; ++g) x.p[g] = __ldg(params + g);
 #pragma unroll
-    for (int y = 0; y < 8; ++y)
-        x.c[y] = p < 128 * G && rb + y < rows_end ? __ldg(vc + (size_t)(rb + y) * 8 * G + word) : 0u;
-}
+            for (int y = 0; y < 8; ++y) x.c[y] = __ldg(codes + y * 8 * G);
+        } else {
+#pragma unroll
+            for (int g = 0; g < G; ++g) x.p[g] = left > 0 ? __ldg(params + g) : 0u;
+#pragma unroll
+            for (int y = 0; y < 8; ++y) x.c[y] = y < left_codes ? __ldg(codes + y * 8 * G) : 0u;
+        }
+        codes += kRowsTile * 8 * G, params += kRowsTile * G;
+        left -= kRowsTile, left_codes -= kRowsTile, whole -= kRowsTile;
+    }
+};
 
 // Exponent e with |low| + 15 step < 2^e for every group, kNoExp for a row of zeros or one that is not finite.
 template <int G>
@@ -204,7 +296,7 @@ template <int G>
 __device__ __forceinline__ void decode_values(const ValueCodes<G>& x, char* sv, const RowParams<G>* rp, int p) {
     const __half2 magic = __float2half2_rn(1024.0f), sixteenth = __float2half2_rn(0.0625f);
     if (p < 128 * G) {
-        const int word = p % (8 * G), b = p / (8 * G);
+        const int word = word_of<G>(p), b = p / (8 * G);
         const int g = G == 1 ? 0 : word & 1, d0 = G == 1 ? word : word >> 1;
         uint32_t out[2][4][4];
 #pragma unroll
@@ -233,32 +325,32 @@ __device__ __forceinline__ void decode_values(const ValueCodes<G>& x, char* sv, 
     }
 }
 
-// The tops of the keys of tile ik and the values of tile iv (-1: none), over all decoding threads; the values'
-// parameters as halves, in units of the running exponent E.
+// The top of the keys of tile i, over the threads that decode keys.
 template <int G>
-__device__ __forceinline__ void find_tops(const KeyCodes<G>& k, const ValueCodes<G>& v, RowParams<G>* rp, int ik, int iv,
-                                          int p, int& E) {
-    bool kbad, vbad;
-    const int kt = __reduce_max_sync(~0u, level_of<G>(k.p, kbad)), vt = __reduce_max_sync(~0u, level_of<G>(v.p, vbad));
-    vbad = vbad && iv >= 0;
-    if ((p & 31) == 0) {
-        if (ik >= 0) atomicMax(&rp->key_top[ik & 3], kt);
-        if (iv >= 0) atomicMax(&rp->value_top[iv & 3], vt);
-    }
-    if (iv >= 0 && p < kRowsTile) {
-        rp->poison[iv & 3][p] = vbad ? __uint_as_float(0x7FC00000u) : 0.0f;
-        if (vbad) rp->bad[iv & 3] = 1;
+__device__ __forceinline__ void find_key_top(const KeyCodes<G>& k, RowParams<G>* rp, int i, int p) {
+    bool bad;
+    const int top = __reduce_max_sync(~0u, level_of<G>(k.p, bad));
+    if ((p & 31) == 0) atomicMax(&rp->key_top[i & 3], top);
+    asm volatile("bar.sync 2, 256;" ::: "memory");
+}
+// The same of the values; their parameters as halves, in units of the running exponent E.
+template <int G>
+__device__ __forceinline__ void find_value_top(const ValueCodes<G>& v, RowParams<G>* rp, int i, int p, int& E) {
+    bool bad;
+    const int top = __reduce_max_sync(~0u, level_of<G>(v.p, bad));
+    if ((p & 31) == 0) atomicMax(&rp->value_top[i & 3], top);
+    if (p < kRowsTile) {
+        rp->poison[i & 3][p] = bad ? __uint_as_float(0x7FC00000u) : 0.0f;
+        if (bad) rp->bad[i & 3] = 1;
     }
     asm volatile("bar.sync 1, 256;" ::: "memory");
-    if (iv >= 0) {
-        E = max(E, rp->value_top[iv & 3]);
-        const float up = pow2(kValueUp - max(E, -110));
-        if (p < kRowsTile)
+    E = max(E, rp->value_top[i & 3]);
+    const float up = pow2(kValueUp - max(E, -110));
+    if (p < kRowsTile)
 #pragma unroll
-            for (int g = 0; g < G; ++g)
-                rp->v[p][g] = vbad ? 0u : pack_h2(__fmul_rn(par_step(v.p[g]), up), __fmul_rn(par_low(v.p[g]), up));
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-    }
+        for (int g = 0; g < G; ++g)
+            rp->v[p][g] = bad ? 0u : pack_h2(__fmul_rn(par_step(v.p[g]), up), __fmul_rn(par_low(v.p[g]), up));
+    asm volatile("bar.sync 1, 256;" ::: "memory");
 }
 
 template <int G>
@@ -268,18 +360,17 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
     cudaTriggerProgrammaticLaunchCompletion();  // the join's blocks wait for this grid's end
     extern __shared__ char s_raw[];
     __shared__ RowParams<G> rp;
-    __shared__ float s_top[2][kWideCols];  // the halves' maxima, later their sums
-    __shared__ uint64_t bar_s, bar_o;
+    __shared__ float s_top[2][kWideCols], s_sum[2][G][kWideCols];  // maxima and sums of a column's two threads
+    __shared__ uint64_t bar_s[2], bar_o;
     __shared__ uint32_t s_tmem;
     __shared__ int s_fail;
     char* sq = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~uintptr_t(1023));
     char* sk = sq + W::kQBytes;
     char* sv = sk + 2 * W::kKBytes;
     const int warp = threadIdx.x >> 5;
-    const bool owns = warp < 8, decodes = !owns;
-    const bool issues = threadIdx.x == 0;
+    const bool owns = warp < 8, decodes_keys = warp >= 16 && warp < 24, issues = warp == 24;
     const int half = warp >> 2;       // rows 64 half .. of a tile
-    const int p = owns ? threadIdx.x & 127 : threadIdx.x - 256;  // column, or decoding thread
+    const int p = owns ? threadIdx.x & 127 : threadIdx.x & 255;  // column, or decoding thread
 
     unsigned b = blockIdx.x;
     const int ct0 = b % kk.col_tiles;
@@ -307,7 +398,8 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
 
     if (warp == 0) umma::tmem_alloc(&s_tmem, kTmemCols);
     if (threadIdx.x == 0) {
-        umma::bar_init(&bar_s, 1);
+        umma::bar_init(&bar_s[0], 1);
+        umma::bar_init(&bar_s[1], 1);
         umma::bar_init(&bar_o, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         s_fail = 0;
@@ -332,236 +424,273 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
         const bool in = col < cols;
         const size_t th = (size_t)(sn.first + tok_i) * a.q_heads + h * a.group + (col - tok_i * a.group);
 
+        // tiles count on over the column tiles for the two places and barriers of the scores
         auto issue_scores = [&](int i) {
+            const int place = (done + i) & 1;
             const uint64_t kd = k_desc + (i & 1) * (W::kKBytes >> 4);
 #pragma unroll
             for (int x = 0; x < 4 * G + 1; ++x) {  // the last sixteen positions hold the low parts
                 const uint32_t at = ((x >> 2) * W::kGroupBytes + 32 * (x & 3)) >> 4;
-                mma_ss(tmem + kColS, q_desc + at, kd + at, kIdS, x > 0);
+                mma_ss(tmem + kColS + kRowsTile * place, q_desc + at, kd + at, kIdS, x > 0);
             }
-            umma::mma_commit(&bar_s);
+            umma::mma_commit(&bar_s[place]);
+        };
+        auto end_step = [] {
+            umma::fence_before_sync();
+            asm volatile("bar.sync 0;" ::: "memory");
         };
         auto issue_values = [&](int i) {
             const uint64_t vd = v_desc + (i & 1) * (W::kVBytes >> 4);
 #pragma unroll
             for (int x = 0; x < 8; ++x)
-                mma_ts(tmem + kColO, tmem + kColP + 8 * x, vd + (((x >> 2) * G * kCacheGroup * 128 + 32 * (x & 3)) >> 4), kIdO,
+                mma_ts(tmem + kColO, tmem + kColP + 64 * (i & 1) + 8 * x, vd + (((x >> 2) * G * kCacheGroup * 128 + 32 * (x & 3)) >> 4), kIdO,
                        i > 0 || x > 0);
             umma::mma_commit(&bar_o);
         };
 
-        KeyCodes<G> keys;
-        ValueCodes<G> values;
         int E = kNoExp;
         float fac = 0.0f, m = kNoMax;
         f2 l2 = 0;
-        // ---- the first tiles; the queries ----
-        if (decodes) {
-            if (p < 4) rp.key_top[p] = rp.value_top[p] = kNoExp, rp.bad[p] = 0;
+        // Each kind of warp has a loop of its own over the tiles, with the block's barrier at the end of a step.
+        if (issues) {
+            end_step();
+            if (n > 0 && (threadIdx.x & 31) == 0) {
+                umma::fence_after_sync();
+                issue_scores(0);
+                if (n > 1) issue_scores(1);
+            }
+            __syncwarp();
+            for (int i = 0; i < n; ++i) {
+                end_step();
+                if ((threadIdx.x & 31) == 0) {
+                    umma::fence_after_sync();
+                    issue_values(i);
+                    if (i + 2 < n) issue_scores(i + 2);
+                }
+                __syncwarp();
+                if (s_fail) break;
+            }
+        } else if (decodes_keys) {
+            KeyCodes<G> keys;
+            KeySource<G> source(kc, kp, start, end, p);
+            if (p < 4) rp.key_top[p] = kNoExp;
             // the second piece of the low parts' positions stays zero
             if (p < 128) {
-                *reinterpret_cast<uint4*>(sk + G * W::kGroupBytes + umma::sw128_offset(p, 1)) = make_uint4(0, 0, 0, 0);
-                *reinterpret_cast<uint4*>(sk + W::kKBytes + G * W::kGroupBytes + umma::sw128_offset(p, 1)) = make_uint4(0, 0, 0, 0);
+                char* const at = sk + G * W::kGroupBytes + umma::sw128_offset(p, 1);
+                *reinterpret_cast<uint4*>(at) = *reinterpret_cast<uint4*>(at + W::kKBytes) = make_uint4(0, 0, 0, 0);
             }
+            asm volatile("bar.sync 2, 256;" ::: "memory");
+            for (int i = 0; i < min(n, 2); ++i) {
+                source.next(keys);
+                find_key_top<G>(keys, &rp, i, p);
+                decode_keys<G>(keys, sk + i * W::kKBytes, rp.key_top[i], p);
+            }
+            if (n > 2) source.next(keys);
+            umma::fence_smem_to_async();
+            end_step();
+            for (int i = 0; i < n; ++i) {
+                if (i + 2 < n) {
+                    if (p == 0) rp.key_top[(i + 3) & 3] = kNoExp;  // last read in the step before
+                    find_key_top<G>(keys, &rp, i + 2, p);
+                    // S of this tile has read the buffer that these keys go to
+                    if (!wait_for(&bar_s[(done + i) & 1], ((done + i) >> 1) & 1)) s_fail = 1;
+                    decode_keys<G>(keys, sk + (i & 1) * W::kKBytes, rp.key_top[(i + 2) & 3], p);
+                    if (i + 3 < n) source.next(keys);
+                }
+                umma::fence_smem_to_async();
+                end_step();
+                if (s_fail) break;
+            }
+        } else if (!owns) {
+            ValueCodes<G> values;
+            ValueSource<G> source(vc, vp, start, end, p);
+            if (p < 4) rp.value_top[p] = kNoExp, rp.bad[p] = 0;
             asm volatile("bar.sync 1, 256;" ::: "memory");
             if (n > 0) {
-                load_keys<G>(keys, kc, kp, start, end, p);
-                load_values<G>(values, vc, vp, start, end, p);
-                find_tops<G>(keys, values, &rp, 0, 0, p, E);
-                decode_keys<G>(keys, sk, rp.key_top[0], p);
-                if (n > 1) load_keys<G>(keys, kc, kp, start + kRowsTile, end, p);
+                source.next(values);
+                find_value_top<G>(values, &rp, 0, p, E);
                 decode_values<G>(values, sv, &rp, p);
-                if (n > 1) {
-                    load_values<G>(values, vc, vp, start + kRowsTile, end, p);
-                    find_tops<G>(keys, values, &rp, 1, -1, p, E);
-                    decode_keys<G>(keys, sk + W::kKBytes, rp.key_top[1], p);
+                if (n > 1) source.next(values);
+            }
+            umma::fence_smem_to_async();
+            end_step();
+            for (int i = 0; i < n; ++i) {
+                if (i + 1 < n) {
+                    if (p == 0) rp.value_top[(i + 2) & 3] = kNoExp, rp.bad[(i + 2) & 3] = 0;
+                    find_value_top<G>(values, &rp, i + 1, p, E);
+                    // P V of the tile before has read the buffer that these values go to
+                    if (i > 0 && !wait_for(&bar_o, (done + i - 1) & 1)) s_fail = 1;
+                    decode_values<G>(values, sv + ((i + 1) & 1) * W::kVBytes, &rp, p);
+                    if (i + 2 < n) source.next(values);
                 }
-                if (n > 2) load_keys<G>(keys, kc, kp, start + 2 * kRowsTile, end, p);
+                umma::fence_smem_to_async();
+                end_step();
+                if (s_fail) break;
             }
         } else {
-            // both threads of a column find its scale; each prepares half of the dimensions' words
-            const size_t qi = (size_t)(sn.first + tok_i) * a.q_stride + (size_t)(h * a.group + (col - tok_i * a.group)) * c.dim;
+            // each of a column's threads takes every second word of eight dimensions; maxima and sums are exchanged
+            const size_t qi = (size_t)(sn.first + tok_i) * a.q_stride +
+                              (size_t)(h * a.group + (col - tok_i * a.group)) * c.dim;
+            uint32_t raw[4 * G][4];
             float top = 0.0f;
-            bool bad = false;
-#pragma unroll 2
-            for (int w = 0; w < 8 * G; ++w) {
-                float x[8];
-                load_query8(a.q, a.type, qi + 8 * w, in ? min(max(c.dim - 8 * w, 0), 8) : 0, x);
 #pragma unroll
-                for (int y = 0; y < 8; ++y) top = fmaxf(top, fabsf(x[y])), bad |= !(fabsf(x[y]) < INFINITY);
+            for (int w = 0; w < 4 * G; ++w) {
+                const int d = 16 * w + 8 * half;
+                load_query8_raw(a.q, qi + d, in ? min(max(c.dim - d, 0), 8) : 0, raw[w]);
             }
+#pragma unroll
+            for (int w = 0; w < 4 * G; ++w)
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const float lo = fabsf(__uint_as_float(raw[w][y] << 16)), hi = fabsf(__uint_as_float(raw[w][y] & 0xFFFF0000u));
+                    // an element that is not finite makes the maximum infinite
+                    top = fmaxf(top, lo < INFINITY ? lo : INFINITY);
+                    top = fmaxf(top, hi < INFINITY ? hi : INFINITY);
+                }
+            s_top[half][p] = top;
+            asm volatile("bar.sync 3, 256;" ::: "memory");
+            top = fmaxf(s_top[0][p], s_top[1][p]);
+            const bool bad = top == INFINITY;
             const int e = top > 0.0f ? min(141 - (int)(__float_as_uint(top) >> 23), 126) : 0;
             // the scale's sign goes into the queries, so that fac is not negative
             const float up = __uint_as_float((uint32_t)max(e + 127, 1) << 23), sgn = a.scale < 0.0f ? -up : up;
             fac = bad ? __uint_as_float(0x7FC00000u) : __fmul_rn(__fmul_rn(__fdiv_rn(1.0f, up), fabsf(a.scale)), kLog2e);
-            uint32_t ext[4] = {0, 0, 0, 0};
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 float sum = 0.0f;
-#pragma unroll 2
-                for (int w = 0; w < 8; ++w) {
+#pragma unroll
+                for (int w = 4 * g; w < 4 * g + 4; ++w) {
                     float x[8];
-                    const int d = kCacheGroup * g + 8 * w;
-                    load_query8(a.q, a.type, qi + d, in && !bad ? min(max(c.dim - d, 0), 8) : 0, x);
 #pragma unroll
                     for (int y = 0; y < 8; ++y) {
-                        x[y] = __fmul_rn(x[y], sgn);
+                        const uint32_t b = raw[w][y / 2];
+                        x[y] = bad ? 0.0f : __fmul_rn(__uint_as_float(y & 1 ? b & 0xFFFF0000u : b << 16), sgn);
                         sum = __fadd_rn(sum, x[y]);
                     }
                     // the order of the codes' nibble pairs
-                    if ((w & 1) == half)
-                        *reinterpret_cast<uint4*>(sq + g * W::kGroupBytes + umma::sw128_offset(p, w)) =
-                            make_uint4(pack_h2(x[0], x[4]), pack_h2(x[1], x[5]), pack_h2(x[2], x[6]), pack_h2(x[3], x[7]));
+                    *reinterpret_cast<uint4*>(sq + g * W::kGroupBytes + umma::sw128_offset(p, 2 * (w & 3) + half)) =
+                        make_uint4(pack_h2(x[0], x[4]), pack_h2(x[1], x[5]), pack_h2(x[2], x[6]), pack_h2(x[3], x[7]));
                 }
+                s_sum[half][g][p] = sum;
+            }
+            asm volatile("bar.sync 3, 256;" ::: "memory");
+            uint32_t ext[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
                 // at most 64 x 2^15, in units of 2^kSumDown; as two halves, once for low and once for 8 step
-                sum = __fmul_rn(sum, 1.0f / (1 << kSumDown));
+                const float sum = __fmul_rn(__fadd_rn(s_sum[0][g][p], s_sum[1][g][p]), 1.0f / (1 << kSumDown));
                 const __half hi = __float2half_rn(sum);
                 ext[2 * g] = ext[2 * g + 1] = pack_h2(__half2float(hi), __fsub_rn(sum, __half2float(hi)));
             }
             *reinterpret_cast<uint4*>(sq + G * W::kGroupBytes + umma::sw128_offset(p, half)) =
                 half ? make_uint4(0, 0, 0, 0) : make_uint4(ext[0], ext[1], ext[2], ext[3]);
-        }
-        const int lim = in ? visible(c, a, sn.len, tok_i) : 0;
-        umma::fence_smem_to_async();
-        umma::fence_before_sync();
-        __syncthreads();
-        if (issues && n > 0) {
-            umma::fence_after_sync();
-            issue_scores(0);
-        }
+            const int lim = in ? visible(c, a, sn.len, tok_i) : 0;
+            umma::fence_smem_to_async();
+            end_step();
 
-        // One tile of this thread's column and half. kEdge: the column does not see some row.
-        auto column_step = [&](int i, auto edge) {
-            constexpr bool kEdge = decltype(edge)::value;
-            const int row0 = start + i * kRowsTile + 64 * half, vis = min(lim, end) - row0;  // rows below vis count
-            bool ok = umma::bar_wait(&bar_s, (done + i) & 1);
-            umma::fence_after_sync();
-            f2 sc[32];
-            float top = -INFINITY;
+            // One tile of this thread's column and half. kEdge: the column does not see some row.
+            auto column_step = [&](int i, auto edge) {
+                constexpr bool kEdge = decltype(edge)::value;
+                const int row0 = start + i * kRowsTile + 64 * half, vis = min(lim, end) - row0;  // rows below vis count
+                const uint32_t s_at = mine + kColS + kRowsTile * ((done + i) & 1) + 64 * half;
+                bool ok = wait_for(&bar_s[(done + i) & 1], ((done + i) >> 1) & 1);
+                umma::fence_after_sync();
+                float top = -INFINITY;
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                uint32_t v[32];
-                tmem_ld32(mine + kColS + 64 * half + 32 * y, v);
-                umma::tmem_wait_ld();
+                for (int y = 0; y < 2; ++y) {
+                    uint32_t v[32];
+                    tmem_ld32(s_at + 32 * y, v);
+                    umma::tmem_wait_ld();
 #pragma unroll
-                for (int x = 0; x < 16; ++x) {
-                    const int r = 16 * y + x;
-                    float s0 = __uint_as_float(v[2 * x]), s1 = __uint_as_float(v[2 * x + 1]);
-                    if constexpr (kEdge) {
-                        if (2 * r >= vis) s0 = -INFINITY;
-                        if (2 * r + 1 >= vis) s1 = -INFINITY;
+                    for (int x = 0; x < 32; x += 2) {
+                        float s0 = __uint_as_float(v[x]), s1 = __uint_as_float(v[x + 1]);
+                        if constexpr (kEdge) {
+                            s0 = 32 * y + x < vis ? s0 : -INFINITY;
+                            s1 = 32 * y + x + 1 < vis ? s1 : -INFINITY;
+                        }
+                        top = max3(top, s0, s1);
                     }
-                    sc[r] = pair(s0, s1);
-                    top = fmaxf(top, fmaxf(s0, s1));
                 }
-            }
-            s_top[half][p] = top;
-            umma::fence_before_sync();
-            asm volatile("bar.sync 3, 256;" ::: "memory");
-            // the scores are in registers: their place, and the buffer of their keys, are free
-            if (issues && i + 1 < n) {
-                umma::fence_after_sync();
-                issue_scores(i + 1);
-            }
-            __syncwarp();
-            if (i + 2 < n) asm volatile("bar.arrive 2, 512;" ::: "memory");
-            // to log2 units: fac is not negative, so the largest stays the largest (-inf where nothing is seen)
-            const float f = __fmul_rn(fac, pow2(max(rp.key_top[i & 3], -120) - kKeyUp));
-            top = fmaxf(s_top[0][p], s_top[1][p]);
-            top = top == -INFINITY ? top : __fmul_rn(top, f);
-            if (kk.logits && in) {
-                float4* lg = reinterpret_cast<float4*>(kk.logits + th * kk.logit_rows + row0);
-#pragma unroll
-                for (int x = 0; x < 16; ++x) {
-                    float4 o;
-                    unpair(mul2(sc[2 * x], pair(f, f)), o.x, o.y);
-                    unpair(mul2(sc[2 * x + 1], pair(f, f)), o.z, o.w);
-                    lg[x] = o;
-                }
-            }
-            // P V of the tile before: its P may be overwritten now, and O be scaled
-            if (i > 0) {
-                ok = umma::bar_wait(&bar_o, (done + i - 1) & 1) && ok;
-                umma::fence_after_sync();
-            }
-            if (!ok) s_fail = 1;
-            const int e_new = max(E, rp.value_top[i & 3]);
-            const bool grow = top > m + kLag;
-            if (__any_sync(~0u, grow) || e_new > E) {
-                const float mn = grow ? fmaxf(m, top) : m;
-                const float fm = ex2(m - mn);
-                m = mn;
-                l2 = mul2(l2, pair(fm, fm));
-                const float fo = __fmul_rn(fm, pow2(max(E, -110) - max(e_new, -110)));
-                if (i > 0) {
+                s_top[half][p] = top;
+                asm volatile("bar.sync 3, 256;" ::: "memory");
+                // to log2 units: fac is not negative, so the largest stays the largest (-inf where nothing is seen)
+                const float f = __fmul_rn(fac, pow2(max(rp.key_top[i & 3], -120) - kKeyUp));
+                top = fmaxf(s_top[0][p], s_top[1][p]);
+                top = top == -INFINITY ? top : __fmul_rn(top, f);
+                const int e_new = max(E, rp.value_top[i & 3]);
+                const bool grow = top > m + kLag;
+                if (__any_sync(~0u, grow) || e_new > E) {
+                    const float mn = grow ? fmaxf(m, top) : m;
+                    const float fm = ex2(m - mn);
+                    m = mn;
+                    l2 = mul2(l2, pair(fm, fm));
+                    const float fo = __fmul_rn(fm, pow2(max(E, -110) - max(e_new, -110)));
+                    // P V of the tile before comes first
+                    if (i > 0) {
+                        ok = wait_for(&bar_o, (done + i - 1) & 1) && ok;
+                        umma::fence_after_sync();
 #pragma unroll 1
-                    for (int y = 0; y < G; ++y) {
-                        uint32_t v[32];
-                        const uint32_t at = mine + kColO + 32 * (half * G + y);
-                        tmem_ld32(at, v);
-                        umma::tmem_wait_ld();
+                        for (int y = 0; y < G; ++y) {
+                            uint32_t v[32];
+                            const uint32_t at = mine + kColO + 32 * (half * G + y);
+                            tmem_ld32(at, v);
+                            umma::tmem_wait_ld();
 #pragma unroll
-                        for (int x = 0; x < 32; ++x) v[x] = __float_as_uint(__fmul_rn(__uint_as_float(v[x]), fo));
-                        tmem_st32(at, v);
+                            for (int x = 0; x < 32; ++x) v[x] = __float_as_uint(__fmul_rn(__uint_as_float(v[x]), fo));
+                            tmem_st32(at, v);
+                        }
                     }
+                    E = e_new;
                 }
-                E = e_new;
-            }
-            const f2 f2x = pair(f, f), neg = pair(kPUp - m, kPUp - m);
-            uint32_t v[32];
+                const f2 f2x = pair(f, f), neg = pair(kPUp - m, kPUp - m);
 #pragma unroll
-            for (int r = 0; r < 32; ++r) {
-                float p0, p1;
-                unpair(fma2(sc[r], f2x, neg), p0, p1);
-                p0 = ex2(p0), p1 = ex2(p1);
-                if constexpr (kEdge) {
-                    // a row the column does not see adds nothing, whatever it holds; one that is not finite poisons
-                    const bool in0 = 2 * r < vis, in1 = 2 * r + 1 < vis;
-                    const float* bad = rp.poison[i & 3] + 64 * half + 2 * r;
-                    p0 = in0 ? p0 : 0.0f, p1 = in1 ? p1 : 0.0f;
-                    l2 = add2(l2, pair(p0, p1));
-                    p0 = in0 ? __fadd_rn(p0, bad[0]) : 0.0f, p1 = in1 ? __fadd_rn(p1, bad[1]) : 0.0f;
-                } else {
-                    l2 = add2(l2, pair(p0, p1));
+                for (int y = 0; y < 2; ++y) {
+                    uint32_t v[32], out[16];
+                    tmem_ld32(s_at + 32 * y, v);
+                    umma::tmem_wait_ld();
+                    if (kk.logits && in) {
+                        float4* lg = reinterpret_cast<float4*>(kk.logits + th * kk.logit_rows + row0 + 32 * y);
+#pragma unroll
+                        for (int x = 0; x < 8; ++x)
+                            lg[x] = make_float4(__fmul_rn(__uint_as_float(v[4 * x]), f), __fmul_rn(__uint_as_float(v[4 * x + 1]), f),
+                                                __fmul_rn(__uint_as_float(v[4 * x + 2]), f),
+                                                __fmul_rn(__uint_as_float(v[4 * x + 3]), f));
+                    }
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) {
+                        const int r = 32 * y + 2 * x;
+                        float p0, p1;
+                        unpair(fma2(pair(__uint_as_float(v[2 * x]), __uint_as_float(v[2 * x + 1])), f2x, neg), p0, p1);
+                        p0 = ex2(p0), p1 = ex2(p1);
+                        if constexpr (kEdge) {
+                            // a row the column does not see adds nothing, whatever it holds; one that is not finite poisons
+                            const bool in0 = r < vis, in1 = r + 1 < vis;
+                            const float* bad = rp.poison[i & 3] + 64 * half + r;
+                            p0 = in0 ? p0 : 0.0f, p1 = in1 ? p1 : 0.0f;
+                            l2 = add2(l2, pair(p0, p1));
+                            p0 = in0 ? __fadd_rn(p0, bad[0]) : 0.0f, p1 = in1 ? __fadd_rn(p1, bad[1]) : 0.0f;
+                        } else {
+                            l2 = add2(l2, pair(p0, p1));
+                        }
+                        out[x] = pack_h2(p0, p1);
+                    }
+                    tmem_st16(mine + kColP + 64 * (i & 1) + 32 * half + 16 * y, out);
                 }
-                v[r] = pack_h2(p0, p1);
-            }
-            tmem_st32(mine + kColP + 32 * half, v);
-            tmem_wait_st();
-        };
+                tmem_wait_st();
+                // P V of the tile before, whose place of P the next tile takes. Every phase is waited for in turn: a
+                // wait for one that another has followed would not end.
+                if (i > 0) ok = wait_for(&bar_o, (done + i - 1) & 1) && ok;
+                if (!ok) s_fail = 1;
+            };
 
-        for (int i = 0; i < n; ++i) {
-            if (owns) {
+            for (int i = 0; i < n; ++i) {
                 if (start + (i + 1) * kRowsTile > min(lim_first, end) || rp.bad[i & 3])
                     column_step(i, std::true_type());
                 else
                     column_step(i, std::false_type());
-            } else {
-                if (i + 1 < n) {
-                    // the slots of the tile after next's successor are free by now
-                    if (p == 0) rp.key_top[(i + 3) & 3] = kNoExp;
-                    if (p == 32) rp.value_top[(i + 2) & 3] = kNoExp, rp.bad[(i + 2) & 3] = 0;
-                    find_tops<G>(keys, values, &rp, i + 2 < n ? i + 2 : -1, i + 1, p, E);
-                    // P V of the tile before has read the buffer that these values go to
-                    if (i > 0 && !umma::bar_wait(&bar_o, (done + i - 1) & 1)) s_fail = 1;
-                    decode_values<G>(values, sv + ((i + 1) & 1) * W::kVBytes, &rp, p);
-                    if (i + 2 < n) {
-                        load_values<G>(values, vc, vp, start + (i + 2) * kRowsTile, end, p);
-                        asm volatile("bar.sync 2, 512;" ::: "memory");  // S of this tile is there: its keys are read
-                        decode_keys<G>(keys, sk + (i & 1) * W::kKBytes, rp.key_top[(i + 2) & 3], p);
-                        if (i + 3 < n) load_keys<G>(keys, kc, kp, start + (i + 3) * kRowsTile, end, p);
-                    }
-                }
-                umma::fence_smem_to_async();
+                end_step();
+                if (s_fail) break;
             }
-            umma::fence_before_sync();
-            __syncthreads();
-            if (issues) {
-                umma::fence_after_sync();
-                issue_values(i);
-            }
-            __syncwarp();
-            if (s_fail) break;
         }
         // ---- the columns' results: each half of the threads half of the dimensions ----
         if (owns) {
@@ -571,7 +700,7 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
             asm volatile("bar.sync 3, 256;" ::: "memory");
             const float l = __fadd_rn(s_top[0][p], s_top[1][p]);
             if (n > 0) {
-                const bool ok = !s_fail && umma::bar_wait(&bar_o, (done + n - 1) & 1);
+                const bool ok = !s_fail && wait_for(&bar_o, (done + n - 1) & 1);
                 umma::fence_after_sync();
                 if (!ok) atomicOr(c.flags, kCacheWait);
             }
@@ -586,15 +715,32 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
                 tmem_ld32(mine + kColO + 32 * (half * G + y), v);
                 umma::tmem_wait_ld();
                 if (in) {
+                    float o[32];
 #pragma unroll
-                    for (int x = 0; x < 32; ++x) {
-                        const int d = 32 * (half * G + y) + x;
-                        if (d >= c.dim) continue;
-                        const float o = none ? 0.0f : __fmul_rn(__uint_as_float(v[x]), inv);
-                        if (kk.parts == 1)
-                            write_out(a.out, a.type, at * c.dim + d, o);
-                        else
-                            kk.part_o[at * c.dim + d] = o;
+                    for (int x = 0; x < 32; ++x) o[x] = none ? 0.0f : __fmul_rn(__uint_as_float(v[x]), inv);
+                    const int d0 = 32 * (half * G + y);
+                    if (kk.parts > 1 && c.dim % 4 == 0) {
+                        float* dst = kk.part_o + at * c.dim + d0;
+#pragma unroll
+                        for (int x = 0; x < 32; x += 4)
+                            if (d0 + x < c.dim)
+                                *reinterpret_cast<float4*>(dst + x) = make_float4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+                    } else if (kk.parts > 1) {
+#pragma unroll
+                        for (int x = 0; x < 32; ++x)
+                            if (d0 + x < c.dim) kk.part_o[at * c.dim + d0 + x] = o[x];
+                    } else if (c.dim % 8 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0) {
+                        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + at * c.dim + d0;
+#pragma unroll
+                        for (int x = 0; x < 32; x += 8)
+                            if (d0 + x < c.dim)
+                                *reinterpret_cast<uint4*>(dst + x) =
+                                    make_uint4(bf16_pair(o[x], o[x + 1]), bf16_pair(o[x + 2], o[x + 3]),
+                                               bf16_pair(o[x + 4], o[x + 5]), bf16_pair(o[x + 6], o[x + 7]));
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 32; ++x)
+                            if (d0 + x < c.dim) write_out(a.out, kBF16, at * c.dim + d0 + x, o[x]);
                     }
                 }
             }
@@ -617,10 +763,9 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
     if (s_fail) {
         // let what was issued land before the memory goes
         if (threadIdx.x == 0) {
-            umma::bar_wait(&bar_s, 0);
-            umma::bar_wait(&bar_s, 1);
-            umma::bar_wait(&bar_o, 0);
-            umma::bar_wait(&bar_o, 1);
+            for (int y = 0; y < 4; ++y) wait_for(&bar_s[y >> 1], y & 1);
+            wait_for(&bar_o, 0);
+            wait_for(&bar_o, 1);
         }
         __syncthreads();
     }
