@@ -87,25 +87,29 @@ __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&v)[32]) 
                  "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(at)
                  : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&v)[16]) {
+// The same of 16 and 8 columns.
+__device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&v)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(v[0]),
-        "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
-        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(at)
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(at)
         : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t at, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(v[0]), "r"(v[1]),
+                 "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(at)
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// A wait of a second at most; false when they ran out.
+// A wait of 2^31 clocks (about a second) at most; false when they ran out.
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity) {
     if (umma::bar_try(bar, parity)) return true;
-    uint64_t first, now;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(first));
+    const long long first = clock64();
     do {
-        for (int i = 0; i < 64; ++i)
-            if (umma::bar_try(bar, parity)) return true;
-        asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
-    } while (now - first < 1000000000ull);
+        if (umma::bar_try(bar, parity)) return true;
+    } while (clock64() - first < 1ll << 31);
     return false;
 }
 
@@ -298,30 +302,28 @@ __device__ __forceinline__ void decode_values(const ValueCodes<G>& x, char* sv, 
     if (p < 128 * G) {
         const int word = word_of<G>(p), b = p / (8 * G);
         const int g = G == 1 ? 0 : word & 1, d0 = G == 1 ? word : word >> 1;
-        uint32_t out[2][4][4];
 #pragma unroll
-        for (int y = 0; y < 4; ++y) {
-            const uint32_t p0 = rp->v[8 * b + 2 * y][g], p1 = rp->v[8 * b + 2 * y + 1][g];
-            const __half2 step = bits_h2(__byte_perm(p0, p1, 0x5410)), low = bits_h2(__byte_perm(p0, p1, 0x7632));
-            const __half2 step16 = __hmul2(step, sixteenth);
+        for (int h = 0; h < 2; ++h) {
+            uint32_t out[4][4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int y = 0; y < 4; ++y) {
+                const uint32_t p0 = rp->v[8 * b + 2 * y][g], p1 = rp->v[8 * b + 2 * y + 1][g];
+                const __half2 step = bits_h2(__byte_perm(p0, p1, 0x5410)), low = bits_h2(__byte_perm(p0, p1, 0x7632));
+                const __half2 step16 = __hmul2(step, sixteenth);
                 const uint32_t u = __byte_perm(x.c[2 * y], x.c[2 * y + 1], h ? 0x7632 : 0x5410);
 #pragma unroll
                 for (int n = 0; n < 4; ++n) {
                     const uint32_t c = ((n >> 1 ? u >> 8 : u) & (n & 1 ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u;
-                    out[h][n][y] = h2_bits(__hfma2(__hsub2(bits_h2(c), magic), n & 1 ? step16 : step, low));
+                    out[n][y] = h2_bits(__hfma2(__hsub2(bits_h2(c), magic), n & 1 ? step16 : step, low));
                 }
             }
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
                 const int d = kCacheGroup * g + 16 * n + 8 * h + d0;
                 *reinterpret_cast<uint4*>(sv + (b >> 3) * G * kCacheGroup * 128 + umma::sw128_offset(d, b & 7)) =
-                    make_uint4(out[h][n][0], out[h][n][1], out[h][n][2], out[h][n][3]);
+                    make_uint4(out[n][0], out[n][1], out[n][2], out[n][3]);
             }
+        }
     }
 }
 
@@ -364,7 +366,7 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
     __shared__ uint64_t bar_s[2], bar_o;
     __shared__ uint32_t s_tmem;
     __shared__ int s_fail;
-    char* sq = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~uintptr_t(1023));
+    char* sq = s_raw + (-umma::smem_addr(s_raw) & 1023u);  // an offset, so that the stores stay shared memory's
     char* sk = sq + W::kQBytes;
     char* sv = sk + 2 * W::kKBytes;
     const int warp = threadIdx.x >> 5;
@@ -391,10 +393,6 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
     if (ct0 * kWideCols >= cols || (part > 0 && start >= rows_all)) return;
 
     const size_t head_row = ((size_t)s * c.heads + h) * c.rows;
-    const uint32_t* kc = c.kc + head_row * 8 * G;
-    const uint32_t* vc = c.vc + head_row * 8 * G;
-    const uint32_t* kp = c.kp + head_row * G;
-    const uint32_t* vp = c.vp + head_row * G;
 
     if (warp == 0) umma::tmem_alloc(&s_tmem, kTmemCols);
     if (threadIdx.x == 0) {
@@ -408,10 +406,7 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
     __syncthreads();
     umma::fence_after_sync();
     const uint32_t tmem = s_tmem, mine = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-    const uint32_t q_at = umma::smem_addr(sq), k_at = umma::smem_addr(sk), v_at = umma::smem_addr(sv);
     constexpr uint32_t kIdS = idesc_f16(128, kRowsTile), kIdO = idesc_f16(128, G * kCacheGroup);
-    // a descriptor's low bits are the address in sixteenths
-    const uint64_t q_desc = umma::desc_k_sw128(q_at), k_desc = umma::desc_k_sw128(k_at), v_desc = umma::desc_k_sw128(v_at);
 
     int done = 0;  // tiles of earlier column tiles: the barriers' phases go on
     for (int ct = ct0; ct * kWideCols < cols; ct += kk.col_tiles) {
@@ -427,11 +422,13 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
         // tiles count on over the column tiles for the two places and barriers of the scores
         auto issue_scores = [&](int i) {
             const int place = (done + i) & 1;
-            const uint64_t kd = k_desc + (i & 1) * (W::kKBytes >> 4);
+            // a descriptor's low bits are the address in sixteenths
+            const uint64_t qd = umma::desc_k_sw128(umma::smem_addr(sq));
+            const uint64_t kd = umma::desc_k_sw128(umma::smem_addr(sk)) + (i & 1) * (W::kKBytes >> 4);
 #pragma unroll
             for (int x = 0; x < 4 * G + 1; ++x) {  // the last sixteen positions hold the low parts
                 const uint32_t at = ((x >> 2) * W::kGroupBytes + 32 * (x & 3)) >> 4;
-                mma_ss(tmem + kColS + kRowsTile * place, q_desc + at, kd + at, kIdS, x > 0);
+                mma_ss(tmem + kColS + kRowsTile * place, qd + at, kd + at, kIdS, x > 0);
             }
             umma::mma_commit(&bar_s[place]);
         };
@@ -440,7 +437,7 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
             asm volatile("bar.sync 0;" ::: "memory");
         };
         auto issue_values = [&](int i) {
-            const uint64_t vd = v_desc + (i & 1) * (W::kVBytes >> 4);
+            const uint64_t vd = umma::desc_k_sw128(umma::smem_addr(sv)) + (i & 1) * (W::kVBytes >> 4);
 #pragma unroll
             for (int x = 0; x < 8; ++x)
                 mma_ts(tmem + kColO, tmem + kColP + 64 * (i & 1) + 8 * x, vd + (((x >> 2) * G * kCacheGroup * 128 + 32 * (x & 3)) >> 4), kIdO,
@@ -472,7 +469,7 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
             }
         } else if (decodes_keys) {
             KeyCodes<G> keys;
-            KeySource<G> source(kc, kp, start, end, p);
+            KeySource<G> source(c.kc + head_row * 8 * G, c.kp + head_row * G, start, end, p);
             if (p < 4) rp.key_top[p] = kNoExp;
             // the second piece of the low parts' positions stays zero
             if (p < 128) {
@@ -503,7 +500,7 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
             }
         } else if (!owns) {
             ValueCodes<G> values;
-            ValueSource<G> source(vc, vp, start, end, p);
+            ValueSource<G> source(c.vc + head_row * 8 * G, c.vp + head_row * G, start, end, p);
             if (p < 4) rp.value_top[p] = kNoExp, rp.bad[p] = 0;
             asm volatile("bar.sync 1, 256;" ::: "memory");
             if (n > 0) {
@@ -603,12 +600,13 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
                     umma::tmem_wait_ld();
 #pragma unroll
                     for (int x = 0; x < 32; x += 2) {
-                        float s0 = __uint_as_float(v[x]), s1 = __uint_as_float(v[x + 1]);
+                        const float s0 = __uint_as_float(v[x]), s1 = __uint_as_float(v[x + 1]);
                         if constexpr (kEdge) {
-                            s0 = 32 * y + x < vis ? s0 : -INFINITY;
-                            s1 = 32 * y + x + 1 < vis ? s1 : -INFINITY;
+                            if (32 * y + x < vis) top = fmaxf(top, s0);
+                            if (32 * y + x + 1 < vis) top = fmaxf(top, s1);
+                        } else {
+                            top = max3(top, s0, s1);
                         }
-                        top = max3(top, s0, s1);
                     }
                 }
                 s_top[half][p] = top;
@@ -644,21 +642,21 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
                 }
                 const f2 f2x = pair(f, f), neg = pair(kPUp - m, kPUp - m);
 #pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    uint32_t v[32], out[16];
-                    tmem_ld32(s_at + 32 * y, v);
+                for (int y = 0; y < 4; ++y) {
+                    uint32_t v[16], out[8];
+                    tmem_ld16(s_at + 16 * y, v);
                     umma::tmem_wait_ld();
                     if (kk.logits && in) {
-                        float4* lg = reinterpret_cast<float4*>(kk.logits + th * kk.logit_rows + row0 + 32 * y);
+                        float4* lg = reinterpret_cast<float4*>(kk.logits + th * kk.logit_rows + row0 + 16 * y);
 #pragma unroll
-                        for (int x = 0; x < 8; ++x)
+                        for (int x = 0; x < 4; ++x)
                             lg[x] = make_float4(__fmul_rn(__uint_as_float(v[4 * x]), f), __fmul_rn(__uint_as_float(v[4 * x + 1]), f),
                                                 __fmul_rn(__uint_as_float(v[4 * x + 2]), f),
                                                 __fmul_rn(__uint_as_float(v[4 * x + 3]), f));
                     }
 #pragma unroll
-                    for (int x = 0; x < 16; ++x) {
-                        const int r = 32 * y + 2 * x;
+                    for (int x = 0; x < 8; ++x) {
+                        const int r = 16 * y + 2 * x;
                         float p0, p1;
                         unpair(fma2(pair(__uint_as_float(v[2 * x]), __uint_as_float(v[2 * x + 1])), f2x, neg), p0, p1);
                         p0 = ex2(p0), p1 = ex2(p1);
@@ -674,7 +672,7 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
                         }
                         out[x] = pack_h2(p0, p1);
                     }
-                    tmem_st16(mine + kColP + 64 * (i & 1) + 32 * half + 16 * y, out);
+                    tmem_st8(mine + kColP + 64 * (i & 1) + 32 * half + 8 * y, out);
                 }
                 tmem_wait_st();
                 // P V of the tile before, whose place of P the next tile takes. Every phase is waited for in turn: a
