@@ -54,6 +54,7 @@ constexpr int kJoinBS = 128;
 constexpr int kMaxCluster = 8;
 constexpr int kMaxParts = 1024;
 constexpr int kWaves = 4;
+constexpr int kPartRows = 1024;
 constexpr int kSoloLists = 2;
 // Up to so many rows a cluster of blocks reads them and joins in shared memory, in one launch; above, its
 // blocks would wait for the slowest and the SMs for a place for all of them.
@@ -996,31 +997,40 @@ AttendPlan make_plan(const CacheView& c, const AttendArgs& a) {
     AttendPlan p{};
     const bool found = a.k > 0;
     const long long cols = found ? a.group : (long long)std::max(1, a.max_tokens) * a.group;
-    // Columns that fill blocks of 128 to four fifths go to k_cache_wide (4 sequences of 20,000 rows, 8 heads of
-    // 128, wide against sixteen columns: 128 columns 236 and 229 us, 192 330 and 316, 256 348 and 406, 512 594
-    // and 741; one sequence, 2048 columns: 437 and 745). Below that, sixteen share a tile's codes where the
-    // registers hold them.
-    const long long full = (cols + kWideCols - 1) / kWideCols * kWideCols;
-    p.wide = !found && a.type == kBF16 && c.G <= 2 && cols >= kWideCols && 5 * cols >= 4 * full;
-    p.nc = p.wide ? kWideCols : a.type != kF32 && c.G <= 2 && cols > 8 ? 16 : 8;
-    p.col_tiles = (int)((cols + p.nc - 1) / p.nc);
-    const long long items = (long long)(found ? a.tok.n_tokens : c.n_seqs) * c.heads * p.col_tiles;
     const int rows = std::max(1, found ? a.k : std::min(a.max_rows, c.capacity));
     const int step = kAttWarps * kTile * sub_tiles(c.G);
-    const long long slots = (long long)(p.wide ? 1 : blocks_of(c.G, p.nc)) * sm_count();
-    // Enough blocks to fill the GPU once; with sequences of different lengths kWaves times as many, of
-    // fixed rows, so that the longest do not run on alone.
     const int most = (rows + step - 1) / step;
     const bool ragged = !found && c.n_seqs > 1;
-    const long long fill = std::max(1ll, slots / std::max(1ll, items));
+    long long slots, items, fill;  // blocks that the GPU holds, blocks without a split of the rows, split that fills it
+    auto tile = [&](int nc, int blocks) {
+        p.nc = nc;
+        p.col_tiles = (int)((cols + nc - 1) / nc);
+        items = (long long)(found ? a.tok.n_tokens : c.n_seqs) * c.heads * p.col_tiles;
+        slots = (long long)blocks * sm_count();
+        fill = std::max(1ll, slots / std::max(1ll, items));
+    };
+    // Sixteen columns share a tile's codes where the registers hold them.
+    const int few = a.type != kF32 && c.G <= 2 && cols > 8 ? 16 : 8;
+    tile(few, blocks_of(c.G, few));
+    const bool join_inside = !found && rows <= kClusterRows && fill >= 2;
+    // From 80 columns on (96 of one group) a block of 128 is faster than blocks of sixteen: 4 sequences of 20,000
+    // rows, 8 heads of 128, wide and narrow: 64 columns 124 and 131 us, 80 130 and 156, 112 139 and 202, 132 203
+    // and 243, 160 206 and 278; heads of 64: 80 98 and 98, 96 100 and 111, 132 162 and 149, 160 165 and 187. Not
+    // where clusters join few rows in one launch (500 rows, 96 columns: 22 and 15 us).
+    p.wide = !found && a.type == kBF16 && c.G <= 2 && cols >= (c.G == 1 ? 96 : 80) && !join_inside;
+    if (p.wide) tile(kWideCols, 1);
+    // Enough blocks to fill the GPU once; with sequences of different lengths kWaves times as many, of
+    // fixed rows, so that the longest do not run on alone. Parts cost their start and the join: more of them than
+    // fill the GPU have kPartRows each (16 sequences of 500 rows, 96 columns: 28 us whole, 86 in five parts).
     p.cluster = p.parts = 1;
     p.share = most * step;
     // Lists enough to fill the GPU by warps: none waits for a block's barriers.
     p.solo = found && c.G <= 2 && p.nc == 8 && items * kSoloLists >= slots * kAttWarps;
-    if (!found && !p.wide && rows <= kClusterRows && fill >= 2) {
+    if (join_inside) {
         p.cluster = (int)std::min<long long>({kMaxCluster, fill, most});
     } else {
-        const long long n = ragged ? std::max(1ll, kWaves * slots / std::max(1ll, items)) : fill;
+        long long n = ragged ? std::max(1ll, kWaves * slots / std::max(1ll, items)) : fill;
+        n = std::max(fill, std::min<long long>(n, rows / kPartRows));
         const int least = (rows + kMaxParts - 1) / kMaxParts;
         p.share = (std::max((int)std::min<long long>(rows, (rows + n - 1) / n), least) + step - 1) / step * step;
         p.parts = (rows + p.share - 1) / p.share;

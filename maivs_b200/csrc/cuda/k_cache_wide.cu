@@ -11,15 +11,21 @@
 // memory, the same words for all lanes, took 5,500 clocks a tile (such a read moves 4 bytes a clock). Here
 // a row's codes are decoded once for 128 columns, where the kernel for few columns decodes them per 16.
 //
-// Warps 0 to 7 own the columns, two threads a column with half a tile's rows each: scores from tensor memory,
-// running maximum (exchanged) and sum in registers, P back. Warps 8 to 15 decode: in step i the values of
-// tile i + 1 and the keys of tile i + 2. Thread 0 issues the products: S of tile i + 1 as soon as S of tile i is
-// in registers, P V of tile i at the end of the step, so both run beside the exponentials.
+// Four kinds of warps, each with a loop of its own, a step a tile and the block's barrier between: in step i
+//   0 to 7    own the columns, two threads a column with half a tile's rows each: scores of tile i from tensor
+//             memory, twice (maximum, exchanged, then exponentials), running maximum and sum in registers, P back;
+//   8 to 15   decode the values of tile i + 1;
+//   16 to 23  decode the keys of tile i + 2;
+//   24        issues the products, as soon as step i - 1 is over: P V of its tile, S of tile i + 1.
+// S and P have two places each, so that the products run beside the exponentials.
 //
-// Bound by the decoding warps: some 5,000 clocks a tile of G = 2, the columns' warps 3,300, the products' arithmetic 550.
-// Chunks of 32 to 64 tokens over 4 sequences of 20,000 to 32,000 rows, 8 heads of 128 with 4 query heads each: 394
-// us, 78 GFLOP, an eighth of the tensor cores' rate. Loads of codes in whole lines that were then exchanged in
-// shared memory took 447.
+// Bound by the issue of instructions and the latencies between a step's barriers: 11,900 warp instructions a tile of
+// G = 2, 3,000 clocks a scheduler at best; a tile takes 4,400 clocks, the products' arithmetic 1,100 of them.
+// Chunks of 32 to 64 tokens over 4 sequences of 20,000 to 32,000 rows, 8 heads of 128 with 4 query heads each:
+// 257 us, 78 GFLOP, a fifth of the tensor cores' rate (with the columns' padding to 128 a third). On the way
+// there: bounds on every load of a tile's codes took 406 us; 16 warps, where the same warps decoded keys and
+// values, 394; 32 columns of scores at a time, with their spills, 284; whole lines of codes exchanged in shared
+// memory were slower (447 for 388 at that time).
 //
 // Rounding: scores are as exact as the other kernel's (the log-sum-exp and the rows' weights come from
 // them); both are scaled by powers of two, the keys by one per tile. V = low + step c is rounded to f16, in
