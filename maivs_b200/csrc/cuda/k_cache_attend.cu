@@ -54,7 +54,7 @@ constexpr int kJoinBS = 128;
 constexpr int kMaxCluster = 8;
 constexpr int kMaxParts = 1024;
 constexpr int kWaves = 4;
-constexpr int kPartRows = 1024;
+constexpr int kPartRows = 1024, kWidePartRows = 16384;
 constexpr int kSoloLists = 2;
 // Up to so many rows a cluster of blocks reads them and joins in shared memory, in one launch; above, its
 // blocks would wait for the slowest and the SMs for a place for all of them.
@@ -1021,7 +1021,9 @@ AttendPlan make_plan(const CacheView& c, const AttendArgs& a) {
     if (p.wide) tile(kWideCols, 1);
     // Enough blocks to fill the GPU once; with sequences of different lengths kWaves times as many, of
     // fixed rows, so that the longest do not run on alone. Parts cost their start and the join: more of them than
-    // fill the GPU have kPartRows each (16 sequences of 500 rows, 96 columns: 28 us whole, 86 in five parts).
+    // fill the GPU have kPartRows each (16 sequences of 500 rows, 96 columns: 28 us whole, 86 in five parts), of
+    // wide blocks, which start with an empty pipeline, kWidePartRows (4 sequences of 20,000 rows, 128 columns: 110
+    // us in four parts, 147 in 18; of 20,000 to 32,000 rows, 128 to 256 columns: 234 and 258).
     p.cluster = p.parts = 1;
     p.share = most * step;
     // Lists enough to fill the GPU by warps: none waits for a block's barriers.
@@ -1030,7 +1032,7 @@ AttendPlan make_plan(const CacheView& c, const AttendArgs& a) {
         p.cluster = (int)std::min<long long>({kMaxCluster, fill, most});
     } else {
         long long n = ragged ? std::max(1ll, kWaves * slots / std::max(1ll, items)) : fill;
-        n = std::max(fill, std::min<long long>(n, rows / kPartRows));
+        n = std::max(fill, std::min<long long>(n, rows / (p.wide ? kWidePartRows : kPartRows)));
         const int least = (rows + kMaxParts - 1) / kMaxParts;
         p.share = (std::max((int)std::min<long long>(rows, (rows + n - 1) / n), least) + step - 1) / step * step;
         p.parts = (rows + p.share - 1) / p.share;
