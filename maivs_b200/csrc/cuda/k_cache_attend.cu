@@ -1013,11 +1013,12 @@ AttendPlan make_plan(const CacheView& c, const AttendArgs& a) {
     const int few = a.type != kF32 && c.G <= 2 && cols > 8 ? 16 : 8;
     tile(few, blocks_of(c.G, few));
     const bool join_inside = !found && rows <= kClusterRows && fill >= 2;
-    // From 80 columns on (96 of one group) a block of 128 is faster than blocks of sixteen: 4 sequences of 20,000
-    // rows, 8 heads of 128, wide and narrow: 64 columns 124 and 131 us, 80 130 and 156, 112 139 and 202, 132 203
-    // and 243, 160 206 and 278; heads of 64: 80 98 and 98, 96 100 and 111, 132 162 and 149, 160 165 and 187. Not
-    // where clusters join few rows in one launch (500 rows, 96 columns: 22 and 15 us).
-    p.wide = !found && a.type == kBF16 && c.G <= 2 && cols >= (c.G == 1 ? 96 : 80) && !join_inside;
+    // From 33 columns on (64 of one group) a block of 128 is faster than blocks of sixteen: 4 sequences of 20,000
+    // rows, 8 heads of 128, wide and narrow: 40 columns 96 and 109 us, 64 98 and 132, 112 104 and 203, 132 179 and
+    // 243, 160 182 and 278; heads of 64: 48 82 and 71, 64 83 and 83, 96 86 and 111, 132 153 and 150, 160 155 and 188;
+    // one sequence of 4000 rows, where the start counts: 40 22 and 18, 128 26 and 24. Not where clusters join few
+    // rows in one launch (500 rows, 96 columns: 22 and 15 us).
+    p.wide = !found && a.type == kBF16 && c.G <= 2 && cols >= (c.G == 1 ? 64 : 33) && !join_inside;
     if (p.wide) tile(kWideCols, 1);
     // Enough blocks to fill the GPU once; with sequences of different lengths kWaves times as many, of
     // fixed rows, so that the longest do not run on alone. Parts cost their start and the join: more of them than

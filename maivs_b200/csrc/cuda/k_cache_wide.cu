@@ -22,10 +22,10 @@
 // Bound by the issue of instructions and the latencies between a step's barriers: 11,900 warp instructions a tile of
 // G = 2, 3,000 clocks a scheduler at best; a tile takes 4,400 clocks, the products' arithmetic 1,100 of them.
 // Chunks of 32 to 64 tokens over 4 sequences of 20,000 to 32,000 rows, 8 heads of 128 with 4 query heads each:
-// 257 us, 78 GFLOP, a fifth of the tensor cores' rate (with the columns' padding to 128 a third). On the way
-// there: bounds on every load of a tile's codes took 406 us; 16 warps, where the same warps decoded keys and
-// values, 394; 32 columns of scores at a time, with their spills, 284; whole lines of codes exchanged in shared
-// memory were slower (447 for 388 at that time).
+// 235 us, 78 GFLOP, a fifth of the tensor cores' rate (with the columns' padding to 128 a third). On the way
+// there, in 18 parts of the rows (258 at the end): bounds on every load of a tile's codes 406 us; 16 warps, where
+// the same warps decoded keys and values, 394; scores 32 at a time, with their spills, 284; whole lines of codes
+// exchanged in shared memory 447 (for 388 at that time).
 //
 // Rounding: scores are as exact as the other kernel's (the log-sum-exp and the rows' weights come from
 // them); both are scaled by powers of two, the keys by one per tile. V = low + step c is rounded to f16, in
