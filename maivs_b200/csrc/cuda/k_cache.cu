@@ -275,8 +275,8 @@ __device__ __forceinline__ void find_places(const CacheView& c, const CacheToken
 // Rows into the cache. blockIdx.x: a run of tokens; blockIdx.y: even keys, odd values, times the slices of a
 // token's units. Eight lanes take a group of 64 dimensions of one head. Every lane goes through the same
 // passes; those without a unit, or whose token has no row, load and store nothing. Bound by its instructions as
-// much as by HBM: 30,000 tokens of 8 heads of 128 in bf16 take 55 us, 158 MB, 2.9 TB/s (75 us with
-// single f32 operations and a bound on every element).
+// much as by HBM: 34,000 tokens of 8 heads of 128 in bf16 take 61 us, 178 MB, 2.9 TB/s (some 20 us
+// more with single f32 operations and a bound on every element).
 template <typename T, int G, int U, bool kWhole>
 __global__ void __launch_bounds__(kStoreBS) k_cache_append(CacheView c, AppendArgs a, bool vec, StoreShape sh) {
     __shared__ long long s_place[kMaxRun];
@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(kStoreBS) k_cache_append(CacheView c, AppendAr
     }
 }
 
-// Rows back as values, in the same order: 39 us for 178 MB, 4.6 TB/s, bound by the writes.
+// Rows back as values, in the same order: 40 us for those 178 MB, 4.4 TB/s, bound by the writes.
 template <typename T, int G, int U, bool kWhole>
 __global__ void __launch_bounds__(kStoreBS) k_cache_read(CacheView c, ReadArgs a, bool vec, StoreShape sh) {
     __shared__ long long s_place[kMaxRun];
