@@ -287,14 +287,41 @@ def test_attend_padding_strides_and_empty_sequences(causal):
                  back=4, q_pad=5, capacity=50)
 
 
+# A capacity above which no cluster joins the rows: calls of many columns take blocks of 128.
+LONG = 2112
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("dim", [40, 64, 80, 128])
 def test_attend_many_columns(dim, dtype):
     """Blocks of 128 columns: full, ragged and several of them, rows in one part and in several."""
     rng = np.random.default_rng(dim)
-    check_attend(rng, [300, 0, 127, 130], [33, 17, 1, 53], 1, 4, dim, dtype, weights=dim == 80)
-    check_attend(rng, [1500], [13], 2, 8, dim, dtype, weights=dim == 64, front=2, back=1, q_pad=3)
-    check_attend(rng, [130, 60], [32, 0], 1, 4, dim, dtype, causal=False, weights=True, capacity=200)
+    check_attend(rng, [300, 0, 127, 130], [33, 17, 1, 53], 1, 4, dim, dtype, weights=dim == 80, capacity=LONG)
+    check_attend(rng, [1500], [13], 2, 8, dim, dtype, weights=dim == 64, front=2, back=1, q_pad=3, capacity=LONG)
+    check_attend(rng, [130, 60], [32, 0], 1, 4, dim, dtype, causal=False, weights=True, capacity=LONG)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("held", [[70, 0], [130, 300], [600, 511]])
+def test_attend_many_columns_beyond_the_hint(held, dim):
+    """More columns than max_tokens promises: a block takes several tiles of them in turn, of 1 to 6 tiles of rows."""
+    rng = np.random.default_rng(35)
+    check_attend(rng, held, [70, 41], 1, 8, dim, "bf16", max_tokens=16, weights=True, capacity=LONG)
+
+
+@pytest.mark.parametrize("max_tokens", [0, 16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attend_many_columns_many_tiles(dim, max_tokens):
+    """Heads enough to fill the GPU, so that a block goes over up to six tiles of rows; maxima and values that rise
+    from tile to tile. With the hint a block takes both tiles of columns."""
+    rng = np.random.default_rng(36)
+    heads, held, new = 24, [701, 389], [33, 40]
+    total = [h + n for h, n in zip(held, new)]
+    rise = np.concatenate([np.linspace(-1, 1, n) for n in total])[:, None, None]
+    keys = (tokens(rng, sum(total), heads, dim) * (1.5 + rise)).astype(np.float32)
+    values = (tokens(rng, sum(total), heads, dim) * 10.0 ** (2 * rise)).astype(np.float32)
+    f = Filled(rng, total, LONG, heads, dim, "bf16", keys, values)
+    check_attend(rng, held, new, heads, 4, dim, "bf16", fill=f, capacity=LONG, max_tokens=max_tokens)
 
 
 def test_attend_many_columns_wide_ranges():
@@ -307,8 +334,8 @@ def test_attend_many_columns_wide_ranges():
     for mag in (np.ones(n), 10.0 ** np.linspace(-3, 3, n), 10.0 ** rng.uniform(-3, 3, n), np.full(n, 1e-20),
                 np.full(n, 1e20)):
         values = (tokens(rng, n, 1, dim) * mag[:, None, None]).astype(np.float32)
-        f = Filled(rng, [n], n, 1, dim, "bf16", keys, values)
-        check_attend(rng, [n - 32], [32], 1, 4, dim, "bf16", fill=f, qs=q, capacity=n, weights=True)
+        f = Filled(rng, [n], LONG, 1, dim, "bf16", keys, values)
+        check_attend(rng, [n - 32], [32], 1, 4, dim, "bf16", fill=f, qs=q, capacity=LONG, weights=True)
 
 
 @pytest.mark.parametrize("new", [1, 32])
@@ -322,11 +349,11 @@ def test_attend_tiles_of_zeros_and_of_extreme_keys(mag, new):
     q = rng.standard_normal((new, 4, dim)).astype(np.float32)
     if mag != 1e30:
         keys[:256] *= mag
-        f = Filled(rng, [n], n, 1, dim, "bf16", keys, values)
-        check_attend(rng, [n - new], [new], 1, 4, dim, "bf16", fill=f, qs=q, capacity=n, weights=True)
+        f = Filled(rng, [n], LONG, 1, dim, "bf16", keys, values)
+        check_attend(rng, [n - new], [new], 1, 4, dim, "bf16", fill=f, qs=q, capacity=LONG, weights=True)
     keys *= mag
-    f = Filled(rng, [n], n, 1, dim, "bf16", keys, np.zeros_like(values))
-    check_attend(rng, [n - new], [new], 1, 4, dim, "bf16", fill=f, qs=q, capacity=n, weights=True,
+    f = Filled(rng, [n], LONG, 1, dim, "bf16", keys, np.zeros_like(values))
+    check_attend(rng, [n - new], [new], 1, 4, dim, "bf16", fill=f, qs=q, capacity=LONG, weights=True,
                  scale=0.1 / mag if mag > 1e-37 else None)  # (a scale past 2^100 is refused)
 
 
@@ -337,14 +364,14 @@ def test_attend_many_columns_ignore_what_they_cannot_see():
     for s in range(2):
         k[s * cap + held[s] + new[s]:(s + 1) * cap] = np.nan
         v[s * cap + held[s] + new[s]:(s + 1) * cap] = np.inf
-    f = Filled(rng, [cap, cap], cap, 1, 128, "bf16", k, v)
-    got, _, _ = check_attend(rng, held, new, 1, 4, 128, "bf16", fill=f, capacity=cap, weights=True)
+    f = Filled(rng, [cap, cap], LONG, 1, 128, "bf16", k, v)
+    got, _, _ = check_attend(rng, held, new, 1, 4, 128, "bf16", fill=f, capacity=LONG, weights=True)
     assert np.isfinite(got).all()
     # a NaN value row of the step: the tokens before it do not see it, those from it on do
     v[held[0] + 11] = np.nan
     k[cap + held[1] + 7] = np.inf
-    f = Filled(rng, [cap, cap], cap, 1, 128, "bf16", k, v)
-    got, lse, _ = check_attend(rng, held, new, 1, 4, 128, "bf16", fill=f, capacity=cap)
+    f = Filled(rng, [cap, cap], LONG, 1, 128, "bf16", k, v)
+    got, lse, _ = check_attend(rng, held, new, 1, 4, 128, "bf16", fill=f, capacity=LONG)
     assert np.isfinite(got[:11]).all() and np.isnan(got[11:44]).all() and np.isfinite(lse[:44]).all()
     assert np.isfinite(got[44:51]).all() and np.isnan(got[51:]).all() and np.isnan(lse[51:]).all()
 
