@@ -73,7 +73,8 @@ __device__ __noinline__ uint32_t codes_exact(float4 a, float4 b, float low, floa
 //    for the exact way there. x - low itself is exact under the same condition;
 //  - f32 elements: wherever t is that close to k + 1/2, which is asked here.
 // Elements i and i + 4 go together in packed f32 operations; the codes of four are summed as
-// c_0 + 16 c_1 + 256 c_2 + 4096 c_3, exact in f32.
+// c_0 + 16 c_1 + 256 c_2 + 4096 c_3, exact in f32: one code outside 0..15 damages the others, so a chunk
+// that is not whole is padded with low.
 template <typename T>
 __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float low, float step, bool fine) {
     constexpr float kMagic = 12582912.0f;
@@ -88,7 +89,7 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float low, flo
         const f2 d = add2(pair(x[i], x[i + 4]), lows);
         f2 t = mul2(d, invs);
         t = fma2(fma2(t, steps, d), invs, t);
-        if constexpr (!std::is_same<T, __nv_bfloat16>::value) {  // bf16: low is the smallest
+        if constexpr (!std::is_same<T, __nv_bfloat16>::value) {  // bf16: low is the smallest, and what pads a chunk
             float a, b;
             unpair(t, a, b);
             t = pair(fminf(fmaxf(a, 0.0f), 15.0f), fminf(fmaxf(b, 0.0f), 15.0f));
@@ -319,10 +320,9 @@ __global__ void __launch_bounds__(kStoreBS) k_cache_append(CacheView c, AppendAr
                 if (step > 0.0f && step < INFINITY) {
                     float x[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = element(raw[i], e);
+                    for (int e = 0; e < 8; ++e) x[e] = e < have ? element(raw[i], e) : low;  // padding: code 0
                     const float few = std::is_same<T, __half>::value ? 0x1p-10f : 0x1p-13f;
                     code = codes_of<T>(x, low, step, sizeof(T) == 2 && small < few * step);
-                    if (have < 8) code &= (1u << (4 * have)) - 1;  // padding
                 }
             }
             if (!is_key) code = transpose_nibbles(code, l8);

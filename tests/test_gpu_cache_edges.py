@@ -1,0 +1,54 @@
+"""The attention cache on the GPU where its arithmetic has an edge: groups that end inside a chunk of eight
+dimensions, smallest elements far below the step, rows of very different magnitude, hints and offsets.
+
+Compared with the definitions in 64 bits (cache_oracle.py), with bounds derived there.
+"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import cache_oracle as O
+import maivs_b200 as M
+from test_gpu_cache import DT, _release_inputs, i32, offsets, rounded, stream  # noqa: F401 (the fixture runs here too)
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+def stored(x, dtype):
+    """Rows [n, heads, dim] written as keys and as values: what each reads back as in f32, and the rounded rows."""
+    n, heads, dim = x.shape
+    xt, xx = rounded(x, dtype)
+    c = M.AttentionCache(1, n, heads, dim)
+    off, ln = offsets([n]), i32([0])
+    c.append(xt.data_ptr(), xt.data_ptr(), n, off.data_ptr(), ln.data_ptr(), dtype=dtype, stream=stream())
+    k, v = (torch.empty(n, heads, dim, device="cuda") for _ in range(2))
+    c.read(k.data_ptr(), v.data_ptr(), n, off.data_ptr(), ln.data_ptr(), dtype="f32", stream=stream())
+    torch.cuda.synchronize()
+    assert c.flags(stream()) == 0
+    return k.cpu().numpy(), v.cpu().numpy(), xx
+
+
+# ---- storage --------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("dim", [2, 3, 5, 6, 7, 61, 66, 67, 69, 70, 71, 73, 74, 127, 131, 197, 259, 383])
+def test_small_spread_beside_a_large_offset(dim, dtype):
+    """The last chunk of eight dimensions is not whole, and the tail's elements lie 10 to 3,000 steps from zero:
+    what pads the chunk must not reach their codes."""
+    rng = np.random.default_rng(dim)
+    rows = []
+    for far in (10, 100, 300, 1000, 3000):
+        for sign in (-1.0, 1.0):
+            # elements low + c of whole numbers c in 0..15, `far` of them from zero
+            rows.append(sign * far + rng.integers(0, 16, (4, dim)))
+    for first in ([-1.0, -1.0078125], [-5.0, -5.0625, -5.03125], [100.0, 101.0]):
+        row = np.full((1, dim), first[0])
+        tail = (dim - 1) % 64 + 1  # dimensions of the last group
+        part = np.resize(first, tail)
+        row[0, dim - tail:] = part
+        rows.append(row)
+    x = np.concatenate(rows).astype(np.float32)[:, None]
+    k, v, xx = stored(x, dtype)
+    want = O.quantise(xx)[0].astype(np.float32)
+    assert np.array_equal(k, want) and np.array_equal(v, want)
