@@ -69,8 +69,9 @@ __device__ __noinline__ uint32_t codes_exact(float4 a, float4 b, float low, floa
 // Rounding to a whole number is an addition of 1.5 * 2^23 (ties to even), whose low bits are the code.
 // That decides wrongly only where the true quotient is within 2^-21 of k + 1/2 and not equal to it:
 //  - 16-bit elements: x - low and (k + 1/2) step are multiples of one power of two, and so is their
-//    difference, unless some element is below 2^-13 (bf16) or 2^-10 (f16) of the step: `fine` asks
-//    for the exact way there. x - low itself is exact under the same condition;
+//    difference, unless an element of this lane, or low (an element of any lane of the group), is below
+//    2^-13 (bf16) or 2^-10 (f16) of the step and is not zero: `fine` asks for the exact way there.
+//    x - low itself is exact under the same condition;
 //  - f32 elements: wherever t is that close to k + 1/2, which is asked here.
 // Elements i and i + 4 go together in packed f32 operations; the codes of four are summed as
 // c_0 + 16 c_1 + 256 c_2 + 4096 c_3, exact in f32: one code outside 0..15 damages the others, so a chunk
@@ -321,8 +322,9 @@ __global__ void __launch_bounds__(kStoreBS) k_cache_append(CacheView c, AppendAr
                     float x[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) x[e] = e < have ? element(raw[i], e) : low;  // padding: code 0
-                    const float few = std::is_same<T, __half>::value ? 0x1p-10f : 0x1p-13f;
-                    code = codes_of<T>(x, low, step, sizeof(T) == 2 && small < few * step);
+                    const float few = (std::is_same<T, __half>::value ? 0x1p-10f : 0x1p-13f) * step;
+                    const bool fine = sizeof(T) == 2 && (small < few || (low != 0.0f && fabsf(low) < few));
+                    code = codes_of<T>(x, low, step, fine);
                 }
             }
             if (!is_key) code = transpose_nibbles(code, l8);

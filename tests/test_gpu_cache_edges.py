@@ -52,3 +52,43 @@ def test_small_spread_beside_a_large_offset(dim, dtype):
     k, v, xx = stored(x, dtype)
     want = O.quantise(xx)[0].astype(np.float32)
     assert np.array_equal(k, want) and np.array_equal(v, want)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("dim", [64, 128, 200])
+def test_smallest_element_far_below_the_step(dim, dtype):
+    """The smallest element of a group is tiny and not zero, or all but; elements of the other chunks lie in the
+    middle between two levels of a range from zero. What is next to a tie is no tie."""
+    rng = np.random.default_rng(dim)
+    rows = []
+    for mag in (2.0 ** -24, 2.0 ** -20, 2.0 ** -14, 2.0 ** -11, 2.0 ** -9) + (() if dtype == "f16" else (2.0 ** -30, 2.0 ** -60)):
+        for sign in (-1.0, 1.0):
+            for step in (1.0, 4.0, 0.25):
+                row = np.tile((rng.integers(0, 15, 8) + 0.5) * step, dim // 8)
+                for g in range(0, dim, 64):
+                    row[g + rng.integers(0, 4)] = sign * mag * step if dtype != "f16" or step > 1 else sign * mag
+                    row[g + 5] = 15 * step
+                rows.append(row)
+    x = np.array(rows, np.float32)[:, None]
+    k, v, xx = stored(x, dtype)
+    want = O.quantise(xx)[0].astype(np.float32)
+    assert np.array_equal(k, want) and np.array_equal(v, want)
+
+
+def test_f16_codes_next_to_the_middle_of_two_levels():
+    """Every f16 neighbour of every border between levels, for steps that are not powers of two."""
+    rng = np.random.default_rng(8)
+    rows = []
+    for _ in range(300):
+        lo, hi = np.sort(rng.standard_normal(2) * 10.0 ** rng.integers(-3, 3)).astype(np.float16)
+        step = float(O.bf16(np.float32([(np.float32(hi) - np.float32(lo)) * (np.float32(1) / np.float32(15))]))[0])
+        low = float(O.bf16(np.float32([lo]))[0])
+        row = [lo, hi]
+        for c in range(15):
+            b = np.float16(low + (c + 0.5) * step)
+            row += [b, np.nextafter(b, np.float16(np.inf)), np.nextafter(b, np.float16(-np.inf))]
+        row = np.clip(np.array(row + [lo] * (64 - len(row)), np.float32), np.float32(lo), np.float32(hi))
+        rows.append(row)
+    k, v, xx = stored(np.array(rows, np.float32)[:, None], "f16")
+    want = O.quantise(xx)[0].astype(np.float32)
+    assert np.array_equal(k, want) and np.array_equal(v, want)
