@@ -264,7 +264,8 @@ int maivs_concurrent_array(maivs_concurrent* cx, long long segment, const char* 
  * named. Rows leave by the attention weight they gathered, as an index's rows leave by id.
  *
  * A row of one head is stored per group of 64 dimensions as step =
- * bf16(f32(f32(max - min) * f32(1 / 15))), low = bf16(min) and 4-bit codes; a code c stands for f32(low + step * c) and is the nearest level
+ * bf16(f32(f32(max - min) * f32(1 / 15))) (a product, not a division), low = bf16(min) and 4-bit codes; a code c
+ * stands for f32(low + step * c) and is the nearest level
  * to its element (ties to the even code). Groups that hold a NaN or an infinity, or whose range
  * overflows f32, read back as NaN. dim is padded to 64, 128, 256 or 384; a padded row of one head
  * takes 36 bytes per 64 dimensions for its key and as many for its value.

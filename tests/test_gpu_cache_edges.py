@@ -92,3 +92,14 @@ def test_f16_codes_next_to_the_middle_of_two_levels():
     k, v, xx = stored(np.array(rows, np.float32)[:, None], "f16")
     want = O.quantise(xx)[0].astype(np.float32)
     assert np.array_equal(k, want) and np.array_equal(v, want)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_step_is_a_product_not_a_quotient(dtype):
+    """step = bf16(f32(max - min) * f32(1 / 15)): 4512 to -3 gives 302, where a division would round to 300."""
+    x = np.full((1, 1, 64), -3.0, np.float32)
+    x[0, 0, 7], x[0, 0, 9], x[0, 0, 20] = 4512.0, 1000.0, 2411.0
+    k, v, xx = stored(x, dtype)
+    assert np.array_equal(xx[0, 0, [0, 7]], [-3.0, 4512.0])
+    want = O.quantise(xx)[0].astype(np.float32)
+    assert want[0, 0, 7] == -3 + 15 * 302 and np.array_equal(k, want) and np.array_equal(v, want)
