@@ -395,8 +395,9 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, TYPE == kF32, (MODE >= Mo
             bad = (__ballot_sync(~0u, bad) >> (lane & ~3)) & 15u;
             const int e = top > 0.0f ? min(141 - (int)(__float_as_uint(top) >> 23), 126) : 0;
             const float up = bad ? 0.0f : __uint_as_float((uint32_t)max(e + 127, 1) << 23);
+            // the scale first: 2^24 / up alone is infinite from elements of 2^118 on
             const float f = bad ? __uint_as_float(0x7FC00000u)
-                                : __fmul_rn(__fmul_rn(__fdiv_rn(S::kUnit, up), a.scale), kLog2e);
+                                : __fmul_rn(__fmul_rn(__fdiv_rn(1.0f, up), a.scale), S::kUnit * kLog2e);
             float qs[G];
 #pragma unroll
             for (int g = 0; g < G; ++g) qs[g] = 0.0f;

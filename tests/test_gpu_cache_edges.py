@@ -10,7 +10,8 @@ import pytest
 
 import cache_oracle as O
 import maivs_b200 as M
-from test_gpu_cache import DT, _release_inputs, i32, offsets, rounded, stream  # noqa: F401 (the fixture runs here too)
+from test_gpu_cache import (DT, LONG, Filled, _release_inputs, check_attend, i32, offsets, rounded,  # noqa: F401
+                            stream, tokens)  # (the fixture runs here too)
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -103,3 +104,14 @@ def test_step_is_a_product_not_a_quotient(dtype):
     assert np.array_equal(xx[0, 0, [0, 7]], [-3.0, 4512.0])
     want = O.quantise(xx)[0].astype(np.float32)
     assert want[0, 0, 7] == -3 + 15 * 302 and np.array_equal(k, want) and np.array_equal(v, want)
+
+
+# ---- attention ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("new", [1, 33])
+@pytest.mark.parametrize("dtype,power", [("bf16", 110), ("bf16", 118), ("bf16", 120), ("bf16", 126), ("bf16", -120),
+                                         ("f32", 120), ("f32", -120)])
+def test_attend_queries_and_scales_of_opposite_magnitude(dtype, power, new):
+    """|query| x scale is moderate where neither is: few columns and blocks of 128."""
+    rng = np.random.default_rng(61)
+    q = (np.clip(rng.standard_normal((new, 4, 128)), -1.9, 1.9) * 2.0 ** power).astype(np.float32)
+    check_attend(rng, [150], [new], 1, 4, 128, dtype, scale=2.0 ** min(-power - 3, 97), qs=q, capacity=LONG)
