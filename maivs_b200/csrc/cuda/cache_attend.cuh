@@ -9,10 +9,13 @@ namespace dev {
 
 constexpr float kNoMax = -3.0e38f;
 constexpr float kLog2e = 1.4426950408889634f;
-// p * step goes into f16 scaled so that the group's largest step becomes 2^12: an old maximum may
-// be exceeded by 2^kLag before the accumulators are rescaled, and 2^12 * 2^kLag is below 65504.
+// An old maximum may be exceeded by 2^kLag before the sums are rescaled. What is summed goes into f16 scaled so
+// that the largest is 2^12 at most when its unit is set (p in blocks of 128 columns, a column's and group's p * step
+// else); 2^12 * 2^kLag is below 65504. The smallest unit of p * step keeps its inverse finite.
 constexpr float kLag = 3.0f;
 constexpr float kPScale = 4096.0f;
+constexpr float kPMost = 32768.0f;
+constexpr float kUnitMin = 0x1p-100f;
 
 struct AttendKernel {
     AttendArgs a;

@@ -12,7 +12,8 @@
 //   keys    S = K Q^T: A = codes (M: 16 rows), B = queries (N: 8 columns, scaled by a power of two to
 //           f16's upper range). Per group g: s += step_g * acc_g + low_g * sum(q in g).
 //   values  O^T = V^T P^T: A = codes (M: 16 dimensions of one group, K: 16 rows), B = p * step_g
-//           rounded to f16 (N: columns); the low terms p * low_g are summed in f32.
+//           rounded to f16 (N: columns), in a unit of its own for every column and group, the power of two above the
+//           largest product so far; the low terms p * low_g are summed in f32.
 //
 // The codes are the A operand of both, so that every register of both fragments is in use whatever
 // the number of columns, and a row's step and low are needed by one lane of every quad only. S's
@@ -21,7 +22,9 @@
 // Rounding: codes are exact, 16-bit queries are exact in f16 down to 2^-24 of their row's largest
 // element. p * step is rounded to f16 in bf16 calls (2^-12 relative, below the output's own rounding) and
 // split into two halves (22 bits) in f16 and f32 calls; one half doubled an f16 output's error where few rows
-// carry the weight. f32 calls split the query as well.
+// carry the weight. f32 calls split the query as well. What p * step loses below f16's smallest half is 2^-36 of
+// the column's largest product, so rows that have no weight, whatever their size, cost the others nothing (with a unit
+// from the largest step alone, f32 outputs beside such a row of 2^60 times the others' size were lost).
 //
 // Bound by instructions, close to HBM: two tiles of 16 rows (G = 2, eight columns) take some 520 of a warp, half
 // of them on the integer pipe (shifts and masks of codes, moves of halves), at 2304 bytes a tile. One token of
@@ -102,6 +105,13 @@ __device__ __forceinline__ uint32_t operand(uint32_t w) {
 template <bool F32>
 __device__ __forceinline__ float low_of(uint32_t par) {
     return F32 ? __fmaf_rn(8.0f, par_step(par), par_low(par)) : par_low(par);
+}
+
+// kPScale / x for a power of two x of 2^-115 to 2^127: a unit's inverse, and the unit of an inverse.
+__device__ __forceinline__ float unit_of(float x) {
+    constexpr uint32_t kSum = (254u + 12u) << 23;  // of the exponents' places
+    static_assert(kPScale == 4096.0f, "2^12");
+    return __uint_as_float(kSum - __float_as_uint(x));
 }
 
 // The part of x that its f16 rounding (in packed pair p, half i) leaves over.
@@ -461,19 +471,18 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, TYPE == kF32, (MODE >= Mo
             logit_at[j] = ((size_t)(FOUND ? item : sn.first + i) * a.q_heads + h * a.group + (col - i * a.group)) *
                           kk.logit_rows;
         }
-        // inv: what brings a step into f16's upper range, kPScale / norm, norm a power of two
-        float m[kCols], l[kCols], low[kCols][G], norm[G], inv[G];
+        // inv: what brings a column's p * step into f16's upper range, kPScale / a power of two (kUnitMin at least)
+        float m[kCols], l[kCols], low[kCols][G], inv[kCols][G];
         float o[G][4][kNt][4];
 #pragma unroll
         for (int j = 0; j < kCols; ++j) {
             m[j] = kNoMax;
             l[j] = 0.0f;
 #pragma unroll
-            for (int g = 0; g < G; ++g) low[j][g] = 0.0f;
+            for (int g = 0; g < G; ++g) low[j][g] = 0.0f, inv[j][g] = kPScale / kUnitMin;
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            norm[g] = inv[g] = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -587,8 +596,9 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, TYPE == kF32, (MODE >= Mo
                     }
             }
 
-            // ---- running maximum and the groups' power of two: rescaled only where they grow ----
-            float top[kCols], big[G];
+            // ---- running maximum and the unit of p * step: rescaled only where they grow. This lane's largest p
+            // times its largest step is no less than any of its products. ----
+            float top[kCols];
             bool grow = false;
 #pragma unroll
             for (int j = 0; j < kCols; ++j) {
@@ -599,10 +609,12 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, TYPE == kF32, (MODE >= Mo
             }
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                big[g] = par_step(vpw[0][g]);
+                float big = par_step(vpw[0][g]);
 #pragma unroll
-                for (int i = 1; i < kR; ++i) big[g] = fmaxf(big[g], par_step(vpw[i][g]));
-                grow |= big[g] > norm[g];
+                for (int i = 1; i < kR; ++i) big = fmaxf(big, par_step(vpw[i][g]));
+#pragma unroll
+                for (int j = 0; j < kCols; ++j)
+                    grow |= __fmul_rn(__fmul_rn(ex2(__fsub_rn(top[j], m[j])), inv[j][g]), big) > kPMost;
             }
             if (__any_sync(~0u, grow)) {
                 float f[kCols];
@@ -620,22 +632,26 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, TYPE == kF32, (MODE >= Mo
                 }
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    // a row with an infinite step is NaN whatever its scale
-                    float x = 0.0f;
+                    float ratio[kCols];
 #pragma unroll
-                    for (int i = 0; i < kR; ++i) {
-                        const float st = par_step(vpw[i][g]);
-                        x = st < INFINITY ? fmaxf(x, st) : x;
-                    }
+                    for (int j = 0; j < kCols; ++j) {
+                        // a row with an infinite step is NaN whatever its scale
+                        float x = 0.0f;
 #pragma unroll
-                    for (int d = 4; d < 32; d *= 2) x = fmaxf(x, __shfl_xor_sync(~0u, x, d));
-                    float ratio = 1.0f;
-                    if (x > norm[g]) {
-                        // a power of two at or above the step, at least 2^-100
-                        const float n = fmaxf(2.0f * __uint_as_float(__float_as_uint(x) & 0x7F800000u), 7.8886e-31f);
-                        ratio = __fdiv_rn(norm[g], n);
-                        norm[g] = n;
-                        inv[g] = __fdiv_rn(kPScale, n);
+                        for (int i = 0; i < kR; ++i) {
+                            const float st = par_step(vpw[i][g]);
+                            x = st < INFINITY ? fmaxf(x, __fmul_rn(ex2(__fsub_rn(sc[j][i], m[j])), st)) : x;
+                        }
+#pragma unroll
+                        for (int d = 4; d < 32; d *= 2) x = fmaxf(x, __shfl_xor_sync(~0u, x, d));
+                        // The sums so far are of f * old now. The unit is the power of two above the largest
+                        // product, of this tile or of those before: of the products as they are now, so that a row
+                        // whose weight has gone takes no digits from the others.
+                        const float old = __fmul_rn(f[j], unit_of(inv[j][g]));
+                        const float above = __uint_as_float(min((__float_as_uint(x) & 0x7F800000u) + 0x00800000u, 0x7F000000u));
+                        const float unit = fmaxf(fmaxf(above, __uint_as_float(__float_as_uint(old) & 0x7F800000u)), kUnitMin);
+                        inv[j][g] = unit_of(unit);
+                        ratio[j] = __fmul_rn(__fmul_rn(old, inv[j][g]), 1.0f / kPScale);
                     }
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
@@ -643,7 +659,7 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, TYPE == kF32, (MODE >= Mo
                         for (int j = 0; j < kNt; ++j)
 #pragma unroll
                             for (int r = 0; r < 4; ++r)
-                                o[g][i][j][r] = __fmul_rn(o[g][i][j][r], __fmul_rn(f[2 * j + (r & 1)], ratio));
+                                o[g][i][j][r] = __fmul_rn(o[g][i][j][r], ratio[2 * j + (r & 1)]);
                 }
             }
 
@@ -681,22 +697,26 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, TYPE == kF32, (MODE >= Mo
                     uint32_t b[kNt][2], c2[kNt][2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const float st = __fmul_rn(par_step(vpw[2 * u + i][g]), inv[g]), lo = low_of<F32>(vpw[2 * u + i][g]);
+                        const float st = par_step(vpw[2 * u + i][g]), lo = low_of<F32>(vpw[2 * u + i][g]);
 #pragma unroll
                         for (int j = 0; j < kNt; ++j) {
                             float ps[2];
+                            unpair(mul2(mul2(pair(p[2 * j][2 * u + i], p[2 * j + 1][2 * u + i]), pair(inv[2 * j][g], inv[2 * j + 1][g])),
+                                        pair(st, st)),
+                                   ps[0], ps[1]);
 #pragma unroll
                             for (int x = 0; x < 2; ++x) {
-                                ps[x] = __fmul_rn(p[2 * j + x][2 * u + i], st);
-                                float& lw = low[2 * j + x][g];
                                 if constexpr (kEdge) {
+                                    float& lw = low[2 * j + x][g];
                                     // a row the column does not see adds nothing, whatever it holds
                                     ps[x] = see[2 * j + x][2 * u + i] ? ps[x] : 0.0f;
                                     lw = see[2 * j + x][2 * u + i] ? __fmaf_rn(p[2 * j + x][2 * u + i], lo, lw) : lw;
-                                } else {
-                                    lw = __fmaf_rn(p[2 * j + x][2 * u + i], lo, lw);
                                 }
                             }
+                            if constexpr (!kEdge)
+                                unpair(fma2(pair(p[2 * j][2 * u + i], p[2 * j + 1][2 * u + i]), pair(lo, lo),
+                                            pair(low[2 * j][g], low[2 * j + 1][g])),
+                                       low[2 * j][g], low[2 * j + 1][g]);
                             b[j][i] = pack_h2(ps[0], ps[1]);
                             if constexpr (kTwoHalves)
                                 c2[j][i] = transpose8(pack_h2(left_over(ps[0], b[j][i], 0), left_over(ps[1], b[j][i], 1)));
@@ -769,14 +789,15 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, TYPE == kF32, (MODE >= Mo
             const float f = ex2(m[j] - mx);
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                // undo the operand's unit (16 for odd i) and kPScale / norm
-                const float n0 = __fmul_rn(S::kUnit / kPScale, norm[g]), n1 = __fmul_rn(S::kUnit / 16.0f / kPScale, norm[g]);
+                // undo the operand's unit (16 for odd i) and inv
+                const float unit = unit_of(inv[j][g]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int y = 0; y < 2; ++y)
                         s_o[(warp * NC + col) * S::kPitch + g * kCacheGroup + 16 * i + gid + 8 * y] =
-                            __fmul_rn(__fmaf_rn(o[g][i][j >> 1][2 * y + (j & 1)], i & 1 ? n1 : n0, low[j][g]), f);
+                            __fmul_rn(__fmaf_rn(__fmul_rn(o[g][i][j >> 1][2 * y + (j & 1)], i & 1 ? S::kUnit / 16.0f / kPScale : S::kUnit / kPScale),
+                                                unit, low[j][g]), f);
             }
         }
         team_sync();

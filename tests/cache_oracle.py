@@ -98,6 +98,37 @@ def attend_head(q, rows, which, scale, dtype):
     return out, lse, p, err, dz + (n + 32) * 2.0 ** -23 + abs(lse) * 2.0 ** -22, p * dp + 2.0 ** -126
 
 
+def attend_head_tight(q, rows, which, scale, dtype):
+    """out, lse, p and the error of each, as attend_head, with every row's error by its own magnitude.
+
+    A score's error is that of its own sum, (dim + 16) roundings of 2^-23 of scale * sum |key| |q| with |key| at most
+    |low| + 15 step, and the query's (2^-22 in f32 calls). p's relative error dp is its score's, the normaliser's (their mean),
+    and the exponential's. p * step is rounded to f16 (2^-12) in bf16 calls and to two halves (2^-22) else, in units where
+    2^11 is at most the largest p * step of the column and group when it was set: half of f16's 2^-24 adds
+    2^-36 of that per row, times a code of 15. Sums over n rows add n roundings of 2^-23.
+    """
+    n, d = len(which), len(q)
+    q = np.asarray(q, np.float64)
+    k, v = rows.k[which], rows.v[which]
+    z = scale * (k @ q)
+    mag = abs(scale) * ((np.abs(rows.k_low[which]) + 15 * rows.k_step[which]) @ np.abs(q))
+    dz = ((d + 16) * 2.0 ** -23 + (2.0 ** -22 if dtype == "f32" else 2.0 ** -30)) * mag
+    top = z.max()
+    e = np.exp(z - top)
+    p = e / e.sum()
+    lse = top + math.log(e.sum())
+    spread = np.minimum((top - z) / math.log(2.0), 160.0)
+    dp = dz + (spread + 8) * 2.0 ** -23
+    dp = dp + p @ dp + (n + 32) * 2.0 ** -23
+    out = p @ v
+    level = 15 * rows.v_step[which] + np.abs(rows.v_low[which])
+    round_p = 2.0 ** -12 if dtype == "bf16" else 2.0 ** -22
+    tiny = 15 * n * (2.0 ** -36 * (p[:, None] * rows.v_step[which]).max(axis=0) + 2.0 ** -136)
+    err = (p * (dp + round_p + (n + 64) * 2.0 ** -23)) @ level + tiny
+    err = err + UNIT[dtype] * (np.abs(out) + err) + TINY[dtype]
+    return out, lse, p, err, p @ dz + (n + 32) * 2.0 ** -23 + abs(lse) * 2.0 ** -22, p * dp + 2.0 ** -126
+
+
 def evict(length, keep, w, ids=None, protect=None):
     """(new length, source row of every new row, rows that leave)."""
     rank = []

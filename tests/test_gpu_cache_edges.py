@@ -10,7 +10,7 @@ import pytest
 
 import cache_oracle as O
 import maivs_b200 as M
-from test_gpu_cache import (DT, LONG, Filled, _release_inputs, check_attend, i32, offsets, rounded,  # noqa: F401
+from test_gpu_cache import (DT, LONG, Filled, _release_inputs, check_attend, check_attend_raw, close, i32, offsets, rounded,  # noqa: F401
                             stream, tokens)  # (the fixture runs here too)
 
 torch = pytest.importorskip("torch")
@@ -115,3 +115,39 @@ def test_attend_queries_and_scales_of_opposite_magnitude(dtype, power, new):
     rng = np.random.default_rng(61)
     q = (np.clip(rng.standard_normal((new, 4, 128)), -1.9, 1.9) * 2.0 ** power).astype(np.float32)
     check_attend(rng, [150], [new], 1, 4, 128, dtype, scale=2.0 ** min(-power - 3, 97), qs=q, capacity=LONG)
+
+
+def check_tight(f, qx, held, new, dtype, only=None):
+    """One causal call, a sequence: outputs and log-sum-exps within the bounds by each row's own magnitude."""
+    got, lse, flags = check_attend_raw(f, qx, [held], [new], dtype)
+    assert flags == 0
+    group = qx.shape[1] // f.heads
+    for i in range(new) if only is None else only:
+        for hh in range(qx.shape[1]):
+            want, wl, _, err, lerr, _ = O.attend_head_tight(qx[i, hh], f.rows[0][hh // group], list(range(held + i + 1)),
+                                                            qx.shape[2] ** -0.5, dtype)
+            close(got[i, hh], want, err, f"out of token {i}, head {hh}")
+            close(lse[i, hh], wl, lerr, f"lse of token {i}, head {hh}")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("dim", [64, 128, 192, 384])
+@pytest.mark.parametrize("power", [14, 24, 30, 60, 120])
+def test_one_large_value_row_takes_nothing_from_the_others(power, dim, dtype):
+    """A value row of 2^power times the others' size, first, in the middle or last, whose weight is nothing, or which
+    only the last token sees: what the others add keeps its digits. Few columns."""
+    rng = np.random.default_rng(71)
+    n, new = 300, 2
+    size = 2.0 ** -14 if dtype == "f16" else 2.0 ** -80 if power > 100 else 1.0
+    power = min(power, 28) if dtype == "f16" else power
+    base = rng.standard_normal(dim)
+    q = (base + 0.3 * rng.standard_normal((new, 4, dim))).astype(np.float32)
+    _, q = rounded(q, dtype)
+    for at in (0, 130, n - new, n - 1):
+        keys = tokens(rng, n, 1, dim)
+        values = (tokens(rng, n, 1, dim, 0.1) * size).astype(np.float32)
+        values[at] *= 2.0 ** power
+        if at < n - 1:
+            keys[at, 0] = -(20 + 0.7 * power) * base / np.sqrt(dim)  # a score of that: e^-20 after the row's size
+        f = Filled(rng, [n], n, 1, dim, dtype, keys, values)
+        check_tight(f, q, n - new, new, dtype, only=None if at < n - 1 else range(new - 1))
