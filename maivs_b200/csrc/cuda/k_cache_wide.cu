@@ -20,18 +20,21 @@
 // S and P have two places each, so that the products run beside the exponentials.
 //
 // Bound by the issue of instructions and the latencies between a step's barriers: 11,900 warp instructions a tile of
-// G = 2, 3,000 clocks a scheduler at best; a tile takes 4,400 clocks, the products' arithmetic 1,100 of them.
+// G = 2, 3,000 clocks a scheduler at best; a tile takes 4,500 clocks, the products' arithmetic 1,100 of them.
 // Chunks of 32 to 64 tokens over 4 sequences of 20,000 to 32,000 rows, 8 heads of 128 with 4 query heads each:
-// 235 us, 78 GFLOP, a fifth of the tensor cores' rate (with the columns' padding to 128 a third). On the way
+// 243 us, 78 GFLOP, a fifth of the tensor cores' rate (with the columns' padding to 128 a third). Where every
+// tile's rows have units of their own, 2.4 times as long (257 us for 107, 32 tokens over four times 20,000 rows). On the way
 // there, in 18 parts of the rows (258 at the end): bounds on every load of a tile's codes 406 us; 16 warps, where
 // the same warps decoded keys and values, 394; scores 32 at a time, with their spills, 284; whole lines of codes
 // exchanged in shared memory 447 (for 388 at that time).
 //
 // Rounding: scores are as exact as the other kernel's (the log-sum-exp and the rows' weights come from
-// them); both are scaled by powers of two, the keys by one per tile. V = low + step c is rounded to f16, in
-// units where the largest level so far is 2^14; P is rounded to f16, in units where the running maximum's is
-// 2^12 (2^-12 relative each, below the output's own rounding). A row whose values are not finite makes every
-// dimension of the columns that see it NaN.
+// them); queries and keys are scaled by powers of two, the keys by one per tile. V = low + step c is rounded to f16, in
+// units where the tile's largest level is 2^14; P is rounded to f16, in units where 2^12 is the largest p * level of
+// the column so far (2^-12 relative each, below the output's own rounding). Where a tile holds rows more than
+// 2^kSpread apart, each of its rows gets a unit of its own, which the columns read from shared memory (two
+// exponentials an element there), so that a row of another size, with or without weight, costs no digits. A row
+// whose values are not finite makes every dimension of the columns that see it NaN.
 #include <type_traits>
 
 #include "cache_attend.cuh"
@@ -48,7 +51,11 @@ constexpr int kRowsTile = 128;
 constexpr uint32_t kColS = 0, kColO = 256, kColP = 384;  // tensor memory columns: two of S, O, two of P
 constexpr uint32_t kTmemCols = 512;
 constexpr int kKeyUp = 6, kValueUp = 14, kSumDown = 8;   // powers of two of the largest key and value, of the query's sums
-constexpr int kNoExp = -200;
+constexpr int kNoExp = -200, kNoLow = 1000;  // of rows of zeros: the largest and the smallest exponent
+constexpr int kSpread = 8;                   // rows of a tile may be so many powers of two apart and share a unit
+constexpr int kKeyLeast = -120, kValueLeast = -110;  // exponents of the smallest units
+constexpr float kFar = 64.0f;  // powers of two between a tile's unit of values and a column's that count
+enum class Tile { kPlain, kEdge, kOwn };
 constexpr float kPUp = 12.0f;  // log2 of kPScale
 
 // kind::f16 with f16 operands, f32 accumulators, both operands K-major.
@@ -160,8 +167,11 @@ __device__ __forceinline__ int word_of(int p) {
 template <int G>
 struct RowParams {
     int key_top[4], value_top[4];    // exponents that hold every key and value element of the tile
+    int key_low[4], value_low[4];    // the smallest exponent of a row that is not all zeros
     int bad[4];                      // some row's values are not finite; which, in `poison` (NaN, else 0)
     float poison[4][kRowsTile];
+    float key_unit[4][kRowsTile];    // unit of a row's keys, over the tile's
+    float value_exp[4][kRowsTile];   // exponent of a row's values' unit
     uint32_t v[kRowsTile][G];        // step and low of the values as halves
 };
 
@@ -249,11 +259,16 @@ __device__ __forceinline__ int level_of(const uint32_t (&par)[G], bool& bad) {
     bad = false;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-        const float most = __fmaf_rn(15.0f, par_step(par[g]), fabsf(par_low(par[g])));
-        bad |= !(most < INFINITY);
-        if (most > 0.0f && most < INFINITY) e = max(e, (int)(__float_as_uint(most) >> 23) - 126);
+        const float step = par_step(par[g]), low = fabsf(par_low(par[g])), most = __fmaf_rn(15.0f, step, low);
+        bad |= !(step < INFINITY && low < INFINITY);
+        // (a sum of two finite terms past f32's range has an infinity's exponent field: 2^129)
+        if (most > 0.0f) e = max(e, (int)(__float_as_uint(most) >> 23) - 126);
     }
-    return bad ? kNoExp : min(e, 126);
+    return bad ? kNoExp : e;
+}
+// This row's unit: the tile's, or its own where the tile's rows are too far apart.
+__device__ __forceinline__ int unit_exp(int own, int top, int low, int least) {
+    return max(low < top - kSpread ? own : top, least);
 }
 
 __device__ __forceinline__ uint32_t h2_bits(__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); }
@@ -262,9 +277,9 @@ __device__ __forceinline__ __half2 bits_h2(uint32_t x) { return *reinterpret_cas
 // step (c - 8) of a row: a word is eight consecutive dimensions, one 16-byte piece, in the order of its nibble
 // pairs. Two threads a row; the first also writes low and 8 step to the positions behind the groups.
 template <int G>
-__device__ __forceinline__ void decode_keys(const KeyCodes<G>& x, char* sk, int top, int p) {
+__device__ __forceinline__ void decode_keys(const KeyCodes<G>& x, char* sk, int unit, int p) {
     const int row = p & 127, part = p >> 7;
-    const float up = pow2(kKeyUp - max(top, -120));
+    const float up = pow2(kKeyUp - unit);
     const __half2 mid = __float2half2_rn(1032.0f), mid16 = __float2half2_rn(1152.0f);
 #pragma unroll
     for (int i = 0; i < G; ++i) {
@@ -333,32 +348,140 @@ __device__ __forceinline__ void decode_values(const ValueCodes<G>& x, char* sv, 
     }
 }
 
-// The top of the keys of tile i, over the threads that decode keys.
+// The top of the keys of tile i, over the threads that decode keys; the exponent of this row's unit.
 template <int G>
-__device__ __forceinline__ void find_key_top(const KeyCodes<G>& k, RowParams<G>* rp, int i, int p) {
+__device__ __forceinline__ int find_key_unit(const KeyCodes<G>& k, RowParams<G>* rp, int i, int p) {
     bool bad;
-    const int top = __reduce_max_sync(~0u, level_of<G>(k.p, bad));
-    if ((p & 31) == 0) atomicMax(&rp->key_top[i & 3], top);
+    const int own = level_of<G>(k.p, bad);
+    const int top = __reduce_max_sync(~0u, own), low = __reduce_min_sync(~0u, own == kNoExp ? kNoLow : own);
+    if ((p & 31) == 0) {
+        atomicMax(&rp->key_top[i & 3], top);
+        atomicMin(&rp->key_low[i & 3], low);
+    }
     asm volatile("bar.sync 2, 256;" ::: "memory");
+    const int all = rp->key_top[i & 3], unit = unit_exp(own, all, rp->key_low[i & 3], kKeyLeast);
+    if (p < kRowsTile) rp->key_unit[i & 3][p] = pow2(unit - max(all, kKeyLeast));
+    return unit;
 }
-// The same of the values; their parameters as halves, in units of the running exponent E.
+// The same of the values; their parameters as halves in that unit.
 template <int G>
-__device__ __forceinline__ void find_value_top(const ValueCodes<G>& v, RowParams<G>* rp, int i, int p, int& E) {
+__device__ __forceinline__ void find_value_unit(const ValueCodes<G>& v, RowParams<G>* rp, int i, int p) {
     bool bad;
-    const int top = __reduce_max_sync(~0u, level_of<G>(v.p, bad));
-    if ((p & 31) == 0) atomicMax(&rp->value_top[i & 3], top);
+    const int own = level_of<G>(v.p, bad);
+    const int top = __reduce_max_sync(~0u, own), low = __reduce_min_sync(~0u, own == kNoExp ? kNoLow : own);
+    if ((p & 31) == 0) {
+        atomicMax(&rp->value_top[i & 3], top);
+        atomicMin(&rp->value_low[i & 3], low);
+    }
     if (p < kRowsTile) {
         rp->poison[i & 3][p] = bad ? __uint_as_float(0x7FC00000u) : 0.0f;
         if (bad) rp->bad[i & 3] = 1;
     }
     asm volatile("bar.sync 1, 256;" ::: "memory");
-    E = max(E, rp->value_top[i & 3]);
-    const float up = pow2(kValueUp - max(E, -110));
-    if (p < kRowsTile)
+    const int unit = unit_exp(own, rp->value_top[i & 3], rp->value_low[i & 3], kValueLeast);
+    const float up = pow2(kValueUp - unit);
+    if (p < kRowsTile) {
+        rp->value_exp[i & 3][p] = (float)unit;
 #pragma unroll
         for (int g = 0; g < G; ++g)
             rp->v[p][g] = bad ? 0u : pack_h2(__fmul_rn(par_step(v.p[g]), up), __fmul_rn(par_low(v.p[g]), up));
+    }
     asm volatile("bar.sync 1, 256;" ::: "memory");
+}
+
+// A column's sums: P is 2^kPUp at a score of m and a level of 2^D (a whole number), l the sum of p as 2^kPUp at m.
+struct ColumnSums {
+    float m, D;
+    f2 l2;
+};
+// Where a column's thread finds things: the tensor memory of its scores, its P and its half of O, the barrier and the
+// phase of the P V before (first: there is none).
+struct ColumnPlace {
+    uint32_t s_at, p_at, o_at;
+    uint64_t* bar_o;
+    uint32_t phase;
+    bool first;
+};
+
+// The unit of P for a tile of largest score `top`: up where the tile asks for it, down with a rising maximum; O and l
+// follow. `most` is the largest exponent of a level (level_exp), or the largest score + exponent. false when a wait
+// ran out.
+template <int G>
+__device__ __forceinline__ bool settle(ColumnSums& c, const ColumnPlace& at, float top, float most, bool level_exp) {
+    const bool grow = top > c.m + kLag;
+    const float mn = grow ? top : c.m, dm = __fsub_rn(mn, c.m);
+    const float need = level_exp ? __fadd_rn(most, __fsub_rn(top, mn)) : __fsub_rn(most, mn);
+    float Dn = ceilf(__fsub_rn(c.D, dm));
+    if (grow || need > Dn + kLag) Dn = fmaxf(Dn, ceilf(need));
+    bool ok = true;
+    if (__any_sync(~0u, grow || Dn != c.D)) {
+        const float fm = ex2(-dm), fo = ex2(__fsub_rn(__fsub_rn(c.D, Dn), dm));
+        c.m = mn, c.D = Dn;
+        c.l2 = mul2(c.l2, pair(fm, fm));
+        // P V of the tile before comes first
+        if (!at.first) {
+            ok = wait_for(at.bar_o, at.phase);
+            umma::fence_after_sync();
+#pragma unroll 1
+            for (int y = 0; y < G; ++y) {
+                uint32_t v[32];
+                tmem_ld32(at.o_at + 32 * y, v);
+                umma::tmem_wait_ld();
+#pragma unroll
+                for (int x = 0; x < 32; ++x) v[x] = __float_as_uint(__fmul_rn(__uint_as_float(v[x]), fo));
+                tmem_st32(at.o_at + 32 * y, v);
+            }
+        }
+    }
+    return ok;
+}
+
+// A column's 64 rows of a tile whose rows have units of their own. Out of line: inlined, it took registers from
+// the common forms (262 us for 234, chunks of 32 to 64 tokens over four times 20,000 to 32,000 rows).
+template <int G>
+__device__ __noinline__ ColumnSums own_step(ColumnSums c, ColumnPlace at, const RowParams<G>* rp, int slot, int half, int p, int vis,
+                                            float f, float (*s_top)[kWideCols], float (*s_most)[kWideCols], float* logits, int* fail) {
+    const float* const key_unit = rp->key_unit[slot] + 64 * half;
+    const float* const value_exp = rp->value_exp[slot] + 64 * half;
+    const float* const poison = rp->poison[slot] + 64 * half;
+    float top = -INFINITY, most = -INFINITY;
+#pragma unroll 1
+    for (int y = 0; y < 64; y += 16) {
+        uint32_t v[16];
+        tmem_ld16(at.s_at + y, v);
+        umma::tmem_wait_ld();
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+            const float z = __fmul_rn(__fmul_rn(__uint_as_float(v[x]), key_unit[y + x]), f);
+            if (y + x < vis) top = fmaxf(top, z), most = fmaxf(most, __fadd_rn(z, value_exp[y + x]));
+        }
+    }
+    s_top[half][p] = top, s_most[half][p] = most;
+    asm volatile("bar.sync 3, 256;" ::: "memory");
+    if (!settle<G>(c, at, fmaxf(s_top[0][p], s_top[1][p]), fmaxf(s_most[0][p], s_most[1][p]), false)) *fail = 1;
+    float l = 0.0f;
+#pragma unroll 1
+    for (int y = 0; y < 64; y += 16) {
+        uint32_t v[16], out[8];
+        tmem_ld16(at.s_at + y, v);
+        umma::tmem_wait_ld();
+#pragma unroll
+        for (int x = 0; x < 16; x += 2) {
+            float pp[2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const int r = y + x + n;
+                const float z = __fmul_rn(__fmul_rn(__uint_as_float(v[x + n]), key_unit[r]), f), up = __fadd_rn(__fsub_rn(z, c.m), kPUp);
+                if (logits) logits[r] = z;
+                l = __fadd_rn(l, r < vis ? ex2(up) : 0.0f);
+                pp[n] = r < vis ? __fadd_rn(ex2(__fadd_rn(up, __fsub_rn(value_exp[r], c.D))), poison[r]) : 0.0f;
+            }
+            out[x / 2] = pack_h2(pp[0], pp[1]);
+        }
+        tmem_st8(at.p_at + y / 2, out);
+    }
+    c.l2 = add2(c.l2, pair(l, 0.0f));
+    return c;
 }
 
 template <int G>
@@ -368,7 +491,8 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
     cudaTriggerProgrammaticLaunchCompletion();  // the join's blocks wait for this grid's end
     extern __shared__ char s_raw[];
     __shared__ RowParams<G> rp;
-    __shared__ float s_top[2][kWideCols], s_sum[2][G][kWideCols];  // maxima and sums of a column's two threads
+    // maxima (of scores, and of scores times levels) and sums of a column's two threads
+    __shared__ float s_top[2][kWideCols], s_most[2][kWideCols], s_sum[2][G][kWideCols];
     __shared__ uint64_t bar_s[2], bar_o;
     __shared__ uint32_t s_tmem;
     __shared__ int s_fail;
@@ -451,9 +575,8 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
             umma::mma_commit(&bar_o);
         };
 
-        int E = kNoExp;
-        float fac = 0.0f, m = kNoMax;
-        f2 l2 = 0;
+        float fac = 0.0f;
+        ColumnSums sums{kNoMax, kValueLeast, 0};
         // Each kind of warp has a loop of its own over the tiles, with the block's barrier at the end of a step.
         if (issues) {
             end_step();
@@ -476,7 +599,7 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
         } else if (decodes_keys) {
             KeyCodes<G> keys;
             KeySource<G> source(c.kc + head_row * 8 * G, c.kp + head_row * G, start, end, p);
-            if (p < 4) rp.key_top[p] = kNoExp;
+            if (p < 4) rp.key_top[p] = kNoExp, rp.key_low[p] = kNoLow;
             // the second piece of the low parts' positions stays zero
             if (p < 128) {
                 char* const at = sk + G * W::kGroupBytes + umma::sw128_offset(p, 1);
@@ -485,19 +608,19 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
             asm volatile("bar.sync 2, 256;" ::: "memory");
             for (int i = 0; i < min(n, 2); ++i) {
                 source.next(keys);
-                find_key_top<G>(keys, &rp, i, p);
-                decode_keys<G>(keys, sk + i * W::kKBytes, rp.key_top[i], p);
+                const int unit = find_key_unit<G>(keys, &rp, i, p);
+                decode_keys<G>(keys, sk + i * W::kKBytes, unit, p);
             }
             if (n > 2) source.next(keys);
             umma::fence_smem_to_async();
             end_step();
             for (int i = 0; i < n; ++i) {
                 if (i + 2 < n) {
-                    if (p == 0) rp.key_top[(i + 3) & 3] = kNoExp;  // last read in the step before
-                    find_key_top<G>(keys, &rp, i + 2, p);
+                    if (p == 0) rp.key_top[(i + 3) & 3] = kNoExp, rp.key_low[(i + 3) & 3] = kNoLow;  // last read in the step before
+                    const int unit = find_key_unit<G>(keys, &rp, i + 2, p);
                     // S of this tile has read the buffer that these keys go to
                     if (!wait_for(&bar_s[(done + i) & 1], ((done + i) >> 1) & 1)) s_fail = 1;
-                    decode_keys<G>(keys, sk + (i & 1) * W::kKBytes, rp.key_top[(i + 2) & 3], p);
+                    decode_keys<G>(keys, sk + (i & 1) * W::kKBytes, unit, p);
                     if (i + 3 < n) source.next(keys);
                 }
                 umma::fence_smem_to_async();
@@ -507,11 +630,11 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
         } else if (!owns) {
             ValueCodes<G> values;
             ValueSource<G> source(c.vc + head_row * 8 * G, c.vp + head_row * G, start, end, p);
-            if (p < 4) rp.value_top[p] = kNoExp, rp.bad[p] = 0;
+            if (p < 4) rp.value_top[p] = kNoExp, rp.value_low[p] = kNoLow, rp.bad[p] = 0;
             asm volatile("bar.sync 1, 256;" ::: "memory");
             if (n > 0) {
                 source.next(values);
-                find_value_top<G>(values, &rp, 0, p, E);
+                find_value_unit<G>(values, &rp, 0, p);
                 decode_values<G>(values, sv, &rp, p);
                 if (n > 1) source.next(values);
             }
@@ -519,8 +642,8 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
             end_step();
             for (int i = 0; i < n; ++i) {
                 if (i + 1 < n) {
-                    if (p == 0) rp.value_top[(i + 2) & 3] = kNoExp, rp.bad[(i + 2) & 3] = 0;
-                    find_value_top<G>(values, &rp, i + 1, p, E);
+                    if (p == 0) rp.value_top[(i + 2) & 3] = kNoExp, rp.value_low[(i + 2) & 3] = kNoLow, rp.bad[(i + 2) & 3] = 0;
+                    find_value_unit<G>(values, &rp, i + 1, p);
                     // P V of the tile before has read the buffer that these values go to
                     if (i > 0 && !wait_for(&bar_o, (done + i - 1) & 1)) s_fail = 1;
                     decode_values<G>(values, sv + ((i + 1) & 1) * W::kVBytes, &rp, p);
@@ -591,94 +714,87 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
             umma::fence_smem_to_async();
             end_step();
 
-            // One tile of this thread's column and half. kEdge: the column does not see some row.
-            auto column_step = [&](int i, auto edge) {
-                constexpr bool kEdge = decltype(edge)::value;
+            // One tile of this thread's column and half. kEdge: the column does not see some row, or one is not
+            // finite. kOwn: rows have units of their own (and the other as well).
+            auto column_step = [&](int i, auto form) {
+                constexpr bool kOwn = decltype(form)::value == Tile::kOwn, kEdge = decltype(form)::value == Tile::kEdge;
+                const int slot = i & 3, vt = rp.value_top[slot];
                 const int row0 = start + i * kRowsTile + 64 * half, vis = min(lim, end) - row0;  // rows below vis count
-                const uint32_t s_at = mine + kColS + kRowsTile * ((done + i) & 1) + 64 * half;
+                const ColumnPlace at{mine + kColS + kRowsTile * ((done + i) & 1) + 64 * half, mine + kColP + 64 * (i & 1) + 32 * half,
+                                     mine + kColO + 32 * G * half, &bar_o, (uint32_t)(done + i - 1) & 1, i == 0};
                 bool ok = wait_for(&bar_s[(done + i) & 1], ((done + i) >> 1) & 1);
                 umma::fence_after_sync();
-                float top = -INFINITY;
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    uint32_t v[32];
-                    tmem_ld32(s_at + 32 * y, v);
-                    umma::tmem_wait_ld();
-#pragma unroll
-                    for (int x = 0; x < 32; x += 2) {
-                        const float s0 = __uint_as_float(v[x]), s1 = __uint_as_float(v[x + 1]);
-                        if constexpr (kEdge) {
-                            if (32 * y + x < vis) top = fmaxf(top, s0);
-                            if (32 * y + x + 1 < vis) top = fmaxf(top, s1);
-                        } else {
-                            top = max3(top, s0, s1);
-                        }
-                    }
-                }
-                s_top[half][p] = top;
-                asm volatile("bar.sync 3, 256;" ::: "memory");
                 // to log2 units: fac is not negative, so the largest stays the largest (-inf where nothing is seen)
-                const float f = __fmul_rn(fac, pow2(max(rp.key_top[i & 3], -120) - kKeyUp));
-                top = fmaxf(s_top[0][p], s_top[1][p]);
-                top = top == -INFINITY ? top : __fmul_rn(top, f);
-                const int e_new = max(E, rp.value_top[i & 3]);
-                const bool grow = top > m + kLag;
-                if (__any_sync(~0u, grow) || e_new > E) {
-                    const float mn = grow ? fmaxf(m, top) : m;
-                    const float fm = ex2(m - mn);
-                    m = mn;
-                    l2 = mul2(l2, pair(fm, fm));
-                    const float fo = __fmul_rn(fm, pow2(max(E, -110) - max(e_new, -110)));
-                    // P V of the tile before comes first
-                    if (i > 0) {
-                        ok = wait_for(&bar_o, (done + i - 1) & 1) && ok;
-                        umma::fence_after_sync();
-#pragma unroll 1
-                        for (int y = 0; y < G; ++y) {
-                            uint32_t v[32];
-                            const uint32_t at = mine + kColO + 32 * (half * G + y);
-                            tmem_ld32(at, v);
-                            umma::tmem_wait_ld();
+                const float f = __fmul_rn(fac, pow2(max(rp.key_top[slot], kKeyLeast) - kKeyUp));
+                float* const lg = kk.logits && in ? kk.logits + th * kk.logit_rows + row0 : nullptr;
+                if constexpr (kOwn) {
+                    sums = own_step<G>(sums, at, &rp, slot, half, p, vis, f, s_top, s_most, lg, &s_fail);
+                } else {
+                    float top = -INFINITY;
 #pragma unroll
-                            for (int x = 0; x < 32; ++x) v[x] = __float_as_uint(__fmul_rn(__uint_as_float(v[x]), fo));
-                            tmem_st32(at, v);
+                    for (int y = 0; y < 2; ++y) {
+                        uint32_t v[32];
+                        tmem_ld32(at.s_at + 32 * y, v);
+                        umma::tmem_wait_ld();
+#pragma unroll
+                        for (int x = 0; x < 32; x += 2) {
+                            const float s0 = __uint_as_float(v[x]), s1 = __uint_as_float(v[x + 1]);
+                            if constexpr (kEdge) {
+                                if (32 * y + x < vis) top = fmaxf(top, s0);
+                                if (32 * y + x + 1 < vis) top = fmaxf(top, s1);
+                            } else {
+                                top = max3(top, s0, s1);
+                            }
                         }
                     }
-                    E = e_new;
-                }
-                const f2 f2x = pair(f, f), neg = pair(kPUp - m, kPUp - m);
+                    s_top[half][p] = top;
+                    asm volatile("bar.sync 3, 256;" ::: "memory");
+                    top = fmaxf(s_top[0][p], s_top[1][p]);
+                    top = top == -INFINITY ? top : __fmul_rn(top, f);
+                    // where nothing is seen, or zeros, the tile takes the column's unit
+                    const float e = vt == kNoExp || !(top > -INFINITY) ? sums.D : (float)max(vt, kValueLeast);
+                    ok = settle<G>(sums, at, top, e, true) && ok;
+                    // P is 2^-off of p, so its sum goes into l times 2^off. That far above, P is nothing as a half; that
+                    // far below, p is nothing beside l.
+                    const float off = fminf(__fsub_rn(sums.D, e), kFar);
+                    const int by = (int)fmaxf(off, -kFar);
+                    f2 l2 = mul2(sums.l2, pair(pow2(-by), pow2(-by)));
+                    const float base = __fsub_rn(__fsub_rn(kPUp, sums.m), off);
+                    const f2 f2x = pair(f, f), neg = pair(base, base);
 #pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    uint32_t v[16], out[8];
-                    tmem_ld16(s_at + 16 * y, v);
-                    umma::tmem_wait_ld();
-                    if (kk.logits && in) {
-                        float4* lg = reinterpret_cast<float4*>(kk.logits + th * kk.logit_rows + row0 + 16 * y);
+                    for (int y = 0; y < 4; ++y) {
+                        uint32_t v[16], out[8];
+                        tmem_ld16(at.s_at + 16 * y, v);
+                        umma::tmem_wait_ld();
+                        if (lg) {
 #pragma unroll
-                        for (int x = 0; x < 4; ++x)
-                            lg[x] = make_float4(__fmul_rn(__uint_as_float(v[4 * x]), f), __fmul_rn(__uint_as_float(v[4 * x + 1]), f),
-                                                __fmul_rn(__uint_as_float(v[4 * x + 2]), f),
-                                                __fmul_rn(__uint_as_float(v[4 * x + 3]), f));
-                    }
-#pragma unroll
-                    for (int x = 0; x < 8; ++x) {
-                        const int r = 16 * y + 2 * x;
-                        float p0, p1;
-                        unpair(fma2(pair(__uint_as_float(v[2 * x]), __uint_as_float(v[2 * x + 1])), f2x, neg), p0, p1);
-                        p0 = ex2(p0), p1 = ex2(p1);
-                        if constexpr (kEdge) {
-                            // a row the column does not see adds nothing, whatever it holds; one that is not finite poisons
-                            const bool in0 = r < vis, in1 = r + 1 < vis;
-                            const float* bad = rp.poison[i & 3] + 64 * half + r;
-                            p0 = in0 ? p0 : 0.0f, p1 = in1 ? p1 : 0.0f;
-                            l2 = add2(l2, pair(p0, p1));
-                            p0 = in0 ? __fadd_rn(p0, bad[0]) : 0.0f, p1 = in1 ? __fadd_rn(p1, bad[1]) : 0.0f;
-                        } else {
-                            l2 = add2(l2, pair(p0, p1));
+                            for (int x = 0; x < 4; ++x)
+                                reinterpret_cast<float4*>(lg + 16 * y)[x] = make_float4(
+                                    __fmul_rn(__uint_as_float(v[4 * x]), f), __fmul_rn(__uint_as_float(v[4 * x + 1]), f),
+                                    __fmul_rn(__uint_as_float(v[4 * x + 2]), f), __fmul_rn(__uint_as_float(v[4 * x + 3]), f));
                         }
-                        out[x] = pack_h2(p0, p1);
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) {
+                            const int r = 16 * y + 2 * x;
+                            float p0, p1;
+                            unpair(fma2(pair(__uint_as_float(v[2 * x]), __uint_as_float(v[2 * x + 1])), f2x, neg), p0, p1);
+                            p0 = ex2(p0), p1 = ex2(p1);
+                            if constexpr (kEdge) {
+                                // a row the column does not see adds nothing, whatever it holds; one that is not finite
+                                // poisons
+                                const bool in0 = r < vis, in1 = r + 1 < vis;
+                                const float* bad = rp.poison[slot] + 64 * half + r;
+                                p0 = in0 ? p0 : 0.0f, p1 = in1 ? p1 : 0.0f;
+                                l2 = add2(l2, pair(p0, p1));
+                                p0 = in0 ? __fadd_rn(p0, bad[0]) : 0.0f, p1 = in1 ? __fadd_rn(p1, bad[1]) : 0.0f;
+                            } else {
+                                l2 = add2(l2, pair(p0, p1));
+                            }
+                            out[x] = pack_h2(p0, p1);
+                        }
+                        tmem_st8(at.p_at + 8 * y, out);
                     }
-                    tmem_st8(mine + kColP + 64 * (i & 1) + 32 * half + 8 * y, out);
+                    sums.l2 = mul2(l2, pair(pow2(by), pow2(by)));
                 }
                 tmem_wait_st();
                 // P V of the tile before, whose place of P the next tile takes. Every phase is waited for in turn: a
@@ -688,10 +804,13 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
             };
 
             for (int i = 0; i < n; ++i) {
-                if (start + (i + 1) * kRowsTile > min(lim_first, end) || rp.bad[i & 3])
-                    column_step(i, std::true_type());
+                const int slot = i & 3;
+                if (rp.key_low[slot] < rp.key_top[slot] - kSpread || rp.value_low[slot] < rp.value_top[slot] - kSpread)
+                    column_step(i, std::integral_constant<Tile, Tile::kOwn>());
+                else if (start + (i + 1) * kRowsTile > min(lim_first, end) || rp.bad[slot])
+                    column_step(i, std::integral_constant<Tile, Tile::kEdge>());
                 else
-                    column_step(i, std::false_type());
+                    column_step(i, std::integral_constant<Tile, Tile::kPlain>());
                 end_step();
                 if (s_fail) break;
             }
@@ -699,7 +818,8 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
         // ---- the columns' results: each half of the threads half of the dimensions ----
         if (owns) {
             float l0, l1;
-            unpair(l2, l0, l1);
+            unpair(sums.l2, l0, l1);
+            const float m = sums.m, D = sums.D;
             s_top[half][p] = __fadd_rn(l0, l1);
             asm volatile("bar.sync 3, 256;" ::: "memory");
             const float l = __fadd_rn(s_top[0][p], s_top[1][p]);
@@ -708,8 +828,8 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
                 umma::fence_after_sync();
                 if (!ok) atomicOr(c.flags, kCacheWait);
             }
-            // l is in units of 2^kPUp as P is, O of 2^E / 2^kValueUp more
-            const float unit = pow2(max(E, -110) - kValueUp);
+            // l is in units of 2^kPUp, O of 2^D / 2^kValueUp more
+            const float unit = pow2((int)fminf(fmaxf(D, -200.0f), 200.0f) - kValueUp);
             const bool none = n == 0 || l == 0.0f;
             const float inv = none ? 0.0f : kk.parts == 1 ? __fdiv_rn(unit, l) : __fmul_rn(unit, 1.0f / kPScale);
             const size_t at = kk.parts == 1 ? th : (size_t)part * a.tok.n_tokens * a.q_heads + th;

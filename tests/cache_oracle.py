@@ -98,7 +98,7 @@ def attend_head(q, rows, which, scale, dtype):
     return out, lse, p, err, dz + (n + 32) * 2.0 ** -23 + abs(lse) * 2.0 ** -22, p * dp + 2.0 ** -126
 
 
-def attend_head_tight(q, rows, which, scale, dtype):
+def attend_head_tight(q, rows, which, scale, dtype, wide=False):
     """out, lse, p and the error of each, as attend_head, with every row's error by its own magnitude.
 
     A score's error is that of its own sum, (dim + 16) roundings of 2^-23 of scale * sum |key| |q| with |key| at most
@@ -106,13 +106,18 @@ def attend_head_tight(q, rows, which, scale, dtype):
     and the exponential's. p * step is rounded to f16 (2^-12) in bf16 calls and to two halves (2^-22) else, in units where
     2^11 is at most the largest p * step of the column and group when it was set: half of f16's 2^-24 adds
     2^-36 of that per row, times a code of 15. Sums over n rows add n roundings of 2^-23.
+
+    wide: blocks of 128 columns. A query's sum meets low and 8 step as two halves, and a key lies up to 2^8 below its
+    tile's unit (2^-20 of the score's magnitudes for both). Values are rounded to f16 as p is (2^-12 each), p in units
+    of the largest p * level, which may be taken 2^9 too large (rows up to 2^8 apart share a unit): 2^-25 / 2^12 * 2^9
+    = 2^-28 of it per row.
     """
     n, d = len(which), len(q)
     q = np.asarray(q, np.float64)
     k, v = rows.k[which], rows.v[which]
     z = scale * (k @ q)
     mag = abs(scale) * ((np.abs(rows.k_low[which]) + 15 * rows.k_step[which]) @ np.abs(q))
-    dz = ((d + 16) * 2.0 ** -23 + (2.0 ** -22 if dtype == "f32" else 2.0 ** -30)) * mag
+    dz = ((d + 16) * 2.0 ** -23 + (2.0 ** -22 if dtype == "f32" else 2.0 ** -30) + (2.0 ** -20 if wide else 0)) * mag
     top = z.max()
     e = np.exp(z - top)
     p = e / e.sum()
@@ -122,8 +127,10 @@ def attend_head_tight(q, rows, which, scale, dtype):
     dp = dp + p @ dp + (n + 32) * 2.0 ** -23
     out = p @ v
     level = 15 * rows.v_step[which] + np.abs(rows.v_low[which])
-    round_p = 2.0 ** -12 if dtype == "bf16" else 2.0 ** -22
+    round_p = 2.0 ** -11 if wide else 2.0 ** -12 if dtype == "bf16" else 2.0 ** -22
     tiny = 15 * n * (2.0 ** -36 * (p[:, None] * rows.v_step[which]).max(axis=0) + 2.0 ** -136)
+    if wide:
+        tiny = tiny + n * 2.0 ** -28 * (p[:, None] * level).max()
     err = (p * (dp + round_p + (n + 64) * 2.0 ** -23)) @ level + tiny
     err = err + UNIT[dtype] * (np.abs(out) + err) + TINY[dtype]
     return out, lse, p, err, p @ dz + (n + 32) * 2.0 ** -23 + abs(lse) * 2.0 ** -22, p * dp + 2.0 ** -126

@@ -117,7 +117,7 @@ def test_attend_queries_and_scales_of_opposite_magnitude(dtype, power, new):
     check_attend(rng, [150], [new], 1, 4, 128, dtype, scale=2.0 ** min(-power - 3, 97), qs=q, capacity=LONG)
 
 
-def check_tight(f, qx, held, new, dtype, only=None):
+def check_tight(f, qx, held, new, dtype, only=None, wide=False):
     """One causal call, a sequence: outputs and log-sum-exps within the bounds by each row's own magnitude."""
     got, lse, flags = check_attend_raw(f, qx, [held], [new], dtype)
     assert flags == 0
@@ -125,7 +125,7 @@ def check_tight(f, qx, held, new, dtype, only=None):
     for i in range(new) if only is None else only:
         for hh in range(qx.shape[1]):
             want, wl, _, err, lerr, _ = O.attend_head_tight(qx[i, hh], f.rows[0][hh // group], list(range(held + i + 1)),
-                                                            qx.shape[2] ** -0.5, dtype)
+                                                            qx.shape[2] ** -0.5, dtype, wide)
             close(got[i, hh], want, err, f"out of token {i}, head {hh}")
             close(lse[i, hh], wl, lerr, f"lse of token {i}, head {hh}")
 
@@ -151,3 +151,78 @@ def test_one_large_value_row_takes_nothing_from_the_others(power, dim, dtype):
             keys[at, 0] = -(20 + 0.7 * power) * base / np.sqrt(dim)  # a score of that: e^-20 after the row's size
         f = Filled(rng, [n], n, 1, dim, dtype, keys, values)
         check_tight(f, q, n - new, new, dtype, only=None if at < n - 1 else range(new - 1))
+
+
+@pytest.mark.parametrize("dim", [40, 64, 128])
+@pytest.mark.parametrize("power", [7, 12, 24, 40, 100])
+@pytest.mark.parametrize("what", ["keys", "values", "both"])
+def test_many_columns_one_large_row_takes_nothing_from_the_others(what, power, dim):
+    """The same in blocks of 128 columns, of a row's keys too: in the first tile, a middle one, the last, and seen by
+    the last token only."""
+    rng = np.random.default_rng(72)
+    n, new = 600, 40
+    size = 2.0 ** -80 if power >= 100 else 1.0
+    base = rng.standard_normal(dim)
+    _, q = rounded((base + 0.3 * rng.standard_normal((new, 4, dim))).astype(np.float32), "bf16")
+    for at in (3, 290, n - new, n - 1):
+        keys, values = tokens(rng, n, 1, dim), tokens(rng, n, 1, dim, 0.1)
+        if at < n - 1:
+            keys[at, 0] = -(20 + 0.7 * power) * base / np.sqrt(dim)
+        if what != "values":
+            keys[at] *= 2.0 ** power / max(1.0, abs(keys[at]).max())
+        if what != "keys":
+            values = (values * size).astype(np.float32)
+            values[at] *= 2.0 ** power
+        f = Filled(rng, [n], LONG, 1, dim, "bf16", keys, values)
+        check_tight(f, q, n - new, new, "bf16", only=(0, 11, new - 2) if at == n - 1 else (0, 25, new - 1), wide=True)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_columns_rows_of_every_size(dim):
+    """Keys and values of rows 10^-9 to 10^9 times the common size, in no order, and values that rise or fall over the
+    tiles: units of their own, a unit that has to grow, and one so large that a tile's weights need another."""
+    rng = np.random.default_rng(73)
+    n, new = 700, 40
+    _, q = rounded(rng.standard_normal((new, 4, dim)).astype(np.float32), "bf16")
+    sizes = [10.0 ** rng.uniform(-9, 9, n), 10.0 ** np.linspace(-25, 25, n), 10.0 ** np.linspace(25, -25, n),
+             10.0 ** np.repeat([-30, 30, -30, 0, -30, 30, -30], 100), np.repeat([0, 1, 0, 1e-30, 0, 0, 1], 100)]
+    for k_size in (np.ones(n), 10.0 ** rng.uniform(-9, 0, n), 10.0 ** np.linspace(-12, 0.5, n)):
+        for v_size in sizes:
+            keys = (tokens(rng, n, 1, dim) * k_size[:, None, None]).astype(np.float32)
+            values = (tokens(rng, n, 1, dim, 0.1) * v_size[:, None, None]).astype(np.float32)
+            f = Filled(rng, [n], LONG, 1, dim, "bf16", keys, values)
+            check_tight(f, q, n - new, new, "bf16", only=(0, 19, new - 1), wide=True)
+
+
+@pytest.mark.parametrize("new", [2, 40])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_value_rows_of_the_lowest_number_without_weight(dtype, new):
+    """Value rows at the end of the type's range whose weight underflows, constant and beside zeros."""
+    rng = np.random.default_rng(74)
+    n, dim = 400, 128
+    base = rng.standard_normal(dim)
+    _, q = rounded((base + 0.3 * rng.standard_normal((new, 4, dim))).astype(np.float32), dtype)
+    keys, values = tokens(rng, n, 1, dim), tokens(rng, n, 1, dim, 0.1)
+    for at, low in ((1, -3.38e38), (170, -3.38e38), (300, 3.38e38)):
+        keys[at, 0] = -200 * base / np.sqrt(dim)
+        values[at] = low
+        values[at, 0, 3:70] = 0.0
+    f = Filled(rng, [n], LONG, 1, dim, dtype, keys, values)
+    assert np.abs(f.rows[0][0].v[1]).max() > 3e38
+    check_tight(f, q, n - new, new, dtype, only=(0, new - 1), wide=new == 40 and dtype == "bf16")
+
+
+def test_many_columns_rows_that_are_not_finite_among_rows_of_every_size():
+    """NaN values and keys in tiles whose rows have units of their own: columns that see them are NaN, others right."""
+    rng = np.random.default_rng(75)
+    n, new, dim = 500, 40, 128
+    _, q = rounded(rng.standard_normal((new, 4, dim)).astype(np.float32), "bf16")
+    keys = tokens(rng, n, 1, dim) * 10.0 ** rng.uniform(-6, 0.3, (n, 1, 1))
+    values = tokens(rng, n, 1, dim, 0.1) * 10.0 ** rng.uniform(-6, 6, (n, 1, 1))
+    values[n - new + 15, 0, 9] = np.nan   # token 15 and those behind it see it
+    keys[n - new + 30, 0, 100] = np.inf
+    f = Filled(rng, [n], LONG, 1, dim, "bf16", keys.astype(np.float32), values.astype(np.float32))
+    got, lse, flags = check_attend_raw(f, q, [n - new], [new], "bf16")
+    assert flags == 0 and np.isnan(got[15:]).all() and np.isfinite(got[:15]).all()
+    assert np.isfinite(lse[:30]).all() and np.isnan(lse[30:]).all()
+    check_tight(f, q, n - new, new, "bf16", only=(0, 7, 14), wide=True)
