@@ -22,8 +22,8 @@
 // Bound by the issue of instructions and the latencies between a step's barriers: 11,900 warp instructions a tile of
 // G = 2, 3,000 clocks a scheduler at best; a tile takes 4,500 clocks, the products' arithmetic 1,100 of them.
 // Chunks of 32 to 64 tokens over 4 sequences of 20,000 to 32,000 rows, 8 heads of 128 with 4 query heads each:
-// 243 us, 78 GFLOP, a fifth of the tensor cores' rate (with the columns' padding to 128 a third). Where every
-// tile's rows have units of their own, 2.4 times as long (257 us for 107, 32 tokens over four times 20,000 rows). On the way
+// 244 us, 78 GFLOP, a fifth of the tensor cores' rate (with the columns' padding to 128 a third). Where every
+// tile's rows have units of their own, 2.5 times as long (270 us for 107, 32 tokens over four times 20,000 rows). On the way
 // there, in 18 parts of the rows (258 at the end): bounds on every load of a tile's codes 406 us; 16 warps, where
 // the same warps decoded keys and values, 394; scores 32 at a time, with their spills, 284; whole lines of codes
 // exchanged in shared memory 447 (for 388 at that time).
@@ -394,6 +394,10 @@ struct ColumnSums {
     float m, D;
     f2 l2;
 };
+struct OwnSums {
+    ColumnSums c;
+    bool ok;  // no wait ran out
+};
 // Where a column's thread finds things: the tensor memory of its scores, its P and its half of O, the barrier and the
 // phase of the P V before (first: there is none).
 struct ColumnPlace {
@@ -439,8 +443,8 @@ __device__ __forceinline__ bool settle(ColumnSums& c, const ColumnPlace& at, flo
 // A column's 64 rows of a tile whose rows have units of their own. Out of line: inlined, it took registers from
 // the common forms (262 us for 234, chunks of 32 to 64 tokens over four times 20,000 to 32,000 rows).
 template <int G>
-__device__ __noinline__ ColumnSums own_step(ColumnSums c, ColumnPlace at, const RowParams<G>* rp, int slot, int half, int p, int vis,
-                                            float f, float (*s_top)[kWideCols], float (*s_most)[kWideCols], float* logits, int* fail) {
+__device__ __noinline__ OwnSums own_step(ColumnSums c, ColumnPlace at, const RowParams<G>* rp, int slot, int half, int p, int vis,
+                                            float f, float (*s_top)[kWideCols], float (*s_most)[kWideCols], float* logits) {
     const float* const key_unit = rp->key_unit[slot] + 64 * half;
     const float* const value_exp = rp->value_exp[slot] + 64 * half;
     const float* const poison = rp->poison[slot] + 64 * half;
@@ -458,7 +462,7 @@ __device__ __noinline__ ColumnSums own_step(ColumnSums c, ColumnPlace at, const 
     }
     s_top[half][p] = top, s_most[half][p] = most;
     asm volatile("bar.sync 3, 256;" ::: "memory");
-    if (!settle<G>(c, at, fmaxf(s_top[0][p], s_top[1][p]), fmaxf(s_most[0][p], s_most[1][p]), false)) *fail = 1;
+    const bool ok = settle<G>(c, at, fmaxf(s_top[0][p], s_top[1][p]), fmaxf(s_most[0][p], s_most[1][p]), false);
     float l = 0.0f;
 #pragma unroll 1
     for (int y = 0; y < 64; y += 16) {
@@ -481,7 +485,7 @@ __device__ __noinline__ ColumnSums own_step(ColumnSums c, ColumnPlace at, const 
         tmem_st8(at.p_at + y / 2, out);
     }
     c.l2 = add2(c.l2, pair(l, 0.0f));
-    return c;
+    return {c, ok};
 }
 
 template <int G>
@@ -495,7 +499,7 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
     __shared__ float s_top[2][kWideCols], s_most[2][kWideCols], s_sum[2][G][kWideCols];
     __shared__ uint64_t bar_s[2], bar_o;
     __shared__ uint32_t s_tmem;
-    __shared__ int s_fail;
+    __shared__ int s_fail;  // 1 + the step in which a wait ran out
     char* sq = s_raw + (-umma::smem_addr(s_raw) & 1023u);  // an offset, so that the stores stay shared memory's
     char* sk = sq + W::kQBytes;
     char* sv = sk + 2 * W::kKBytes;
@@ -566,6 +570,12 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
             umma::fence_before_sync();
             asm volatile("bar.sync 0;" ::: "memory");
         };
+        // Every thread leaves after the same step: a thread ahead may have failed in the next one already, which those
+        // still here have to enter, or its barrier would miss them.
+        auto failed = [&](int i) {
+            const int f = s_fail;  // (read after the barrier, which clobbers memory)
+            return f != 0 && f <= i + 1;
+        };
         auto issue_values = [&](int i) {
             const uint64_t vd = umma::desc_k_sw128(umma::smem_addr(sv)) + (i & 1) * (W::kVBytes >> 4);
 #pragma unroll
@@ -594,7 +604,7 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
                     if (i + 2 < n) issue_scores(i + 2);
                 }
                 __syncwarp();
-                if (s_fail) break;
+                if (failed(i)) break;
             }
         } else if (decodes_keys) {
             KeyCodes<G> keys;
@@ -619,13 +629,13 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
                     if (p == 0) rp.key_top[(i + 3) & 3] = kNoExp, rp.key_low[(i + 3) & 3] = kNoLow;  // last read in the step before
                     const int unit = find_key_unit<G>(keys, &rp, i + 2, p);
                     // S of this tile has read the buffer that these keys go to
-                    if (!wait_for(&bar_s[(done + i) & 1], ((done + i) >> 1) & 1)) s_fail = 1;
+                    if (!wait_for(&bar_s[(done + i) & 1], ((done + i) >> 1) & 1)) s_fail = i + 1;
                     decode_keys<G>(keys, sk + (i & 1) * W::kKBytes, unit, p);
                     if (i + 3 < n) source.next(keys);
                 }
                 umma::fence_smem_to_async();
                 end_step();
-                if (s_fail) break;
+                if (failed(i)) break;
             }
         } else if (!owns) {
             ValueCodes<G> values;
@@ -645,13 +655,13 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
                     if (p == 0) rp.value_top[(i + 2) & 3] = kNoExp, rp.value_low[(i + 2) & 3] = kNoLow, rp.bad[(i + 2) & 3] = 0;
                     find_value_unit<G>(values, &rp, i + 1, p);
                     // P V of the tile before has read the buffer that these values go to
-                    if (i > 0 && !wait_for(&bar_o, (done + i - 1) & 1)) s_fail = 1;
+                    if (i > 0 && !wait_for(&bar_o, (done + i - 1) & 1)) s_fail = i + 1;
                     decode_values<G>(values, sv + ((i + 1) & 1) * W::kVBytes, &rp, p);
                     if (i + 2 < n) source.next(values);
                 }
                 umma::fence_smem_to_async();
                 end_step();
-                if (s_fail) break;
+                if (failed(i)) break;
             }
         } else {
             // each of a column's threads takes every second word of eight dimensions; maxima and sums are exchanged
@@ -728,7 +738,8 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
                 const float f = __fmul_rn(fac, pow2(max(rp.key_top[slot], kKeyLeast) - kKeyUp));
                 float* const lg = kk.logits && in ? kk.logits + th * kk.logit_rows + row0 : nullptr;
                 if constexpr (kOwn) {
-                    sums = own_step<G>(sums, at, &rp, slot, half, p, vis, f, s_top, s_most, lg, &s_fail);
+                    const OwnSums r = own_step<G>(sums, at, &rp, slot, half, p, vis, f, s_top, s_most, lg);
+                    sums = r.c, ok = r.ok && ok;
                 } else {
                     float top = -INFINITY;
 #pragma unroll
@@ -800,7 +811,7 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
                 // P V of the tile before, whose place of P the next tile takes. Every phase is waited for in turn: a
                 // wait for one that another has followed would not end.
                 if (i > 0) ok = wait_for(&bar_o, (done + i - 1) & 1) && ok;
-                if (!ok) s_fail = 1;
+                if (!ok) s_fail = i + 1;
             };
 
             for (int i = 0; i < n; ++i) {
@@ -812,7 +823,7 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
                 else
                     column_step(i, std::integral_constant<Tile, Tile::kPlain>());
                 end_step();
-                if (s_fail) break;
+                if (failed(i)) break;
             }
         }
         // ---- the columns' results: each half of the threads half of the dimensions ----
