@@ -280,7 +280,9 @@ int maivs_concurrent_array(maivs_concurrent* cx, long long segment, const char* 
  * (int32, n_seqs + 1 of them, ascending within 0..n_tokens); d_lengths[s] (int32) is the number of
  * rows it held before this step. Tokens before the first or behind the last sequence are padding:
  * nothing is read or written for them. A call takes at most 2^27 tokens, and 2^30 query heads of them
- * together. Row tables (weights f32, ids u64) are [n_seqs][capacity].
+ * together. Offsets that do not ascend within 0..n_tokens set flag 4: their sequences are skipped, and tokens
+ * of others may be; nothing outside the tensors is touched. Row tables (weights f32, ids u64) are
+ * [n_seqs][capacity].
  * dtype is that of keys, values, queries and outputs. A stride counts elements from token to token
  * (0: packed); a token's heads are adjacent. */
 typedef struct maivs_cache maivs_cache;
@@ -315,7 +317,7 @@ int maivs_cache_read(maivs_cache* cx, void* d_keys, void* d_values, int dtype, s
  * row below d_lengths[s] for a sequence without tokens); other entries are left as they are.
  * max_rows (0: capacity) bounds the rows of a sequence: a longer one is read up to it and sets flag
  * 2. max_tokens (0: n_tokens) is the expected number of tokens of a sequence; it only sizes the
- * launch. Offsets that do not ascend within 0..n_tokens set flag 4; those sequences are skipped. Flag 8:
+ * launch. Flag 8:
  * a bounded wait of the kernel for many columns ran out, and the call's results are invalid. A value row that
  * is not finite makes the outputs that see it NaN, at least in its groups of 64 dimensions. |scale| is at
  * most 2^100, and a query whose largest element times scale passes that gives NaN. d_out overlaps no input. */

@@ -80,13 +80,14 @@ __device__ __forceinline__ void write_out(void* out, int type, size_t i, float x
 // Rows of a sequence that its last token sees, and the number of its tokens.
 struct Span {
     int first, count, len;
+    bool good;  // its offsets ascend within the call's tokens (if not: no tokens)
 };
 __device__ __forceinline__ Span span_of(const CacheView& c, const AttendArgs& a, int s) {
     Span p;
     const int lo = __ldg(a.tok.offsets + s), hi = __ldg(a.tok.offsets + s + 1);
-    const bool good = lo >= 0 && hi >= lo && hi <= a.tok.n_tokens;
+    p.good = good_offsets(lo, hi, a.tok.n_tokens);
     p.first = lo;
-    p.count = good ? hi - lo : 0;
+    p.count = p.good ? hi - lo : 0;
     p.len = min(max(__ldg(a.tok.lengths + s), 0), c.capacity);
     return p;
 }

@@ -68,11 +68,22 @@ __device__ __forceinline__ f2 add2(f2 a, f2 b) {
     return r;
 }
 
+// Whether a sequence's tokens lo .. hi - 1 ascend within the call's.
+__device__ __forceinline__ bool good_offsets(int lo, int hi, int n_tokens) { return lo >= 0 && hi >= lo && hi <= n_tokens; }
+
+// Sets `bit` of *flags where some sequence's do not; the threads of one block share the sequences.
+__device__ __forceinline__ void check_offsets(const int32_t* __restrict__ off, int n_seqs, int n_tokens, uint32_t* flags,
+                                              uint32_t bit) {
+    bool bad = false;
+    for (int s = threadIdx.x; s < n_seqs; s += blockDim.x) bad |= !good_offsets(__ldg(off + s), __ldg(off + s + 1), n_tokens);
+    if (bad) atomicOr(flags, bit);
+}
+
 // The sequence of packed token `tok`: offsets[s] <= tok < offsets[s + 1], or -1 for a token before
 // the first or behind the last sequence. Called by an aligned group of 8 lanes (lane8, mask), which
 // count the starts at or below tok together: one round of loads per 8 sequences, none dependent;
 // above 512 sequences every lane bisects instead.
-__device__ __forceinline__ int find_sequence(const int32_t* __restrict__ off, int n_seqs, int tok, int lane8,
+__device__ __forceinline__ int find_sequence(const int32_t* __restrict__ off, int n_seqs, int n_tokens, int tok, int lane8,
                                              unsigned mask) {
     int s;
     if (n_seqs <= 512) {
@@ -94,8 +105,9 @@ __device__ __forceinline__ int find_sequence(const int32_t* __restrict__ off, in
         s = lo - 1;
     }
     if (s < 0 || s >= n_seqs) return -1;
-    // offsets that do not ascend map a token nowhere rather than to a wrong row
-    return __ldg(off + s) <= tok && tok < __ldg(off + s + 1) ? s : -1;
+    // offsets that do not ascend, or leave the call's tokens, map a token nowhere rather than to a wrong row
+    const int lo = __ldg(off + s), hi = __ldg(off + s + 1);
+    return good_offsets(lo, hi, n_tokens) && lo <= tok && tok < hi ? s : -1;
 }
 
 // Launches the second kernel of a pair: its blocks may be set up while the first still runs (the first says

@@ -43,7 +43,7 @@ struct Place {
 __device__ __forceinline__ Place place_of(const CacheView& c, const CacheTokens& tk, int tok, int lane8, unsigned mask) {
     Place p{-1, -1};
     if (tok >= tk.n_tokens) return p;
-    p.seq = find_sequence(tk.offsets, c.n_seqs, tok, lane8, mask);
+    p.seq = find_sequence(tk.offsets, c.n_seqs, tk.n_tokens, tok, lane8, mask);
     if (p.seq < 0) return p;
     const long long row =
         (long long)min(max(__ldg(tk.lengths + p.seq), 0), c.capacity) + (tok - __ldg(tk.offsets + p.seq));
@@ -257,6 +257,7 @@ __device__ __forceinline__ void find_places(const CacheView& c, const CacheToken
                                             const uint64_t* token_ids) {
     const int l8 = threadIdx.x % kUnit;
     const unsigned mask = 0xFFu << (threadIdx.x % 32 / kUnit * kUnit);
+    if (blockIdx.x == 0 && blockIdx.y == 0) check_offsets(tk.offsets, c.n_seqs, tk.n_tokens, c.flags, kCacheOffsets);
     for (int i = threadIdx.x / kUnit; i < n_tok; i += kUnits) {
         const Place p = place_of(c, tk, tok0 + i, l8, mask);
         if (l8 == 0) {

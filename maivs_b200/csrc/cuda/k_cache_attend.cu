@@ -318,13 +318,14 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, TYPE == kF32, (MODE >= Mo
     b /= kk.parts;
     const int h = b % c.heads;
     const int item = b / c.heads;  // sequence, or token of a found list
+    if (FOUND && blockIdx.x == 0) check_offsets(a.tok.offsets, c.n_seqs, a.tok.n_tokens, c.flags, kCacheOffsets);
     if (kSolo && item >= a.tok.n_tokens) return;
 
     Span sn;
     int s, cols, rows_all;
     if (FOUND) {
         const unsigned m8 = 0xFFu << (lane / 8 * 8);
-        s = find_sequence(a.tok.offsets, c.n_seqs, item, lane & 7, m8);
+        s = find_sequence(a.tok.offsets, c.n_seqs, a.tok.n_tokens, item, lane & 7, m8);
         if (s < 0) return;
         sn = span_of(c, a, s);
         cols = a.group;
@@ -335,8 +336,7 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, TYPE == kF32, (MODE >= Mo
         cols = sn.count * a.group;
         rows_all = sn.count ? visible(c, a, sn.len, sn.count - 1) : 0;
         if (threadIdx.x == 0 && h == 0 && part == 0 && rank == 0 && ct0 == 0) {
-            const int lo = __ldg(a.tok.offsets + s), hi = __ldg(a.tok.offsets + s + 1);
-            if (lo < 0 || hi < lo || hi > a.tok.n_tokens) atomicOr(c.flags, kCacheOffsets);
+            if (!sn.good) atomicOr(c.flags, kCacheOffsets);
             if (sn.count && min(sn.len + (a.causal ? sn.count : 0), c.capacity) > a.max_rows)
                 atomicOr(c.flags, kCacheTooLong);
         }
@@ -914,7 +914,7 @@ __global__ void __launch_bounds__(kJoinBS) k_cache_join(CacheView c, AttendKerne
     const int tk = (int)(th / a.q_heads);
     cudaTriggerProgrammaticLaunchCompletion();
     cudaGridDependencySynchronize();
-    const int s = find_sequence(a.tok.offsets, c.n_seqs, tk, lane & 7, 0xFFu << (lane / 8 * 8));
+    const int s = find_sequence(a.tok.offsets, c.n_seqs, a.tok.n_tokens, tk, lane & 7, 0xFFu << (lane / 8 * 8));
     if (s < 0) return;
     const Span sn = span_of(c, a, s);
     if (sn.count == 0) return;
@@ -979,6 +979,10 @@ __global__ void __launch_bounds__(256) k_cache_weights(CacheView c, AttendKernel
     cudaGridDependencySynchronize();
     const int s = blockIdx.y;
     const Span sn = span_of(c, a, s);
+    if (!sn.good) {  // a call without tokens has no other kernel that says so
+        if (blockIdx.x == 0 && threadIdx.x == 0) atomicOr(c.flags, kCacheOffsets);
+        return;
+    }
     const int rows = min(sn.len + (a.causal ? sn.count : 0), c.capacity);
     for (int r = blockIdx.x * 256 + threadIdx.x; r < rows; r += gridDim.x * 256) {
         float sum = 0.0f;
@@ -999,7 +1003,7 @@ __global__ void __launch_bounds__(128) k_cache_found_weights(CacheView c, Attend
     cudaGridDependencySynchronize();
     const int blocks = (a.k + 127) / 128;  // of one token
     const int tk = blockIdx.x / blocks, lane = threadIdx.x & 31;
-    const int s = find_sequence(a.tok.offsets, c.n_seqs, tk, lane & 7, 0xFFu << (lane / 8 * 8));
+    const int s = find_sequence(a.tok.offsets, c.n_seqs, a.tok.n_tokens, tk, lane & 7, 0xFFu << (lane / 8 * 8));
     if (s < 0) return;
     const size_t th = (size_t)tk * a.q_heads;
     const int e = (blockIdx.x - tk * blocks) * 128 + threadIdx.x;

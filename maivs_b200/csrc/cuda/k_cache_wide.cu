@@ -518,8 +518,7 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
     const int cols = sn.count * a.group;
     const int rows_all = sn.count ? visible(c, a, sn.len, sn.count - 1) : 0;
     if (threadIdx.x == 0 && h == 0 && part == 0 && ct0 == 0) {
-        const int lo = __ldg(a.tok.offsets + s), hi = __ldg(a.tok.offsets + s + 1);
-        if (lo < 0 || hi < lo || hi > a.tok.n_tokens) atomicOr(c.flags, kCacheOffsets);
+        if (!sn.good) atomicOr(c.flags, kCacheOffsets);
         if (sn.count && min(sn.len + (a.causal ? sn.count : 0), c.capacity) > a.max_rows)
             atomicOr(c.flags, kCacheTooLong);
     }

@@ -226,3 +226,61 @@ def test_many_columns_rows_that_are_not_finite_among_rows_of_every_size():
     assert flags == 0 and np.isnan(got[15:]).all() and np.isfinite(got[:15]).all()
     assert np.isfinite(lse[:30]).all() and np.isnan(lse[30:]).all()
     check_tight(f, q, n - new, new, "bf16", only=(0, 7, 14), wide=True)
+
+
+# ---- offsets --------------------------------------------------------------------------------------
+@pytest.mark.parametrize("bad", [[0, 9, 8], [-3, 4, 8], [0, 1 << 30, 8], [0, 4, 9], [0, 4, 2]])
+def test_offsets_out_of_order_are_flagged_and_skipped(bad):
+    """By every call on tokens; nothing is read or written for the sequences concerned, their weights included."""
+    rng = np.random.default_rng(81)
+    t, heads, dim, cap = 8, 2, 64, 12
+    x = torch.tensor(tokens(rng, t, heads, dim)).cuda()
+    c = M.AttentionCache(2, cap, heads, dim)
+    full = torch.tensor(tokens(rng, 2 * cap, heads, dim)).cuda()
+    c.append(full.data_ptr(), full.data_ptr(), 2 * cap, offsets([cap, cap]).data_ptr(), i32([0, 0]).data_ptr(), dtype="f32",
+             stream=stream())
+    off, ln = i32(bad), i32([3, 3])
+    skipped = [s for s in range(2) if not 0 <= bad[s] <= bad[s + 1] <= t]
+    kept = [s for s in range(2) if s not in skipped]
+    assert skipped and c.flags(stream()) == 0
+
+    def rows(s):
+        k, v = torch.empty(cap, heads, dim, device="cuda"), torch.empty(cap, heads, dim, device="cuda")
+        one = i32([0, cap, cap] if s == 0 else [0, 0, cap])
+        c.read(k.data_ptr(), v.data_ptr(), cap, one.data_ptr(), i32([0, 0]).data_ptr(), dtype="f32", stream=stream())
+        return k.cpu()
+
+    before = [rows(s) for s in range(2)]
+    w = torch.full((2, cap), 3.0, device="cuda")
+    c.append(x.data_ptr(), x.data_ptr(), t, off.data_ptr(), ln.data_ptr(), dtype="f32", d_weights=w.data_ptr(), stream=stream())
+    assert c.flags(stream()) == 4
+    for s in skipped:
+        assert torch.equal(rows(s), before[s]) and (w[s] == 3).all()
+    k, v = torch.full_like(x, 7.0), torch.full_like(x, 7.0)
+    c.read(k.data_ptr(), v.data_ptr(), t, off.data_ptr(), ln.data_ptr(), dtype="f32", stream=stream())
+    assert c.flags(stream()) == 4
+    # (tokens between the two offsets of a skipped sequence may be skipped with it)
+    others = [i for i in range(t) if not any(bad[s] <= i < bad[s + 1] for s in kept)]
+    mine = [i for i in range(t) if i not in others and not any(bad[s + 1] <= i < bad[s] for s in skipped)]
+    assert (k[others] == 7).all() and (v[others] == 7).all() and (k[mine] != 7).all()
+    out = torch.full((t, heads, dim), 7.0, device="cuda")
+    w_in, w_out = torch.full((2, cap), 2.0, device="cuda"), torch.full((2, cap), 7.0, device="cuda")
+    ws = torch.empty(c.attend_workspace(t, heads, weights=True), dtype=torch.uint8, device="cuda")
+    c.attend(x.data_ptr(), t, heads, off.data_ptr(), ln.data_ptr(), out.data_ptr(), dtype="f32", decay=0.5,
+             d_weights_in=w_in.data_ptr(), d_weights_out=w_out.data_ptr(), d_workspace=ws.data_ptr(), workspace_bytes=ws.numel(),
+             stream=stream())
+    assert c.flags(stream()) == 4 and (out[others] == 7).all()
+    assert (w_out[skipped] == 7).all() and all((w_out[s, :3] != 7).all() for s in kept)
+    list_ = torch.zeros(t, 5, dtype=torch.int64, device="cuda")
+    out.fill_(7.0)
+    fw = torch.full((t, 5), 7.0, device="cuda")
+    ws = torch.empty(c.attend_found_workspace(t, heads, 5), dtype=torch.uint8, device="cuda")
+    c.attend_found(x.data_ptr(), t, heads, off.data_ptr(), ln.data_ptr(), list_.data_ptr(), 5, out.data_ptr(), dtype="f32",
+                   d_weights=fw.data_ptr(), d_workspace=ws.data_ptr(), workspace_bytes=ws.numel(), stream=stream())
+    assert c.flags(stream()) == 4 and (out[others] == 7).all() and (fw[others] == 7).all() and (out[mine] != 7).all()
+    # a call without tokens, which may still age the weights
+    w_out.fill_(7.0)
+    zero = i32([0, 1, 0])
+    c.attend(0, 0, heads, zero.data_ptr(), ln.data_ptr(), 0, dtype="f32", decay=0.5, d_weights_in=w_in.data_ptr(),
+             d_weights_out=w_out.data_ptr(), stream=stream())
+    assert c.flags(stream()) == 4 and (w_out == 7).all()
