@@ -606,10 +606,12 @@ def _cache_dtype(dtype: str) -> int:
     return _CACHE_DTYPES[dtype]
 
 
-def _size(x, name: str) -> int:
+def _size(x, name: str, bits: int = 64) -> int:
     x = int(x)
     if x < 0:
         raise ValueError(f"{name} must not be negative")
+    if x >> bits:  # ctypes would drop the upper bits
+        raise ValueError(f"{name} must be below 2^{bits}")
     return x
 
 
@@ -632,7 +634,7 @@ class AttentionCache:
         self._h = None
         self._free = L.maivs_cache_free  # still there when the interpreter takes the module down
         rc = L.maivs_cache_new(_size(n_seqs, "n_seqs"), _size(capacity, "capacity"), _size(n_heads, "n_heads"),
-                               _size(dim, "dim"), -1 if device is None else _size(device, "device"), C.byref(h))
+                               _size(dim, "dim"), -1 if device is None else _size(device, "device", 31), C.byref(h))
         self._h = h
         self._dim = int(dim)
         if rc != _lib.OK:
