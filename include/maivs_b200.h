@@ -296,7 +296,8 @@ int maivs_cache_new(size_t n_seqs, size_t capacity, size_t n_heads, size_t dim, 
 void maivs_cache_free(maivs_cache* cx);
 const char* maivs_cache_last_error(maivs_cache* cx);
 /* "n_seqs", "capacity", "n_heads", "dim", "device", "device_bytes", "row_bytes" (key and value of one
- * row of one head) */
+ * row of one head), "block_columns" (query columns, tokens times query heads of one cache head, that a block of the
+ * last attend or attend_found took: 8, 16 or 128) */
 int maivs_cache_stat(maivs_cache* cx, const char* name, double* value);
 /* Token i of sequence s becomes row d_lengths[s] + i - d_offsets[s] (keys and values
  * [n_tokens][n_heads][dim]). Rows past the capacity are left out and set flag 1. The new rows'

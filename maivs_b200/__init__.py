@@ -739,7 +739,7 @@ class AttentionCache:
         self._check(_lib.lib().maivs_cache_flags(self._h, stream, C.byref(f)))
         return int(f.value)
 
-    _STATS = ("n_seqs", "capacity", "n_heads", "dim", "device", "device_bytes", "row_bytes")
+    _STATS = ("n_seqs", "capacity", "n_heads", "dim", "device", "device_bytes", "row_bytes", "block_columns")
 
     def stats(self) -> dict:
         out = {}

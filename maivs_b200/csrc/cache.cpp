@@ -24,6 +24,7 @@ struct maivs_cache {
     int device = -1;  // -1: no storage, sizes and argument checks only
     void* mem = nullptr;
     size_t bytes = 0;
+    int columns = 0;  // of a block of the last attend or attend_found
     std::string err;
     std::mutex mu;
 };
@@ -229,6 +230,7 @@ int maivs_cache_stat(maivs_cache* cx, const char* name, double* value) {
         if (!std::strcmp(name, "row_bytes")) return *value = 72.0 * v.G, MAIVS_OK;
         if (!std::strcmp(name, "device_bytes")) return *value = (double)cx->bytes, MAIVS_OK;
         if (!std::strcmp(name, "device")) return *value = cx->device, MAIVS_OK;
+        if (!std::strcmp(name, "block_columns")) return *value = cx->columns, MAIVS_OK;
         return cfail(cx, MAIVS_NOT_FOUND, std::string("no such value: ") + name);
     });
 }
@@ -345,7 +347,7 @@ int maivs_cache_attend(maivs_cache* cx, const void* d_queries, int dtype, size_t
         OnDevice d(cx->device < 0 ? 0 : cx->device);
         e = check_workspace(ws, maivs::dev::cache_attend_workspace(cx->v, a));
         if (!e.empty()) return cfail(cx, MAIVS_BAD_ARG, e);
-        return on_device(cx, [&] { maivs::dev::launch_cache_attend(cx->v, a, (cudaStream_t)stream); });
+        return on_device(cx, [&] { cx->columns = maivs::dev::launch_cache_attend(cx->v, a, (cudaStream_t)stream); });
     });
 }
 
@@ -375,7 +377,7 @@ int maivs_cache_attend_found(maivs_cache* cx, const void* d_queries, int dtype, 
         OnDevice d(cx->device < 0 ? 0 : cx->device);
         e = check_workspace(ws, maivs::dev::cache_attend_workspace(cx->v, a));
         if (!e.empty()) return cfail(cx, MAIVS_BAD_ARG, e);
-        return on_device(cx, [&] { maivs::dev::launch_cache_attend(cx->v, a, (cudaStream_t)stream); });
+        return on_device(cx, [&] { cx->columns = maivs::dev::launch_cache_attend(cx->v, a, (cudaStream_t)stream); });
     });
 }
 

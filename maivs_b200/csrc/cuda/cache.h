@@ -89,7 +89,8 @@ struct AttendArgs {
 size_t cache_attend_workspace(const CacheView& c, const AttendArgs& a);
 // Blocks of its grid (a launch takes at most 2^31 - 1).
 long long cache_attend_blocks(const CacheView& c, const AttendArgs& a);
-void launch_cache_attend(const CacheView& c, const AttendArgs& a, cudaStream_t st);
+// Returns the query columns that a block of it takes (0: nothing was launched over columns).
+int launch_cache_attend(const CacheView& c, const AttendArgs& a, cudaStream_t st);
 
 struct EvictArgs {
     const int32_t* lengths;

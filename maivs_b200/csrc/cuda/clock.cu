@@ -51,7 +51,7 @@ const char* kernel_name(int id) {
                                              "k_seed_finish", "k_local_list", "k_merge_topk", "k_scan_mma",
                                              "k_seed_scan", "nccl_all_gather", "k_segment_merge", "k_rescore_dots", "k_probe_select",
                                              "k_cache_append", "k_cache_read", "k_cache_attend", "k_cache_join",
-                                             "k_cache_weights", "k_cache_select", "k_cache_move"};
+                                             "k_cache_weights", "k_cache_select", "k_cache_move", "k_cache_wide"};
     return id >= 0 && id < kNumNamed ? names[id] : "?";
 }
 

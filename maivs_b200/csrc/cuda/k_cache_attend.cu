@@ -1135,10 +1135,10 @@ long long cache_attend_blocks(const CacheView& c, const AttendArgs& a) {
     return (long long)(a.k > 0 ? a.tok.n_tokens : c.n_seqs) * c.heads * p.cluster * p.parts * p.col_tiles;
 }
 
-void launch_cache_attend(const CacheView& c, const AttendArgs& a, cudaStream_t st) {
-    if (a.tok.n_tokens <= 0 && !a.w_out) return;
+int launch_cache_attend(const CacheView& c, const AttendArgs& a, cudaStream_t st) {
+    if (a.tok.n_tokens <= 0 && !a.w_out) return 0;
     const bool found = a.k > 0;
-    if (found && a.tok.n_tokens <= 0) return;
+    if (found && a.tok.n_tokens <= 0) return 0;
     const AttendPlan p = make_plan(c, a);
     char* ws = static_cast<char*>(a.workspace);
     AttendKernel k{};
@@ -1159,7 +1159,7 @@ void launch_cache_attend(const CacheView& c, const AttendArgs& a, cudaStream_t s
         const unsigned grid =
             (unsigned)((long long)(found ? a.tok.n_tokens : c.n_seqs) * c.heads * p.cluster * p.parts * p.col_tiles);
         {
-            Tick tk(kKCacheAttend, st);
+            Tick tk(p.wide ? kKCacheWide : kKCacheAttend, st);
             if (p.wide)
                 launch_cache_wide(c, k, grid, st);
             else if (c.G == 1)
@@ -1187,6 +1187,7 @@ void launch_cache_attend(const CacheView& c, const AttendArgs& a, cudaStream_t s
         else
             launch_after(k_cache_weights, dim3((std::min(a.max_rows, c.capacity) + 255) / 256, c.n_seqs), 256, st, c, k);
     }
+    return a.tok.n_tokens > 0 ? p.nc : 0;
 }
 
 }  // namespace dev

@@ -67,6 +67,7 @@ enum KernelId : int {
     kKScanMma, kKSeedScan, kKAllGather, kKSegMerge, kKRescoreDots, kKProbeSelect, kNumKernels,
     // the attention cache's kernels: named and counted, but no index's clock times them
     kKCacheAppend = kNumKernels, kKCacheRead, kKCacheAttend, kKCacheJoin, kKCacheWeights, kKCacheSelect, kKCacheMove,
+    kKCacheWide,
     kNumNamed
 };
 const char* kernel_name(int id);

@@ -120,7 +120,7 @@ def test_attend_queries_and_scales_of_opposite_magnitude(dtype, power, new):
 def check_tight(f, qx, held, new, dtype, only=None, wide=False):
     """One causal call, a sequence: outputs and log-sum-exps within the bounds by each row's own magnitude."""
     got, lse, flags = check_attend_raw(f, qx, [held], [new], dtype)
-    assert flags == 0
+    assert flags == 0 and (columns(f) == 128) == wide
     group = qx.shape[1] // f.heads
     for i in range(new) if only is None else only:
         for hh in range(qx.shape[1]):
@@ -284,3 +284,58 @@ def test_offsets_out_of_order_are_flagged_and_skipped(bad):
     c.attend(0, 0, heads, zero.data_ptr(), ln.data_ptr(), 0, dtype="f32", decay=0.5, d_weights_in=w_in.data_ptr(),
              d_weights_out=w_out.data_ptr(), stream=stream())
     assert c.flags(stream()) == 4 and (w_out == 7).all()
+
+
+# ---- blocks of 128 columns: each test says that they ran ------------------------------------------
+def columns(f):
+    return f.cache.stats()["block_columns"]
+
+
+@pytest.mark.parametrize("dim", [61, 70, 100, 127])
+def test_many_columns_dims_of_no_whole_pieces(dim):
+    """Outputs, and parts of long rows, that are stored element by element."""
+    rng = np.random.default_rng(91)
+    for held, new in (([300, 40], [33, 40]), ([1500], [40])):
+        total = [h + n for h, n in zip(held, new)]
+        f = Filled(rng, total, LONG, 1, dim, "bf16")
+        check_attend(rng, held, new, 1, 4, dim, "bf16", fill=f, capacity=LONG, weights=True)
+        assert columns(f) == 128
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 2.0, 1e-6])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_columns_scales(dim, scale):
+    rng = np.random.default_rng(92)
+    f = Filled(rng, [330], LONG, 1, dim, "bf16")
+    check_attend(rng, [290], [40], 1, 4, dim, "bf16", fill=f, scale=scale, capacity=LONG, weights=True)
+    assert columns(f) == 128
+
+
+@pytest.mark.parametrize("dim", [40, 64, 128])
+def test_blocks_of_many_columns_non_finite_queries(dim):
+    """A column whose query is not finite is NaN; its neighbours, and the other half of its rows, are right."""
+    rng = np.random.default_rng(93)
+    n, new = 400, 40
+    _, q = rounded(rng.standard_normal((new, 4, dim)).astype(np.float32), "bf16")
+    good = q.copy()
+    q[3, 1, 5], q[20, 0, 33], q[20, 1, dim - 1], q[39, 3, 0] = np.nan, -np.inf, np.inf, np.nan
+    bad = ~np.isfinite(q).all(axis=2)
+    f = Filled(rng, [n], LONG, 1, dim, "bf16")
+    got, lse, flags = check_attend_raw(f, q, [n - new], [new], "bf16")
+    assert columns(f) == 128 and flags == 0
+    assert np.isnan(got[bad]).all() and np.isnan(lse[bad]).all()
+    want, want_l, _ = check_attend_raw(f, good, [n - new], [new], "bf16")
+    assert np.array_equal(got[~bad], want[~bad]) and np.array_equal(lse[~bad], want_l[~bad])
+    check_tight(f, good, n - new, new, "bf16", only=(3, 20, 39), wide=True)
+
+
+def test_which_form_runs():
+    """Few columns in blocks of 8 or 16, many in blocks of 128; the widths that the tests above mean to reach."""
+    rng = np.random.default_rng(94)
+    for dtype, dim, new, group, want in (("bf16", 128, 1, 4, 8), ("bf16", 128, 3, 4, 16), ("bf16", 128, 40, 4, 128),
+                                         ("bf16", 64, 40, 4, 128), ("bf16", 64, 15, 4, 16), ("f16", 128, 40, 4, 16),
+                                         ("f32", 128, 40, 4, 8), ("bf16", 192, 40, 4, 8)):
+        f = Filled(rng, [60], LONG, 1, dim, dtype)
+        assert columns(f) == 0
+        check_attend_raw(f, rng.standard_normal((new, group, dim)).astype(np.float32), [60 - new], [new], dtype)
+        assert columns(f) == want
