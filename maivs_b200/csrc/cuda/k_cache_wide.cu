@@ -841,7 +841,7 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
             // l is in units of 2^kPUp, O of 2^D / 2^kValueUp more
             const float unit = pow2((int)fminf(fmaxf(D, -200.0f), 200.0f) - kValueUp);
             const bool none = n == 0 || l == 0.0f;
-            const float inv = none ? 0.0f : kk.parts == 1 ? __fdiv_rn(unit, l) : __fmul_rn(unit, 1.0f / kPScale);
+            const float inv = none ? 0.0f : kk.parts == 1 ? __fdiv_rn(1.0f, l) : 1.0f / kPScale;
             const size_t at = kk.parts == 1 ? th : (size_t)part * a.tok.n_tokens * a.q_heads + th;
 #pragma unroll 1
             for (int y = 0; y < G; ++y) {
@@ -851,7 +851,7 @@ __global__ void __launch_bounds__(kWideBS, 1) k_cache_wide(CacheView c, AttendKe
                 if (in) {
                     float o[32];
 #pragma unroll
-                    for (int x = 0; x < 32; ++x) o[x] = none ? 0.0f : __fmul_rn(__uint_as_float(v[x]), inv);
+                    for (int x = 0; x < 32; ++x) o[x] = none ? 0.0f : __fmul_rn(__fmul_rn(__uint_as_float(v[x]), inv), unit);
                     const int d0 = 32 * (half * G + y);
                     if (kk.parts > 1 && c.dim % 4 == 0) {
                         float* dst = kk.part_o + at * c.dim + d0;

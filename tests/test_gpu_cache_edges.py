@@ -228,6 +228,28 @@ def test_many_columns_rows_that_are_not_finite_among_rows_of_every_size():
     check_tight(f, q, n - new, new, "bf16", only=(0, 7, 14), wide=True)
 
 
+@pytest.mark.parametrize("new", [2, 40])
+@pytest.mark.parametrize("mag", [1e-30, 1e-33, 1e-36])
+@pytest.mark.parametrize("n,heads", [(100, 1), (900, 1), (900, 80)])
+def test_tiny_values(n, heads, mag, new):
+    """Values near the end of the normal numbers, rows of all but equal weight, in several parts and,
+    with heads enough, in one."""
+    rng = np.random.default_rng(76)
+    dim = 128
+    _, q = rounded((0.01 * rng.standard_normal((new, 4 * heads, dim))).astype(np.float32), "bf16")
+    values = (np.clip(tokens(rng, n, heads, dim, 0.1), -2, 2) + 4).astype(np.float32) * np.float32(mag)
+    f = Filled(rng, [n], LONG, heads, dim, "bf16", tokens(rng, n, heads, dim), values)
+    got, _, flags = check_attend_raw(f, q, [n - new], [new], "bf16")
+    assert flags == 0
+    for i in (0, new - 1):
+        for hh in (0, 4 * heads - 2):
+            want = O.attend_head_tight(q[i, hh], f.rows[0][hh // 4], list(range(n - new + i + 1)), dim ** -0.5, "bf16")[0]
+            # bf16 keeps 8 bits: a rounded output is off by up to half of 2^-7. p and V have 11 bits (2^-12 each) of a
+            # level of at most 6.2 for values of at least 2 (4 + 2 and 4 - 2), so 2^-11 * 3.1 < 2^-9. Half a step of
+            # p * step's smallest half is 2^-137, times a code of 15.
+            close(got[i, hh], want, np.abs(want) * (2.0 ** -8 + 2.0 ** -9) + 15 * 2.0 ** -136, f"token {i}, head {hh}")
+
+
 # ---- offsets --------------------------------------------------------------------------------------
 @pytest.mark.parametrize("bad", [[0, 9, 8], [-3, 4, 8], [0, 1 << 30, 8], [0, 4, 9], [0, 4, 2]])
 def test_offsets_out_of_order_are_flagged_and_skipped(bad):
