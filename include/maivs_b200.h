@@ -318,8 +318,9 @@ int maivs_cache_read(maivs_cache* cx, void* d_keys, void* d_values, int dtype, s
  * row below d_lengths[s] for a sequence without tokens); other entries are left as they are.
  * max_rows (0: capacity) bounds the rows of a sequence: a longer one is read up to it and sets flag
  * 2. max_tokens (0: n_tokens) is the expected number of tokens of a sequence; it only sizes the
- * launch. Flag 8:
- * a bounded wait of the kernel for many columns ran out, and the call's results are invalid. A value row that
+ * launch, which may change roundings (a decoding step of many sequences is faster with 1). Flag 8:
+ * a bounded wait of the kernel for many columns ran out, and the call's results are invalid. Scores and sums
+ * over rows are f32: keys past 2^96, or values past 2^127 over the number of rows, may overflow them. A value row that
  * is not finite makes the outputs that see it NaN, at least in its groups of 64 dimensions. |scale| is at
  * most 2^100, and a query whose largest element times scale passes that gives NaN. d_out overlaps no input. */
 int maivs_cache_attend(maivs_cache* cx, const void* d_queries, int dtype, size_t n_tokens, size_t query_stride,

@@ -277,9 +277,10 @@ __device__ __forceinline__ void find_places(const CacheView& c, const CacheToken
 
 // Rows into the cache. blockIdx.x: a run of tokens; blockIdx.y: even keys, odd values, times the slices of a
 // token's units. Eight lanes take a group of 64 dimensions of one head. Every lane goes through the same
-// passes; those without a unit, or whose token has no row, load and store nothing. Bound by its instructions as
-// much as by HBM: 34,000 tokens of 8 heads of 128 in bf16 take 61 us, 178 MB, 2.9 TB/s (some 20 us
-// more with single f32 operations and a bound on every element).
+// passes; those without a unit, or whose token has no row, load and store nothing. Bound by the issue of
+// instructions: 34,000 tokens of 8 heads of 128 in bf16 take 63 us, 178 MB, 2.8 TB/s, with an instruction in 67 % of the
+// cycles and the integer pipe busy in 57 %; the rest are fixed latencies and loads (some 20 us more with single f32
+// operations and a bound on every element).
 template <typename T, int G, int U, bool kWhole>
 __global__ void __launch_bounds__(kStoreBS) k_cache_append(CacheView c, AppendArgs a, bool vec, StoreShape sh) {
     __shared__ long long s_place[kMaxRun];
@@ -467,8 +468,9 @@ __device__ __forceinline__ void scan_counts(int (*s_cnt)[kCounts], int warp, int
 // A cluster per sequence: the keep-th largest weight by three rounds of counting over the
 // order-preserving keys (11, 11 and 10 bits from the top), then which rows stay, which leave and which
 // move where. A block takes one stretch of the rows and keeps their keys in shared memory; counts are
-// gathered over the cluster, ranks follow the rows' order. Bound by the latency of its five barriers
-// of the cluster and of the loads between them.
+// gathered over the cluster, ranks follow the rows' order. Bound by latency: 16 sequences of 3,000 to 32,768 rows take
+// 32 us, with an instruction in 30 % of the cycles; warps wait for loads and at the cluster's five barriers
+// in equal parts, half as long for shared memory.
 template <int N>
 __global__ void __launch_bounds__(kSelBS) k_cache_select(CacheView c, EvictArgs a, int key_cap) {
     const auto cl = cooperative_groups::this_cluster();

@@ -26,11 +26,14 @@
 // the column's largest product, so rows that have no weight, whatever their size, cost the others nothing (with a unit
 // from the largest step alone, f32 outputs beside such a row of 2^60 times the others' size were lost).
 //
-// Bound by instructions, close to HBM: two tiles of 16 rows (G = 2, eight columns) take some 520 of a warp, half
-// of them on the integer pipe (shifts and masks of codes, moves of halves), at 2304 bytes a tile. One token of
-// 8 query heads a head over 262,144 rows of 8 heads of 128, f16: 80 us, 302 MB (a copy's rate would be 46); with
-// one half for p * step, as in bf16, 69, of them 61 in this kernel, 4.9 TB/s. A token each of 64 sequences of 500
-// to 8,000 rows, 4 query heads a head, bf16: 97 us with the rows' weights (297 MB), 77 of them here.
+// Nothing is saturated: three warps a scheduler (168 registers a thread) leave 43 % of the issue slots empty, mostly to
+// the fixed latency of one instruction on the next; the integer pipe (shifts and masks of codes, moves of halves) is
+// busy 49 % of the time, the tensor pipe 37 %, HBM half. Two tiles of 16 rows (G = 2, eight columns) take 590
+// instructions of a warp, 4608 bytes. One token of 8 query heads a head over 262,144 rows of 8 heads of 128, f16: 80 us,
+// 302 MB (a copy's rate would be 46), 71 in this kernel; with one half for p * step, as in bf16, 69 and 61. A token
+// each of 64 sequences of 500 to 8,000 rows, 4 query heads a head, bf16: 97 us with the rows' weights (297 MB), 77 of
+// them here. Small calls of G = 6 wait for their code: 5 sequences of up to 5,001 rows, one head of 384, f32, issue
+// in 18 % of the cycles, and four of the seven cycles a warp spends on an instruction are waits for its fetch.
 // Measured and not kept: a multiplication for the codes' shifts (86 us for 83), clusters that join long rows in
 // shared memory (98 for 69), four or two blocks of two groups a SM for three, three and six waves of ragged
 // parts for four.
@@ -60,7 +63,9 @@ constexpr int kWaves = 4;
 constexpr int kPartRows = 1024, kWidePartRows = 16384;
 constexpr int kSoloLists = 2;
 // Up to so many rows a cluster of blocks reads them and joins in shared memory, in one launch; above, its
-// blocks would wait for the slowest and the SMs for a place for all of them.
+// blocks would wait for the slowest and the SMs for a place for all of them. One token of 8 heads of 128, 4 query
+// heads each, in a cluster and in parts: 256 rows 9.9 and 14.4 us, 2,048 11.1 and 14.3, 4,096 12.5 and 13.8, 8,192
+// 15.4 and 14.5; of 8 sequences 2,048 14.6 and 16.7.
 constexpr int kClusterRows = 2048;
 struct AttendPlan {
     int nc;         // columns per tile
@@ -1040,10 +1045,10 @@ AttendPlan make_plan(const CacheView& c, const AttendArgs& a) {
     tile(few, blocks_of(c.G, few));
     const bool join_inside = !found && rows <= kClusterRows && fill >= 2;
     // From 33 columns on (64 of one group) a block of 128 is faster than blocks of sixteen: 4 sequences of 20,000
-    // rows, 8 heads of 128, wide and narrow: 40 columns 96 and 109 us, 64 98 and 132, 112 104 and 203, 132 179 and
-    // 243, 160 182 and 278; heads of 64: 48 82 and 71, 64 83 and 83, 96 86 and 111, 132 153 and 150, 160 155 and 188;
-    // one sequence of 4000 rows, where the start counts: 40 22 and 18, 128 26 and 24. Not where clusters join few
-    // rows in one launch (500 rows, 96 columns: 22 and 15 us).
+    // rows, 8 heads of 128, wide and narrow: 32 columns 97 and 89 us, 36 97 and 112, 64 102 and 138, 112 108 and 211, 132
+    // 184 and 253, 160 186 and 316; heads of 64: 48 88 and 74, 64 88 and 86, 80 90 and 103, 128 95 and 154, 132 163 and
+    // 156, 160 166 and 193; one sequence of 4000 rows, where the start counts: 40 24 and 21, 128 27 and 27. Not where
+    // clusters join few rows in one launch (500 rows, 96 columns: 22 and 15 us).
     p.wide = !found && a.type == kBF16 && c.G <= 2 && cols >= (c.G == 1 ? 64 : 33) && !join_inside;
     if (p.wide) tile(kWideCols, 1);
     // Enough blocks to fill the GPU once; with sequences of different lengths kWaves times as many, of
@@ -1053,7 +1058,9 @@ AttendPlan make_plan(const CacheView& c, const AttendArgs& a) {
     // us in four parts, 147 in 18; of 20,000 to 32,000 rows, 128 to 256 columns: 234 and 258).
     p.cluster = p.parts = 1;
     p.share = most * step;
-    // Lists enough to fill the GPU by warps: none waits for a block's barriers.
+    // Lists enough to fill half the GPU by warps: none waits for a block's barriers. 257 rows a list, two heads of 64,
+    // f32, a warp and a block each: 250 lists 18.7 and 14.5 us, 500 22.7 and 22.8, 1,000 33.0 and 35.8, 4,000 90 and
+    // 115; one head of 128, 8 query heads, bf16: 500 20.9 and 21.6, 1,000 26.8 and 32.9.
     p.solo = found && c.G <= 2 && p.nc == 8 && items * kSoloLists >= slots * kAttWarps;
     if (join_inside) {
         p.cluster = (int)std::min<long long>({kMaxCluster, fill, most});

@@ -19,10 +19,10 @@
 //   24        issues the products, as soon as step i - 1 is over: P V of its tile, S of tile i + 1.
 // S and P have two places each, so that the products run beside the exponentials.
 //
-// Bound by the issue of instructions and the latencies between a step's barriers: 11,900 warp instructions a tile of
-// G = 2, 3,000 clocks a scheduler at best; a tile takes 4,500 clocks, the products' arithmetic 1,100 of them.
+// Bound by the issue of instructions and the latencies between a step's barriers: 9,100 warp instructions a tile of
+// G = 2, 2,300 clocks a scheduler at best; a tile takes 4,800 clocks, the products' arithmetic 1,100 of them.
 // Chunks of 32 to 64 tokens over 4 sequences of 20,000 to 32,000 rows, 8 heads of 128 with 4 query heads each:
-// 244 us, 78 GFLOP, a fifth of the tensor cores' rate (with the columns' padding to 128 a third). Where every
+// 243 us, 78 GFLOP, a fifth of the tensor cores' rate (with the columns' padding to 128 a third). Where every
 // tile's rows have units of their own, 2.5 times as long (270 us for 107, 32 tokens over four times 20,000 rows). On the way
 // there, in 18 parts of the rows (258 at the end): bounds on every load of a tile's codes 406 us; 16 warps, where
 // the same warps decoded keys and values, 394; scores 32 at a time, with their spills, 284; whole lines of codes
