@@ -71,11 +71,12 @@ __device__ __forceinline__ f2 add2(f2 a, f2 b) {
 // Whether a sequence's tokens lo .. hi - 1 ascend within the call's.
 __device__ __forceinline__ bool good_offsets(int lo, int hi, int n_tokens) { return lo >= 0 && hi >= lo && hi <= n_tokens; }
 
-// Sets `bit` of *flags where some sequence's do not; the threads of one block share the sequences.
+// Sets `bit` of *flags where some sequence's do not; the threads of a row of blocks share the sequences.
 __device__ __forceinline__ void check_offsets(const int32_t* __restrict__ off, int n_seqs, int n_tokens, uint32_t* flags,
                                               uint32_t bit) {
     bool bad = false;
-    for (int s = threadIdx.x; s < n_seqs; s += blockDim.x) bad |= !good_offsets(__ldg(off + s), __ldg(off + s + 1), n_tokens);
+    for (int s = blockIdx.x * blockDim.x + threadIdx.x; s < n_seqs; s += gridDim.x * blockDim.x)
+        bad |= !good_offsets(__ldg(off + s), __ldg(off + s + 1), n_tokens);
     if (bad) atomicOr(flags, bit);
 }
 

@@ -257,7 +257,7 @@ __device__ __forceinline__ void find_places(const CacheView& c, const CacheToken
                                             const uint64_t* token_ids) {
     const int l8 = threadIdx.x % kUnit;
     const unsigned mask = 0xFFu << (threadIdx.x % 32 / kUnit * kUnit);
-    if (blockIdx.x == 0 && blockIdx.y == 0) check_offsets(tk.offsets, c.n_seqs, tk.n_tokens, c.flags, kCacheOffsets);
+    if (blockIdx.y == 0) check_offsets(tk.offsets, c.n_seqs, tk.n_tokens, c.flags, kCacheOffsets);
     for (int i = threadIdx.x / kUnit; i < n_tok; i += kUnits) {
         const Place p = place_of(c, tk, tok0 + i, l8, mask);
         if (l8 == 0) {

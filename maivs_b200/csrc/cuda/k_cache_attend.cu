@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(kAttBS, Shape<G, NC, TYPE == kF32, (MODE >= Mo
     b /= kk.parts;
     const int h = b % c.heads;
     const int item = b / c.heads;  // sequence, or token of a found list
-    if (FOUND && blockIdx.x == 0) check_offsets(a.tok.offsets, c.n_seqs, a.tok.n_tokens, c.flags, kCacheOffsets);
+    if (FOUND) check_offsets(a.tok.offsets, c.n_seqs, a.tok.n_tokens, c.flags, kCacheOffsets);
     if (kSolo && item >= a.tok.n_tokens) return;
 
     Span sn;

@@ -308,6 +308,51 @@ def test_offsets_out_of_order_are_flagged_and_skipped(bad):
     assert c.flags(stream()) == 4 and (w_out == 7).all()
 
 
+@pytest.mark.parametrize("n_seqs", [513, 700, 3000])
+def test_many_sequences(n_seqs):
+    """More sequences than a group of lanes counts through: tokens, rows and lists find theirs by bisection; offsets out of
+    order are seen wherever they are."""
+    rng = np.random.default_rng(82)
+    cap, dim = 12, 64
+    held, new = rng.integers(0, 6, n_seqs), rng.integers(0, 4, n_seqs)
+    new[[0, n_seqs - 1]] = 0, 2
+    f = Filled(rng, [int(h + n) for h, n in zip(held, new)], cap, 1, dim, "f32")
+    t = int(new.sum())
+    _, q = rounded(rng.standard_normal((t, 2, dim)).astype(np.float32), "f32")
+    qt = torch.tensor(q).cuda()
+    out, lse, off, ln = torch.empty_like(qt), torch.empty(t, 2, device="cuda"), offsets(new), i32(held)
+    ws = torch.empty(max(1, f.cache.attend_workspace(t, 2)), dtype=torch.uint8, device="cuda")
+    f.cache.attend(qt.data_ptr(), t, 2, off.data_ptr(), ln.data_ptr(), out.data_ptr(), dtype="f32", d_lse=lse.data_ptr(),
+                   d_workspace=ws.data_ptr(), workspace_bytes=ws.numel(), stream=stream())
+    # every row that a token sees, as a list
+    lists = torch.arange(cap, device="cuda").repeat(t, 1)
+    out2, w = torch.empty_like(out), torch.empty(t, cap, device="cuda")
+    ws2 = torch.empty(f.cache.attend_found_workspace(t, 2, cap), dtype=torch.uint8, device="cuda")
+    f.cache.attend_found(qt.data_ptr(), t, 2, off.data_ptr(), ln.data_ptr(), lists.data_ptr(), cap, out2.data_ptr(), dtype="f32",
+                         causal=True, d_weights=w.data_ptr(), d_workspace=ws2.data_ptr(), workspace_bytes=ws2.numel(),
+                         stream=stream())
+    k, v = torch.empty(t, 1, dim, device="cuda"), torch.empty(t, 1, dim, device="cuda")
+    f.cache.read(k.data_ptr(), v.data_ptr(), t, off.data_ptr(), ln.data_ptr(), dtype="f32", stream=stream())
+    assert f.cache.flags(stream()) == 0
+    got, got2, k = out.cpu().numpy(), out2.cpu().numpy(), k.cpu().numpy()
+    tok = 0
+    for s in range(n_seqs):
+        for i in range(new[s]):
+            r = f.rows[s][0]
+            assert np.array_equal(k[tok, 0], r.k[held[s] + i].astype(np.float32))
+            for hh in range(2):
+                want, _, _, err, _, _ = O.attend_head_tight(q[tok, hh], r, list(range(held[s] + i + 1)), dim ** -0.5, "f32")
+                close(got[tok, hh], want, err, f"attend, sequence {s}")
+                close(got2[tok, hh], want, err, f"found, sequence {s}")
+            tok += 1
+    assert tok == t and torch.allclose(w.sum(dim=1), torch.full((t,), 2.0, device="cuda"), atol=1e-5)
+    bad = off.clone()
+    bad[n_seqs - 1] = t + 1
+    f.cache.read(torch.empty(t, dim, device="cuda").data_ptr(), torch.empty(t, dim, device="cuda").data_ptr(), t, bad.data_ptr(),
+                 ln.data_ptr(), dtype="f32", stream=stream())
+    assert f.cache.flags(stream()) == 4
+
+
 # ---- blocks of 128 columns: each test says that they ran ------------------------------------------
 def columns(f):
     return f.cache.stats()["block_columns"]
