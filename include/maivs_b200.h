@@ -353,7 +353,8 @@ int maivs_cache_evict(maivs_cache* cx, const int32_t* d_lengths, size_t keep, co
                       const uint64_t* d_protect_from, uint64_t* d_evicted, void* d_workspace, size_t workspace_bytes,
                       void* stream);
 int maivs_cache_evict_workspace(maivs_cache* cx, size_t* bytes);
-/* Flags that earlier work set (see above), cleared by the call; synchronises `stream`. */
+/* Flags that earlier work set (see above), cleared by the call; synchronises `stream`, which must not be capturing
+ * (MAIVS_BAD_STATE, and the capture goes on). */
 int maivs_cache_flags(maivs_cache* cx, void* stream, uint32_t* flags);
 
 /* profile(on) / profile_read(reset=True) (src/prof.rs:76-98): device time per query phase. The

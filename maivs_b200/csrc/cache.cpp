@@ -426,6 +426,12 @@ int maivs_cache_flags(maivs_cache* cx, void* stream, uint32_t* flags) {
         if (cx->device < 0) return no_storage(cx);
         OnDevice d(cx->device);
         cudaStream_t st = (cudaStream_t)stream;
+        // a wait in a capture would end it
+        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(st, &capture) != cudaSuccess || capture != cudaStreamCaptureStatusNone) {
+            cudaGetLastError();
+            return cfail(cx, MAIVS_BAD_STATE, "flags cannot be read while the stream is being captured");
+        }
         cudaError_t e = cudaMemcpyAsync(flags, cx->v.flags, sizeof(uint32_t), cudaMemcpyDeviceToHost, st);
         if (e == cudaSuccess) e = cudaMemsetAsync(cx->v.flags, 0, sizeof(uint32_t), st);
         if (e == cudaSuccess) e = cudaStreamSynchronize(st);

@@ -406,3 +406,30 @@ def test_which_form_runs():
         assert columns(f) == 0
         check_attend_raw(f, rng.standard_normal((new, group, dim)).astype(np.float32), [60 - new], [new], dtype)
         assert columns(f) == want
+
+
+# ---- capture --------------------------------------------------------------------------------------
+def test_flags_are_refused_in_a_capture_which_goes_on():
+    rng = np.random.default_rng(95)
+    f = Filled(rng, [40], LONG, 1, 64, "f32")
+    x = torch.randn(1, 1, 64, device="cuda")
+    out = torch.zeros_like(x)
+    off, ln = offsets([1]), i32([39])
+    ws = torch.empty(max(1, f.cache.attend_workspace(1, 1)), dtype=torch.uint8, device="cuda")
+
+    def go():
+        f.cache.attend(x.data_ptr(), 1, 1, off.data_ptr(), ln.data_ptr(), out.data_ptr(), dtype="f32", d_workspace=ws.data_ptr(),
+                       workspace_bytes=ws.numel(), stream=stream())
+
+    go()
+    torch.cuda.synchronize()
+    want = out.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        go()
+        with pytest.raises(ValueError, match="captured"):
+            f.cache.flags(stream())
+    out.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and f.cache.flags(stream()) == 0
